@@ -263,6 +263,26 @@ int ulm_swiglu_bwd(const ulm_swiglu_args* a);
  * two halves of one [rows, 2d] projection; y and dy are dense, n = rows * d.  d and row_stride: whole 16-byte vectors. */
 int ulm_swiglu_rows(const ulm_swiglu_args* a, int32_t backward, int64_t d, int64_t row_stride);
 
+/* ---- dropout with a mask that is computed and never stored -----------------
+ * The reference drops with F.dropout (train.py:1966-1994), which keeps a byte mask per element for its backward.
+ * Here the mask is a function of a 64-bit seed and the element's row-major index i alone: Philox4x32 with ten rounds, key =
+ * seed (low word first), counter = i / 8 (low word first), and of its 128 bits the (i % 8)-th 16, low halves first.  The element is
+ * dropped where they are below t = 65536 p rounded to an integer (ties to even; at least 1 for p > 0, at most 65535 for
+ * p < 1), the others are multiplied by 65536 / (65536 - t).  A dropped element is 0 whatever it held.  p in [0, 1].
+ *
+ * ulm_dropout: y = drop(x), n elements, both 16-byte aligned; y may be x.  Its own backward, on dy.
+ * ulm_swiglu_dropout: y = drop(silu(a) * b), or da and db from dy (backward != 0); d = 0: dense operands, else rows as in
+ *   ulm_swiglu_rows.  The mask goes by y's index.  fp32 arithmetic from the loads to the one rounding of each store.
+ * ulm_add_dropout_norm_fwd: x_out = x + drop(branch), y = rms_norm(x_out); ulm_rmsnorm_fwd's arguments with fp32 x and w,
+ *   a branch, and a 16-bit y_kind; rows of at most 8192 elements, a multiple of 4.  16-bit rows 8-byte aligned or better.
+ * ulm_add_dropout_norm_bwd: ulm_rmsnorm_bwd's arguments (x: the forward's x_out; rstd required; g_add may be NULL); dx is the
+ *   whole gradient of x_out and d_branch = drop(dx).  `partial`: ulm_add_dropout_norm_partial_rows(rows) * d floats. */
+int ulm_dropout(const void* x, void* y, int64_t n, int32_t dtype, double p, uint64_t seed, void* stream);
+int ulm_swiglu_dropout(const ulm_swiglu_args* a, int32_t backward, int64_t d, int64_t row_stride, double p, uint64_t seed);
+int ulm_add_dropout_norm_fwd(const ulm_rmsnorm_fwd_args* a, double p, uint64_t seed);
+int ulm_add_dropout_norm_bwd(const ulm_rmsnorm_bwd_args* a, double p, uint64_t seed);
+int64_t ulm_add_dropout_norm_partial_rows(int64_t rows);
+
 /* ---- chunked cross-entropy row kernels -----------------------------------
  * The reference loops fc_out + F.cross_entropy(reduction='sum') over chunks of
  * rows (train.py:2075-2079).  These kernels are the softmax part over one

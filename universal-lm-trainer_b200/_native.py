@@ -23,8 +23,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
-            'grad_post.cu', 'selftest.cu']          # slowest first: they are compiled in parallel
-_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
+            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu']          # slowest first: they are compiled in parallel
+_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
 _EXT_SOURCE = 'torch_ops.cpp'
@@ -39,6 +39,7 @@ ULM_F16, ULM_BF16, ULM_F32 = 0, 1, 2
 ULM_Y_SAME, ULM_Y_F16, ULM_Y_BF16 = 0, 1, 2
 ABI_VERSION = 4
 i64, i32, u32, f32, vp = C.c_int64, C.c_int32, C.c_uint32, C.c_float, C.c_void_p
+u64, f64 = C.c_uint64, C.c_double
 
 
 class RopeArgs(C.Structure):
@@ -132,6 +133,11 @@ EXPORTS = {
     'ulm_swiglu_fwd': (C.c_int, [C.POINTER(SwigluArgs)]),
     'ulm_swiglu_bwd': (C.c_int, [C.POINTER(SwigluArgs)]),
     'ulm_swiglu_rows': (C.c_int, [C.POINTER(SwigluArgs), C.c_int32, i64, i64]),
+    'ulm_dropout': (C.c_int, [vp, vp, i64, i32, f64, u64, vp]),
+    'ulm_swiglu_dropout': (C.c_int, [C.POINTER(SwigluArgs), i32, i64, i64, f64, u64]),
+    'ulm_add_dropout_norm_fwd': (C.c_int, [C.POINTER(RmsFwdArgs), f64, u64]),
+    'ulm_add_dropout_norm_bwd': (C.c_int, [C.POINTER(RmsBwdArgs), f64, u64]),
+    'ulm_add_dropout_norm_partial_rows': (i64, [i64]),
     'ulm_grad_unscale_sumsq': (C.c_int, [vp, i64, vp, vp, vp, vp]),
     'ulm_grad_clip': (C.c_int, [vp, i64, vp, f32, vp, vp]),
     'ulm_token_targets': (C.c_int, [vp, vp, i64, i64, i64, i64, vp, vp, vp]),

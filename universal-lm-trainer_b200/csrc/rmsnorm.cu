@@ -16,6 +16,7 @@
 // caller-provided scratch; a second small kernel sums the partials in a fixed order
 // (deterministic, no atomics).
 #include "common.cuh"
+#include "col_sum.cuh"
 
 #include <mutex>
 
@@ -692,26 +693,6 @@ rmsnorm_bwd_quad_kernel(const BwdParams p) {
   }
 }
 
-// dw[c] = sum over the partial rows, in a fixed order: a CTA takes 32 columns, its 32 x 32 threads each add
-// every 32nd partial row of one column (coalesced 128-byte reads, short independent chains), and the 32
-// sub-sums of a column are added in index order.
-__global__ void __launch_bounds__(1024)
-rmsnorm_dw_reduce_kernel(const float* __restrict__ partial, float* __restrict__ dw, int nparts, int d) {
-  __shared__ float sub[32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  float t = 0.f;
-  if (c < d)
-    for (int p = threadIdx.y; p < nparts; p += 32) t += partial[(int64_t)p * d + c];
-  sub[threadIdx.y][threadIdx.x] = t;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < d) {
-    float sum = 0.f;
-#pragma unroll
-    for (int g = 0; g < 32; ++g) sum += sub[g][threadIdx.x];
-    dw[c] = sum;
-  }
-}
-
 // y / dy may be 16-bit next to an fp32 x (autocast's layout); otherwise they have x's dtype
 int check_kind(const char* who, int kind, int x_dtype) {
   if (kind == ULM_Y_SAME) return ULM_OK;
@@ -889,7 +870,7 @@ int rmsnorm_bwd_launch(const ulm_rmsnorm_bwd_args* a, float* partial, const char
     rc = check_launch(who);
     if (rc) return rc;
   }
-  rmsnorm_dw_reduce_kernel<<<(a->d + 31) / 32, dim3(32, 32), 0, st>>>(partial, a->dw, a->rows > 0 ? (int)blocks : 0, a->d);
+  col_sum_kernel<<<(a->d + 31) / 32, dim3(32, 32), 0, st>>>(partial, a->dw, a->rows > 0 ? (int)blocks : 0, a->d);
   return check_launch(who);
 }
 }  // namespace ulm

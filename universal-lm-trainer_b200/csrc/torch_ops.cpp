@@ -705,34 +705,154 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& branch, c
   return {x_new, y};
 }
 
-struct SwigluBwd : OpNode {
+// ---------------------------------------------------------------------------
+// dropout with a mask that is never stored
+// ---------------------------------------------------------------------------
+// A probability and the seed of its mask; none: nothing is dropped and the op without dropout runs.
+struct Drop {
+  double p = 0;
+  int64_t seed = 0;
+  bool none() const { return p == 0; }
+};
+void check_drop(double p, const char* who) { TORCH_CHECK_VALUE(p >= 0 && p <= 1, who, ": p must lie between 0 and 1, got ", p); }
+bool aligned_to(const Tensor& t, int64_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
+// contiguous and 16-byte aligned
+Tensor dense16(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return aligned_to(c, 16) ? c : c.clone();
+}
+// [.., d] as [rows, d] with contiguous rows that all start on a multiple of `bytes`
+Tensor rows_on(const Tensor& x, int64_t bytes) {
+  const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  return x2.stride(1) == 1 && aligned_to(x2, bytes) && x2.stride(0) * x2.element_size() % bytes == 0 ? x2 : dense16(x2);
+}
+
+Tensor dropout_launch(const Tensor& x_in, const Drop& drop) {
+  OpScope scope;
+  c10::cuda::CUDAGuard dev(x_in.device());
+  const Tensor x = dense16(x_in), y = empty_cuda(x.sizes(), x.scalar_type(), x);
+  check(ulm_dropout(x.data_ptr(), y.data_ptr(), x.numel(), code_of(x.scalar_type()), drop.p, (uint64_t)drop.seed, stream_of(x)), "dropout");
+  return y;
+}
+
+Tensor dropout(const Tensor& x, double p, int64_t seed);
+
+struct DropoutBwd : OpNode {
+  Drop drop;
+  at::ScalarType dtype;
+  variable_list backward(variable_list& g, const variable_list&) override { return {dropout_launch(g[0].to(dtype), drop)}; }
+  // linear in x: the gradient is the op itself, which autograd can differentiate again
+  variable_list backward_recorded(variable_list& g, const variable_list&) override { return {::dropout(g[0].to(dtype), drop.p, drop.seed)}; }
+};
+
+Tensor dropout(const Tensor& x, double p, int64_t seed) {
+  TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()), "dropout needs a CUDA fp16/bf16/fp32 tensor");
+  check_drop(p, "dropout");
+  const Drop drop{p, seed};
+  const Tensor y = dropout_launch(x, drop);
+  if (!no_graph(x)) {
+    auto node = make_node<DropoutBwd>(x);
+    node->drop = drop; node->dtype = x.scalar_type();
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+struct DropNormBwd : OpNode {
+  Drop drop;
+  std::vector<int64_t> shape;
+  at::ScalarType wdtype, bdtype;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor a = kept[0], b = kept[1], dy = g[0].to(a.scalar_type()).contiguous();
+    const Tensor w = kept[1], rstd = kept[2], x = kept[0].view({-1, kept[0].size(-1)});
+    const int64_t rows = x.size(0), d = x.size(1);
+    // a y that nobody used has the gradient zero
+    const Tensor dy = g[1].defined() ? rows_on(g[1].to(bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
+    const Tensor ga = g[0].defined() ? rows_on(g[0].to(at::kFloat), 16) : Tensor();
+    const Tensor dx = empty_cuda({rows, d}, at::kFloat, x), db = empty_cuda({rows, d}, bdtype, x), dw = empty_cuda({d}, at::kFloat, x);
+    const Tensor partial = empty_cuda({ulm_add_dropout_norm_partial_rows(rows), d}, at::kFloat, x);
+    ulm_rmsnorm_bwd_args a{};
+    a.x = x.data_ptr(); a.w = w.data_ptr(); a.dy = dy.data_ptr(); a.rstd = rstd.data_ptr<float>();
+    a.dx = dx.data_ptr(); a.dw = dw.data_ptr<float>(); a.partial = partial.data_ptr<float>();
+    a.x_stride = d; a.dy_stride = dy.stride(0); a.dx_stride = d; a.rows = rows; a.d = (int32_t)d;
+    a.x_dtype = ULM_F32; a.w_dtype = ULM_F32; a.stream = stream_of(x); a.dy_kind = y_kind(bdtype, at::kFloat);
+    if (ga.defined()) { a.g_add = ga.data_ptr(); a.gadd_stride = ga.stride(0); }
+    a.d_branch = db.data_ptr(); a.dbranch_stride = d;
+    check(ulm_add_dropout_norm_bwd(&a, drop.p, (uint64_t)drop.seed), "dropout_add_rms_norm backward");
+    return {dx.view(shape), db.view(shape), dw.to(wdtype)};
+  }
+};
+
+std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& branch, const Tensor& weight, double p, int64_t seed, double eps) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kFloat && is_16bit(branch.scalar_type()) && branch.device() == x.device() && branch.sizes() == x.sizes(),
+                    "dropout_add_rms_norm needs an fp32 CUDA x and a 16-bit branch of the same shape and device");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) <= 8192 && x.size(-1) % 4 == 0, "dropout_add_rms_norm takes rows of at most 8192 elements, a multiple of 4");
+  TORCH_CHECK_VALUE(weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == x.size(-1) && weight.is_floating_point(),
+                    "dropout_add_rms_norm needs one weight per column, on the device of x");
+  check_drop(p, "dropout_add_rms_norm");
+  const Drop drop{p, seed};
+  Tensor x_new, y, w, rstd;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(x.device());
+    const int64_t d = x.size(-1);
+    const Tensor x2 = rows_on(x, 16), b2 = rows_on(branch, 8);
+    x_new = empty_cuda(x.sizes(), at::kFloat, x);
+    y = empty_cuda(x.sizes(), branch.scalar_type(), x);
+    rstd = empty_cuda({x2.size(0)}, at::kFloat, x);
+    w = dense16(weight.to(at::kFloat));
+    ulm_rmsnorm_fwd_args a{};
+    a.x = x2.data_ptr(); a.w = w.data_ptr(); a.y = y.data_ptr(); a.rstd = rstd.data_ptr<float>();
+    a.x_stride = x2.stride(0); a.y_stride = d; a.rows = x2.size(0); a.d = (int32_t)d;
+    a.x_dtype = ULM_F32; a.w_dtype = ULM_F32; a.eps = (float)eps; a.stream = stream_of(x); a.y_kind = y_kind(branch.scalar_type(), at::kFloat);
+    a.branch = b2.data_ptr(); a.x_out = x_new.data_ptr(); a.branch_stride = b2.stride(0); a.xout_stride = d;
+    check(ulm_add_dropout_norm_fwd(&a, p, (uint64_t)seed), "dropout_add_rms_norm forward");
+  }
+  if (!no_graph(x, branch, weight)) {
+    auto node = make_node<DropNormBwd>(x, branch, weight);
+    node->drop = drop; node->shape = x.sizes().vec(); node->wdtype = weight.scalar_type(); node->bdtype = branch.scalar_type();
+    torch::autograd::set_history(x_new, node);
+    torch::autograd::set_history(y, node);
+    node->keep(x_new, true); node->keep(w); node->keep(rstd);
+  }
+  return {x_new, y};
+}
+
+struct SwigluBwd : OpNode {
+  Drop drop;
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor a = kept[0], b = kept[1], gy = g[0].to(a.scalar_type()), dy = drop.none() ? gy.contiguous() : dense16(gy);
     const Tensor da = empty_cuda(a.sizes(), a.scalar_type(), a), db = empty_cuda(a.sizes(), a.scalar_type(), a);
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), nullptr, dy.data_ptr(), da.data_ptr(), db.data_ptr(), a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
-    check(ulm_swiglu_bwd(&p), "swiglu backward");
+    check(drop.none() ? ulm_swiglu_bwd(&p) : ulm_swiglu_dropout(&p, true, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu backward");
     return {da, db};
   }
 };
 
-Tensor swiglu(const Tensor& a_in, const Tensor& b_in) {
+Tensor gate(const Tensor& a_in, const Tensor& b_in, const Drop& drop) {
   TORCH_CHECK_VALUE(a_in.is_cuda() && known(a_in.scalar_type()) && b_in.scalar_type() == a_in.scalar_type() && b_in.sizes() == a_in.sizes(),
                     "swiglu needs two CUDA tensors of one shape and one of fp16/bf16/fp32");
   Tensor a, b, y;
   {
     OpScope scope;
     c10::cuda::CUDAGuard dev(a_in.device());
-    a = a_in.contiguous(); b = b_in.contiguous();
+    a = drop.none() ? a_in.contiguous() : dense16(a_in);
+    b = drop.none() ? b_in.contiguous() : dense16(b_in);
     y = empty_cuda(a.sizes(), a.scalar_type(), a);
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), y.data_ptr(), nullptr, nullptr, nullptr, a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
-    check(ulm_swiglu_fwd(&p), "swiglu forward");
+    check(drop.none() ? ulm_swiglu_fwd(&p) : ulm_swiglu_dropout(&p, false, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu forward");
   }
   if (!no_graph(a_in, b_in)) {
     auto node = make_node<SwigluBwd>(a_in, b_in);
+    node->drop = drop;
     node->keep(a); node->keep(b);
     torch::autograd::set_history(y, node);
   }
   return y;
+}
+Tensor swiglu(const Tensor& a, const Tensor& b) { return gate(a, b, Drop{}); }
+Tensor swiglu_dropout(const Tensor& a, const Tensor& b, double p, int64_t seed) {
+  check_drop(p, "swiglu_dropout");
+  return gate(a, b, Drop{p, seed});
 }
 
 // ---------------------------------------------------------------------------
@@ -920,21 +1040,22 @@ Tensor stacked(const Tensor& a, const Tensor& b) {
   return a.as_strided({a.size(0) + b.size(0), a.size(1)}, {a.size(1), 1}, a.storage_offset());
 }
 
-void swiglu_rows(const Tensor& ab, const Tensor& y, const Tensor& dy, const Tensor& dab, bool backward) {
+void swiglu_rows(const Tensor& ab, const Tensor& y, const Tensor& dy, const Tensor& dab, bool backward, const Drop& drop) {
   const int64_t d = ab.size(1) / 2, half = d * ab.element_size();
   auto at_half = [&](const Tensor& t, int h) -> void* { return t.defined() ? static_cast<char*>(t.data_ptr()) + h * half : nullptr; };
   ulm_swiglu_args p{at_half(ab, 0), at_half(ab, 1), at_half(y, 0), at_half(dy, 0), at_half(dab, 0), at_half(dab, 1), ab.size(0) * d,
                     code_of(ab.scalar_type()), 0, stream_of(ab)};
-  check(ulm_swiglu_rows(&p, backward, d, 2 * d), backward ? "swiglu backward" : "swiglu forward");
+  check(drop.none() ? ulm_swiglu_rows(&p, backward, d, 2 * d) : ulm_swiglu_dropout(&p, backward, d, 2 * d, drop.p, (uint64_t)drop.seed), backward ? "swiglu backward" : "swiglu forward");
 }
 
 struct GatedBwd : OpNode {
   at::ScalarType cd, x_dtype;
+  Drop drop;
   variable_list backward(variable_list& g, const variable_list& kept) override {
     const Tensor x = kept[0], w1 = kept[1], w3 = kept[2], ab = kept[3];
     const Tensor dy = g[0].reshape({-1, g[0].size(-1)}).to(cd).contiguous(), x2 = x.reshape({-1, x.size(-1)});
     const Tensor dab = empty_cuda(ab.sizes(), cd, ab);
-    swiglu_rows(ab, Tensor(), dy, dab, true);
+    swiglu_rows(ab, Tensor(), dy, dab, true, drop);
     const int64_t ff = w1.size(0);
     const Tensor da = dab.narrow(1, 0, ff), db = dab.narrow(1, ff, ff);
     Tensor dx, dw1, dw3;
@@ -966,11 +1087,11 @@ struct GatedBwd : OpNode {
 // Both projections write the two halves of one [rows, 2 ff] matrix: as one GEMM where the weights' 16-bit copies lie one
 // behind the other (WeightCopies).  Against two linears and a gate that is one GEMM less forward, two less backward,
 // and no pass that adds the two branches' gradients of x.
-Tensor gated_linear(const Tensor& x, const Tensor& w1, const Tensor& w3) {
+Tensor gated(const Tensor& x, const Tensor& w1, const Tensor& w3, const Drop& drop) {
   at::ScalarType cd = x.scalar_type();
   if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) cd = at::autocast::get_autocast_dtype(at::kCUDA);
   const int64_t ff = w1.size(0);
-  if (!x.is_cuda() || !known(cd) || w3.sizes() != w1.sizes() || ff % (16 / (int64_t)c10::elementSize(cd))) return ::swiglu(::linear(x, w1), ::linear(x, w3));
+  if (!x.is_cuda() || !known(cd) || w3.sizes() != w1.sizes() || ff % (16 / (int64_t)c10::elementSize(cd))) return gate(::linear(x, w1), ::linear(x, w3), drop);
   Tensor xc, ab, y;
   {
     OpScope scope;
@@ -988,15 +1109,21 @@ Tensor gated_linear(const Tensor& x, const Tensor& w1, const Tensor& w3) {
     auto n = xc.sizes().vec();
     n.back() = ff;
     y = empty_cuda(n, cd, x2);
-    swiglu_rows(ab, y, Tensor(), Tensor(), false);
+    swiglu_rows(ab, y, Tensor(), Tensor(), false, drop);
   }
   if (!no_graph(x, w1, w3)) {
     auto node = make_node<GatedBwd>(x, w1, w3);
-    node->cd = cd; node->x_dtype = x.scalar_type();
+    node->cd = cd; node->x_dtype = x.scalar_type(); node->drop = drop;
     node->keep(xc); node->keep(w1); node->keep(w3); node->keep(ab);
     torch::autograd::set_history(y, node);
   }
   return y;
+}
+
+Tensor gated_linear(const Tensor& x, const Tensor& w1, const Tensor& w3) { return gated(x, w1, w3, Drop{}); }
+Tensor gated_linear_dropout(const Tensor& x, const Tensor& w1, const Tensor& w3, double p, int64_t seed) {
+  check_drop(p, "gated_linear");
+  return gated(x, w1, w3, Drop{p, seed});
 }
 
 // ---------------------------------------------------------------------------
@@ -1180,6 +1307,9 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "rms_norm", &::rms_norm);
   def_op(m, "add_rms_norm", &::add_rms_norm);
   def_op(m, "swiglu", &::swiglu);
+  def_op(m, "swiglu_dropout", &::swiglu_dropout);
+  def_op(m, "dropout", &::dropout);
+  def_op(m, "dropout_add_rms_norm", &::dropout_add_rms_norm);
   py::class_<ContextToken>(m, "ContextToken").def("leave", &leave_context);
   m.def("enter_wgrad_in_place", [](bool on) { return enter_context([on](OpContext& c) { c.wgrad_in_place = on; }); });
   py::class_<WeightCopies, std::shared_ptr<WeightCopies>>(m, "WeightCopies")
@@ -1195,6 +1325,7 @@ PYBIND11_MODULE(_ulm_torch, m) {
   }, no_gil());
   def_op(m, "linear", &::linear);
   def_op(m, "gated_linear", &::gated_linear);
+  def_op(m, "gated_linear_dropout", &::gated_linear_dropout);
   m.def("lm_head_lse", &lm_head_lse, no_gil());
   m.def("lm_head_score", &lm_head_score, no_gil());
   m.def("token_targets", &token_targets, no_gil());

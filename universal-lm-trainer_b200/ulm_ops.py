@@ -70,6 +70,63 @@ def swiglu(a, b):
 
 
 # ---------------------------------------------------------------------------
+# Dropout with a mask that is never stored
+# ---------------------------------------------------------------------------
+def dropout(x, p, seed):
+    """Inverted dropout of a CUDA fp16/bf16/fp32 tensor: each element is zero with probability ``p`` (in steps of 2^-16) and
+    otherwise divided by the share that stays.  Which ones are dropped is a function of ``seed`` (any 64-bit integer) and of the
+    element's row-major index alone (`Philox4x32`, include/ulm_b200.h says how), so nothing is kept for the backward: it forms
+    the mask again.  The same seed drops the same elements of another tensor of that size."""
+    return N.ext().dropout(x, float(p), _as_i64(seed))
+
+
+def swiglu_dropout(a, b, p, seed):
+    """``dropout(silu(a) * b)`` in one kernel each way (the reference's feed-forward, train.py:1975); p = 0 is `swiglu`.
+    Values stay in fp32 up to the one rounding of the result."""
+    return N.ext().swiglu_dropout(a, b, float(p), _as_i64(seed))
+
+
+def dropout_add_rms_norm(x, branch, weight, p, seed, eps: float = 1e-6):
+    """`add_rms_norm` with dropout on the branch: ``x_new = x + dropout(branch)`` and ``y = rms_norm(x_new)`` in one pass
+    (train.py:1993 with the norm behind it), returns ``(x_new, y)``.  x and x_new fp32, branch and y 16-bit, rows of at most 8192
+    elements, a multiple of 4.  The backward gives the gradients of x, branch and weight in one pass and a column sum."""
+    return N.ext().dropout_add_rms_norm(x, branch, weight, float(p), _as_i64(seed), float(eps))
+
+
+def _as_i64(seed):
+    """The 64 bits of ``seed`` as the signed integer the extension takes."""
+    seed = int(seed)
+    if not -(1 << 63) <= seed < 1 << 64:
+        raise ValueError('a dropout seed is a 64-bit integer')
+    return seed - (1 << 64) if seed >= 1 << 63 else seed
+
+
+def next_dropout_seed():
+    """A seed from torch's default CPU generator: `torch.manual_seed` fixes the sequence, and a checkpointed forward that is run
+    again draws the same ones.  No device is asked."""
+    return int(torch.randint(0, 1 << 62, ()))
+
+
+class Dropout(nn.Module):
+    """`nn.Dropout` on `dropout`: the same ``p`` and the same training switch, no stored mask, a mask of its own per call."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f'dropout probability has to be between 0 and 1, but got {p}')
+        self.p = p
+
+    def active(self):
+        return self.training and self.p > 0.0
+
+    def forward(self, x):
+        return dropout(x, self.p, next_dropout_seed()) if self.active() else x
+
+    def extra_repr(self):
+        return f'p={self.p}'
+
+
+# ---------------------------------------------------------------------------
 # Bias-free linear layers with the weight gradient accumulated where it lives
 # ---------------------------------------------------------------------------
 @contextlib.contextmanager
@@ -119,9 +176,12 @@ def linear_copies(model, dtype):
     return weight_copies(ws, dtype) if ws and dtype in _16BIT else None
 
 
-def gated_linear(x, w1, w3):
+def gated_linear(x, w1, w3, dropout_p=0.0, seed=0):
     """``swiglu(linear(x, w1), linear(x, w3))`` (train.py:1975) as one op: both projections write the halves of one
-    [rows, 2 d_ff] matrix, which the gate's kernels read and differentiate in place of two."""
+    [rows, 2 d_ff] matrix, which the gate's kernels read and differentiate in place of two.  ``dropout_p``, ``seed``: with the
+    gate of `swiglu_dropout`."""
+    if dropout_p:
+        return N.ext().gated_linear_dropout(x, w1, w3, float(dropout_p), _as_i64(seed))
     return N.ext().gated_linear(x, w1, w3)
 
 
