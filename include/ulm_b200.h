@@ -356,6 +356,43 @@ int64_t ulm_lmhead_parts(int64_t rows, int32_t V);
  * ignored rows.  part_i: int32 scratch of the size of part_m. */
 int ulm_lmhead_score(const ulm_lmhead_lse_args* a, uint8_t* hit, int32_t* part_i);
 
+/* ---- lm head + cross-entropy without the logits ----------------------------
+ * The loss of train.py:2069-2082 over a vocabulary too large to keep [rows, V] logits for: the forward goes over the
+ * vocabulary once with a running maximum and sum per row, the backward forms the logits again, `piece` columns at a time,
+ * and keeps softmax - onehot of one piece in 16 bits.  z = h w^T stays in fp32 throughout (it is not rounded to the 16-bit type).
+ * fwd: lse[r] and loss[r] = lse[r] - z[r, target[r]] in fp32; loss 0 where target[r] is ignore_index or no column.
+ *      scratch: ulm_streamed_ce_scratch(rows, V, d) floats.
+ * bwd: with f = *factor_dev (d total / d row loss) and G = softmax - onehot, 0 on the rows above:
+ *      dh [rows, d] = f G w, dense, of the 16-bit type; dw [V, d] = f G^T h, 16-bit, or fp32 with dw_f32, or added to an fp32
+ *      dw with dw_add; either may be NULL.  lse is the forward's.
+ *      workspace: ulm_streamed_ce_workspace(rows, V, piece) 16-bit elements; slots: ulm_streamed_ce_slots(...) floats (may
+ *      be 0); dh_sum: fp32 [rows, d], needed with a dh and a piece below V.  piece: a multiple of 256.
+ * h [rows, d], w [V, d]: fp16 or bf16, 16-byte aligned, row strides multiples of 8 elements, d a multiple of 8; rows and V of
+ * any size.  All sums run in a fixed order.  status_dev: optional, see ULM_STATUS_*. */
+typedef struct {
+  const void* h; const void* w; const int64_t* target;
+  float* lse; float* loss; float* scratch;             /* loss, scratch: forward only */
+  int64_t h_stride, w_stride;
+  int64_t rows; int32_t V; int32_t d;
+  int32_t dtype; int32_t reserved;
+  int64_t ignore_index;
+  uint32_t* status_dev;
+  void* stream;
+} ulm_streamed_ce_args;
+typedef struct {
+  const float* factor_dev;
+  void* dh; void* dw;
+  int64_t dw_stride;
+  int32_t dw_f32, dw_add;
+  void* workspace; float* slots; float* dh_sum;
+  int64_t piece;
+} ulm_streamed_ce_grads;
+int ulm_streamed_ce_fwd(const ulm_streamed_ce_args* a);
+int ulm_streamed_ce_bwd(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g);
+int64_t ulm_streamed_ce_scratch(int64_t rows, int32_t V, int32_t d);
+int64_t ulm_streamed_ce_workspace(int64_t rows, int32_t V, int64_t piece);
+int64_t ulm_streamed_ce_slots(int64_t rows, int32_t V, int32_t d, int64_t piece, int32_t want_dh, int32_t want_dw);
+
 /* ---- gradient post-processing after the data-parallel all-reduce ----------
  * No counterpart kernel in the reference: fuses what scaler.unscale_ and
  * clip_grad_norm_ do in separate passes (train.py:2364-2365) over one flat fp32

@@ -23,8 +23,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
-            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu']          # slowest first: they are compiled in parallel
-_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
+            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu']          # slowest first: they are compiled in parallel
+_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
 _EXT_SOURCE = 'torch_ops.cpp'
@@ -109,6 +109,17 @@ class LmHeadLseArgs(C.Structure):
                 ('ignore_index', i64), ('status_dev', vp), ('stream', vp)]
 
 
+class StreamedCeArgs(C.Structure):
+    _fields_ = [('h', vp), ('w', vp), ('target', vp), ('lse', vp), ('loss', vp), ('scratch', vp), ('h_stride', i64), ('w_stride', i64),
+                ('rows', i64), ('V', i32), ('d', i32), ('dtype', i32), ('reserved', i32), ('ignore_index', i64),
+                ('status_dev', vp), ('stream', vp)]
+
+
+class StreamedCeGrads(C.Structure):
+    _fields_ = [('factor_dev', vp), ('dh', vp), ('dw', vp), ('dw_stride', i64), ('dw_f32', i32), ('dw_add', i32),
+                ('workspace', vp), ('slots', vp), ('dh_sum', vp), ('piece', i64)]
+
+
 # every symbol include/ulm_b200.h declares: name -> (restype, argtypes)
 EXPORTS = {
     'ulm_abi_version': (C.c_int, []),
@@ -138,6 +149,11 @@ EXPORTS = {
     'ulm_add_dropout_norm_fwd': (C.c_int, [C.POINTER(RmsFwdArgs), f64, u64]),
     'ulm_add_dropout_norm_bwd': (C.c_int, [C.POINTER(RmsBwdArgs), f64, u64]),
     'ulm_add_dropout_norm_partial_rows': (i64, [i64]),
+    'ulm_streamed_ce_fwd': (C.c_int, [C.POINTER(StreamedCeArgs)]),
+    'ulm_streamed_ce_bwd': (C.c_int, [C.POINTER(StreamedCeArgs), C.POINTER(StreamedCeGrads)]),
+    'ulm_streamed_ce_scratch': (i64, [i64, i32, i32]),
+    'ulm_streamed_ce_workspace': (i64, [i64, i32, i64]),
+    'ulm_streamed_ce_slots': (i64, [i64, i32, i32, i64, i32, i32]),
     'ulm_grad_unscale_sumsq': (C.c_int, [vp, i64, vp, vp, vp, vp]),
     'ulm_grad_clip': (C.c_int, [vp, i64, vp, f32, vp, vp]),
     'ulm_token_targets': (C.c_int, [vp, vp, i64, i64, i64, i64, vp, vp, vp]),

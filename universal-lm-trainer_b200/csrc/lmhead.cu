@@ -19,6 +19,7 @@
 // 25 column tiles): the running statistics stay in registers across the group's tiles; all CTAs sweep the
 // same column group at the same time, so the W tiles are shared through L2.
 // All barrier waits are bounded (status bit + clean exit on expiry), like the attention kernels'.
+#include "lmhead_tiles.cuh"
 #include "tc.cuh"
 
 namespace ulm {
@@ -26,9 +27,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int LM_BM = 128, LM_BN = 256, LM_BK = 64;
 constexpr int kLmStages = 4;
-constexpr int kLmGroupTiles = 25;                      // column tiles per work item (upper bound)
 constexpr uint32_t kLmATile = LM_BM * LM_BK * 2;       // 16 KB
 constexpr uint32_t kLmBTile = LM_BN * LM_BK * 2;       // 32 KB
 constexpr uint32_t kLmStage = kLmATile + kLmBTile;
@@ -51,65 +50,6 @@ static_assert(kLmSmem <= 227 * 1024, "shared memory");
 
 template <typename T> struct LmFmt { static constexpr int v = 0; };
 template <> struct LmFmt<__nv_bfloat16> { static constexpr int v = 1; };
-
-// 4-D tiled store shared -> global (the counterpart of tma_load_4d), completion tracked by bulk groups
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* smem_src, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-      ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Barrier over the 128 threads of one column half (ids 1, 2) whose OR-reduction tells every one of them
-// whether any of them (or another role of the CTA) has given up.
-__device__ __forceinline__ bool half_sync_any(int half, bool fail) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.or.pred p, %2, 128, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(any) : "r"((uint32_t)fail), "r"(half + 1) : "memory");
-  return any != 0;
-}
-
-// Column tiles per work item: the count whose rounds of items over the SMs take the fewest tile times, an item's own
-// cost (pipeline fill, statistics) being worth about a quarter of a tile.  At 32768 x 32000 that is 5 (220 tile times,
-// 216 ideal; the fixed 25 of before took 225); with 2048 rows x 4096 columns, 1 instead of 16: 256 items on 148 SMs
-// where 16 SMs had one each.
-int lm_group_tiles(int64_t rows, int V) {
-  const int64_t n_rb = (rows + LM_BM - 1) / LM_BM, n_ct = (V + LM_BN - 1) / LM_BN;
-  int best = 1;
-  int64_t best_cost = INT64_MAX;
-  for (int want = 1; want <= kLmGroupTiles; ++want) {
-    const int64_t groups = (n_ct + want - 1) / want, tiles = (n_ct + groups - 1) / groups;
-    const int64_t cost = ((n_rb * groups + kNumSMs - 1) / kNumSMs) * (4 * tiles + 1);
-    if (cost < best_cost) { best_cost = cost; best = (int)tiles; }
-  }
-  return best;
-}
-
-struct LmItems {
-  int n_rb, n_ct, n_groups, group_tiles;
-  __host__ __device__ LmItems(int64_t rows, int V, int tiles) {
-    n_rb = (int)((rows + LM_BM - 1) / LM_BM);
-    n_ct = (V + LM_BN - 1) / LM_BN;
-    group_tiles = tiles;
-    n_groups = (n_ct + tiles - 1) / tiles;
-  }
-  __host__ __device__ int n_items() const { return n_rb * n_groups; }
-  // all CTAs are on one column group at a time: its W tiles are read from L2 by everyone
-  __device__ void decode(int idx, int& rb, int& g, int& ct0, int& nct) const {
-    g = idx / n_rb;
-    rb = idx - g * n_rb;
-    ct0 = g * group_tiles;
-    nct = n_ct - ct0 < group_tiles ? n_ct - ct0 : group_tiles;
-  }
-};
 
 // TOP1 (scoring): instead of storing the logits the epilogue picks out what a score needs of them, the target's logit
 // (into z_target) and the column of the largest one (part_i, the lowest on ties; ~column of the first NaN if there is one).

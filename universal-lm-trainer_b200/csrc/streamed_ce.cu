@@ -1,0 +1,642 @@
+// lm head + softmax cross-entropy over a large vocabulary in pieces of the vocabulary, with its gradient, without the logits
+// (sm_100a).
+//
+//   z = H W^T (fp32 accumulators, never stored),  l_r = ln sum_c exp z[r,c],  loss_r = l_r - z[r, target_r]
+//   G[r,c] = exp(z[r,c] - l_r) - [c = target_r]          (0 on ignored rows)
+//   dH = g G W,   dW = g G^T H                           g: one factor for all rows, in device memory
+//
+// Forward: one pass over the vocabulary that keeps a running maximum and sum per row, and the target's logit.  Backward, for
+// one piece of the vocabulary at a time: z again, G of the piece in 16 bits into a workspace [rows, piece], then the two
+// products that read it; dH is summed over the pieces in fp32.  So 8 rows V d flops where keeping the logits takes 6, and
+// a workspace whose size does not depend on the vocabulary.
+//
+// G is the only rounding before the results': to 16 bits, which the tensor cores take, with fp32 sums of exact
+// products behind it.  fp16 would lose probabilities below 2^-24, so its G is held times 2^14 (|G| <= 1) and the factor taken
+// back in the fp32 epilogue.  z is not rounded to 16 bits.
+//
+// All four products run through one main loop: persistent CTAs of 320 threads, one per SM (warps 0-7 epilogue, warp 8 one-lane
+// TMA producer, warp 9 one-lane tcgen05.mma issuer), output tiles of 128 x 256, M128 x N256 x K16 instructions, four
+// stages of 128x64 + 256x64 operands in 128-byte-swizzled shared memory, two accumulators of 256 TMEM columns so that a
+// tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
+// contiguous, so dH reads W, and dW reads both G and H, as MN-major operands: rows of 64-element atoms, no transposed copies.
+// Waits are bounded (status bit and clean exit on expiry), like the attention kernels'.
+#include "lmhead_tiles.cuh"
+#include "tc.cuh"
+
+#include <algorithm>
+
+namespace ulm {
+namespace {
+
+using namespace tc;
+
+enum Mode { kStats, kGrad, kRowGrad, kColGrad };         // statistics; G; dH = G W; dW = G^T H
+
+constexpr int kStages = 4;
+constexpr uint32_t kATile = LM_BM * LM_BK * 2;           // 16 KB
+constexpr uint32_t kBTile = LM_BN * LM_BK * 2;           // 32 KB
+constexpr uint32_t kStage = kATile + kBTile;
+constexpr uint32_t kAtom = 64 * 64 * 2;                  // one MN-major box: 64 (MN) x 64 (K)
+constexpr uint32_t kStaging = 128 * 64 * 2;              // one 128-row x 64-column block of G
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int64_t kSlot = (int64_t)LM_BM * LM_BN;        // floats of one partial tile
+
+template <typename T> struct Fmt { static constexpr int idesc = 0, g_shift = 14; };
+template <> struct Fmt<__nv_bfloat16> { static constexpr int idesc = 1, g_shift = 0; };
+
+struct Ctl {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_free[2];
+  uint32_t tmem_base;
+  int abort;
+  uint32_t fail_bits;
+};
+constexpr size_t kCtlBytes = 1024;
+static_assert(sizeof(Ctl) <= kCtlBytes, "control block");
+constexpr size_t smem_bytes(int mode) { return 1024 + (size_t)kStages * kStage + (mode == kGrad ? 2 * (size_t)kStaging : 0) + kCtlBytes; }
+static_assert(smem_bytes(kGrad) <= 227 * 1024, "shared memory");
+
+// One launch's work.  Items are numbered and dealt round the CTAs.
+//   statistics: 128 rows x a group of column tiles, whose statistics stay in registers;
+//   G: one tile each, rows fastest, so that all CTAs read one stretch of W;
+//   products: `whole` tiles, then the `rest` tiles that would not fill a round of the SMs, cut into `split` stretches of the inner
+//   dimension each; every stretch leaves its fp32 tile in a slot, and a second kernel adds up a tile's slots in order.
+struct Work {
+  int n_mt, n_nt, n_kb, group;
+  int whole, rest, split;
+};
+struct Item { int mt, nt, count, kb0, kb1, slot; };
+
+template <int MODE>
+__host__ __device__ inline int n_items(const Work& w) {
+  if (MODE == kStats) return w.n_mt * ((w.n_nt + w.group - 1) / w.group);
+  if (MODE == kGrad) return w.n_mt * w.n_nt;
+  return w.whole + w.rest * w.split;
+}
+template <int MODE>
+__device__ __forceinline__ Item item_of(const Work& w, int q) {
+  Item it{0, 0, 1, 0, w.n_kb, -1};
+  if constexpr (MODE == kStats) {
+    const int g = q / w.n_mt;
+    it.mt = q - g * w.n_mt;
+    it.nt = g * w.group;
+    it.count = min(w.group, w.n_nt - it.nt);
+  } else if constexpr (MODE == kGrad) {
+    it.nt = q / w.n_mt;
+    it.mt = q - it.nt * w.n_mt;
+  } else {
+    int t = q;
+    if (q >= w.whole) {
+      const int part = q - w.whole, s = part / w.rest, j = part - s * w.rest;
+      t = w.whole + j;
+      it.kb0 = (int)((int64_t)w.n_kb * s / w.split);
+      it.kb1 = (int)((int64_t)w.n_kb * (s + 1) / w.split);
+      if (w.split > 1) it.slot = j * w.split + s;
+    }
+    it.mt = t / w.n_nt;                                  // the column tiles of one row tile side by side: they share its A panel in L2
+    it.nt = t - it.mt * w.n_nt;
+  }
+  return it;
+}
+
+// How the accumulators leave: out = factor * acc (+ prev)
+struct Out {
+  const float* factor_dev;
+  float factor;
+  const float* prev;
+  void* out;
+  int64_t ld, rows;                                      // of out and prev
+  int cols, is_f32;
+  float* slots;
+};
+struct Params {
+  Work w;
+  int64_t rows;
+  int V, v0;                                             // vocabulary; first column of the piece
+  const int64_t* target;
+  int64_t ignore_index;
+  float *part_m, *part_s, *z_target;                     // statistics
+  const float* lse;                                      // G
+  int g_cols;                                            // the workspace's columns
+  Out out;                                               // products
+  uint32_t* status;
+};
+
+__device__ __forceinline__ int target_column(const Params& p, int64_t row) {
+  if (row >= p.rows) return -1;
+  const int64_t t = p.target[row];
+  return t != p.ignore_index && t >= 0 && t < p.V ? (int)t : -1;
+}
+
+// 64 accumulator columns of one row: columns col .. col + 63 of the output (or of a slot)
+template <typename T>
+__device__ __forceinline__ void put_row(const Out& o, float factor, int64_t row, int col, const uint32_t (&acc)[64]) {
+  if (row >= o.rows) return;
+#pragma unroll
+  for (int c = 0; c < 64; c += 8) {
+    if (col + c < o.cols) {                              // the width is whole vectors of 8
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = factor * __uint_as_float(acc[c + j]);
+      const int64_t at = row * o.ld + col + c;
+      if (o.prev) {
+        const float4 a = *reinterpret_cast<const float4*>(o.prev + at), b = *reinterpret_cast<const float4*>(o.prev + at + 4);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+      if (o.is_f32) {
+        float4* q = reinterpret_cast<float4*>(static_cast<float*>(o.out) + at);
+        q[0] = make_float4(v[0], v[1], v[2], v[3]);
+        q[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<T*>(o.out) + at) =
+            make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]), Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7]));
+      }
+    }
+  }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
+                   const __grid_constant__ Params p) {
+  constexpr bool kAmn = MODE == kColGrad, kBmn = MODE == kRowGrad || MODE == kColGrad;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* stages = base;                                             // [stage][A tile | B tile]
+  uint8_t* staging = base + (size_t)kStages * kStage;                 // G: [column half] one 128x64 block each
+  Ctl* ctl = reinterpret_cast<Ctl*>(staging + (MODE == kGrad ? 2 * (size_t)kStaging : 0));
+  volatile int* abort_flag = &ctl->abort;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int items = n_items<MODE>(p.w);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&ctl->acc_full[b], 1); mbar_init(&ctl->acc_free[b], kEpiWarps * 32); }
+    ctl->abort = 0;
+    ctl->fail_bits = 0;
+    fence_mbar_init();
+  }
+  if (warp == kEpiWarps + 1) { tmem_alloc(&ctl->tmem_base, 512); tmem_relinquish(); }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);   // warp-uniform
+
+  if (warp == kEpiWarps) {
+    // ---------------- TMA producer ----------------
+    if (elect_one()) {
+      tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB);
+      uint32_t it = 0;                                   // k-blocks issued so far, over all tiles
+      bool ok = true;
+      for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+        const Item im = item_of<MODE>(p.w, q);
+        for (int t = 0; ok && t < im.count; ++t) {
+          const int m0 = im.mt * LM_BM, n0 = (im.nt + t) * LM_BN;
+          for (int kb = im.kb0; kb < im.kb1; ++kb, ++it) {
+            const uint32_t s = it % kStages;
+            if (it >= (uint32_t)kStages && !mbar_wait(&ctl->empty[s], ((it / kStages) - 1) & 1, abort_flag)) {
+              atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_MMA);
+              ok = false;
+              break;
+            }
+            uint8_t* a = stages + (size_t)s * kStage;
+            uint8_t* b = a + kATile;
+            const int k0 = kb * LM_BK;
+            mbar_expect_tx(&ctl->full[s], kStage);
+            if constexpr (kAmn) {
+#pragma unroll
+              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d(a + i * kAtom, &tmA, &ctl->full[s], m0 + 64 * i, k0, 0, 0);
+            } else {
+              tma_load_4d(a, &tmA, &ctl->full[s], k0, m0, 0, 0);
+            }
+            // W's rows are vocabulary columns, counted from the piece's first
+            if constexpr (kBmn) {
+#pragma unroll
+              for (int i = 0; i < LM_BN / 64; ++i) tma_load_4d(b + i * kAtom, &tmB, &ctl->full[s], n0 + 64 * i, MODE == kRowGrad ? p.v0 + k0 : k0, 0, 0);
+            } else {
+              tma_load_4d(b, &tmB, &ctl->full[s], k0, p.v0 + n0, 0, 0);
+            }
+          }
+        }
+      }
+      if (*abort_flag) {   // let our own copies land before the CTA's shared memory goes away
+        for (uint32_t u = it > (uint32_t)kStages ? it - kStages : 0; u < it; ++u) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try(&ctl->full[u % kStages], (u / kStages) & 1))
+            if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+        }
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // ---------------- MMA issuer ----------------
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc(Fmt<T>::idesc, LM_BM, LM_BN, kBmn, kAmn);
+      constexpr uint64_t kStepA = kAmn ? 2048 >> 4 : 32 >> 4, kStepB = kBmn ? 2048 >> 4 : 32 >> 4;      // 16 elements of the inner dimension on
+      uint32_t it = 0, tt = 0;                           // k-blocks / tiles so far
+      bool ok = true;
+      for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+        const Item im = item_of<MODE>(p.w, q);
+        for (int t = 0; ok && t < im.count; ++t, ++tt) {
+          const uint32_t b = tt & 1;
+          // the accumulator still holds tile tt-2 until the epilogue warps have read it
+          if (tt >= 2 && !mbar_wait(&ctl->acc_free[b], ((tt >> 1) - 1) & 1, abort_flag)) { atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_SOFTMAX); ok = false; break; }
+          fence_after_sync();
+          for (int kb = im.kb0; kb < im.kb1; ++kb, ++it) {
+            const uint32_t s = it % kStages;
+            if (!mbar_wait(&ctl->full[s], (it / kStages) & 1, abort_flag)) { atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_LOAD); ok = false; break; }
+            fence_after_sync();
+            const uint32_t sa = smem_u32(stages + (size_t)s * kStage);
+            const uint64_t da = kAmn ? make_sdesc_sw128_mn(sa, kAtom) : make_sdesc_sw128(sa);
+            const uint64_t db = kBmn ? make_sdesc_sw128_mn(sa + kATile, kAtom) : make_sdesc_sw128(sa + kATile);
+#pragma unroll
+            for (int kk = 0; kk < LM_BK / 16; ++kk)
+              mma_ss(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
+            mma_commit(&ctl->empty[s]);                  // the stage is free once these MMAs have read it
+          }
+          if (ok) mma_commit(&ctl->acc_full[b]);
+        }
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int half = warp >> 2;                          // columns [128 half, 128 half + 128) of the tile
+    const int r = ((warp & 3) << 5) | lane;              // row within the tile == TMEM lane
+    const int tg = (int)threadIdx.x - half * 128;        // thread within its half (0..127)
+    const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    [[maybe_unused]] uint8_t* my_staging = staging + (size_t)half * kStaging;
+    [[maybe_unused]] float factor = 0.f;
+    if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = *p.out.factor_dev * p.out.factor;
+    uint32_t tt = 0;
+    bool ok = true;
+    for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+      const Item im = item_of<MODE>(p.w, q);
+      const int64_t grow = (int64_t)im.mt * LM_BM + r;
+      [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
+      [[maybe_unused]] float shift = 0.f;                // G: 2^(z log2e + shift)
+      [[maybe_unused]] int tgt = -1;
+      if constexpr (MODE == kStats || MODE == kGrad) tgt = target_column(p, grow);
+      if constexpr (MODE == kGrad) shift = tgt >= 0 ? (float)Fmt<T>::g_shift - p.lse[grow] * kLog2e : 0.f;
+      for (int t = 0; ok && t < im.count; ++t, ++tt) {
+        const uint32_t b = tt & 1;
+        const bool waited = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[b], (tt >> 1) & 1, abort_flag));
+        if (!waited && lane == 0) atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_MMA);
+        // every thread of the half learns the same verdict (a barrier follows inside the passes)
+        if (half_sync_any(half, !waited || *abort_flag != 0)) { ok = false; break; }
+        fence_after_sync();
+        const int col_tile = (im.nt + t) * LM_BN;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          const int c_blk = half * 128 + pass * 64;      // first column of this pass within the tile
+          uint32_t acc[64];
+          tmem_ld32(t_row + b * LM_BN + c_blk, *reinterpret_cast<uint32_t(*)[32]>(&acc[0]));
+          tmem_ld32(t_row + b * LM_BN + c_blk + 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[32]));
+          tmem_wait_ld();
+          if (pass == 1) {                               // everything of this tile is in registers: hand the accumulator back
+            fence_before_sync();
+            mbar_arrive(&ctl->acc_free[b]);
+          }
+          if constexpr (MODE == kStats) {
+            const int col0 = col_tile + c_blk;
+            if (col0 + 64 > p.V) {
+#pragma unroll
+              for (int c = 0; c < 64; ++c)
+                if (col0 + c >= p.V) acc[c] = __float_as_uint(-INFINITY);
+            }
+            if ((unsigned)(tgt - col0) < 64u) {          // one block of one thread holds the row's target
+              float z = 0.f;
+#pragma unroll
+              for (int c = 0; c < 64; ++c) z = tgt - col0 == c ? __uint_as_float(acc[c]) : z;
+              p.z_target[grow] = z;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) mx = fmax3(mx, __uint_as_float(acc[c]), __uint_as_float(acc[c + 1]));
+            const float m_new = fmaxf(m, mx * kLog2e);
+            if (m_new > -INFINITY) {
+              ssum *= ex2(m - m_new);                    // 2^(-inf) = 0 on the first block
+              const float nm = -m_new;
+              float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+              for (int c = 0; c < 64; c += 4) {
+                s0 += ex2(fmaf(__uint_as_float(acc[c]), kLog2e, nm));
+                s1 += ex2(fmaf(__uint_as_float(acc[c + 1]), kLog2e, nm));
+                s2 += ex2(fmaf(__uint_as_float(acc[c + 2]), kLog2e, nm));
+                s3 += ex2(fmaf(__uint_as_float(acc[c + 3]), kLog2e, nm));
+              }
+              ssum += (s0 + s1) + (s2 + s3);
+              m = m_new;
+            } else {                                     // nothing but -inf, or NaN, which fmaxf passes over
+#pragma unroll
+              for (int c = 0; c < 64; ++c)
+                if (__uint_as_float(acc[c]) != __uint_as_float(acc[c])) ssum = __uint_as_float(acc[c]);
+            }
+          } else if constexpr (MODE == kGrad) {
+            const int col0 = p.v0 + col_tile + c_blk;
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+              const float g0 = ex2(fmaf(__uint_as_float(acc[c]), kLog2e, shift)), g1 = ex2(fmaf(__uint_as_float(acc[c + 1]), kLog2e, shift));
+              acc[c] = __float_as_uint(g0);
+              acc[c + 1] = __float_as_uint(g1);
+            }
+            if ((unsigned)(tgt - col0) < 64u) {
+#pragma unroll
+              for (int c = 0; c < 64; ++c)
+                if (tgt - col0 == c) acc[c] = __float_as_uint(__uint_as_float(acc[c]) - (float)(1 << Fmt<T>::g_shift));
+            }
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) pk[c >> 1] = tgt >= 0 ? Cvt<T>::pack2(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1])) : 0u;
+            if (col0 + 64 > p.V) {                       // the workspace's columns past the vocabulary are zero
+#pragma unroll
+              for (int c = 0; c < 64; c += 2) {
+                if (col0 + c >= p.V) pk[c >> 1] = 0u;
+                else if (col0 + c + 1 >= p.V) pk[c >> 1] &= 0xffffu;
+              }
+            }
+            // the previous store out of this staging block must have read it
+            if (tg == 0) bulk_wait_read0();
+            if (half_sync_any(half, *abort_flag != 0)) { ok = false; break; }
+            // row r of a 128-byte-swizzled block: 16-byte chunk c sits at chunk position c ^ (r & 7)
+            uint8_t* row = my_staging + (size_t)r * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+            fence_proxy_async_smem();
+            if (half_sync_any(half, *abort_flag != 0)) { ok = false; break; }
+            if (tg == 0 && col_tile + c_blk < p.g_cols) {
+              tma_store_4d(&tmG, my_staging, col_tile + c_blk, im.mt * LM_BM, 0, 0);
+              bulk_commit();
+            }
+          } else {
+            if (im.slot >= 0) {
+              float4* s = reinterpret_cast<float4*>(p.out.slots + im.slot * kSlot + r * LM_BN + c_blk);
+#pragma unroll
+              for (int c = 0; c < 64; c += 4)
+                s[c >> 2] = make_float4(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1]), __uint_as_float(acc[c + 2]), __uint_as_float(acc[c + 3]));
+            } else {
+              put_row<T>(p.out, factor, grow, col_tile + c_blk, acc);
+            }
+          }
+        }
+      }
+      if constexpr (MODE == kStats) {
+        if (!ok) break;
+        if (grow < p.rows) {                             // [row][group][half]: the finishing kernel merges a row's pairs
+          const int64_t o = (grow * ((p.w.n_nt + p.w.group - 1) / p.w.group) + im.nt / p.w.group) * 2 + half;
+          p.part_m[o] = m;
+          p.part_s[o] = ssum;
+        }
+      }
+    }
+    if (MODE == kGrad && tg == 0) bulk_wait0();          // our stores must be complete before the CTA ends
+  }
+
+  fence_before_sync();
+  __syncthreads();
+  if (warp == kEpiWarps + 1) tmem_dealloc(tmem_base, 512);
+  if (threadIdx.x == 0 && ctl->fail_bits && p.status) atomicOr(p.status, ctl->fail_bits);
+}
+
+// The tiles that were cut: out = factor * (sum of the tile's slots, in order) (+ prev).  A CTA takes eight rows of a tile, a
+// thread eight columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+streamed_ce_join_kernel(const Work w, const Out o) {
+  const int j = blockIdx.x, t = w.whole + j, mt = t / w.n_nt, nt = t - mt * w.n_nt;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 8;
+  const int64_t row = (int64_t)mt * LM_BM + r;
+  const int col = nt * LM_BN + c;
+  if (row >= o.rows || col >= o.cols) return;
+  const float* s = o.slots + (int64_t)j * w.split * kSlot + r * LM_BN + c;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  for (int k = 0; k < w.split; ++k, s += kSlot) {
+    const float4 a = *reinterpret_cast<const float4*>(s), b = *reinterpret_cast<const float4*>(s + 4);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  const float factor = *o.factor_dev * o.factor;
+  const int64_t at = row * o.ld + col;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = factor * v[i] + (o.prev ? o.prev[at + i] : 0.f);
+  if (o.is_f32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(o.out) + at);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<T*>(o.out) + at) =
+        make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]), Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7]));
+  }
+}
+
+// lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry).
+// One warp per row.
+__global__ void __launch_bounds__(256)
+streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int n_parts, const int64_t* __restrict__ target,
+                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows) {
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  float m = -INFINITY;
+  for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, part_m[r * n_parts + i]);
+  m = warp_max(m);
+  float s = 0.f;
+  for (int i = lane; i < n_parts; i += 32) {
+    const float mi = part_m[r * n_parts + i], si = part_s[r * n_parts + i];
+    s += mi > -INFINITY ? si * exp2f(mi - m) : si;       // a group of nothing but -inf has the sum 0; of NaN, NaN
+  }
+  s = warp_sum(s);
+  if (lane) return;
+  const float l = (m + log2f(s)) * kLn2;
+  lse[r] = l;
+  const int64_t t = target[r];
+  loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : l - loss[r];
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+// The rest tiles' split: the fewest rounds over the SMs, in k-blocks, an item's own cost (fill, epilogue, its slot's way
+// through memory) being worth about 12 of them; stretches of at least 4 k-blocks.
+Work product_work(int64_t m, int64_t n, int64_t k) {
+  Work w{};
+  w.n_mt = (int)((m + LM_BM - 1) / LM_BM);
+  w.n_nt = (int)((n + LM_BN - 1) / LM_BN);
+  w.n_kb = (int)((k + LM_BK - 1) / LM_BK);
+  const int64_t tiles = (int64_t)w.n_mt * w.n_nt;
+  w.whole = (int)(tiles / kNumSMs * kNumSMs);
+  w.rest = (int)(tiles - w.whole);
+  w.split = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= 64 && w.rest && (s == 1 || w.n_kb / s >= 4); ++s) {
+    const int64_t rounds = ((int64_t)w.rest * s + kNumSMs - 1) / kNumSMs, cost = rounds * ((w.n_kb + s - 1) / s + 12) + (s > 1 ? 12 : 0);
+    if (cost < best) { best = cost; w.split = s; }
+  }
+  return w;
+}
+int64_t slot_floats(const Work& w) { return w.split > 1 ? (int64_t)w.rest * w.split * kSlot : 0; }
+
+template <typename T, int MODE>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, const Params& p, int device, cudaStream_t st, const char* who) {
+  static std::atomic<bool> attr_set[kMaxDevices];
+  auto kern = streamed_ce_kernel<T, MODE>;
+  if (int rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who)) return rc;
+  const int items = n_items<MODE>(p.w), grid = items < kNumSMs ? items : kNumSMs;
+  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mg, p);
+  if (int rc = check_launch(who)) return rc;
+  if (MODE >= kRowGrad && p.w.split > 1) {
+    streamed_ce_join_kernel<T><<<dim3(p.w.rest, LM_BM / 8), 256, 0, st>>>(p.w, p.out);
+    return check_launch(who);
+  }
+  return ULM_OK;
+}
+
+int check_args(const ulm_streamed_ce_args* a, const char* who) {
+  if (!a) return fail(ULM_ERR_ARG, "%s: null args", who);
+  if (a->dtype != ULM_F16 && a->dtype != ULM_BF16) return fail(ULM_ERR_ARG, "%s: dtype must be fp16 or bf16", who);
+  if (a->rows < 0 || a->V <= 0 || a->d <= 0 || a->d % 8) return fail(ULM_ERR_ARG, "%s: need rows >= 0, V > 0, d a positive multiple of 8", who);
+  // tile numbers and TMA coordinates are 32-bit
+  if (a->rows > (1 << 30) || a->V > (1 << 30) || a->d > (1 << 20)) return fail(ULM_ERR_TOO_LARGE, "%s: too many rows or columns", who);
+  if (((a->rows + 127) / 128) * (((int64_t)a->V + 255) / 256) > 0x7fffffffLL) return fail(ULM_ERR_TOO_LARGE, "%s: too many output tiles", who);
+  if (a->rows == 0) return ULM_OK;
+  if (!a->h || !a->w || !a->target || !a->lse) return fail(ULM_ERR_ARG, "%s: null tensor", who);
+  return ULM_OK;
+}
+bool ok_out(const void* p, int64_t stride, int d) { return !(reinterpret_cast<uintptr_t>(p) & 15) && stride % 8 == 0 && stride >= d; }
+
+Params common_params(const ulm_streamed_ce_args* a) {
+  Params p{};
+  p.rows = a->rows; p.V = a->V; p.target = a->target; p.ignore_index = a->ignore_index; p.status = a->status_dev;
+  return p;
+}
+
+Work stats_work(int64_t rows, int V, int d) {
+  Work w{};
+  w.n_mt = (int)((rows + LM_BM - 1) / LM_BM);
+  w.n_nt = (V + LM_BN - 1) / LM_BN;
+  w.n_kb = (d + LM_BK - 1) / LM_BK;
+  w.group = lm_group_tiles(rows, V);
+  return w;
+}
+
+template <typename T>
+int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
+  CUtensorMap mh, mw;
+  if (int rc = encode_matrix_map(&mh, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who)) return rc;
+  if (int rc = encode_matrix_map(&mw, a->w, a->dtype, a->V, a->d, a->w_stride, LM_BN, who)) return rc;
+  Params p = common_params(a);
+  p.w = stats_work(a->rows, a->V, a->d);
+  const int parts = 2 * ((p.w.n_nt + p.w.group - 1) / p.w.group);
+  p.part_m = a->scratch; p.part_s = a->scratch + a->rows * parts; p.z_target = a->loss;
+  cudaStream_t st = (cudaStream_t)a->stream;
+  if (int rc = launch<T, kStats>(mh, mw, mh, p, device, st, who)) return rc;
+  streamed_ce_finish_kernel<<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V, a->lse, a->loss, a->rows);
+  return check_launch(who);
+}
+
+int64_t g_stride(int64_t piece) { return (piece + 63) / 64 * 64; }
+
+template <typename T>
+int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int device, const char* who) {
+  cudaStream_t st = (cudaStream_t)a->stream;
+  CUtensorMap h_rows, h_mn, w_rows, w_mn;                // K-major and MN-major boxes of both
+  int rc;
+  if ((rc = encode_matrix_map(&h_rows, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who))) return rc;
+  if ((rc = encode_matrix_map(&h_mn, a->h, a->dtype, a->rows, a->d, a->h_stride, 64, who))) return rc;
+  if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, LM_BN, who))) return rc;
+  if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
+  for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
+    const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece, stride = g_stride(n);
+    CUtensorMap g_rows, g_mn;
+    if ((rc = encode_matrix_map(&g_rows, g->workspace, a->dtype, a->rows, stride, stride, LM_BM, who))) return rc;
+    if ((rc = encode_matrix_map(&g_mn, g->workspace, a->dtype, a->rows, stride, stride, 64, who))) return rc;
+    Params p = common_params(a);
+    p.v0 = (int)v0;
+    p.lse = a->lse;
+    p.g_cols = (int)stride;
+    p.w = stats_work(a->rows, (int)n, a->d);
+    if ((rc = launch<T, kGrad>(h_rows, w_rows, g_rows, p, device, st, who))) return rc;
+    p.out.factor_dev = g->factor_dev;
+    p.out.factor = 1.f / (float)(1 << Fmt<T>::g_shift);
+    p.out.slots = g->slots;
+    p.out.cols = a->d;
+    if (g->dw) {
+      p.w = product_work(n, a->d, a->rows);
+      p.out.ld = g->dw_stride; p.out.rows = n; p.out.is_f32 = g->dw_f32;
+      p.out.out = g->dw_f32 ? (void*)((float*)g->dw + v0 * g->dw_stride) : (void*)((T*)g->dw + v0 * g->dw_stride);
+      p.out.prev = g->dw_add ? (const float*)p.out.out : nullptr;
+      if ((rc = launch<T, kColGrad>(g_mn, h_mn, g_mn, p, device, st, who))) return rc;
+    }
+    if (g->dh) {
+      const bool first = v0 == 0, last = v0 + n >= a->V;
+      p.w = product_work(a->rows, a->d, n);
+      p.out.rows = a->rows;
+      p.out.is_f32 = !last;
+      p.out.out = last ? g->dh : (void*)g->dh_sum;
+      p.out.prev = first ? nullptr : g->dh_sum;
+      p.out.ld = a->d;                                   // dh and dh_sum are dense
+      if ((rc = launch<T, kRowGrad>(g_rows, w_mn, g_rows, p, device, st, who))) return rc;
+    }
+  }
+  return ULM_OK;
+}
+
+}  // namespace
+}  // namespace ulm
+
+extern "C" int64_t ulm_streamed_ce_scratch(int64_t rows, int32_t V, int32_t d) {
+  if (rows <= 0 || V <= 0 || d <= 0) return 0;
+  const ulm::Work w = ulm::stats_work(rows, V, d);
+  return rows * 4 * ((w.n_nt + w.group - 1) / w.group);
+}
+
+extern "C" int64_t ulm_streamed_ce_workspace(int64_t rows, int32_t V, int64_t piece) {
+  return rows * ulm::g_stride(piece < V ? piece : V);
+}
+
+extern "C" int64_t ulm_streamed_ce_slots(int64_t rows, int32_t V, int32_t d, int64_t piece, int32_t want_dh, int32_t want_dw) {
+  using namespace ulm;
+  if (rows <= 0 || V <= 0 || d <= 0 || piece <= 0) return 0;
+  int64_t most = 0;
+  const int64_t tail = V % piece ? V % piece : piece;    // the pieces have two sizes at most
+  for (int64_t n : {piece < V ? piece : (int64_t)V, tail < V ? tail : (int64_t)V}) {
+    if (want_dw) most = std::max(most, slot_floats(product_work(n, d, rows)));
+    if (want_dh) most = std::max(most, slot_floats(product_work(rows, d, n)));
+  }
+  return most;
+}
+
+extern "C" int ulm_streamed_ce_fwd(const ulm_streamed_ce_args* a) {
+  using namespace ulm;
+  const char* who = "ulm_streamed_ce_fwd";
+  int rc = check_args(a, who);
+  if (rc || a->rows == 0) return rc;
+  if (!a->loss || !a->scratch) return fail(ULM_ERR_ARG, "%s: null tensor", who);
+  DeviceScope scope(a->h, who);
+  if (scope.rc) return scope.rc;
+  return a->dtype == ULM_BF16 ? forward<__nv_bfloat16>(a, scope.device, who) : forward<__half>(a, scope.device, who);
+}
+
+extern "C" int ulm_streamed_ce_bwd(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g) {
+  using namespace ulm;
+  const char* who = "ulm_streamed_ce_bwd";
+  int rc = check_args(a, who);
+  if (rc) return rc;
+  if (!g) return fail(ULM_ERR_ARG, "%s: null grads", who);
+  if (g->piece <= 0 || g->piece % LM_BN) return fail(ULM_ERR_ARG, "%s: piece must be a positive multiple of %d columns", who, LM_BN);
+  if (a->rows == 0 || (!g->dh && !g->dw)) return ULM_OK;
+  if (!g->factor_dev || !g->workspace || (g->dh && g->piece < a->V && !g->dh_sum)) return fail(ULM_ERR_ARG, "%s: null tensor", who);
+  if (!g->slots && ulm_streamed_ce_slots(a->rows, a->V, a->d, g->piece, g->dh != nullptr, g->dw != nullptr) > 0) return fail(ULM_ERR_ARG, "%s: null slots", who);
+  if ((g->dw && !ok_out(g->dw, g->dw_stride, a->d)) || (g->dh && !ok_out(g->dh, a->d, a->d)) || (reinterpret_cast<uintptr_t>(g->dh_sum) & 15) ||
+      (reinterpret_cast<uintptr_t>(g->slots) & 15))
+    return fail(ULM_ERR_ARG, "%s: gradients must be 16-byte aligned, dw's row stride a multiple of 8 and at least d", who);
+  if (g->dw_add && !g->dw_f32) return fail(ULM_ERR_ARG, "%s: only an fp32 dw can be added to", who);
+  DeviceScope scope(a->h, who);
+  if (scope.rc) return scope.rc;
+  return a->dtype == ULM_BF16 ? backward<__nv_bfloat16>(a, g, scope.device, who) : backward<__half>(a, g, scope.device, who);
+}

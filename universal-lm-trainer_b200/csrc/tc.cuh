@@ -98,6 +98,30 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
         "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+// 4-D tiled store shared -> global (the counterpart of tma_load_4d), completion tracked by bulk groups
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* smem_src, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+      ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Barrier over the 128 threads of one half of the epilogue warps (ids 1, 2) whose OR-reduction tells every one of them
+// whether any of them (or another role of the CTA) has given up.
+__device__ __forceinline__ bool half_sync_any(int half, bool fail) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(any) : "r"((uint32_t)fail), "r"(half + 1) : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -131,9 +155,9 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // tcgen05.mma descriptors
 // ---------------------------------------------------------------------------
 // Instruction descriptor for kind::f16: fp32 accumulate, A and B both `fmt`
-// (0 = f16, 1 = bf16), A always K-major, B K-major (b_mn = 0) or MN-major (1).
-__host__ __device__ constexpr uint32_t make_idesc(int fmt, int M, int N, int b_mn) {
-  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)b_mn << 16) |
+// (0 = f16, 1 = bf16), each K-major (a_mn, b_mn = 0) or MN-major (1).
+__host__ __device__ constexpr uint32_t make_idesc(int fmt, int M, int N, int b_mn, int a_mn = 0) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // Shared-memory matrix descriptor, 128-byte swizzle, rows of exactly 128 bytes
@@ -148,6 +172,12 @@ __device__ __forceinline__ uint64_t make_sdesc_sw128(uint32_t smem_addr) {
   d |= (uint64_t)1 << 46;                     // version
   d |= (uint64_t)2 << 61;                     // SWIZZLE_128B
   return d;
+}
+
+// The same for an MN-major operand wider than one 64-element atom: the tile is a row of TMA boxes of 64 (MN) x box_rows (K)
+// elements, `atom_bytes` apart; groups of 8 K rows lie 1024 bytes apart within each.  16 K rows on: + 2048 bytes.
+__device__ __forceinline__ uint64_t make_sdesc_sw128_mn(uint32_t smem_addr, uint32_t atom_bytes) {
+  return (make_sdesc_sw128(smem_addr) & ~((uint64_t)0x3FFF << 16)) | (uint64_t)(atom_bytes >> 4) << 16;
 }
 
 // D[tmem] (+)= A[smem] * B[smem]
@@ -286,6 +316,11 @@ struct ItemIter {
 // reuses its buffers pays for the driver call once per buffer instead of once per launch.
 int encode_bhsd_map(CUtensorMap* out, const void* base, int dtype, int B, int H, int S,
                     int64_t sb, int64_t sh, int64_t ss, int box_rows, const char* what);
+
+// Describes a row-major 16-bit matrix [rows, cols], rows `stride` elements apart (a multiple of 8), for boxes of box_rows
+// rows x 64 columns with the 128-byte swizzle: a 4-D tensor {cols, rows, 1, 1}, coordinates (column, row, 0, 0).  Loads read zeros
+// past either end, stores leave them out.  Same cache.
+int encode_matrix_map(CUtensorMap* out, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* what);
 
 void map_cache_stats(uint64_t* hits, uint64_t* misses);
 

@@ -27,7 +27,7 @@ void fetch_entry_point() {
 struct MapKey {
   const void* base;
   int64_t sb, sh, ss;
-  int32_t dtype, B, H, S, box_rows, pad;
+  int32_t dtype, B, H, S, box_rows, matrix;
   bool operator==(const MapKey& o) const { return std::memcmp(this, &o, sizeof(MapKey)) == 0; }
 };
 struct MapKeyHash {
@@ -46,6 +46,35 @@ std::unordered_map<MapKey, CUtensorMap, MapKeyHash>& cache() {
   return *m;
 }
 std::atomic<uint64_t> g_cache_hits{0}, g_cache_misses{0};
+
+// The map of `key` with these dimensions and byte strides, from the cache or from the driver.
+int cached_map(CUtensorMap* out, const MapKey& key, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], const char* what) {
+  std::call_once(g_once, fetch_entry_point);
+  if (!g_encode) return fail(ULM_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available (%s)", what, cudaGetErrorString(g_once_err));
+  {
+    std::lock_guard<std::mutex> lock(g_cache_mu);
+    auto it = cache().find(key);
+    if (it != cache().end()) {
+      *out = it->second;
+      g_cache_hits.fetch_add(1, std::memory_order_relaxed);
+      return ULM_OK;
+    }
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)key.box_rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType dt = key.dtype == ULM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = g_encode(out, dt, 4, const_cast<void*>(key.base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ULM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", what, (int)r);
+  g_cache_misses.fetch_add(1, std::memory_order_relaxed);
+  {
+    std::lock_guard<std::mutex> lock(g_cache_mu);
+    if (cache().size() >= kCacheMax) cache().clear();
+    cache().emplace(key, *out);
+  }
+  return ULM_OK;
+}
 
 }  // namespace
 
@@ -78,8 +107,6 @@ void map_cache_stats(uint64_t* hits, uint64_t* misses) {
 
 int encode_bhsd_map(CUtensorMap* out, const void* base, int dtype, int B, int H, int S,
                     int64_t sb, int64_t sh, int64_t ss, int box_rows, const char* what) {
-  std::call_once(g_once, fetch_entry_point);
-  if (!g_encode) return fail(ULM_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available (%s)", what, cudaGetErrorString(g_once_err));
   if (reinterpret_cast<uintptr_t>(base) & 15) return fail(ULM_ERR_ARG, "%s: base pointer must be 16-byte aligned", what);
   // A dimension of extent 1 never advances, so its stride only has to be legal.
   const int64_t dense_s = 64;
@@ -96,31 +123,24 @@ int encode_bhsd_map(CUtensorMap* out, const void* base, int dtype, int B, int H,
   std::memset(&key, 0, sizeof(key));
   key.base = base; key.sb = sb; key.sh = sh; key.ss = ss;
   key.dtype = dtype; key.B = B; key.H = H; key.S = S; key.box_rows = box_rows;
-  {
-    std::lock_guard<std::mutex> lock(g_cache_mu);
-    auto it = cache().find(key);
-    if (it != cache().end()) {
-      *out = it->second;
-      g_cache_hits.fetch_add(1, std::memory_order_relaxed);
-      return ULM_OK;
-    }
-  }
   const cuuint64_t dims[4] = {64, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType dt = dtype == ULM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = g_encode(out, dt, 4, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(ULM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", what, (int)r);
-  g_cache_misses.fetch_add(1, std::memory_order_relaxed);
-  {
-    std::lock_guard<std::mutex> lock(g_cache_mu);
-    if (cache().size() >= kCacheMax) cache().clear();
-    cache().emplace(key, *out);
-  }
-  return ULM_OK;
+  return cached_map(out, key, dims, strides, what);
+}
+
+int encode_matrix_map(CUtensorMap* out, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* what) {
+  if (reinterpret_cast<uintptr_t>(base) & 15) return fail(ULM_ERR_ARG, "%s: base pointer must be 16-byte aligned", what);
+  if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || cols > 0x7fffffffLL) return fail(ULM_ERR_ARG, "%s: bad matrix size", what);
+  if (rows == 1) stride = (cols + 7) / 8 * 8;            // never applied
+  if (stride < cols || stride % 8 || stride >= (int64_t)1 << 39)
+    return fail(ULM_ERR_ARG, "%s: the row stride must be a multiple of 8 elements and at least the row", what);
+  MapKey key;
+  std::memset(&key, 0, sizeof(key));
+  key.base = base; key.ss = stride; key.dtype = dtype; key.H = (int32_t)cols; key.S = (int32_t)rows; key.box_rows = box_rows;
+  key.matrix = 1;
+  const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, 1, 1};
+  const cuuint64_t strides[3] = {(cuuint64_t)stride * 2, (cuuint64_t)stride * 2, (cuuint64_t)stride * 2};   // the last two: of extent 1
+  return cached_map(out, key, dims, strides, what);
 }
 
 }  // namespace tc

@@ -1264,6 +1264,95 @@ Tensor kept_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tens
 }
 
 // ---------------------------------------------------------------------------
+// lm head + cross-entropy, the form that never has the logits
+// ---------------------------------------------------------------------------
+// operands and stream of one launch; hc and wc have rows on 16-byte boundaries
+ulm_streamed_ce_args streamed_args(const Tensor& hc, const Tensor& wc, const Tensor& target, const Tensor& lse, int64_t ignore_index) {
+  ulm_streamed_ce_args a{};
+  a.h = hc.data_ptr(); a.w = wc.data_ptr(); a.target = target.data_ptr<int64_t>(); a.lse = lse.data_ptr<float>();
+  a.h_stride = hc.stride(0); a.w_stride = wc.stride(0);
+  a.rows = hc.size(0); a.V = (int32_t)wc.size(0); a.d = (int32_t)hc.size(1); a.dtype = code_of(hc.scalar_type());
+  a.ignore_index = ignore_index; a.status_dev = status_ptr(hc); a.stream = stream_of(hc);
+  return a;
+}
+
+struct StreamedCeBwd : OpNode {
+  int64_t ignore_index = 0, piece_bytes = 0;
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor hidden = kept[0], weight = kept[1], target = kept[2], lse = kept[3], inv = kept[4], wc = kept[5], hc = kept[6];
+    const bool want_h = task_should_compute_output(0), want_w = task_should_compute_output(1);
+    if (!want_h && !want_w) return {Tensor(), Tensor()};
+    const at::ScalarType cd = hc.scalar_type();
+    const int64_t rows = hc.size(0), d = hc.size(1), V = wc.size(0);
+    ulm_streamed_ce_args a = streamed_args(hc, wc, target, lse, ignore_index);
+    ulm_streamed_ce_grads o{};
+    const Tensor factor = g[0].to(at::kFloat).mul(inv);                         // d loss / d row loss
+    o.factor_dev = factor.data_ptr<float>();
+    o.piece = std::max<int64_t>(256, piece_bytes / (2 * rows) / 256 * 256);
+    Tensor dh, dw, dh_sum, slots;
+    bool added = false;
+    if (want_h) {
+      dh = empty_cuda({rows, d}, cd, hc);
+      o.dh = dh.data_ptr();
+      if (o.piece < V) { dh_sum = empty_cuda({rows, d}, at::kFloat, hc); o.dh_sum = dh_sum.data_ptr<float>(); }
+    }
+    if (want_w) {
+      const Tensor into = weight.grad();
+      added = wgrad_in_place() && into.defined() && into.scalar_type() == at::kFloat && into.is_contiguous() && aligned_to(into, 16);
+      // fp32 parameters get the fp32 sums: no 16-bit rounding and no cast pass
+      dw = added ? into : empty_cuda({V, d}, weight.scalar_type() == at::kFloat ? at::kFloat : cd, hc);
+      o.dw = dw.data_ptr(); o.dw_stride = d; o.dw_f32 = dw.scalar_type() == at::kFloat; o.dw_add = added;
+    }
+    const Tensor workspace = empty_cuda({ulm_streamed_ce_workspace(rows, a.V, o.piece)}, cd, hc);
+    o.workspace = workspace.data_ptr();
+    if (const int64_t n = ulm_streamed_ce_slots(rows, a.V, a.d, o.piece, want_h, want_w)) {
+      slots = empty_cuda({n}, at::kFloat, hc);
+      o.slots = slots.data_ptr<float>();
+    }
+    check(ulm_streamed_ce_bwd(&a, &o), "streamed cross-entropy backward");
+    return {want_h ? dh.to(hidden.scalar_type()) : Tensor(), want_w && !added ? dw.to(weight.scalar_type()) : Tensor()};
+  }
+};
+
+Tensor streamed_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t ignore_index, at::ScalarType cd,
+                              const OptTensor& denom_dev, double denom, int64_t piece_bytes) {
+  TORCH_CHECK_VALUE(hidden.is_cuda() && weight.device() == hidden.device() && hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1) &&
+                    hidden.is_floating_point() && weight.is_floating_point(), "streamed_cross_entropy takes hidden [rows, d] and weight [V, d] on one CUDA device");
+  TORCH_CHECK_VALUE(is_16bit(cd), "streamed_cross_entropy computes in fp16 or bf16");
+  TORCH_CHECK_VALUE(hidden.size(1) > 0 && hidden.size(1) % 8 == 0 && weight.size(0) > 0 && weight.size(0) <= INT32_MAX,
+                    "streamed_cross_entropy needs a width that is a positive multiple of 8 and at least one vocabulary column");
+  TORCH_CHECK_VALUE(target.scalar_type() == at::kLong && target.device() == hidden.device() && target.dim() == 1 && target.size(0) == hidden.size(0) && target.is_contiguous(),
+                    "streamed_cross_entropy takes one int64 target per row, on the device of hidden");
+  Tensor loss, lse, inv, wc, hc;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(hidden.device());
+    wc = rows_on(cast_cached(weight, cd), 16);
+    hc = rows_on(hidden.to(cd), 16);
+    const int64_t rows = hc.size(0);
+    lse = empty_cuda({rows}, at::kFloat, hc);
+    const Tensor rows_loss = empty_cuda({rows}, at::kFloat, hc);
+    ulm_streamed_ce_args a = streamed_args(hc, wc, target, lse, ignore_index);
+    const Tensor scratch = empty_cuda({ulm_streamed_ce_scratch(rows, a.V, a.d)}, at::kFloat, hc);
+    a.loss = rows_loss.data_ptr<float>(); a.scratch = scratch.data_ptr<float>();
+    check(ulm_streamed_ce_fwd(&a), "streamed cross-entropy forward");
+    loss = empty_cuda({}, at::kFloat, hc);                  // sum of the row losses / denominator
+    inv = empty_cuda({}, at::kFloat, hc);                   // 1 / denominator
+    Tensor dd;
+    if (denom_dev) dd = denom_dev->to(hidden.device(), at::kFloat);
+    check(ulm_loss_mean(rows_loss.data_ptr<float>(), target.data_ptr<int64_t>(), rows, ignore_index, dd.defined() ? dd.data_ptr<float>() : nullptr,
+                        (float)denom, loss.data_ptr<float>(), inv.data_ptr<float>(), stream_of(hc)), "loss mean");
+  }
+  if (!no_graph(hidden, weight)) {
+    auto node = make_node<StreamedCeBwd>(hidden, weight);
+    node->ignore_index = ignore_index; node->piece_bytes = piece_bytes;
+    node->keep(hidden); node->keep(weight); node->keep(target); node->keep(lse); node->keep(inv); node->keep(wc); node->keep(hc);
+    torch::autograd::set_history(loss, node);
+  }
+  return loss;
+}
+
+// ---------------------------------------------------------------------------
 // bindings
 // ---------------------------------------------------------------------------
 template <typename T> bool has_tangent(const T&) { return false; }
@@ -1332,4 +1421,5 @@ PYBIND11_MODULE(_ulm_torch, m) {
   m.def("grad_clip", &grad_clip, no_gil());
   m.def("check_target", &check_target);
   def_op(m, "kept_cross_entropy", &::kept_cross_entropy);
+  def_op(m, "streamed_cross_entropy", &::streamed_cross_entropy);
 }

@@ -294,6 +294,25 @@ class _ChunkedCE(torch.autograd.Function):
         return dh, (None if dw is None else dw.to(weight.dtype)), None, None, None, None, None
 
 
+def _loss_dtype(hidden):
+    """The 16-bit type the loss computes in where none is given."""
+    return torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled() else (hidden.dtype if hidden.dtype in _16BIT else torch.bfloat16)
+
+
+def _divided(loss_over, denominator, hidden):
+    """``loss_over(device scalar or None, host number)`` for any denominator: none, a number, a tensor of any shape."""
+    dev = denominator.detach() if torch.is_tensor(denominator) else None
+    host, shaped = 0.0, dev is not None and dev.dim() > 0
+    if dev is None and denominator is not None:
+        host = float(denominator)
+        if not host > 0.0:                                # the kernel counts then; a division by this number was asked for
+            dev = torch.full((), host, dtype=torch.float32, device=hidden.device)
+    elif shaped:                                          # one sum, divided as the tensor's shape says
+        dev, host = None, 1.0
+    loss = loss_over(dev, host)
+    return loss / denominator.detach().to(device=hidden.device, dtype=torch.float32) if shaped else loss
+
+
 def chunked_cross_entropy(hidden, weight, target, ignore_index=0, chunk_rows=2048,
                           compute_dtype=None, denominator=None):
     """hidden [rows, d], weight [V, d] (the tied lm head), target int64 [rows]
@@ -307,24 +326,39 @@ def chunked_cross_entropy(hidden, weight, target, ignore_index=0, chunk_rows=204
                for dW (no recomputation);
       chunked  one tile of rows at a time with recomputation (`_ChunkedCE`; buffers beyond KEEP_LOGITS_BYTES)."""
     if compute_dtype is None:
-        compute_dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled() else (
-            hidden.dtype if hidden.dtype in (torch.float16, torch.bfloat16) else torch.bfloat16)
+        compute_dtype = _loss_dtype(hidden)
     if hidden.shape[0] == 0:
         return torch.zeros((), device=hidden.device, requires_grad=True)
     target = target.contiguous()
     if hidden.shape[0] * weight.shape[0] * 2 <= KEEP_LOGITS_BYTES:
-        dev = denominator.detach() if torch.is_tensor(denominator) else None
-        host, shaped = 0.0, dev is not None and dev.dim() > 0
-        if dev is None and denominator is not None:
-            host = float(denominator)
-            if not host > 0.0:                            # the kernel counts then; a division by this number was asked for
-                dev = torch.full((), host, dtype=torch.float32, device=hidden.device)
-        elif shaped:                                      # one sum, divided as the tensor's shape says
-            dev, host = None, 1.0
-        loss = N.ext().kept_cross_entropy(hidden, weight, target, int(ignore_index), compute_dtype, dev, host, FUSED_LM_HEAD)
-        return loss / denominator.detach().to(device=hidden.device, dtype=torch.float32) if shaped else loss
+        return _divided(lambda dev, host: N.ext().kept_cross_entropy(hidden, weight, target, int(ignore_index), compute_dtype, dev, host, FUSED_LM_HEAD),
+                        denominator, hidden)
     N.ext().check_target(hidden, target)
     return _ChunkedCE.apply(hidden, weight, target, int(ignore_index), int(chunk_rows), compute_dtype, denominator)
+
+
+# Largest workspace the backward of `streamed_cross_entropy` takes for one piece of the vocabulary: 16 bits per row and column.
+# At 32768 rows this is 8192 columns, four pieces of a vocabulary of 32000.
+PIECE_BYTES = 512 << 20
+
+
+def streamed_cross_entropy(hidden, weight, target, ignore_index=0, compute_dtype=None, denominator=None):
+    """`chunked_cross_entropy` without logits: hidden [rows, d], weight [V, d], target int64 [rows] -> the mean cross-entropy over the
+    targets that are not ``ignore_index`` (or the sum over ``denominator``), for any number of rows and vocabulary columns and a
+    width that is a multiple of 8.  The forward keeps one fp32 log-sum-exp per row; the backward forms the logits again, one piece
+    of the vocabulary at a time, in a workspace of at most about PIECE_BYTES, whatever the vocabulary.  The logits are never
+    rounded to 16 bits, so the loss is the fp32 loss of the 16-bit operands.  Gradients: in the operands' types; an fp32 weight's is
+    the fp32 sum, under `wgrad_in_place` added into its ``grad``.
+
+    Against the kept form: a quarter more arithmetic, none of its 2 rows V bytes between forward and backward, and the backward
+    may run more than once."""
+    if compute_dtype is None:
+        compute_dtype = _loss_dtype(hidden)
+    if hidden.shape[0] == 0:
+        return torch.zeros((), device=hidden.device, requires_grad=True)
+    target = target.contiguous()
+    return _divided(lambda dev, host: N.ext().streamed_cross_entropy(hidden, weight, target, int(ignore_index), compute_dtype, dev, host, int(PIECE_BYTES)),
+                    denominator, hidden)
 
 
 def token_targets(ids, labels, padded, ignore_index):
