@@ -13,17 +13,18 @@ constexpr int kLmGroupTiles = 25;                      // column tiles per work 
 // cost (pipeline fill, statistics) being worth about a quarter of a tile.  At 32768 x 32000 that is 5 (220 tile times,
 // 216 ideal; the fixed 25 of before took 225); with 2048 rows x 4096 columns, 1 instead of 16: 256 items on 148 SMs
 // where 16 SMs had one each.
-int lm_group_tiles(int64_t rows, int V) {
-  const int64_t n_rb = (rows + LM_BM - 1) / LM_BM, n_ct = (V + LM_BN - 1) / LM_BN;
+inline int lm_group_tiles(int64_t n_rb, int64_t n_ct, int workers) {
   int best = 1;
   int64_t best_cost = INT64_MAX;
   for (int want = 1; want <= kLmGroupTiles; ++want) {
     const int64_t groups = (n_ct + want - 1) / want, tiles = (n_ct + groups - 1) / groups;
-    const int64_t cost = ((n_rb * groups + kNumSMs - 1) / kNumSMs) * (4 * tiles + 1);
+    const int64_t cost = ((n_rb * groups + workers - 1) / workers) * (4 * tiles + 1);
     if (cost < best_cost) { best_cost = cost; best = (int)tiles; }
   }
   return best;
 }
+
+inline int lm_group_tiles(int64_t rows, int V) { return lm_group_tiles((rows + LM_BM - 1) / LM_BM, ((int64_t)V + LM_BN - 1) / LM_BN, kNumSMs); }
 
 struct LmItems {
   int n_rb, n_ct, n_groups, group_tiles;

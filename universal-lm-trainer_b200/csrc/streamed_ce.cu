@@ -14,10 +14,10 @@
 // products behind it.  fp16 would lose probabilities below 2^-24, so its G is held times 2^14 (|G| <= 1) and the factor taken
 // back in the fp32 epilogue.  z is not rounded to 16 bits.
 //
-// All four products run through one main loop: persistent CTAs of 320 threads, one per SM (warps 0-7 epilogue, warp 8 one-lane
-// TMA producer, warp 9 one-lane tcgen05.mma issuer), output tiles of 128 x 256, M128 x N256 x K16 instructions, four
-// stages of 128x64 + 256x64 operands in 128-byte-swizzled shared memory, two accumulators of 256 TMEM columns so that a
-// tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
+// All four products run through one main loop: persistent pairs of CTAs of 320 threads, one CTA per SM (warps 0-7 epilogue, warp
+// 8 one-lane TMA producer, warp 9 of the pair's first CTA one-lane tcgen05.mma issuer), output tiles of 256 x 256, M256 x
+// N256 x K16 instructions over both CTAs, six stages of 128x64 + 128x64 operands a CTA in 128-byte-swizzled shared memory, two
+// accumulators of 256 TMEM columns so that a tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
 // contiguous, so dH reads W, and dW reads both G and H, as MN-major operands: rows of 64-element atoms, no transposed copies.
 // Waits are bounded (status bit and clean exit on expiry), like the attention kernels'.
 #include "lmhead_tiles.cuh"
@@ -32,17 +32,20 @@ using namespace tc;
 
 enum Mode { kStats, kGrad, kRowGrad, kColGrad };         // statistics; G; dH = G W; dW = G^T H
 
-constexpr int kStages = 4;
+constexpr int kPairM = 2 * LM_BM;                         // rows of a pair's output tile
+constexpr int kPairs = kNumSMs / 2;
+constexpr int kStages = 6;
+constexpr int kBRows = LM_BN / 2;                        // columns of B that each CTA of a pair holds
 constexpr uint32_t kATile = LM_BM * LM_BK * 2;           // 16 KB
-constexpr uint32_t kBTile = LM_BN * LM_BK * 2;           // 32 KB
-constexpr uint32_t kStage = kATile + kBTile;
+constexpr uint32_t kBTile = kBRows * LM_BK * 2;          // 16 KB
+constexpr uint32_t kStage = kATile + kBTile;             // of one CTA
 constexpr uint32_t kAtom = 64 * 64 * 2;                  // one MN-major box: 64 (MN) x 64 (K)
 constexpr uint32_t kStaging = 128 * 64 * 2;              // one 128-row x 64-column block of G
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int64_t kSlot = (int64_t)LM_BM * LM_BN;        // floats of one partial tile
+constexpr int64_t kSlot = (int64_t)kPairM * LM_BN;       // floats of one partial tile
 
 template <typename T> struct Fmt { static constexpr int idesc = 0, g_shift = 14; };
 template <> struct Fmt<__nv_bfloat16> { static constexpr int idesc = 1, g_shift = 0; };
@@ -159,7 +162,7 @@ __device__ __forceinline__ void put_row(const Out& o, float factor, int64_t row,
 }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
                    const __grid_constant__ Params p) {
   constexpr bool kAmn = MODE == kColGrad, kBmn = MODE == kRowGrad || MODE == kColGrad;
@@ -172,17 +175,22 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int items = n_items<MODE>(p.w);
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
+  // full and acc_free are awaited in the CTA of rank 0, which issues the products: its full counts the bytes of both CTAs,
+  // its acc_free an arrival of every epilogue warp of both
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&ctl->acc_full[b], 1); mbar_init(&ctl->acc_free[b], kEpiWarps * 32); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&ctl->acc_full[b], 1); mbar_init(&ctl->acc_free[b], 2 * kEpiWarps); }
     ctl->abort = 0;
     ctl->fail_bits = 0;
     fence_mbar_init();
   }
-  if (warp == kEpiWarps + 1) { tmem_alloc(&ctl->tmem_base, 512); tmem_relinquish(); }
+  if (warp == kEpiWarps + 1) { tmem_alloc_pair(&ctl->tmem_base, 512); tmem_relinquish_pair(); }
   fence_before_sync();
   __syncthreads();
+  cluster_sync();                                        // the other CTA's barriers are set up before anything signals them
   fence_after_sync();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);   // warp-uniform
 
@@ -192,10 +200,10 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB);
       uint32_t it = 0;                                   // k-blocks issued so far, over all tiles
       bool ok = true;
-      for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+      for (int q = pair; ok && q < items; q += pairs) {
         const Item im = item_of<MODE>(p.w, q);
         for (int t = 0; ok && t < im.count; ++t) {
-          const int m0 = im.mt * LM_BM, n0 = (im.nt + t) * LM_BN;
+          const int m0 = im.mt * kPairM + (int)rank * LM_BM, n0 = (im.nt + t) * LM_BN + (int)rank * kBRows;
           for (int kb = im.kb0; kb < im.kb1; ++kb, ++it) {
             const uint32_t s = it % kStages;
             if (it >= (uint32_t)kStages && !mbar_wait(&ctl->empty[s], ((it / kStages) - 1) & 1, abort_flag)) {
@@ -206,44 +214,44 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             uint8_t* a = stages + (size_t)s * kStage;
             uint8_t* b = a + kATile;
             const int k0 = kb * LM_BK;
-            mbar_expect_tx(&ctl->full[s], kStage);
+            if (rank == 0) mbar_expect_tx(&ctl->full[s], 2 * kStage);
+            const uint32_t full = peer_smem(&ctl->full[s], 0);
             if constexpr (kAmn) {
 #pragma unroll
-              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d(a + i * kAtom, &tmA, &ctl->full[s], m0 + 64 * i, k0, 0, 0);
+              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, &tmA, full, m0 + 64 * i, k0, 0, 0);
             } else {
-              tma_load_4d(a, &tmA, &ctl->full[s], k0, m0, 0, 0);
+              tma_load_4d_pair(a, &tmA, full, k0, m0, 0, 0);
             }
             // W's rows are vocabulary columns, counted from the piece's first
             if constexpr (kBmn) {
 #pragma unroll
-              for (int i = 0; i < LM_BN / 64; ++i) tma_load_4d(b + i * kAtom, &tmB, &ctl->full[s], n0 + 64 * i, MODE == kRowGrad ? p.v0 + k0 : k0, 0, 0);
+              for (int i = 0; i < kBRows / 64; ++i) tma_load_4d_pair(b + i * kAtom, &tmB, full, n0 + 64 * i, MODE == kRowGrad ? p.v0 + k0 : k0, 0, 0);
             } else {
-              tma_load_4d(b, &tmB, &ctl->full[s], k0, p.v0 + n0, 0, 0);
+              tma_load_4d_pair(b, &tmB, full, k0, p.v0 + n0, 0, 0);
             }
           }
         }
       }
-      if (*abort_flag) {   // let our own copies land before the CTA's shared memory goes away
-        for (uint32_t u = it > (uint32_t)kStages ? it - kStages : 0; u < it; ++u) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try(&ctl->full[u % kStages], (u / kStages) & 1))
-            if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-        }
+      // Given up: our copies land before the pair's shared memory goes away.  Their barrier is rank 0's and may lack the other
+      // CTA's half, so it is time that is waited for: a thousand times what a load takes.
+      if (*abort_flag) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000ull) {}
       }
     }
   } else if (warp == kEpiWarps + 1) {
-    // ---------------- MMA issuer ----------------
-    if (elect_one()) {
-      constexpr uint32_t idesc = make_idesc(Fmt<T>::idesc, LM_BM, LM_BN, kBmn, kAmn);
+    // ---------------- MMA issuer: rank 0 for both ----------------
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = make_idesc(Fmt<T>::idesc, kPairM, LM_BN, kBmn, kAmn);
       constexpr uint64_t kStepA = kAmn ? 2048 >> 4 : 32 >> 4, kStepB = kBmn ? 2048 >> 4 : 32 >> 4;      // 16 elements of the inner dimension on
       uint32_t it = 0, tt = 0;                           // k-blocks / tiles so far
       bool ok = true;
-      for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+      for (int q = pair; ok && q < items; q += pairs) {
         const Item im = item_of<MODE>(p.w, q);
         for (int t = 0; ok && t < im.count; ++t, ++tt) {
           const uint32_t b = tt & 1;
           // the accumulator still holds tile tt-2 until the epilogue warps have read it
-          if (tt >= 2 && !mbar_wait(&ctl->acc_free[b], ((tt >> 1) - 1) & 1, abort_flag)) { atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_SOFTMAX); ok = false; break; }
+          if (tt >= 2 && !mbar_wait<true>(&ctl->acc_free[b], ((tt >> 1) - 1) & 1, abort_flag)) { atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_SOFTMAX); ok = false; break; }
           fence_after_sync();
           for (int kb = im.kb0; kb < im.kb1; ++kb, ++it) {
             const uint32_t s = it % kStages;
@@ -254,10 +262,10 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint64_t db = kBmn ? make_sdesc_sw128_mn(sa + kATile, kAtom) : make_sdesc_sw128(sa + kATile);
 #pragma unroll
             for (int kk = 0; kk < LM_BK / 16; ++kk)
-              mma_ss(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
-            mma_commit(&ctl->empty[s]);                  // the stage is free once these MMAs have read it
+              mma_ss_pair(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
+            mma_commit_pair(&ctl->empty[s]);             // the stage is free in both CTAs once these MMAs have read it
           }
-          if (ok) mma_commit(&ctl->acc_full[b]);
+          if (ok) mma_commit_pair(&ctl->acc_full[b]);
         }
       }
     }
@@ -272,9 +280,9 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = *p.out.factor_dev * p.out.factor;
     uint32_t tt = 0;
     bool ok = true;
-    for (int q = blockIdx.x; ok && q < items; q += gridDim.x) {
+    for (int q = pair; ok && q < items; q += pairs) {
       const Item im = item_of<MODE>(p.w, q);
-      const int64_t grow = (int64_t)im.mt * LM_BM + r;
+      const int64_t grow = (int64_t)im.mt * kPairM + rank * LM_BM + r;
       [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
       [[maybe_unused]] float shift = 0.f;                // G: 2^(z log2e + shift)
       [[maybe_unused]] int tgt = -1;
@@ -297,7 +305,8 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           tmem_wait_ld();
           if (pass == 1) {                               // everything of this tile is in registers: hand the accumulator back
             fence_before_sync();
-            mbar_arrive(&ctl->acc_free[b]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_peer(peer_smem(&ctl->acc_free[b], 0));
           }
           if constexpr (MODE == kStats) {
             const int col0 = col_tile + c_blk;
@@ -368,12 +377,12 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             fence_proxy_async_smem();
             if (half_sync_any(half, *abort_flag != 0)) { ok = false; break; }
             if (tg == 0 && col_tile + c_blk < p.g_cols) {
-              tma_store_4d(&tmG, my_staging, col_tile + c_blk, im.mt * LM_BM, 0, 0);
+              tma_store_4d(&tmG, my_staging, col_tile + c_blk, im.mt * kPairM + (int)rank * LM_BM, 0, 0);
               bulk_commit();
             }
           } else {
             if (im.slot >= 0) {
-              float4* s = reinterpret_cast<float4*>(p.out.slots + im.slot * kSlot + r * LM_BN + c_blk);
+              float4* s = reinterpret_cast<float4*>(p.out.slots + im.slot * kSlot + ((int)rank * LM_BM + r) * LM_BN + c_blk);
 #pragma unroll
               for (int c = 0; c < 64; c += 4)
                 s[c >> 2] = make_float4(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1]), __uint_as_float(acc[c + 2]), __uint_as_float(acc[c + 3]));
@@ -397,7 +406,8 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
   fence_before_sync();
   __syncthreads();
-  if (warp == kEpiWarps + 1) tmem_dealloc(tmem_base, 512);
+  cluster_sync();                                        // neither CTA leaves while the other's products or arrivals may reach it
+  if (warp == kEpiWarps + 1) tmem_dealloc_pair(tmem_base, 512);
   if (threadIdx.x == 0 && ctl->fail_bits && p.status) atomicOr(p.status, ctl->fail_bits);
 }
 
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(256)
 streamed_ce_join_kernel(const Work w, const Out o) {
   const int j = blockIdx.x, t = w.whole + j, mt = t / w.n_nt, nt = t - mt * w.n_nt;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 8;
-  const int64_t row = (int64_t)mt * LM_BM + r;
+  const int64_t row = (int64_t)mt * kPairM + r;
   const int col = nt * LM_BN + c;
   if (row >= o.rows || col >= o.cols) return;
   const float* s = o.slots + (int64_t)j * w.split * kSlot + r * LM_BN + c;
@@ -465,16 +475,16 @@ streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restr
 // through memory) being worth about 12 of them; stretches of at least 4 k-blocks.
 Work product_work(int64_t m, int64_t n, int64_t k) {
   Work w{};
-  w.n_mt = (int)((m + LM_BM - 1) / LM_BM);
+  w.n_mt = (int)((m + kPairM - 1) / kPairM);
   w.n_nt = (int)((n + LM_BN - 1) / LM_BN);
   w.n_kb = (int)((k + LM_BK - 1) / LM_BK);
   const int64_t tiles = (int64_t)w.n_mt * w.n_nt;
-  w.whole = (int)(tiles / kNumSMs * kNumSMs);
+  w.whole = (int)(tiles / kPairs * kPairs);
   w.rest = (int)(tiles - w.whole);
   w.split = 1;
   int64_t best = INT64_MAX;
   for (int s = 1; s <= 64 && w.rest && (s == 1 || w.n_kb / s >= 4); ++s) {
-    const int64_t rounds = ((int64_t)w.rest * s + kNumSMs - 1) / kNumSMs, cost = rounds * ((w.n_kb + s - 1) / s + 12) + (s > 1 ? 12 : 0);
+    const int64_t rounds = ((int64_t)w.rest * s + kPairs - 1) / kPairs, cost = rounds * ((w.n_kb + s - 1) / s + 12) + (s > 1 ? 12 : 0);
     if (cost < best) { best = cost; w.split = s; }
   }
   return w;
@@ -486,11 +496,11 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, 
   static std::atomic<bool> attr_set[kMaxDevices];
   auto kern = streamed_ce_kernel<T, MODE>;
   if (int rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who)) return rc;
-  const int items = n_items<MODE>(p.w), grid = items < kNumSMs ? items : kNumSMs;
+  const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
   kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mg, p);
   if (int rc = check_launch(who)) return rc;
   if (MODE >= kRowGrad && p.w.split > 1) {
-    streamed_ce_join_kernel<T><<<dim3(p.w.rest, LM_BM / 8), 256, 0, st>>>(p.w, p.out);
+    streamed_ce_join_kernel<T><<<dim3(p.w.rest, kPairM / 8), 256, 0, st>>>(p.w, p.out);
     return check_launch(who);
   }
   return ULM_OK;
@@ -517,10 +527,10 @@ Params common_params(const ulm_streamed_ce_args* a) {
 
 Work stats_work(int64_t rows, int V, int d) {
   Work w{};
-  w.n_mt = (int)((rows + LM_BM - 1) / LM_BM);
+  w.n_mt = (int)((rows + kPairM - 1) / kPairM);
   w.n_nt = (V + LM_BN - 1) / LM_BN;
   w.n_kb = (d + LM_BK - 1) / LM_BK;
-  w.group = lm_group_tiles(rows, V);
+  w.group = lm_group_tiles(w.n_mt, w.n_nt, kPairs);
   return w;
 }
 
@@ -528,7 +538,7 @@ template <typename T>
 int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
   CUtensorMap mh, mw;
   if (int rc = encode_matrix_map(&mh, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who)) return rc;
-  if (int rc = encode_matrix_map(&mw, a->w, a->dtype, a->V, a->d, a->w_stride, LM_BN, who)) return rc;
+  if (int rc = encode_matrix_map(&mw, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who)) return rc;
   Params p = common_params(a);
   p.w = stats_work(a->rows, a->V, a->d);
   const int parts = 2 * ((p.w.n_nt + p.w.group - 1) / p.w.group);
@@ -548,7 +558,7 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
   int rc;
   if ((rc = encode_matrix_map(&h_rows, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who))) return rc;
   if ((rc = encode_matrix_map(&h_mn, a->h, a->dtype, a->rows, a->d, a->h_stride, 64, who))) return rc;
-  if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, LM_BN, who))) return rc;
+  if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who))) return rc;
   if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
   for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
     const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece, stride = g_stride(n);
