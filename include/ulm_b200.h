@@ -362,7 +362,7 @@ int ulm_lmhead_score(const ulm_lmhead_lse_args* a, uint8_t* hit, int32_t* part_i
  * and keeps softmax - onehot of one piece in 16 bits.  z = h w^T stays in fp32 throughout (it is not rounded to the 16-bit type).
  * fwd: lse[r] and loss[r] = lse[r] - z[r, target[r]] in fp32; loss 0 where target[r] is ignore_index or no column.
  *      scratch: ulm_streamed_ce_scratch(rows, V, d) floats.
- * bwd: with f = *factor_dev (d total / d row loss) and G = softmax - onehot, 0 on the rows above:
+ * bwd: with f = *factor_dev (times *factor2_dev; d total / d row loss) and G = softmax - onehot, 0 on the rows above:
  *      dh [rows, d] = f G w, dense, of the 16-bit type; dw [V, d] = f G^T h, 16-bit, or fp32 with dw_f32, or added to an fp32
  *      dw with dw_add; either may be NULL.  lse is the forward's.
  *      workspace: ulm_streamed_ce_workspace(rows, V, piece) 16-bit elements; slots: ulm_streamed_ce_slots(...) floats (may
@@ -380,7 +380,7 @@ typedef struct {
   void* stream;
 } ulm_streamed_ce_args;
 typedef struct {
-  const float* factor_dev;
+  const float* factor_dev; const float* factor2_dev;   /* the second may be NULL */
   void* dh; void* dw;
   int64_t dw_stride;
   int32_t dw_f32, dw_add;

@@ -75,4 +75,4 @@ def test_python_refusals(bad):
 
 def test_struct_sizes():
     assert C.sizeof(N.StreamedCeArgs) == 6 * 8 + 2 * 8 + 8 + 4 * 4 + 8 + 2 * 8
-    assert C.sizeof(N.StreamedCeGrads) == 3 * 8 + 8 + 2 * 4 + 3 * 8 + 8
+    assert C.sizeof(N.StreamedCeGrads) == 4 * 8 + 8 + 2 * 4 + 3 * 8 + 8

@@ -116,7 +116,7 @@ class StreamedCeArgs(C.Structure):
 
 
 class StreamedCeGrads(C.Structure):
-    _fields_ = [('factor_dev', vp), ('dh', vp), ('dw', vp), ('dw_stride', i64), ('dw_f32', i32), ('dw_add', i32),
+    _fields_ = [('factor_dev', vp), ('factor2_dev', vp), ('dh', vp), ('dw', vp), ('dw_stride', i64), ('dw_f32', i32), ('dw_add', i32),
                 ('workspace', vp), ('slots', vp), ('dh_sum', vp), ('piece', i64)]
 
 

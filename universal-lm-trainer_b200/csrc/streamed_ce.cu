@@ -40,7 +40,7 @@ constexpr uint32_t kATile = LM_BM * LM_BK * 2;           // 16 KB
 constexpr uint32_t kBTile = kBRows * LM_BK * 2;          // 16 KB
 constexpr uint32_t kStage = kATile + kBTile;             // of one CTA
 constexpr uint32_t kAtom = 64 * 64 * 2;                  // one MN-major box: 64 (MN) x 64 (K)
-constexpr uint32_t kStaging = 128 * 64 * 2;              // one 128-row x 64-column block of G
+constexpr uint32_t kStaging = 32 * 128;                  // a warp's 32 rows x 128 bytes of output
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -58,7 +58,7 @@ struct Ctl {
 };
 constexpr size_t kCtlBytes = 1024;
 static_assert(sizeof(Ctl) <= kCtlBytes, "control block");
-constexpr size_t smem_bytes(int mode) { return 1024 + (size_t)kStages * kStage + (mode == kGrad ? 2 * (size_t)kStaging : 0) + kCtlBytes; }
+constexpr size_t smem_bytes(int mode) { return 1024 + (size_t)kStages * kStage + (mode == kStats ? 0 : kEpiWarps * (size_t)kStaging) + kCtlBytes; }
 static_assert(smem_bytes(kGrad) <= 227 * 1024, "shared memory");
 
 // One launch's work.  Items are numbered and dealt round the CTAs.
@@ -104,9 +104,11 @@ __device__ __forceinline__ Item item_of(const Work& w, int q) {
   return it;
 }
 
-// How the accumulators leave: out = factor * acc (+ prev)
+// How the accumulators leave: out = factor * acc (+ prev).  A whole tile goes through shared memory and a TMA store, or where an
+// fp32 out is its own prev a TMA addition (one to each element: no order to depend on); where a 16-bit out adds an fp32 prev,
+// straight from the registers.  A cut tile's parts go to their slots, fp32 and without factor, and out by the join kernel.
 struct Out {
-  const float* factor_dev;
+  const float *factor_dev, *factor2_dev;
   float factor;
   const float* prev;
   void* out;
@@ -133,44 +135,66 @@ __device__ __forceinline__ int target_column(const Params& p, int64_t row) {
   return t != p.ignore_index && t >= 0 && t < p.V ? (int)t : -1;
 }
 
-// 64 accumulator columns of one row: columns col .. col + 63 of the output (or of a slot)
+__device__ __forceinline__ float out_factor(const Out& o) { return *o.factor_dev * (o.factor2_dev ? *o.factor2_dev : 1.f) * o.factor; }
+
+// 128 bytes of a row of a warp's block into shared memory, lane = row, as the 128-byte swizzle has them: 16-byte chunk c at chunk
+// position c ^ (lane & 7); then one TMA store or addition of the block to (col, row) of `map`.  Whole warp.
+template <bool ADD>
+__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* block, int lane, const uint32_t (&u)[32], int col, int row) {
+  if (lane == 0) bulk_wait_read0();                      // the warp's previous store must have read the block
+  __syncwarp();
+  uint8_t* line = block + lane * 128;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = make_uint4(u[4 * c], u[4 * c + 1], u[4 * c + 2], u[4 * c + 3]);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (ADD) tma_add_4d(map, block, col, row, 0, 0); else tma_store_4d(map, block, col, row, 0, 0);
+    bulk_commit();
+  }
+}
+// 64 fp32 columns as two blocks
+template <bool ADD>
+__device__ __forceinline__ void store_f32(const CUtensorMap* map, uint8_t* block, int lane, const uint32_t (&acc)[64], float factor, int col, int cols, int row) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (col + 32 * h >= cols) break;
+    uint32_t u[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) u[c] = __float_as_uint(factor * __uint_as_float(acc[32 * h + c]));
+    store_block<ADD>(map, block, lane, u, col + 32 * h, row);
+  }
+}
+
+// 64 accumulator columns of one row plus fp32 values, rounded to 16 bits
 template <typename T>
-__device__ __forceinline__ void put_row(const Out& o, float factor, int64_t row, int col, const uint32_t (&acc)[64]) {
+__device__ __forceinline__ void add_and_round(const Out& o, float factor, int64_t row, int col, const uint32_t (&acc)[64]) {
   if (row >= o.rows) return;
 #pragma unroll
   for (int c = 0; c < 64; c += 8) {
     if (col + c < o.cols) {                              // the width is whole vectors of 8
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = factor * __uint_as_float(acc[c + j]);
       const int64_t at = row * o.ld + col + c;
-      if (o.prev) {
-        const float4 a = *reinterpret_cast<const float4*>(o.prev + at), b = *reinterpret_cast<const float4*>(o.prev + at + 4);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-      }
-      if (o.is_f32) {
-        float4* q = reinterpret_cast<float4*>(static_cast<float*>(o.out) + at);
-        q[0] = make_float4(v[0], v[1], v[2], v[3]);
-        q[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<T*>(o.out) + at) =
-            make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]), Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7]));
-      }
+      const float4 a = *reinterpret_cast<const float4*>(o.prev + at), b = *reinterpret_cast<const float4*>(o.prev + at + 4);
+      float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += factor * __uint_as_float(acc[c + j]);
+      *reinterpret_cast<uint4*>(static_cast<T*>(o.out) + at) =
+          make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]), Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7]));
     }
   }
 }
 
 template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmG,
-                   const __grid_constant__ Params p) {
+streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut,
+                   const __grid_constant__ CUtensorMap tmSlots, const __grid_constant__ Params p) {
   constexpr bool kAmn = MODE == kColGrad, kBmn = MODE == kRowGrad || MODE == kColGrad;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stages = base;                                             // [stage][A tile | B tile]
-  uint8_t* staging = base + (size_t)kStages * kStage;                 // G: [column half] one 128x64 block each
-  Ctl* ctl = reinterpret_cast<Ctl*>(staging + (MODE == kGrad ? 2 * (size_t)kStaging : 0));
+  uint8_t* staging = base + (size_t)kStages * kStage;                 // [epilogue warp] one block each
+  Ctl* ctl = reinterpret_cast<Ctl*>(staging + (MODE == kStats ? 0 : kEpiWarps * (size_t)kStaging));
   volatile int* abort_flag = &ctl->abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -273,16 +297,16 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     // ---------------- epilogue ----------------
     const int half = warp >> 2;                          // columns [128 half, 128 half + 128) of the tile
     const int r = ((warp & 3) << 5) | lane;              // row within the tile == TMEM lane
-    const int tg = (int)threadIdx.x - half * 128;        // thread within its half (0..127)
     const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-    [[maybe_unused]] uint8_t* my_staging = staging + (size_t)half * kStaging;
+    [[maybe_unused]] uint8_t* my_staging = staging + (size_t)warp * kStaging;
     [[maybe_unused]] float factor = 0.f;
-    if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = *p.out.factor_dev * p.out.factor;
+    if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = out_factor(p.out);
     uint32_t tt = 0;
     bool ok = true;
     for (int q = pair; ok && q < items; q += pairs) {
       const Item im = item_of<MODE>(p.w, q);
       const int64_t grow = (int64_t)im.mt * kPairM + rank * LM_BM + r;
+      [[maybe_unused]] const int row0 = (int)grow - lane;                        // the warp's first row
       [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
       [[maybe_unused]] float shift = 0.f;                // G: 2^(z log2e + shift)
       [[maybe_unused]] int tgt = -1;
@@ -292,8 +316,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const uint32_t b = tt & 1;
         const bool waited = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[b], (tt >> 1) & 1, abort_flag));
         if (!waited && lane == 0) atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_MMA);
-        // every thread of the half learns the same verdict (a barrier follows inside the passes)
-        if (half_sync_any(half, !waited || *abort_flag != 0)) { ok = false; break; }
+        if (!waited) { ok = false; break; }              // the whole warp; nothing below waits for another one
         fence_after_sync();
         const int col_tile = (im.nt + t) * LM_BN;
 #pragma unroll 1
@@ -366,28 +389,24 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 else if (col0 + c + 1 >= p.V) pk[c >> 1] &= 0xffffu;
               }
             }
-            // the previous store out of this staging block must have read it
-            if (tg == 0) bulk_wait_read0();
-            if (half_sync_any(half, *abort_flag != 0)) { ok = false; break; }
-            // row r of a 128-byte-swizzled block: 16-byte chunk c sits at chunk position c ^ (r & 7)
-            uint8_t* row = my_staging + (size_t)r * 128;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-            fence_proxy_async_smem();
-            if (half_sync_any(half, *abort_flag != 0)) { ok = false; break; }
-            if (tg == 0 && col_tile + c_blk < p.g_cols) {
-              tma_store_4d(&tmG, my_staging, col_tile + c_blk, im.mt * kPairM + (int)rank * LM_BM, 0, 0);
-              bulk_commit();
-            }
+            if (col_tile + c_blk < p.g_cols && row0 < p.rows) store_block<false>(&tmOut, my_staging, lane, pk, col_tile + c_blk, row0);
           } else {
+            const int col = col_tile + c_blk;
             if (im.slot >= 0) {
-              float4* s = reinterpret_cast<float4*>(p.out.slots + im.slot * kSlot + ((int)rank * LM_BM + r) * LM_BN + c_blk);
+              store_f32<false>(&tmSlots, my_staging, lane, acc, 1.f, c_blk, LM_BN, im.slot * kPairM + (int)rank * LM_BM + (warp & 3) * 32);
+            } else if (col < p.out.cols && row0 < p.out.rows) {
+              if (p.out.is_f32 && p.out.prev) {
+                store_f32<true>(&tmOut, my_staging, lane, acc, factor, col, p.out.cols, row0);
+              } else if (p.out.is_f32) {
+                store_f32<false>(&tmOut, my_staging, lane, acc, factor, col, p.out.cols, row0);
+              } else if (p.out.prev) {
+                add_and_round<T>(p.out, factor, grow, col, acc);
+              } else {
+                uint32_t pk[32];
 #pragma unroll
-              for (int c = 0; c < 64; c += 4)
-                s[c >> 2] = make_float4(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1]), __uint_as_float(acc[c + 2]), __uint_as_float(acc[c + 3]));
-            } else {
-              put_row<T>(p.out, factor, grow, col_tile + c_blk, acc);
+                for (int c = 0; c < 64; c += 2) pk[c >> 1] = Cvt<T>::pack2(factor * __uint_as_float(acc[c]), factor * __uint_as_float(acc[c + 1]));
+                store_block<false>(&tmOut, my_staging, lane, pk, col, row0);
+              }
             }
           }
         }
@@ -401,7 +420,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
       }
     }
-    if (MODE == kGrad && tg == 0) bulk_wait0();          // our stores must be complete before the CTA ends
+    if (MODE != kStats && lane == 0) bulk_wait0();       // our stores must be complete before the CTA ends
   }
 
   fence_before_sync();
@@ -430,7 +449,7 @@ streamed_ce_join_kernel(const Work w, const Out o) {
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
     v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
   }
-  const float factor = *o.factor_dev * o.factor;
+  const float factor = out_factor(o);
   const int64_t at = row * o.ld + col;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = factor * v[i] + (o.prev ? o.prev[at + i] : 0.f);
@@ -492,18 +511,30 @@ Work product_work(int64_t m, int64_t n, int64_t k) {
 int64_t slot_floats(const Work& w) { return w.split > 1 ? (int64_t)w.rest * w.split * kSlot : 0; }
 
 template <typename T, int MODE>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, const Params& p, int device, cudaStream_t st, const char* who) {
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Params& p, int device, cudaStream_t st, const char* who) {
   static std::atomic<bool> attr_set[kMaxDevices];
   auto kern = streamed_ce_kernel<T, MODE>;
   if (int rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who)) return rc;
   const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
-  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mg, p);
-  if (int rc = check_launch(who)) return rc;
-  if (MODE >= kRowGrad && p.w.split > 1) {
-    streamed_ce_join_kernel<T><<<dim3(p.w.rest, kPairM / 8), 256, 0, st>>>(p.w, p.out);
-    return check_launch(who);
-  }
-  return ULM_OK;
+  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, mo, p);
+  return check_launch(who);
+}
+// A product and, where tiles were cut, their sum
+template <typename T, int MODE>
+int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int dtype, int device, cudaStream_t st, const char* who) {
+  static std::atomic<bool> attr_set[kMaxDevices];
+  auto kern = streamed_ce_kernel<T, MODE>;
+  CUtensorMap mo, ms;
+  int rc;
+  if ((rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who))) return rc;
+  if ((rc = encode_matrix_map(&mo, p.out.out, p.out.is_f32 ? (int)ULM_F32 : dtype, p.out.rows, p.out.cols, p.out.ld, 32, who))) return rc;
+  ms = mo;
+  if (p.w.split > 1 && (rc = encode_matrix_map(&ms, p.out.slots, ULM_F32, (int64_t)p.w.rest * p.w.split * kPairM, LM_BN, LM_BN, 32, who))) return rc;
+  const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
+  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, ms, p);
+  if ((rc = check_launch(who)) || p.w.split == 1) return rc;
+  streamed_ce_join_kernel<T><<<dim3(p.w.rest, kPairM / 8), 256, 0, st>>>(p.w, p.out);
+  return check_launch(who);
 }
 
 int check_args(const ulm_streamed_ce_args* a, const char* who) {
@@ -562,16 +593,18 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
   if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
   for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
     const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece, stride = g_stride(n);
-    CUtensorMap g_rows, g_mn;
+    CUtensorMap g_rows, g_mn, g_out;
     if ((rc = encode_matrix_map(&g_rows, g->workspace, a->dtype, a->rows, stride, stride, LM_BM, who))) return rc;
     if ((rc = encode_matrix_map(&g_mn, g->workspace, a->dtype, a->rows, stride, stride, 64, who))) return rc;
+    if ((rc = encode_matrix_map(&g_out, g->workspace, a->dtype, a->rows, stride, stride, 32, who))) return rc;
     Params p = common_params(a);
     p.v0 = (int)v0;
     p.lse = a->lse;
     p.g_cols = (int)stride;
     p.w = stats_work(a->rows, (int)n, a->d);
-    if ((rc = launch<T, kGrad>(h_rows, w_rows, g_rows, p, device, st, who))) return rc;
+    if ((rc = launch<T, kGrad>(h_rows, w_rows, g_out, p, device, st, who))) return rc;
     p.out.factor_dev = g->factor_dev;
+    p.out.factor2_dev = g->factor2_dev;
     p.out.factor = 1.f / (float)(1 << Fmt<T>::g_shift);
     p.out.slots = g->slots;
     p.out.cols = a->d;
@@ -580,7 +613,7 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
       p.out.ld = g->dw_stride; p.out.rows = n; p.out.is_f32 = g->dw_f32;
       p.out.out = g->dw_f32 ? (void*)((float*)g->dw + v0 * g->dw_stride) : (void*)((T*)g->dw + v0 * g->dw_stride);
       p.out.prev = g->dw_add ? (const float*)p.out.out : nullptr;
-      if ((rc = launch<T, kColGrad>(g_mn, h_mn, g_mn, p, device, st, who))) return rc;
+      if ((rc = launch_product<T, kColGrad>(g_mn, h_mn, p, a->dtype, device, st, who))) return rc;
     }
     if (g->dh) {
       const bool first = v0 == 0, last = v0 + n >= a->V;
@@ -590,7 +623,7 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
       p.out.out = last ? g->dh : (void*)g->dh_sum;
       p.out.prev = first ? nullptr : g->dh_sum;
       p.out.ld = a->d;                                   // dh and dh_sum are dense
-      if ((rc = launch<T, kRowGrad>(g_rows, w_mn, g_rows, p, device, st, who))) return rc;
+      if ((rc = launch_product<T, kRowGrad>(g_rows, w_mn, p, a->dtype, device, st, who))) return rc;
     }
   }
   return ULM_OK;

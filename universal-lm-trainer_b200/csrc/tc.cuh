@@ -117,6 +117,13 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
       ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+// The same, adding fp32 elements to what is there
+__device__ __forceinline__ void tma_add_4d(const CUtensorMap* map, const void* smem_src, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.4d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+      ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
@@ -380,9 +387,9 @@ struct ItemIter {
 int encode_bhsd_map(CUtensorMap* out, const void* base, int dtype, int B, int H, int S,
                     int64_t sb, int64_t sh, int64_t ss, int box_rows, const char* what);
 
-// Describes a row-major 16-bit matrix [rows, cols], rows `stride` elements apart (a multiple of 8), for boxes of box_rows
-// rows x 64 columns with the 128-byte swizzle: a 4-D tensor {cols, rows, 1, 1}, coordinates (column, row, 0, 0).  Loads read zeros
-// past either end, stores leave them out.  Same cache.
+// Describes a row-major matrix [rows, cols] of 16-bit or fp32 elements, rows `stride` elements apart (whole 16 bytes), for boxes of
+// box_rows rows x 128 bytes with the 128-byte swizzle: a 4-D tensor {cols, rows, 1, 1}, coordinates (column, row, 0, 0).  Loads
+// read zeros past either end, stores leave them out.  Same cache.
 int encode_matrix_map(CUtensorMap* out, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* what);
 
 void map_cache_stats(uint64_t* hits, uint64_t* misses);

@@ -60,9 +60,10 @@ int cached_map(CUtensorMap* out, const MapKey& key, const cuuint64_t (&dims)[4],
       return ULM_OK;
     }
   }
-  const cuuint32_t box[4] = {64, (cuuint32_t)key.box_rows, 1, 1};
+  const cuuint32_t box[4] = {key.dtype == ULM_F32 ? 32u : 64u, (cuuint32_t)key.box_rows, 1, 1};         // 128 bytes wide
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType dt = key.dtype == ULM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapDataType dt = key.dtype == ULM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : key.dtype == ULM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = g_encode(out, dt, 4, const_cast<void*>(key.base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -131,15 +132,16 @@ int encode_bhsd_map(CUtensorMap* out, const void* base, int dtype, int B, int H,
 int encode_matrix_map(CUtensorMap* out, const void* base, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows, const char* what) {
   if (reinterpret_cast<uintptr_t>(base) & 15) return fail(ULM_ERR_ARG, "%s: base pointer must be 16-byte aligned", what);
   if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || cols > 0x7fffffffLL) return fail(ULM_ERR_ARG, "%s: bad matrix size", what);
-  if (rows == 1) stride = (cols + 7) / 8 * 8;            // never applied
-  if (stride < cols || stride % 8 || stride >= (int64_t)1 << 39)
-    return fail(ULM_ERR_ARG, "%s: the row stride must be a multiple of 8 elements and at least the row", what);
+  const int size = dtype == ULM_F32 ? 4 : 2, vec = 16 / size;
+  if (rows == 1) stride = (cols + vec - 1) / vec * vec;  // never applied
+  if (stride < cols || stride % vec || stride * size >= (int64_t)1 << 40)
+    return fail(ULM_ERR_ARG, "%s: the row stride must be a multiple of %d elements and at least the row", what, vec);
   MapKey key;
   std::memset(&key, 0, sizeof(key));
   key.base = base; key.ss = stride; key.dtype = dtype; key.H = (int32_t)cols; key.S = (int32_t)rows; key.box_rows = box_rows;
   key.matrix = 1;
   const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, 1, 1};
-  const cuuint64_t strides[3] = {(cuuint64_t)stride * 2, (cuuint64_t)stride * 2, (cuuint64_t)stride * 2};   // the last two: of extent 1
+  const cuuint64_t bytes = (cuuint64_t)stride * size, strides[3] = {bytes, bytes, bytes};                   // the last two: of extent 1
   return cached_map(out, key, dims, strides, what);
 }
 

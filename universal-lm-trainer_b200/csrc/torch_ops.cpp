@@ -760,15 +760,15 @@ Tensor dropout(const Tensor& x, double p, int64_t seed) {
 
 struct DropNormBwd : OpNode {
   Drop drop;
-  std::vector<int64_t> shape;
   at::ScalarType wdtype, bdtype;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor w = kept[1], rstd = kept[2], x = kept[0].view({-1, kept[0].size(-1)});
-    const int64_t rows = x.size(0), d = x.size(1);
+    const Tensor x = kept[0], w = kept[1], rstd = kept[2];
+    const int64_t rows = rstd.size(0), d = w.size(0);
+    auto as = [](const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); };
     // a y that nobody used has the gradient zero
-    const Tensor dy = g[1].defined() ? rows_on(g[1].to(bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
-    const Tensor ga = g[0].defined() ? rows_on(g[0].to(at::kFloat), 16) : Tensor();
-    const Tensor dx = empty_cuda({rows, d}, at::kFloat, x), db = empty_cuda({rows, d}, bdtype, x), dw = empty_cuda({d}, at::kFloat, x);
+    const Tensor dy = g[1].defined() ? rows_on(as(g[1], bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
+    const Tensor ga = g[0].defined() ? rows_on(as(g[0], at::kFloat), 16) : Tensor();
+    const Tensor dx = empty_cuda(x.sizes(), at::kFloat, x), db = empty_cuda(x.sizes(), bdtype, x), dw = empty_cuda({d}, at::kFloat, x);
     const Tensor partial = empty_cuda({ulm_add_dropout_norm_partial_rows(rows), d}, at::kFloat, x);
     ulm_rmsnorm_bwd_args a{};
     a.x = x.data_ptr(); a.w = w.data_ptr(); a.dy = dy.data_ptr(); a.rstd = rstd.data_ptr<float>();
@@ -778,7 +778,7 @@ struct DropNormBwd : OpNode {
     if (ga.defined()) { a.g_add = ga.data_ptr(); a.gadd_stride = ga.stride(0); }
     a.d_branch = db.data_ptr(); a.dbranch_stride = d;
     check(ulm_add_dropout_norm_bwd(&a, drop.p, (uint64_t)drop.seed), "dropout_add_rms_norm backward");
-    return {dx.view(shape), db.view(shape), dw.to(wdtype)};
+    return {dx, db, as(dw, wdtype)};
   }
 };
 
@@ -809,7 +809,7 @@ std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& b
   }
   if (!no_graph(x, branch, weight)) {
     auto node = make_node<DropNormBwd>(x, branch, weight);
-    node->drop = drop; node->shape = x.sizes().vec(); node->wdtype = weight.scalar_type(); node->bdtype = branch.scalar_type();
+    node->drop = drop; node->wdtype = weight.scalar_type(); node->bdtype = branch.scalar_type();
     torch::autograd::set_history(x_new, node);
     torch::autograd::set_history(y, node);
     node->keep(x_new, true); node->keep(w); node->keep(rstd);
@@ -1267,9 +1267,9 @@ Tensor kept_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tens
 // lm head + cross-entropy, the form that never has the logits
 // ---------------------------------------------------------------------------
 // operands and stream of one launch; hc and wc have rows on 16-byte boundaries
-ulm_streamed_ce_args streamed_args(const Tensor& hc, const Tensor& wc, const Tensor& target, const Tensor& lse, int64_t ignore_index) {
+ulm_streamed_ce_args streamed_args(const Tensor& hc, const Tensor& wc, const Tensor& target, float* lse, int64_t ignore_index) {
   ulm_streamed_ce_args a{};
-  a.h = hc.data_ptr(); a.w = wc.data_ptr(); a.target = target.data_ptr<int64_t>(); a.lse = lse.data_ptr<float>();
+  a.h = hc.data_ptr(); a.w = wc.data_ptr(); a.target = target.data_ptr<int64_t>(); a.lse = lse;
   a.h_stride = hc.stride(0); a.w_stride = wc.stride(0);
   a.rows = hc.size(0); a.V = (int32_t)wc.size(0); a.d = (int32_t)hc.size(1); a.dtype = code_of(hc.scalar_type());
   a.ignore_index = ignore_index; a.status_dev = status_ptr(hc); a.stream = stream_of(hc);
@@ -1278,23 +1278,23 @@ ulm_streamed_ce_args streamed_args(const Tensor& hc, const Tensor& wc, const Ten
 
 struct StreamedCeBwd : OpNode {
   int64_t ignore_index = 0, piece_bytes = 0;
+  at::ScalarType hdtype;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor hidden = kept[0], weight = kept[1], target = kept[2], lse = kept[3], inv = kept[4], wc = kept[5], hc = kept[6];
+    const Tensor weight = kept[0], target = kept[1], stats = kept[2], wc = kept[3], hc = kept[4];
     const bool want_h = task_should_compute_output(0), want_w = task_should_compute_output(1);
     if (!want_h && !want_w) return {Tensor(), Tensor()};
     const at::ScalarType cd = hc.scalar_type();
     const int64_t rows = hc.size(0), d = hc.size(1), V = wc.size(0);
-    ulm_streamed_ce_args a = streamed_args(hc, wc, target, lse, ignore_index);
+    ulm_streamed_ce_args a = streamed_args(hc, wc, target, stats.data_ptr<float>(), ignore_index);
     ulm_streamed_ce_grads o{};
-    const Tensor factor = g[0].to(at::kFloat).mul(inv);                         // d loss / d row loss
-    o.factor_dev = factor.data_ptr<float>();
+    const Tensor up = g[0].scalar_type() == at::kFloat ? g[0] : g[0].to(at::kFloat);
+    o.factor_dev = up.data_ptr<float>(); o.factor2_dev = a.lse + rows;          // their product: d total / d row loss
     o.piece = std::max<int64_t>(256, piece_bytes / (2 * rows) / 256 * 256);
-    Tensor dh, dw, dh_sum, slots;
+    Tensor dh, dw;
     bool added = false;
     if (want_h) {
       dh = empty_cuda({rows, d}, cd, hc);
       o.dh = dh.data_ptr();
-      if (o.piece < V) { dh_sum = empty_cuda({rows, d}, at::kFloat, hc); o.dh_sum = dh_sum.data_ptr<float>(); }
     }
     if (want_w) {
       const Tensor into = weight.grad();
@@ -1303,14 +1303,19 @@ struct StreamedCeBwd : OpNode {
       dw = added ? into : empty_cuda({V, d}, weight.scalar_type() == at::kFloat ? at::kFloat : cd, hc);
       o.dw = dw.data_ptr(); o.dw_stride = d; o.dw_f32 = dw.scalar_type() == at::kFloat; o.dw_add = added;
     }
-    const Tensor workspace = empty_cuda({ulm_streamed_ce_workspace(rows, a.V, o.piece)}, cd, hc);
-    o.workspace = workspace.data_ptr();
-    if (const int64_t n = ulm_streamed_ce_slots(rows, a.V, a.d, o.piece, want_h, want_w)) {
-      slots = empty_cuda({n}, at::kFloat, hc);
-      o.slots = slots.data_ptr<float>();
-    }
+    // one buffer: the pieces' softmax, dh's sum over the pieces, the cut tiles' slots
+    auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    const int64_t n_g = whole(2 * ulm_streamed_ce_workspace(rows, a.V, o.piece)), n_sum = want_h && o.piece < V ? whole(4 * rows * d) : 0;
+    const Tensor buffer = empty_cuda({n_g + n_sum + 4 * ulm_streamed_ce_slots(rows, a.V, a.d, o.piece, want_h, want_w)}, at::kByte, hc);
+    char* at = static_cast<char*>(buffer.data_ptr());
+    o.workspace = at;
+    o.dh_sum = reinterpret_cast<float*>(at + n_g);
+    o.slots = reinterpret_cast<float*>(at + n_g + n_sum);
     check(ulm_streamed_ce_bwd(&a, &o), "streamed cross-entropy backward");
-    return {want_h ? dh.to(hidden.scalar_type()) : Tensor(), want_w && !added ? dw.to(weight.scalar_type()) : Tensor()};
+    if (want_h && dh.scalar_type() != hdtype) dh = dh.to(hdtype);
+    if (added) dw = Tensor();
+    else if (want_w && dw.scalar_type() != weight.scalar_type()) dw = dw.to(weight.scalar_type());
+    return {dh, dw};
   }
 };
 
@@ -1323,30 +1328,28 @@ Tensor streamed_cross_entropy(const Tensor& hidden, const Tensor& weight, const 
                     "streamed_cross_entropy needs a width that is a positive multiple of 8 and at least one vocabulary column");
   TORCH_CHECK_VALUE(target.scalar_type() == at::kLong && target.device() == hidden.device() && target.dim() == 1 && target.size(0) == hidden.size(0) && target.is_contiguous(),
                     "streamed_cross_entropy takes one int64 target per row, on the device of hidden");
-  Tensor loss, lse, inv, wc, hc;
+  Tensor loss, stats, wc, hc;                               // stats: the rows' log-sum-exp, then 1 / denominator
   {
     OpScope scope;
     c10::cuda::CUDAGuard dev(hidden.device());
     wc = rows_on(cast_cached(weight, cd), 16);
     hc = rows_on(hidden.to(cd), 16);
     const int64_t rows = hc.size(0);
-    lse = empty_cuda({rows}, at::kFloat, hc);
-    const Tensor rows_loss = empty_cuda({rows}, at::kFloat, hc);
-    ulm_streamed_ce_args a = streamed_args(hc, wc, target, lse, ignore_index);
-    const Tensor scratch = empty_cuda({ulm_streamed_ce_scratch(rows, a.V, a.d)}, at::kFloat, hc);
-    a.loss = rows_loss.data_ptr<float>(); a.scratch = scratch.data_ptr<float>();
-    check(ulm_streamed_ce_fwd(&a), "streamed cross-entropy forward");
+    stats = empty_cuda({rows + 1}, at::kFloat, hc);
     loss = empty_cuda({}, at::kFloat, hc);                  // sum of the row losses / denominator
-    inv = empty_cuda({}, at::kFloat, hc);                   // 1 / denominator
+    ulm_streamed_ce_args a = streamed_args(hc, wc, target, stats.data_ptr<float>(), ignore_index);
+    const Tensor scratch = empty_cuda({rows + ulm_streamed_ce_scratch(rows, a.V, a.d)}, at::kFloat, hc);
+    a.loss = scratch.data_ptr<float>(); a.scratch = a.loss + rows;
+    check(ulm_streamed_ce_fwd(&a), "streamed cross-entropy forward");
     Tensor dd;
     if (denom_dev) dd = denom_dev->to(hidden.device(), at::kFloat);
-    check(ulm_loss_mean(rows_loss.data_ptr<float>(), target.data_ptr<int64_t>(), rows, ignore_index, dd.defined() ? dd.data_ptr<float>() : nullptr,
-                        (float)denom, loss.data_ptr<float>(), inv.data_ptr<float>(), stream_of(hc)), "loss mean");
+    check(ulm_loss_mean(a.loss, a.target, rows, ignore_index, dd.defined() ? dd.data_ptr<float>() : nullptr, (float)denom, loss.data_ptr<float>(),
+                        a.lse + rows, a.stream), "loss mean");
   }
   if (!no_graph(hidden, weight)) {
     auto node = make_node<StreamedCeBwd>(hidden, weight);
-    node->ignore_index = ignore_index; node->piece_bytes = piece_bytes;
-    node->keep(hidden); node->keep(weight); node->keep(target); node->keep(lse); node->keep(inv); node->keep(wc); node->keep(hc);
+    node->ignore_index = ignore_index; node->piece_bytes = piece_bytes; node->hdtype = hidden.scalar_type();
+    node->keep(weight); node->keep(target); node->keep(stats); node->keep(wc); node->keep(hc);
     torch::autograd::set_history(loss, node);
   }
   return loss;
