@@ -319,18 +319,18 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (!waited) { ok = false; break; }              // the whole warp; nothing below waits for another one
         fence_after_sync();
         const int col_tile = (im.nt + t) * LM_BN;
-#pragma unroll 1
+        // the thread's 128 columns at once, and the accumulator goes back before any of them is worked on
+        uint32_t both[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(t_row + b * LM_BN + half * 128 + c, *reinterpret_cast<uint32_t(*)[32]>(&both[c]));
+        tmem_wait_ld();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_peer(peer_smem(&ctl->acc_free[b], 0));
+#pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
           const int c_blk = half * 128 + pass * 64;      // first column of this pass within the tile
-          uint32_t acc[64];
-          tmem_ld32(t_row + b * LM_BN + c_blk, *reinterpret_cast<uint32_t(*)[32]>(&acc[0]));
-          tmem_ld32(t_row + b * LM_BN + c_blk + 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[32]));
-          tmem_wait_ld();
-          if (pass == 1) {                               // everything of this tile is in registers: hand the accumulator back
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_peer(peer_smem(&ctl->acc_free[b], 0));
-          }
+          uint32_t (&acc)[64] = *reinterpret_cast<uint32_t(*)[64]>(&both[64 * pass]);
           if constexpr (MODE == kStats) {
             const int col0 = col_tile + c_blk;
             if (col0 + 64 > p.V) {
@@ -350,16 +350,19 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const float m_new = fmaxf(m, mx * kLog2e);
             if (m_new > -INFINITY) {
               ssum *= ex2(m - m_new);                    // 2^(-inf) = 0 on the first block
-              const float nm = -m_new;
-              float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+              const uint64_t log2e2 = f2_pack(kLog2e, kLog2e), nm2 = f2_pack(-m_new, -m_new);
+              uint64_t sa = f2_pack(0.f, 0.f), sb = sa;
 #pragma unroll
               for (int c = 0; c < 64; c += 4) {
-                s0 += ex2(fmaf(__uint_as_float(acc[c]), kLog2e, nm));
-                s1 += ex2(fmaf(__uint_as_float(acc[c + 1]), kLog2e, nm));
-                s2 += ex2(fmaf(__uint_as_float(acc[c + 2]), kLog2e, nm));
-                s3 += ex2(fmaf(__uint_as_float(acc[c + 3]), kLog2e, nm));
+                float e0, e1, e2, e3;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1])), log2e2, nm2), e0, e1);
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(acc[c + 2]), __uint_as_float(acc[c + 3])), log2e2, nm2), e2, e3);
+                sa = f2_add(sa, f2_pack(ex2(e0), ex2(e1)));
+                sb = f2_add(sb, f2_pack(ex2(e2), ex2(e3)));
               }
-              ssum += (s0 + s1) + (s2 + s3);
+              float s0, s1;
+              f2_unpack(f2_add(sa, sb), s0, s1);
+              ssum += s0 + s1;
               m = m_new;
             } else {                                     // nothing but -inf, or NaN, which fmaxf passes over
 #pragma unroll
@@ -368,12 +371,14 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             }
           } else if constexpr (MODE == kGrad) {
             const int col0 = p.v0 + col_tile + c_blk;
+            const uint64_t log2e2 = f2_pack(kLog2e, kLog2e), shift2 = f2_pack(shift, shift);
             uint32_t pk[32];
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
-              const float g0 = ex2(fmaf(__uint_as_float(acc[c]), kLog2e, shift)), g1 = ex2(fmaf(__uint_as_float(acc[c + 1]), kLog2e, shift));
-              acc[c] = __float_as_uint(g0);
-              acc[c + 1] = __float_as_uint(g1);
+              float g0, g1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1])), log2e2, shift2), g0, g1);
+              acc[c] = __float_as_uint(ex2(g0));
+              acc[c + 1] = __float_as_uint(ex2(g1));
             }
             if ((unsigned)(tgt - col0) < 64u) {
 #pragma unroll
