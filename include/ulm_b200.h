@@ -360,8 +360,8 @@ int ulm_lmhead_score(const ulm_lmhead_lse_args* a, uint8_t* hit, int32_t* part_i
  * The loss of train.py:2069-2082 over a vocabulary too large to keep [rows, V] logits for: the forward goes over the
  * vocabulary once with a running maximum and sum per row, the backward forms the logits again, `piece` columns at a time,
  * and keeps softmax - onehot of one piece in 16 bits.  z = h w^T stays in fp32 throughout (it is not rounded to the 16-bit type).
- * fwd: lse[r] and loss[r] = lse[r] - z[r, target[r]] in fp32; loss 0 where target[r] is ignore_index or no column.
- *      scratch: ulm_streamed_ce_scratch(rows, V, d) floats.
+ * fwd: lse[r] and loss[r] = lse[r] - z[r, target[r]] in fp32; loss 0 where target[r] is ignore_index or no column; and the
+ *      mean of the losses, *mean and *inv as ulm_loss_mean gives them.  scratch: ulm_streamed_ce_scratch(rows, V, d) floats.
  * bwd: with f = *factor_dev (times *factor2_dev; d total / d row loss) and G = softmax - onehot, 0 on the rows above:
  *      dh [rows, d] = f G w, dense, of the 16-bit type; dw [V, d] = f G^T h, 16-bit, or fp32 with dw_f32, or added to an fp32
  *      dw with dw_add; either may be NULL.  lse is the forward's.
@@ -371,8 +371,11 @@ int ulm_lmhead_score(const ulm_lmhead_lse_args* a, uint8_t* hit, int32_t* part_i
  * any size.  All sums run in a fixed order.  status_dev: optional, see ULM_STATUS_*. */
 typedef struct {
   const void* h; const void* w; const int64_t* target;
-  float* lse; float* loss; float* scratch;             /* loss, scratch: forward only */
-  int64_t h_stride, w_stride;
+  float* lse;
+  float* loss; float* scratch;                         /* from here on: forward only */
+  float* mean; float* inv;
+  const float* denom_dev; float denom; int32_t reserved0;
+  int64_t h_stride, w_stride;                          /* of both */
   int64_t rows; int32_t V; int32_t d;
   int32_t dtype; int32_t reserved;
   int64_t ignore_index;

@@ -110,7 +110,8 @@ class LmHeadLseArgs(C.Structure):
 
 
 class StreamedCeArgs(C.Structure):
-    _fields_ = [('h', vp), ('w', vp), ('target', vp), ('lse', vp), ('loss', vp), ('scratch', vp), ('h_stride', i64), ('w_stride', i64),
+    _fields_ = [('h', vp), ('w', vp), ('target', vp), ('lse', vp), ('loss', vp), ('scratch', vp), ('mean', vp), ('inv', vp),
+                ('denom_dev', vp), ('denom', f32), ('reserved0', i32), ('h_stride', i64), ('w_stride', i64),
                 ('rows', i64), ('V', i32), ('d', i32), ('dtype', i32), ('reserved', i32), ('ignore_index', i64),
                 ('status_dev', vp), ('stream', vp)]
 

@@ -25,6 +25,24 @@ inline int check_launch(const char* what) {
   return ULM_OK;
 }
 
+// Programmatic dependent launch: a kernel launched by launch_dependent may be set up, and its blocks started on SMs that are
+// free, while the one before it in the stream still runs.  Such a kernel calls grid_dependency_wait before it touches
+// anything another kernel writes or reads; that returns once all kernels before it have ended and their writes can be seen.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next such launch begin.
+__device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_dependent(const char* what, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  if (e != cudaSuccess) { cudaGetLastError(); return fail(ULM_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e)); }
+  return check_launch(what);
+}
+
 constexpr int kNumSMs = 148;          // B200: 2 dies x 74 SMs
 
 // ---- 16-bit <-> fp32, round-to-nearest-even --------------------------------

@@ -123,6 +123,7 @@ struct Params {
   const int64_t* target;
   int64_t ignore_index;
   float *part_m, *part_s, *z_target;                     // statistics
+  uint32_t* done;
   const float* lse;                                      // G
   int g_cols;                                            // the workspace's columns
   Out out;                                               // products
@@ -140,7 +141,7 @@ __device__ __forceinline__ float out_factor(const Out& o) { return *o.factor_dev
 // 128 bytes of a row of a warp's block into shared memory, lane = row, as the 128-byte swizzle has them: 16-byte chunk c at chunk
 // position c ^ (lane & 7); then one TMA store or addition of the block to (col, row) of `map`.  Whole warp.
 template <bool ADD>
-__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* block, int lane, const uint32_t (&u)[32], int col, int row) {
+__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* block, int lane, const uint32_t (&u)[32], int col, int row, int z = 0) {
   if (lane == 0) bulk_wait_read0();                      // the warp's previous store must have read the block
   __syncwarp();
   uint8_t* line = block + lane * 128;
@@ -150,7 +151,7 @@ __device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* blo
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) {
-    if (ADD) tma_add_4d(map, block, col, row, 0, 0); else tma_store_4d(map, block, col, row, 0, 0);
+    if (ADD) tma_add_4d(map, block, col, row, z, 0); else tma_store_4d(map, block, col, row, z, 0);
     bulk_commit();
   }
 }
@@ -216,8 +217,11 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   __syncthreads();
   cluster_sync();                                        // the other CTA's barriers are set up before anything signals them
   fence_after_sync();
+  grid_dependents_go();
+  grid_dependency_wait();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);   // warp-uniform
 
+  if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0u;
   if (warp == kEpiWarps) {
     // ---------------- TMA producer ----------------
     if (elect_one()) {
@@ -242,7 +246,9 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint32_t full = peer_smem(&ctl->full[s], 0);
             if constexpr (kAmn) {
 #pragma unroll
-              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, &tmA, full, m0 + 64 * i, k0, 0, 0);
+              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, &tmA, full, 0, k0, (m0 >> 6) + i, 0);
+            } else if constexpr (MODE == kRowGrad) {
+              tma_load_4d_pair(a, &tmA, full, 0, m0, kb, 0);
             } else {
               tma_load_4d_pair(a, &tmA, full, k0, m0, 0, 0);
             }
@@ -394,11 +400,11 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 else if (col0 + c + 1 >= p.V) pk[c >> 1] &= 0xffffu;
               }
             }
-            if (col_tile + c_blk < p.g_cols && row0 < p.rows) store_block<false>(&tmOut, my_staging, lane, pk, col_tile + c_blk, row0);
+            if (col_tile + c_blk < p.g_cols && row0 < p.rows) store_block<false>(&tmOut, my_staging, lane, pk, 0, row0, (col_tile + c_blk) >> 6);
           } else {
             const int col = col_tile + c_blk;
             if (im.slot >= 0) {
-              store_f32<false>(&tmSlots, my_staging, lane, acc, 1.f, c_blk, LM_BN, im.slot * kPairM + (int)rank * LM_BM + (warp & 3) * 32);
+              if (row0 < p.out.rows) store_f32<false>(&tmSlots, my_staging, lane, acc, 1.f, c_blk, LM_BN, im.slot * kPairM + (int)rank * LM_BM + (warp & 3) * 32);
             } else if (col < p.out.cols && row0 < p.out.rows) {
               if (p.out.is_f32 && p.out.prev) {
                 store_f32<true>(&tmOut, my_staging, lane, acc, factor, col, p.out.cols, row0);
@@ -440,6 +446,8 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 template <typename T>
 __global__ void __launch_bounds__(256)
 streamed_ce_join_kernel(const Work w, const Out o) {
+  grid_dependents_go();
+  grid_dependency_wait();
   const int j = blockIdx.x, t = w.whole + j, mt = t / w.n_nt, nt = t - mt * w.n_nt;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 8;
   const int64_t row = (int64_t)mt * kPairM + r;
@@ -449,6 +457,7 @@ streamed_ce_join_kernel(const Work w, const Out o) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll 4
   for (int k = 0; k < w.split; ++k, s += kSlot) {
     const float4 a = *reinterpret_cast<const float4*>(s), b = *reinterpret_cast<const float4*>(s + 4);
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
@@ -468,28 +477,65 @@ streamed_ce_join_kernel(const Work w, const Out o) {
   }
 }
 
-// lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry).
-// One warp per row.
+// lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry): a
+// warp per row.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
+// n = *denom_dev, denom if that is positive, or the number of targets that are not ignore_index (at least 1).
+struct Mean {
+  const float* denom_dev;
+  float denom;
+  float *mean, *inv;
+  uint32_t* done;                                        // CTAs that have finished: zeroed by the statistics kernel
+};
 __global__ void __launch_bounds__(256)
 streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int n_parts, const int64_t* __restrict__ target,
-                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows) {
+                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows, const Mean mean) {
+  __shared__ double s_sum[8];
+  __shared__ int s_n[8];
+  __shared__ uint32_t s_before;
+  grid_dependents_go();
+  grid_dependency_wait();
   const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  float m = -INFINITY;
-  for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, part_m[r * n_parts + i]);
-  m = warp_max(m);
-  float s = 0.f;
-  for (int i = lane; i < n_parts; i += 32) {
-    const float mi = part_m[r * n_parts + i], si = part_s[r * n_parts + i];
-    s += mi > -INFINITY ? si * exp2f(mi - m) : si;       // a group of nothing but -inf has the sum 0; of NaN, NaN
+  if (r < rows) {
+    float m = -INFINITY;
+    for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, part_m[r * n_parts + i]);
+    m = warp_max(m);
+    float s = 0.f;
+    for (int i = lane; i < n_parts; i += 32) {
+      const float mi = part_m[r * n_parts + i], si = part_s[r * n_parts + i];
+      s += mi > -INFINITY ? si * exp2f(mi - m) : si;     // a group of nothing but -inf has the sum 0; of NaN, NaN
+    }
+    s = warp_sum(s);
+    if (lane == 0) {
+      const float l = (m + log2f(s)) * kLn2;
+      lse[r] = l;
+      const int64_t t = target[r];
+      loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : l - loss[r];
+    }
   }
-  s = warp_sum(s);
-  if (lane) return;
-  const float l = (m + log2f(s)) * kLn2;
-  lse[r] = l;
-  const int64_t t = target[r];
-  loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : l - loss[r];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_before = atomicAdd(mean.done, 1u);
+  __syncthreads();
+  if (s_before != gridDim.x - 1) return;
+  __threadfence();
+  double sum = 0.;
+  int n = 0;
+  const bool count = !mean.denom_dev && !(mean.denom > 0.f);
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < rows; i += 256) {
+    sum += __ldcg(loss + i);
+    if (count) n += target[i] != ignore_index;
+  }
+  sum = warp_sum(sum);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0) { s_sum[threadIdx.x >> 5] = sum; s_n[threadIdx.x >> 5] = n; }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 8; ++w) { sum += s_sum[w]; n += s_n[w]; }
+  const float d = mean.denom_dev ? *mean.denom_dev : count ? (float)(n > 0 ? n : 1) : mean.denom;
+  *mean.mean = (float)(sum / d);
+  *mean.inv = 1.f / d;
 }
 
 // ---------------------------------------------------------------------------
@@ -521,8 +567,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   auto kern = streamed_ce_kernel<T, MODE>;
   if (int rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who)) return rc;
   const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
-  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, mo, p);
-  return check_launch(who);
+  return launch_dependent(who, kern, grid, kThreads, smem_bytes(MODE), st, ma, mb, mo, mo, p);
 }
 // A product and, where tiles were cut, their sum
 template <typename T, int MODE>
@@ -536,10 +581,9 @@ int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p
   ms = mo;
   if (p.w.split > 1 && (rc = encode_matrix_map(&ms, p.out.slots, ULM_F32, (int64_t)p.w.rest * p.w.split * kPairM, LM_BN, LM_BN, 32, who))) return rc;
   const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
-  kern<<<grid, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, ms, p);
-  if ((rc = check_launch(who)) || p.w.split == 1) return rc;
-  streamed_ce_join_kernel<T><<<dim3(p.w.rest, kPairM / 8), 256, 0, st>>>(p.w, p.out);
-  return check_launch(who);
+  rc = launch_dependent(who, kern, grid, kThreads, smem_bytes(MODE), st, ma, mb, mo, ms, p);
+  if (rc || p.w.split == 1) return rc;
+  return launch_dependent(who, streamed_ce_join_kernel<T>, dim3(p.w.rest, (unsigned)((p.out.rows < kPairM ? p.out.rows : kPairM) + 7) / 8), 256, 0, st, p.w, p.out);
 }
 
 int check_args(const ulm_streamed_ce_args* a, const char* who) {
@@ -579,13 +623,17 @@ int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
   p.w = stats_work(a->rows, a->V, a->d);
   const int parts = 2 * ((p.w.n_nt + p.w.group - 1) / p.w.group);
   p.part_m = a->scratch; p.part_s = a->scratch + a->rows * parts; p.z_target = a->loss;
+  p.done = reinterpret_cast<uint32_t*>(a->scratch + 2 * a->rows * parts);
   cudaStream_t st = (cudaStream_t)a->stream;
   if (int rc = launch<T, kStats>(mh, mw, mh, p, device, st, who)) return rc;
-  streamed_ce_finish_kernel<<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V, a->lse, a->loss, a->rows);
-  return check_launch(who);
+  const Mean mean{a->denom_dev, a->denom, a->mean, a->inv, p.done};
+  return launch_dependent(who, streamed_ce_finish_kernel, (unsigned)((a->rows + 7) / 8), 256, 0, st, p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V,
+                          a->lse, a->loss, a->rows, mean);
 }
 
-int64_t g_stride(int64_t piece) { return (piece + 63) / 64 * 64; }
+// G's workspace: blocks of 64 columns, [block][row][64], so that every box that is stored or loaded is one stretch of memory.
+// As a row-major matrix, whose boxes are 128-byte pieces of far-apart rows, the whole op took 0.5 % longer (32768 x 768 x 32000).
+int64_t g_blocks(int64_t piece) { return (piece + 63) / 64; }
 
 template <typename T>
 int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int device, const char* who) {
@@ -597,15 +645,16 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
   if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who))) return rc;
   if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
   for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
-    const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece, stride = g_stride(n);
+    const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece;
     CUtensorMap g_rows, g_mn, g_out;
-    if ((rc = encode_matrix_map(&g_rows, g->workspace, a->dtype, a->rows, stride, stride, LM_BM, who))) return rc;
-    if ((rc = encode_matrix_map(&g_mn, g->workspace, a->dtype, a->rows, stride, stride, 64, who))) return rc;
-    if ((rc = encode_matrix_map(&g_out, g->workspace, a->dtype, a->rows, stride, stride, 32, who))) return rc;
+    auto g_map = [&](CUtensorMap* m, int box_rows) {
+      return encode_bhsd_map(m, g->workspace, a->dtype, 1, (int)g_blocks(n), (int)a->rows, 0, a->rows * 64, 64, box_rows, who);
+    };
+    if ((rc = g_map(&g_rows, LM_BM)) || (rc = g_map(&g_mn, 64)) || (rc = g_map(&g_out, 32))) return rc;
     Params p = common_params(a);
     p.v0 = (int)v0;
     p.lse = a->lse;
-    p.g_cols = (int)stride;
+    p.g_cols = (int)g_blocks(n) * 64;
     p.w = stats_work(a->rows, (int)n, a->d);
     if ((rc = launch<T, kGrad>(h_rows, w_rows, g_out, p, device, st, who))) return rc;
     p.out.factor_dev = g->factor_dev;
@@ -640,11 +689,11 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
 extern "C" int64_t ulm_streamed_ce_scratch(int64_t rows, int32_t V, int32_t d) {
   if (rows <= 0 || V <= 0 || d <= 0) return 0;
   const ulm::Work w = ulm::stats_work(rows, V, d);
-  return rows * 4 * ((w.n_nt + w.group - 1) / w.group);
+  return rows * 4 * ((w.n_nt + w.group - 1) / w.group) + 1;
 }
 
 extern "C" int64_t ulm_streamed_ce_workspace(int64_t rows, int32_t V, int64_t piece) {
-  return rows * ulm::g_stride(piece < V ? piece : V);
+  return rows * 64 * ulm::g_blocks(piece < V ? piece : V);
 }
 
 extern "C" int64_t ulm_streamed_ce_slots(int64_t rows, int32_t V, int32_t d, int64_t piece, int32_t want_dh, int32_t want_dw) {
@@ -664,7 +713,7 @@ extern "C" int ulm_streamed_ce_fwd(const ulm_streamed_ce_args* a) {
   const char* who = "ulm_streamed_ce_fwd";
   int rc = check_args(a, who);
   if (rc || a->rows == 0) return rc;
-  if (!a->loss || !a->scratch) return fail(ULM_ERR_ARG, "%s: null tensor", who);
+  if (!a->loss || !a->scratch || !a->mean || !a->inv) return fail(ULM_ERR_ARG, "%s: null tensor", who);
   DeviceScope scope(a->h, who);
   if (scope.rc) return scope.rc;
   return a->dtype == ULM_BF16 ? forward<__nv_bfloat16>(a, scope.device, who) : forward<__half>(a, scope.device, who);

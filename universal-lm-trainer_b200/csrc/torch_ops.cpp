@@ -810,9 +810,10 @@ std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& b
   if (!no_graph(x, branch, weight)) {
     auto node = make_node<DropNormBwd>(x, branch, weight);
     node->drop = drop; node->wdtype = weight.scalar_type(); node->bdtype = branch.scalar_type();
+    // an alias of x_new, so that the node does not hold its own output; it shares the version counter
+    node->keep(x_new.detach()); node->keep(w); node->keep(rstd);
     torch::autograd::set_history(x_new, node);
     torch::autograd::set_history(y, node);
-    node->keep(x_new, true); node->keep(w); node->keep(rstd);
   }
   return {x_new, y};
 }
@@ -1340,11 +1341,11 @@ Tensor streamed_cross_entropy(const Tensor& hidden, const Tensor& weight, const 
     ulm_streamed_ce_args a = streamed_args(hc, wc, target, stats.data_ptr<float>(), ignore_index);
     const Tensor scratch = empty_cuda({rows + ulm_streamed_ce_scratch(rows, a.V, a.d)}, at::kFloat, hc);
     a.loss = scratch.data_ptr<float>(); a.scratch = a.loss + rows;
-    check(ulm_streamed_ce_fwd(&a), "streamed cross-entropy forward");
     Tensor dd;
     if (denom_dev) dd = denom_dev->to(hidden.device(), at::kFloat);
-    check(ulm_loss_mean(a.loss, a.target, rows, ignore_index, dd.defined() ? dd.data_ptr<float>() : nullptr, (float)denom, loss.data_ptr<float>(),
-                        a.lse + rows, a.stream), "loss mean");
+    a.denom_dev = dd.defined() ? dd.data_ptr<float>() : nullptr; a.denom = (float)denom;
+    a.mean = loss.data_ptr<float>(); a.inv = a.lse + rows;
+    check(ulm_streamed_ce_fwd(&a), "streamed cross-entropy forward");
   }
   if (!no_graph(hidden, weight)) {
     auto node = make_node<StreamedCeBwd>(hidden, weight);
