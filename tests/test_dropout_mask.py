@@ -98,4 +98,4 @@ def test_refusals_come_before_any_launch():
     f.d, f.rows = 64, 0
     assert lib.ulm_add_dropout_norm_fwd(C.byref(f), 0.1, 0) == 0
     assert lib.ulm_add_dropout_norm_bwd(None, 0.1, 0) == -1
-    assert lib.ulm_add_dropout_norm_partial_rows(0) == 1 and lib.ulm_add_dropout_norm_partial_rows(10 ** 9) == 296
+    assert lib.ulm_add_dropout_norm_partial_rows(0) == 1 and lib.ulm_add_dropout_norm_partial_rows(10 ** 9) == 444

@@ -5,10 +5,11 @@
 //
 // drop and its mask: philox.cuh, over the branch's elements.  Sums and statistics are fp32; y, db are rounded once.
 //
-// What bounds it: HBM, 12 bytes an element forward and 16 backward.  A row belongs to W warps of a CTA (W = 1 up to 1024
+// What bounds it: HBM, 12 bytes an element forward and 16 backward: 32768 x 768 fp16 45.5 us (6.6 TB/s) and 67.6 us (6.0 TB/s) and
+// 3 us for dw's column sums.  A row belongs to W warps of a CTA (W = 1 up to 1024
 // elements forward) and is held in registers between its two uses; a lane owns vectors of E elements: eight where all
 // rows are whole 16-byte vectors of the 16-bit tensors, so that a vector is exactly one group of the mask, else four
-// (two lanes then form the same group: 2x the generator's work, beside 12-16 bytes an element still hidden).
+// (two lanes then form the same group, twice the generator's work: 20000 x 772 41 and 69 us).
 // dw: per-lane sums over a CTA's rows, added up over the CTA's groups in shared memory, one partial row per CTA, column
 // sums in a fixed order: no atomics.
 #include "col_sum.cuh"
@@ -106,12 +107,12 @@ add_dropout_norm_fwd_kernel(const FwdParams p, const __grid_constant__ DropMask 
     for (int it = 0; it < NV; ++it) {
       const int vi = first + it * hop;
       if (vi < nvec) {
-        const uint32_t bits = keep_bits<E>(mask, (uint64_t)r * nvec + vi);
+        const Keep<E> keep = keep_of<E>(mask, (uint64_t)r * nvec + vi);
         float f[E];
         unpack_raw<TY, E>(b[it], f);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          v[it][j] += dropped(mask, bits, j, f[j]);
+          v[it][j] += dropped(mask, keep(j), f[j]);
           ss += v[it][j] * v[it][j];
         }
         store_f32<E>(p.x_out + r * p.xout_stride + vi * E, v[it]);
@@ -202,9 +203,9 @@ add_dropout_norm_bwd_kernel(const BwdParams p, const __grid_constant__ DropMask 
 #pragma unroll
         for (int j = 0; j < E; ++j) o[j] = inv * (g[j] * wv[j] - z[it][j] * dm) + ga[it][j];
         store_f32<E>(p.dx + r * p.dx_stride + vi * E, o);
-        const uint32_t bits = keep_bits<E>(mask, (uint64_t)r * nvec + vi);
+        const Keep<E> keep = keep_of<E>(mask, (uint64_t)r * nvec + vi);
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = dropped(mask, bits, j, o[j]);
+        for (int j = 0; j < E; ++j) o[j] = dropped(mask, keep(j), o[j]);
         store_16<TY, E>(db + r * p.dbranch_stride + vi * E, o);
       }
     }
@@ -237,14 +238,21 @@ Split split_rows(int64_t rows, int nvec, int nv, int warps) {
   if (spread < s.groups) s.groups = spread < 1 ? 1 : (int)spread;
   return s;
 }
-// Vectors a lane holds: of 4 floats each as many as make one warp enough for 1024 elements forward; backward, where a
-// row's z, dy, g and dw are alive together, 8 elements up to rows of 1024 (up to four warps a row), 16 beyond.
-int fwd_nv(int nvec, int E) { const int most = 32 / E, need = ceil_div(nvec, 32); return need < most ? need : most; }
-int bwd_nv(int d, int E) { return (d <= 1024 ? 8 : 16) / E; }
+// Elements a lane holds.  Forward 32 with vectors of eight (one warp a row up to 1024), with vectors of four 16 up to rows of
+// 4096 and 32 beyond.  Backward, where a
+// row's z, dy, g and dw are alive together, 8 up to rows of 2048 and 16 beyond: us with 8 / 16, bf16,
+// 4096 x 2048 28.5 / 29.3, x 2560 39.2 / 36.3, x 4096 77.6 / 54.5 (4.7, 4.6 and 4.9 TB/s
+// with what is taken).
+int fwd_nv(int nvec, int E) { const int most = E == 8 || nvec <= 1024 ? 4 : 8, need = ceil_div(nvec, 32); return need < most ? need : most; }
+int bwd_nv(int d, int E) { return (d <= 2048 ? 8 : 16) / E; }
 
-int64_t bwd_blocks(int64_t rows, int groups) {
-  const int64_t want = (rows + groups - 1) / groups, cap = 2 * kNumSMs;
-  return want < 1 ? 1 : want < cap ? want : cap;
+// A CTA of the backward per `groups` rows, 24 warps per SM at most (their registers fill it): each leaves one partial row
+constexpr int kBwdWarpsPerSm = 24, kMostBwdCtas = 3;
+int64_t bwd_blocks(int64_t rows, const Split& s) {
+  const int64_t want = (rows + s.groups - 1) / s.groups;
+  int per_sm = kBwdWarpsPerSm / (s.W * s.groups);
+  per_sm = per_sm < 1 ? 1 : per_sm > kMostBwdCtas ? kMostBwdCtas : per_sm;
+  return want < per_sm * kNumSMs ? want : per_sm * kNumSMs;
 }
 
 bool ok16(const void* p, int64_t stride, int E) { return !(reinterpret_cast<uintptr_t>(p) & (2 * E - 1)) && stride % E == 0; }
@@ -285,7 +293,7 @@ int64_t launch_bwd(BwdParams p, int E, const DropMask& mask, cudaStream_t st) {
   const int nvec = p.d / E, nv = bwd_nv(p.d, E);
   const Split s = split_rows(p.rows, nvec, nv, kBwdWarps);
   p.W = s.W;
-  const int64_t blocks = bwd_blocks(p.rows, s.groups);
+  const int64_t blocks = bwd_blocks(p.rows, s);
   const int threads = s.W * s.groups * 32;
   const size_t smem = (size_t)s.groups * p.d * sizeof(float);            // at most 12 x 512 floats: below 48 KB
   auto go = [&](auto kern) { kern<<<(unsigned)blocks, threads, smem, st>>>(p, mask); };
@@ -323,8 +331,11 @@ extern "C" int ulm_add_dropout_norm_fwd(const ulm_rmsnorm_fwd_args* a, double p,
   return check_launch(who);
 }
 
-// groups is never below one, so one CTA per row is the most
-extern "C" int64_t ulm_add_dropout_norm_partial_rows(int64_t rows) { return ulm::bwd_blocks(rows, 1); }
+// one CTA a row, or as many as run at a time
+extern "C" int64_t ulm_add_dropout_norm_partial_rows(int64_t rows) {
+  const int64_t most = ulm::kMostBwdCtas * ulm::kNumSMs;
+  return rows < 1 ? 1 : rows < most ? rows : most;
+}
 
 extern "C" int ulm_add_dropout_norm_bwd(const ulm_rmsnorm_bwd_args* a, double p, uint64_t seed) {
   using namespace ulm;

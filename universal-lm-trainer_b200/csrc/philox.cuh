@@ -20,7 +20,8 @@ constexpr int kPhiloxRounds = 10;
 
 struct DropMask {
   uint32_t k0[kPhiloxRounds], k1[kPhiloxRounds];         // the rounds' keys: the same for all threads, so made on the host
-  uint32_t threshold;                                    // 0 (nothing is dropped) .. 65536 (everything is)
+  uint32_t least;                                        // threshold << 16: 16 bits in the upper half of a word stay from here on
+  uint32_t bits;                                         // ANDed to the generator's words: 0 where everything is dropped
   float scale;
 };
 
@@ -32,8 +33,10 @@ inline DropMask make_drop_mask(double p, uint64_t seed) {
     m.k1[r] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
   }
   const double t = nearbyint(p * 65536.0);
-  m.threshold = p <= 0. ? 0u : p >= 1. ? 65536u : t < 1. ? 1u : t > 65535. ? 65535u : (uint32_t)t;
-  m.scale = m.threshold < 65536u ? (float)(65536.0 / (65536.0 - m.threshold)) : 0.f;
+  const uint32_t threshold = p <= 0. ? 0u : t < 1. ? 1u : t > 65535. ? 65535u : (uint32_t)t;
+  m.least = p >= 1. ? 0xffffffffu : threshold << 16;
+  m.bits = p >= 1. ? 0u : 0xffffffffu;
+  m.scale = p >= 1. ? 0.f : (float)(65536.0 / (65536.0 - threshold));
   return m;
 }
 inline bool drop_p_ok(double p) { return p >= 0. && p <= 1.; }      // false for NaN
@@ -51,30 +54,38 @@ __device__ __forceinline__ uint4 philox(const DropMask& m, uint64_t group) {
   return make_uint4(c0, c1, c2, c3);
 }
 
-// The mask of N consecutive elements that start at index v * N: bit j of the answer is set where element j stays.
-template <int N>
-__device__ __forceinline__ uint32_t keep_bits(const DropMask& m, uint64_t v) {
+// The mask of N consecutive elements that start at index v * N.  Kept as the generator's words and compared where an element is
+// used: a shift for every second element, a compare and a select, instead of gathering the N answers into bits first
+// (dropout of 32768 x 768 bf16 20.9 -> 17.9 us; the gate's backward at 32768 x 2048 113 -> 101).
+template <int N> struct Keep {
   static_assert(N == 8 || N == 4, "a group or half of one");
+  uint32_t w[N / 2], least;
+  __device__ __forceinline__ bool operator()(int j) const { return (j & 1 ? w[j >> 1] : w[j >> 1] << 16) >= least; }
+};
+template <int N>
+__device__ __forceinline__ Keep<N> keep_of(const DropMask& m, uint64_t v) {
   const uint4 u = philox(m, N == 8 ? v : v >> 1);
-  uint32_t w[N / 2];
+  Keep<N> k;
+  k.least = m.least;
   if constexpr (N == 8) {
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    k.w[0] = u.x & m.bits; k.w[1] = u.y & m.bits; k.w[2] = u.z & m.bits; k.w[3] = u.w & m.bits;
   } else {
     const bool upper = v & 1;
-    w[0] = upper ? u.z : u.x;
-    w[1] = upper ? u.w : u.y;
+    k.w[0] = (upper ? u.z : u.x) & m.bits;
+    k.w[1] = (upper ? u.w : u.y) & m.bits;
   }
-  uint32_t bits = 0;
-#pragma unroll
-  for (int j = 0; j < N / 2; ++j) {
-    bits |= (uint32_t)((w[j] & 0xffffu) >= m.threshold) << (2 * j);
-    bits |= (uint32_t)((w[j] >> 16) >= m.threshold) << (2 * j + 1);
-  }
-  return bits;
+  return k;
 }
-__device__ __forceinline__ bool keep_one(const DropMask& m, uint64_t i) { return keep_bits<8>(m, i >> 3) >> (i & 7) & 1u; }
+// element i by itself
+__device__ __forceinline__ bool keep_one(const DropMask& m, uint64_t i) {
+  const Keep<8> k = keep_of<8>(m, i >> 3);
+  bool stays = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) stays = (int)(i & 7) == j ? k(j) : stays;
+  return stays;
+}
 
 // A dropped element is zero whatever it held, infinities and NaN included.
-__device__ __forceinline__ float dropped(const DropMask& m, uint32_t bits, int j, float v) { return bits >> j & 1u ? v * m.scale : 0.f; }
+__device__ __forceinline__ float dropped(const DropMask& m, bool stays, float v) { return stays ? v * m.scale : 0.f; }
 
 }  // namespace ulm
