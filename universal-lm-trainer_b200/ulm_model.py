@@ -30,6 +30,9 @@ class ModelConfig:  # train.py:725-737
     use_rope: bool = True
     tie_weights: bool = True
     use_gradient_checkpointing: bool = False
+    # not the reference's: what a training step need not store between forward and backward
+    counter_dropout: bool = False   # feed-forward and residual dropout by ulm_ops.Dropout, inside the gate and the residual add + norm
+    streamed_loss: bool = False     # ulm_ops.streamed_cross_entropy: no logits
 
 
 # compute_loss pads the flattened token dimension to a multiple of this (see DecoderOnlyTransformer._forward_flat)
@@ -130,15 +133,29 @@ def _drop(dropout, x):
     return x if idle else dropout(x)
 
 
+def _mask_of(dropout):
+    """(p, seed) where ``dropout`` is a plain `ulm_ops.Dropout` at work, for the kernel that works in its place; None where it has
+    to be called (or is idle)."""
+    plain = type(dropout) is ulm_ops.Dropout and not (dropout._forward_hooks or dropout._forward_pre_hooks)
+    return (dropout.p, ulm_ops.next_dropout_seed()) if plain and dropout.active() else None
+
+
+def _make_dropout(p, counter):
+    return ulm_ops.Dropout(p) if counter else nn.Dropout(p)
+
+
 class FeedForward(nn.Module):  # train.py:1966-1975
-    def __init__(self, d_model: int, d_ff: int, dropout: float):
+    def __init__(self, d_model: int, d_ff: int, dropout: float, counter_dropout: bool = False):
         super().__init__()
         self.w1 = nn.Linear(d_model, d_ff, bias=False)
         self.w3 = nn.Linear(d_model, d_ff, bias=False)
         self.w2 = nn.Linear(d_ff, d_model, bias=False)
-        self.dropout = nn.Dropout(dropout)
+        self.dropout = _make_dropout(dropout, counter_dropout)
 
     def forward(self, x):
+        mask = _mask_of(self.dropout)
+        if mask is not None:
+            return linear(gated_linear(x, self.w1.weight, self.w3.weight, *mask), self.w2.weight)
         return linear(_drop(self.dropout, gated_linear(x, self.w1.weight, self.w3.weight)), self.w2.weight)
 
 
@@ -147,24 +164,32 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
     residual add is fused with the norm that FOLLOWS it (one pass over the residual stream instead of
     two), so a block receives the residual stream together with the branch output that has not been
     added yet (`pending`: the previous block's feed-forward output, None for the first block) and hands
-    its own feed-forward output on in the same way; the model's final norm absorbs the last one.  Same
-    values, same parameter names."""
+    its own feed-forward output on in the same way; the model's final norm absorbs the last one.  With
+    `counter_dropout` the output is handed on undropped, as (output, p, seed), and dropped where it is added.
+    Same values, same parameter names."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
         self.self_attn = MultiHeadAttention(config)
-        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout)
+        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout, config.counter_dropout)
         self.norm1 = FusedRMSNorm(config.d_model)
         self.norm2 = FusedRMSNorm(config.d_model)
-        self.dropout = nn.Dropout(config.dropout)
+        self.dropout = _make_dropout(config.dropout, config.counter_dropout)
 
     def forward(self, x, pending=None, cos=None, sin=None, shape=None):
         if pending is None:
             h = self.norm1(x)
         else:
-            x, h = self.norm1.add_forward(x, pending)                 # train.py:1993 of the previous block + 1988
+            x, h = self.norm1.add_forward(x, *_branch(pending))       # train.py:1993 of the previous block + 1988
         x, h = self.norm2.add_forward(x, self.self_attn(h, cos=cos, sin=sin, shape=shape))   # train.py:1989 + 1991
-        return x, _drop(self.dropout, self.ff(h))                            # added by whoever normalises next
+        out = self.ff(h)                                              # added by whoever normalises next
+        mask = _mask_of(self.dropout)
+        return x, (out, *mask) if mask is not None else _drop(self.dropout, out)
+
+
+def _branch(pending):
+    """What a block hands on, as `FusedRMSNorm.add_forward` takes it."""
+    return pending if isinstance(pending, tuple) else (pending,)
 
 
 class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
@@ -210,7 +235,7 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
                 x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), use_reentrant=False)
             else:
                 x, pending = layer(x, pending, cos=cos, sin=sin, shape=(n, L))
-        x = self.norm(x) if pending is None else self.norm.add_forward(x, pending)[1]
+        x = self.norm(x) if pending is None else self.norm.add_forward(x, *_branch(pending))[1]
         return x, T
 
     def forward_hidden(self, x):
@@ -232,5 +257,7 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
         Tp = n * L if TOKEN_QUANTUM <= 1 else -(-n * L // TOKEN_QUANTUM) * TOKEN_QUANTUM
         flat_ids, target = ulm_ops.token_targets(input_ids.contiguous(), labels.contiguous(), Tp, ignore_index)
         hidden, _ = self._forward_flat(input_ids, TOKEN_QUANTUM, flat_ids)
+        if self.config.streamed_loss:
+            return ulm_ops.streamed_cross_entropy(hidden, self.fc_out.weight, target, ignore_index=ignore_index, denominator=denominator)
         return ulm_ops.chunked_cross_entropy(hidden, self.fc_out.weight, target, ignore_index=ignore_index,
                                              chunk_rows=chunk_rows, denominator=denominator)

@@ -53,14 +53,18 @@ class FusedRMSNorm(nn.Module):
     def forward(self, x):
         return rms_norm(x, self.weight, self.eps)
 
-    def add_forward(self, x, branch):
+    def add_forward(self, x, branch, dropout_p=0.0, seed=0):
         """(x + branch, norm(x + branch)); the fused kernel when the tensors have the training layout
-        (fp32 residual stream, 16-bit branch, d <= 1024), the two separate ops otherwise."""
-        if (x.is_cuda and x.dtype == torch.float32 and branch.dtype in _16BIT and x.shape[-1] <= 1024
-                and x.shape[-1] % 4 == 0 and torch.is_autocast_enabled('cuda')
+        (fp32 residual stream, 16-bit branch, d <= 1024), the two separate ops otherwise.  With ``dropout_p`` the branch
+        is dropped first, in the fused kernel (d <= 8192) or by `dropout`."""
+        d = x.shape[-1]
+        if (x.is_cuda and x.dtype == torch.float32 and branch.dtype in _16BIT and d <= (8192 if dropout_p else 1024)
+                and d % 4 == 0 and torch.is_autocast_enabled('cuda')
                 and torch.get_autocast_dtype('cuda') == branch.dtype):
+            if dropout_p:
+                return dropout_add_rms_norm(x, branch, self.weight, dropout_p, seed, self.eps)
             return add_rms_norm(x, branch, self.weight, self.eps)
-        x = x + branch
+        x = x + (dropout(branch, dropout_p, seed) if dropout_p else branch)
         return x, rms_norm(x, self.weight, self.eps)
 
 

@@ -24,10 +24,12 @@ PRESETS = {
 BOS, EOS, PAD = 2, 3, 0
 
 
-def build(preset, device, seed=0):
+def build(preset, device, seed=0, **config):
+    """A preset's model in training mode and the preset; ``config`` sets further fields of `ulm_model.ModelConfig`, for instance
+    ``dropout=0.1, counter_dropout=True, streamed_loss=True``: regularised training that stores neither masks nor logits."""
     p = PRESETS[preset]
     torch.manual_seed(seed)
-    cfg = ulm_model.ModelConfig(**p['model'], dropout=0.0, use_gradient_checkpointing=p['checkpointing'])
+    cfg = ulm_model.ModelConfig(**{**p['model'], 'dropout': 0.0, 'use_gradient_checkpointing': p['checkpointing'], **config})
     model = ulm_model.DecoderOnlyTransformer(cfg).to(device)
     model.train()
     return model, p
