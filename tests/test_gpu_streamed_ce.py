@@ -112,7 +112,7 @@ def test_shapes_of_training(rows, V, dtype):
     check(*run(h, w, t, up=float(rows)), h, w, t, 0, up=float(rows))
 
 
-@pytest.mark.parametrize('rows,V,columns', [(300, 1000, 256), (1000, 1025, 256), (129, 5003, 1024), (2000, 4096, 1536), (4000, 2900, 768)])
+@pytest.mark.parametrize('rows,V,columns', [(300, 1000, 256), (1000, 1025, 256), (129, 5003, 1024), (2000, 4096, 1536), (4000, 2900, 768), (10000, 1100, 512)])
 def test_pieces_of_the_vocabulary(rows, V, columns):
     h, w, t = case(rows, V, 328, BF16)
     with piece_bytes(2 * rows * columns):
@@ -214,6 +214,39 @@ def test_strided_operands_and_other_streams():
             assert torch.equal(a, b)
 
 
+def test_broadcast_rows():
+    h, w, t = case(1, 520, 128, BF16)
+    t = torch.arange(1, 6, device='cuda')
+    for a, b in zip(run(h.expand(5, 128), w, t), run(h.expand(5, 128).contiguous(), w, t)):
+        assert torch.equal(a, b)
+
+
+def test_in_a_graph():
+    h, w, t = case(700, 3000, 128, BF16)
+    h.requires_grad_(), w.requires_grad_()
+    up = torch.ones((), device='cuda')
+
+    def step():
+        loss = ulm_ops.streamed_cross_entropy(h, w, t)
+        return [loss.detach(), *torch.autograd.grad(loss, [h, w], up)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        h.mul_(1.5)
+        t[::7] = 0
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b)
+
+
 def test_the_same_bits_every_time():
     h, w, t = case(1111, 3001, 776, F16)
     first = run(h, w, t)
@@ -258,19 +291,20 @@ def test_denominators(denominator):
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16])
-def test_fp32_parameters_under_autocast(dtype):
-    h, w, t = case(200, 700, 128, dtype)
+@pytest.mark.parametrize('rows,V,d', [(200, 700, 128), (5000, 700, 128), (300, 40000, 264)])       # whole tiles, cut ones, both
+def test_fp32_parameters_under_autocast(dtype, rows, V, d):
+    h, w, t = case(rows, V, d, dtype)
     wp = w.float().requires_grad_()
     hp = h.float().requires_grad_()
     with torch.autocast('cuda', dtype=dtype):
         loss = ulm_ops.streamed_cross_entropy(hp, wp, t)
-    dh, dw = torch.autograd.grad(loss, [hp, wp], torch.tensor(200.0, device='cuda'))
+    dh, dw = torch.autograd.grad(loss, [hp, wp], torch.tensor(float(rows), device='cuda'))
     assert dh.dtype == F32 and dw.dtype == F32
-    check(loss.detach(), dh.to(dtype), dw, h, w, t, 0, up=200.0, w_out=F32)
+    check(loss.detach(), dh.to(dtype), dw, h, w, t, 0, up=float(rows), w_out=F32)
     # into existing gradients, as the data-parallel step has it
     wp.grad = torch.full_like(wp, 0.5)
     with torch.autocast('cuda', dtype=dtype), ulm_ops.wgrad_in_place():
-        (ulm_ops.streamed_cross_entropy(hp, wp, t) * 200).backward()
+        (ulm_ops.streamed_cross_entropy(hp, wp, t) * rows).backward()
     assert float((wp.grad - 0.5 - dw).abs().max()) <= 2.0 ** -23 * (0.5 + float(dw.abs().max()))
 
 

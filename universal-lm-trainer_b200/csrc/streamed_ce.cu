@@ -130,12 +130,6 @@ struct Params {
   uint32_t* status;
 };
 
-__device__ __forceinline__ int target_column(const Params& p, int64_t row) {
-  if (row >= p.rows) return -1;
-  const int64_t t = p.target[row];
-  return t != p.ignore_index && t >= 0 && t < p.V ? (int)t : -1;
-}
-
 __device__ __forceinline__ float out_factor(const Out& o) { return *o.factor_dev * (o.factor2_dev ? *o.factor2_dev : 1.f) * o.factor; }
 
 // 128 bytes of a row of a warp's block into shared memory, lane = row, as the 128-byte swizzle has them: 16-byte chunk c at chunk
@@ -309,15 +303,29 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = out_factor(p.out);
     uint32_t tt = 0;
     bool ok = true;
+    // the row's target column and, for G, its shift of the exponent 2^(z log2e + shift); asked for an item ahead
+    struct Row { int64_t target; float lse; };
+    auto row_of = [&](int q) {
+      Row w{-1, 0.f};
+      if constexpr (MODE == kStats || MODE == kGrad) {
+        const int64_t row = (int64_t)item_of<MODE>(p.w, q < items ? q : pair).mt * kPairM + rank * LM_BM + r;
+        if (row < p.rows) {
+          w.target = p.target[row];
+          if (w.target == p.ignore_index || w.target >= p.V) w.target = -1;
+          if constexpr (MODE == kGrad) w.lse = p.lse[row];
+        }
+      }
+      return w;
+    };
+    [[maybe_unused]] Row next = row_of(pair);
     for (int q = pair; ok && q < items; q += pairs) {
       const Item im = item_of<MODE>(p.w, q);
       const int64_t grow = (int64_t)im.mt * kPairM + rank * LM_BM + r;
       [[maybe_unused]] const int row0 = (int)grow - lane;                        // the warp's first row
       [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
-      [[maybe_unused]] float shift = 0.f;                // G: 2^(z log2e + shift)
-      [[maybe_unused]] int tgt = -1;
-      if constexpr (MODE == kStats || MODE == kGrad) tgt = target_column(p, grow);
-      if constexpr (MODE == kGrad) shift = tgt >= 0 ? (float)Fmt<T>::g_shift - p.lse[grow] * kLog2e : 0.f;
+      [[maybe_unused]] const int tgt = next.target >= 0 ? (int)next.target : -1;
+      [[maybe_unused]] const float shift = (float)Fmt<T>::g_shift - next.lse * kLog2e;
+      if constexpr (MODE == kStats || MODE == kGrad) next = row_of(q + pairs);
       for (int t = 0; ok && t < im.count; ++t, ++tt) {
         const uint32_t b = tt & 1;
         const bool waited = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[b], (tt >> 1) & 1, abort_flag));
@@ -350,24 +358,24 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
               for (int c = 0; c < 64; ++c) z = tgt - col0 == c ? __uint_as_float(acc[c]) : z;
               p.z_target[grow] = z;
             }
-            float mx = -INFINITY;
+            // four chains each for maximum and sum: two warps a scheduler do not hide the latency of one
+            float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) mx = fmax3(mx, __uint_as_float(acc[c]), __uint_as_float(acc[c + 1]));
+            for (int c = 0; c < 64; c += 2) mq[c >> 1 & 3] = fmax3(mq[c >> 1 & 3], __uint_as_float(acc[c]), __uint_as_float(acc[c + 1]));
+            const float mx = fmax3(fmaxf(mq[0], mq[1]), mq[2], mq[3]);
             const float m_new = fmaxf(m, mx * kLog2e);
             if (m_new > -INFINITY) {
               ssum *= ex2(m - m_new);                    // 2^(-inf) = 0 on the first block
               const uint64_t log2e2 = f2_pack(kLog2e, kLog2e), nm2 = f2_pack(-m_new, -m_new);
-              uint64_t sa = f2_pack(0.f, 0.f), sb = sa;
+              uint64_t sq[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-              for (int c = 0; c < 64; c += 4) {
-                float e0, e1, e2, e3;
+              for (int c = 0; c < 64; c += 2) {
+                float e0, e1;
                 f2_unpack(f2_fma(f2_pack(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1])), log2e2, nm2), e0, e1);
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(acc[c + 2]), __uint_as_float(acc[c + 3])), log2e2, nm2), e2, e3);
-                sa = f2_add(sa, f2_pack(ex2(e0), ex2(e1)));
-                sb = f2_add(sb, f2_pack(ex2(e2), ex2(e3)));
+                sq[c >> 1 & 3] = f2_add(sq[c >> 1 & 3], f2_pack(ex2(e0), ex2(e1)));
               }
               float s0, s1;
-              f2_unpack(f2_add(sa, sb), s0, s1);
+              f2_unpack(f2_add(f2_add(sq[0], sq[1]), f2_add(sq[2], sq[3])), s0, s1);
               ssum += s0 + s1;
               m = m_new;
             } else {                                     // nothing but -inf, or NaN, which fmaxf passes over

@@ -724,7 +724,8 @@ Tensor dense16(const Tensor& t) {
 // [.., d] as [rows, d] with contiguous rows that all start on a multiple of `bytes`
 Tensor rows_on(const Tensor& x, int64_t bytes) {
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  return x2.stride(1) == 1 && aligned_to(x2, bytes) && x2.stride(0) * x2.element_size() % bytes == 0 ? x2 : dense16(x2);
+  const bool in_place = x2.stride(1) == 1 && (x2.size(0) <= 1 || x2.stride(0) >= x2.size(1)) && aligned_to(x2, bytes) && x2.stride(0) * x2.element_size() % bytes == 0;
+  return in_place ? x2 : dense16(x2);                     // a broadcast row among others
 }
 
 Tensor dropout_launch(const Tensor& x_in, const Drop& drop) {
