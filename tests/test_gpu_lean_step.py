@@ -133,3 +133,58 @@ def test_no_logits_are_alive_between_forward_and_backward():
         loss.backward()
         return alive
     assert held(True) <= 1 << 20 and held(False) >= 2 * rows * V
+
+
+class Traced(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.w = torch.nn.Parameter(torch.ones(64, device='cuda'))
+
+    def forward(self, x):
+        b = ulm_ops.swiglu_dropout(x, ulm_ops.dropout(x, 0.3, 1), 0.3, 2)
+        x_new, y = ulm_ops.dropout_add_rms_norm(x, b.half(), self.w, 0.3, 3)
+        return x_new + y
+
+
+def test_traced_ops_run_again_on_other_inputs():
+    m, x = Traced(), torch.randn(24, 64, device='cuda')
+    got, want = torch.jit.trace(m, torch.randn(8, 64, device='cuda'))(x), m(x)
+    assert torch.equal(got, want)
+    a, b = torch.autograd.grad(got.sum(), m.w)[0], torch.autograd.grad(want.sum(), m.w)[0]
+    assert float((a - b).norm()) <= 2.0 ** -11 * float(b.norm())
+
+
+@pytest.mark.parametrize('op', [
+    lambda x: ulm_ops.dropout(x, 0.5, 1),
+    lambda x: ulm_ops.swiglu_dropout(x, x, 0.5, 1),
+    lambda x: ulm_ops.dropout_add_rms_norm(x, torch.ones(4, 64, device='cuda').half(), torch.ones(64, device='cuda'), 0.5, 1)[0],
+    lambda x: ulm_ops.streamed_cross_entropy(x, torch.ones(9, 64, device='cuda'), torch.ones(4, device='cuda', dtype=torch.long), compute_dtype=torch.bfloat16),
+])
+def test_transforms_without_a_rule_are_refused(op):
+    with pytest.raises((RuntimeError, NotImplementedError), match='autograd.Function'):
+        torch.func.grad(lambda x: op(x).sum())(torch.ones(4, 64, device='cuda'))
+
+
+def test_checkpointed_loss_and_saved_tensor_hooks():
+    g = torch.Generator(device='cuda').manual_seed(1)
+    h, w = torch.randn(300, 128, generator=g, device='cuda').half(), torch.randn(500, 128, generator=g, device='cuda').half()
+    t = torch.randint(0, 500, (300,), generator=g, device='cuda')
+
+    def grads(call):
+        a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(call(a, b), [a, b])
+    plain = grads(lambda a, b: ulm_ops.streamed_cross_entropy(a, b, t))
+    again = grads(lambda a, b: torch.utils.checkpoint.checkpoint(ulm_ops.streamed_cross_entropy, a, b, t, use_reentrant=False))
+    with torch.autograd.graph.save_on_cpu():
+        parked = grads(lambda a, b: ulm_ops.streamed_cross_entropy(a, b, t))
+    for other in (again, parked):
+        assert all(torch.equal(x, y) for x, y in zip(other, plain))
+
+
+def test_an_operand_changed_in_place_is_noticed():
+    x, b, w = torch.randn(4, 64, device='cuda', requires_grad=True), torch.randn(4, 64, device='cuda').half(), torch.ones(64, device='cuda', requires_grad=True)
+    x_new, y = ulm_ops.dropout_add_rms_norm(x, b, w, 0.5, 1)
+    with torch.no_grad():
+        x_new.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.float().sum().backward()

@@ -515,10 +515,11 @@ streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restr
     }
     s = warp_sum(s);
     if (lane == 0) {
-      const float l = (m + log2f(s)) * kLn2;
-      lse[r] = l;
+      const float log2_s = log2f(s);
+      lse[r] = (m + log2_s) * kLn2;
       const int64_t t = target[r];
-      loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : l - loss[r];
+      // lse - z_target, with the large parts subtracted first and exactly: their difference is as small as the loss
+      loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : (fmaf(-loss[r], kLog2e, m) + log2_s) * kLn2;
     }
   }
   __threadfence();
