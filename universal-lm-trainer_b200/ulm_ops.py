@@ -1,7 +1,7 @@
-"""RMSNorm, the SwiGLU gate and chunked cross-entropy on the sm_100a library, as autograd ops.
+"""RMSNorm, the SwiGLU gate, dropout and the cross-entropy on the sm_100a library, as autograd ops.
 
 The reference has no custom kernels for these: ``FusedRMSNorm`` calls
-F.rms_norm (train.py:1862-1875) and ``compute_loss`` loops fc_out +
+F.rms_norm (train.py:1862-1875), dropout is nn.Dropout and ``compute_loss`` loops fc_out +
 F.cross_entropy over row chunks (train.py:2059-2082).  The classes and functions
 below keep those names and argument meanings.
 """
