@@ -490,7 +490,9 @@ streamed_ce_join_kernel(const Work w, const Out o) {
 }
 
 // lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry): a
-// warp per row.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
+// warp per row.  The target's logit is formed once more here, by fp32 fused multiply-adds, and takes the place of the tensor
+// core's in the sum and in the difference: their additions round towards zero, some 5e-6 of a logit of 8 at d = 1024, always the
+// same way, so that it stays in the mean (loss against 64 bits, d = 1024: 1.0e-6 -> 0.45e-6).  2 d bytes of H and W a row each.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
 // n = *denom_dev, denom if that is positive, or the number of targets that are not ignore_index (at least 1).
 struct Mean {
   const float* denom_dev;
@@ -498,9 +500,11 @@ struct Mean {
   float *mean, *inv;
   uint32_t* done;                                        // CTAs that have finished: zeroed by the statistics kernel
 };
+struct Operands { const void *h, *w; int64_t h_stride, w_stride; int d; };
+template <typename T>
 __global__ void __launch_bounds__(256)
 streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int n_parts, const int64_t* __restrict__ target,
-                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows, const Mean mean) {
+                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows, const Operands op, const Mean mean) {
   __shared__ double s_sum[8];
   __shared__ int s_n[8];
   __shared__ uint32_t s_before;
@@ -518,12 +522,30 @@ streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restr
       s += mi > -INFINITY ? si * exp2f(mi - m) : si;     // a group of nothing but -inf has the sum 0; of NaN, NaN
     }
     s = warp_sum(s);
+    const int64_t t = target[r];
+    const bool counts = t != ignore_index && t >= 0 && t < V;
+    float z = 0.f;
+    if (counts) {
+      const T *h = static_cast<const T*>(op.h) + r * op.h_stride, *w = static_cast<const T*>(op.w) + t * op.w_stride;
+      float z0 = 0.f, z1 = 0.f;
+      for (int k = lane * 8; k < op.d; k += 256) {
+        const uint4 a = *reinterpret_cast<const uint4*>(h + k), b = *reinterpret_cast<const uint4*>(w + k);
+        const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = Cvt<T>::unpack2(au[j]), y = Cvt<T>::unpack2(bu[j]);
+          z0 = fmaf(x.x, y.x, z0);
+          z1 = fmaf(x.y, y.y, z1);
+        }
+      }
+      z = warp_sum(z0 + z1);
+    }
     if (lane == 0) {
+      if (counts) s += exp2f(fmaf(z, kLog2e, -m)) - exp2f(fmaf(loss[r], kLog2e, -m));
       const float log2_s = log2f(s);
       lse[r] = (m + log2_s) * kLn2;
-      const int64_t t = target[r];
-      // lse - z_target, with the large parts subtracted first and exactly: their difference is as small as the loss
-      loss[r] = t == ignore_index || t < 0 || t >= V ? 0.f : (fmaf(-loss[r], kLog2e, m) + log2_s) * kLn2;
+      // lse - z, with the large parts subtracted first and exactly: their difference is as small as the loss
+      loss[r] = counts ? (fmaf(-z, kLog2e, m) + log2_s) * kLn2 : 0.f;
     }
   }
   __threadfence();
@@ -640,8 +662,9 @@ int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
   cudaStream_t st = (cudaStream_t)a->stream;
   if (int rc = launch<T, kStats>(mh, mw, mh, p, device, st, who)) return rc;
   const Mean mean{a->denom_dev, a->denom, a->mean, a->inv, p.done};
-  return launch_dependent(who, streamed_ce_finish_kernel, (unsigned)((a->rows + 7) / 8), 256, 0, st, p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V,
-                          a->lse, a->loss, a->rows, mean);
+  const Operands op{a->h, a->w, a->h_stride, a->w_stride, a->d};
+  return launch_dependent(who, streamed_ce_finish_kernel<T>, (unsigned)((a->rows + 7) / 8), 256, 0, st, p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V,
+                          a->lse, a->loss, a->rows, op, mean);
 }
 
 // G's workspace: blocks of 64 columns, [block][row][64], so that every box that is stored or loaded is one stretch of memory.

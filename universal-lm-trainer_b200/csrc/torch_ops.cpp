@@ -716,6 +716,8 @@ struct Drop {
 };
 void check_drop(double p, const char* who) { TORCH_CHECK_VALUE(p >= 0 && p <= 1, who, ": p must lie between 0 and 1, got ", p); }
 bool aligned_to(const Tensor& t, int64_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
+// t.to(type) without a way through the dispatcher where nothing is to be done
+Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
 // contiguous and 16-byte aligned
 Tensor dense16(const Tensor& t) {
   const Tensor c = t.contiguous();
@@ -741,7 +743,7 @@ Tensor dropout(const Tensor& x, double p, int64_t seed);
 struct DropoutBwd : OpNode {
   Drop drop;
   at::ScalarType dtype;
-  variable_list backward(variable_list& g, const variable_list&) override { return {dropout_launch(g[0].to(dtype), drop)}; }
+  variable_list backward(variable_list& g, const variable_list&) override { return {dropout_launch(as_type(g[0], dtype), drop)}; }
   // linear in x: the gradient is the op itself, which autograd can differentiate again
   variable_list backward_recorded(variable_list& g, const variable_list&) override { return {::dropout(g[0].to(dtype), drop.p, drop.seed)}; }
 };
@@ -765,10 +767,9 @@ struct DropNormBwd : OpNode {
   variable_list backward(variable_list& g, const variable_list& kept) override {
     const Tensor x = kept[0], w = kept[1], rstd = kept[2];
     const int64_t rows = rstd.size(0), d = w.size(0);
-    auto as = [](const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); };
     // a y that nobody used has the gradient zero
-    const Tensor dy = g[1].defined() ? rows_on(as(g[1], bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
-    const Tensor ga = g[0].defined() ? rows_on(as(g[0], at::kFloat), 16) : Tensor();
+    const Tensor dy = g[1].defined() ? rows_on(as_type(g[1], bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
+    const Tensor ga = g[0].defined() ? rows_on(as_type(g[0], at::kFloat), 16) : Tensor();
     const Tensor dx = empty_cuda(x.sizes(), at::kFloat, x), db = empty_cuda(x.sizes(), bdtype, x), dw = empty_cuda({d}, at::kFloat, x);
     const Tensor partial = empty_cuda({ulm_add_dropout_norm_partial_rows(rows), d}, at::kFloat, x);
     ulm_rmsnorm_bwd_args a{};
@@ -779,7 +780,7 @@ struct DropNormBwd : OpNode {
     if (ga.defined()) { a.g_add = ga.data_ptr(); a.gadd_stride = ga.stride(0); }
     a.d_branch = db.data_ptr(); a.dbranch_stride = d;
     check(ulm_add_dropout_norm_bwd(&a, drop.p, (uint64_t)drop.seed), "dropout_add_rms_norm backward");
-    return {dx, db, as(dw, wdtype)};
+    return {dx, db, as_type(dw, wdtype)};
   }
 };
 
@@ -822,7 +823,7 @@ std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& b
 struct SwigluBwd : OpNode {
   Drop drop;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor a = kept[0], b = kept[1], gy = g[0].to(a.scalar_type()), dy = drop.none() ? gy.contiguous() : dense16(gy);
+    const Tensor a = kept[0], b = kept[1], gy = as_type(g[0], a.scalar_type()), dy = drop.none() ? gy.contiguous() : dense16(gy);
     const Tensor da = empty_cuda(a.sizes(), a.scalar_type(), a), db = empty_cuda(a.sizes(), a.scalar_type(), a);
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), nullptr, dy.data_ptr(), da.data_ptr(), db.data_ptr(), a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
     check(drop.none() ? ulm_swiglu_bwd(&p) : ulm_swiglu_dropout(&p, true, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu backward");
