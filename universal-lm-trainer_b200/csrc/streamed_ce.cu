@@ -132,6 +132,11 @@ struct Params {
   int g_cols;                                            // the workspace's columns
   Out out;                                               // products
   uint32_t* status;
+  // Bytes of A that the CTAs of a pair load per k-block, and of B each; the K16 steps of a k-block.  Where all rows fit one
+  // CTA's half tile, boxes end with them and the other CTA loads no A; an inner dimension of less than one
+  // k-block ends with its last step.  Zeros past a tensor's end cost a load more than data does: 7 rows, forward 25 -> 21 us.
+  uint32_t a_bytes[2], b_bytes;
+  int k_steps;
 };
 
 __device__ __forceinline__ float out_factor(const Out& o) { return *o.factor_dev * (o.factor2_dev ? *o.factor2_dev : 1.f) * o.factor; }
@@ -240,15 +245,14 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             uint8_t* a = stages + (size_t)s * kStage;
             uint8_t* b = a + kATile;
             const int k0 = kb * LM_BK;
-            if (rank == 0) mbar_expect_tx(&ctl->full[s], 2 * kStage);
+            if (rank == 0) mbar_expect_tx(&ctl->full[s], p.a_bytes[0] + p.a_bytes[1] + 2 * p.b_bytes);
             const uint32_t full = peer_smem(&ctl->full[s], 0);
             if constexpr (kAmn) {
 #pragma unroll
               for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, &tmA, full, 0, k0, (m0 >> 6) + i, 0);
-            } else if constexpr (MODE == kRowGrad) {
-              tma_load_4d_pair(a, &tmA, full, 0, m0, kb, 0);
-            } else {
-              tma_load_4d_pair(a, &tmA, full, k0, m0, 0, 0);
+            } else if (p.a_bytes[rank]) {
+              if constexpr (MODE == kRowGrad) tma_load_4d_pair(a, &tmA, full, 0, m0, kb, 0);
+              else tma_load_4d_pair(a, &tmA, full, k0, m0, 0, 0);
             }
             // W's rows are vocabulary columns, counted from the piece's first
             if constexpr (kBmn) {
@@ -290,7 +294,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint64_t db = kBmn ? make_sdesc_sw128_mn(sa + kATile, kAtom) : make_sdesc_sw128(sa + kATile);
 #pragma unroll
             for (int kk = 0; kk < LM_BK / 16; ++kk)
-              mma_ss_pair(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
+              if (MODE != kColGrad || kk < p.k_steps) mma_ss_pair(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
             mma_commit_pair(&ctl->empty[s]);             // the stage is free in both CTAs once these MMAs have read it
           }
           if (ok) mma_commit_pair(&ctl->acc_full[b]);
@@ -466,16 +470,16 @@ streamed_ce_join_kernel(const Work w, const Out o) {
   const int col = nt * LM_BN + c;
   if (row >= o.rows || col >= o.cols) return;
   const float* s = o.slots + (int64_t)j * w.split * kSlot + r * LM_BN + c;
+  const float factor = out_factor(o);
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < w.split; ++k, s += kSlot) {
     const float4 a = *reinterpret_cast<const float4*>(s), b = *reinterpret_cast<const float4*>(s + 4);
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
     v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
   }
-  const float factor = out_factor(o);
   const int64_t at = row * o.ld + col;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = factor * v[i] + (o.prev ? o.prev[at + i] : 0.f);
@@ -513,17 +517,20 @@ streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restr
   const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (r < rows) {
-    float m = -INFINITY;
-    for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, part_m[r * n_parts + i]);
-    m = warp_max(m);
-    float s = 0.f;
-    for (int i = lane; i < n_parts; i += 32) {
-      const float mi = part_m[r * n_parts + i], si = part_s[r * n_parts + i];
-      s += mi > -INFINITY ? si * exp2f(mi - m) : si;     // a group of nothing but -inf has the sum 0; of NaN, NaN
-    }
-    s = warp_sum(s);
     const int64_t t = target[r];
+    const float z_tensor = loss[r];
     const bool counts = t != ignore_index && t >= 0 && t < V;
+    float m = -INFINITY, s = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < n_parts; i += 32) {
+      const float mi = part_m[r * n_parts + i], si = part_s[r * n_parts + i], mn = fmaxf(m, mi);
+      // a group of nothing but -inf has the sum 0; of NaN, NaN
+      s = (m > -INFINITY ? s * exp2f(m - mn) : s) + (mi > -INFINITY ? si * exp2f(mi - mn) : si);
+      m = mn;
+    }
+    const float lane_m = m;
+    m = warp_max(m);
+    s = warp_sum(lane_m > -INFINITY ? s * exp2f(lane_m - m) : s);
     float z = 0.f;
     if (counts) {
       const T *h = static_cast<const T*>(op.h) + r * op.h_stride, *w = static_cast<const T*>(op.w) + t * op.w_stride;
@@ -541,7 +548,7 @@ streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restr
       z = warp_sum(z0 + z1);
     }
     if (lane == 0) {
-      if (counts) s += exp2f(fmaf(z, kLog2e, -m)) - exp2f(fmaf(loss[r], kLog2e, -m));
+      if (counts) s += exp2f(fmaf(z, kLog2e, -m)) - exp2f(fmaf(z_tensor, kLog2e, -m));
       const float log2_s = log2f(s);
       lse[r] = (m + log2_s) * kLn2;
       // lse - z, with the large parts subtracted first and exactly: their difference is as small as the loss
@@ -634,6 +641,17 @@ int check_args(const ulm_streamed_ce_args* a, const char* who) {
 }
 bool ok_out(const void* p, int64_t stride, int d) { return !(reinterpret_cast<uintptr_t>(p) & 15) && stride % 8 == 0 && stride >= d; }
 
+// rows of a box of A where A's rows are the tensor's: all there are, if they fit
+int a_box(int64_t rows) { return rows < LM_BM ? (int)(rows + 7) / 8 * 8 : LM_BM; }
+// K16 steps of dW's k-blocks, which go over the rows
+int col_steps(int64_t rows) { return rows < LM_BK ? (int)(rows + 15) / 16 : LM_BK / 16; }
+void set_bytes(Params& p, bool col_grad) {
+  p.k_steps = col_grad ? col_steps(p.rows) : LM_BK / 16;
+  p.a_bytes[0] = col_grad ? kATile / 4 * p.k_steps : (uint32_t)a_box(p.rows) * LM_BK * 2;
+  p.a_bytes[1] = !col_grad && p.rows <= LM_BM ? 0u : p.a_bytes[0];
+  p.b_bytes = col_grad ? kBTile / 4 * p.k_steps : kBTile;
+}
+
 Params common_params(const ulm_streamed_ce_args* a) {
   Params p{};
   p.rows = a->rows; p.V = a->V; p.target = a->target; p.ignore_index = a->ignore_index; p.status = a->status_dev;
@@ -652,9 +670,10 @@ Work stats_work(int64_t rows, int V, int d) {
 template <typename T>
 int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
   CUtensorMap mh, mw;
-  if (int rc = encode_matrix_map(&mh, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who)) return rc;
+  if (int rc = encode_matrix_map(&mh, a->h, a->dtype, a->rows, a->d, a->h_stride, a_box(a->rows), who)) return rc;
   if (int rc = encode_matrix_map(&mw, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who)) return rc;
   Params p = common_params(a);
+  set_bytes(p, false);
   p.w = stats_work(a->rows, a->V, a->d);
   const int parts = 2 * ((p.w.n_nt + p.w.group - 1) / p.w.group);
   p.part_m = a->scratch; p.part_s = a->scratch + a->rows * parts; p.z_target = a->loss;
@@ -676,8 +695,8 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
   cudaStream_t st = (cudaStream_t)a->stream;
   CUtensorMap h_rows, h_mn, w_rows, w_mn;                // K-major and MN-major boxes of both
   int rc;
-  if ((rc = encode_matrix_map(&h_rows, a->h, a->dtype, a->rows, a->d, a->h_stride, LM_BM, who))) return rc;
-  if ((rc = encode_matrix_map(&h_mn, a->h, a->dtype, a->rows, a->d, a->h_stride, 64, who))) return rc;
+  if ((rc = encode_matrix_map(&h_rows, a->h, a->dtype, a->rows, a->d, a->h_stride, a_box(a->rows), who))) return rc;
+  if ((rc = encode_matrix_map(&h_mn, a->h, a->dtype, a->rows, a->d, a->h_stride, 16 * col_steps(a->rows), who))) return rc;
   if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who))) return rc;
   if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
   for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
@@ -686,9 +705,10 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
     auto g_map = [&](CUtensorMap* m, int box_rows) {
       return encode_bhsd_map(m, g->workspace, a->dtype, 1, (int)g_blocks(n), (int)a->rows, 0, a->rows * 64, 64, box_rows, who);
     };
-    if ((rc = g_map(&g_rows, LM_BM)) || (rc = g_map(&g_mn, 64)) || (rc = g_map(&g_out, 32))) return rc;
+    if ((rc = g_map(&g_rows, a_box(a->rows))) || (rc = g_map(&g_mn, 16 * col_steps(a->rows))) || (rc = g_map(&g_out, 32))) return rc;
     Params p = common_params(a);
     p.v0 = (int)v0;
+    set_bytes(p, false);
     p.lse = a->lse;
     p.g_cols = (int)g_blocks(n) * 64;
     p.w = stats_work(a->rows, (int)n, a->d);
@@ -700,6 +720,7 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
     p.out.cols = a->d;
     if (g->dw) {
       p.w = product_work(n, a->d, a->rows);
+      set_bytes(p, true);
       p.out.ld = g->dw_stride; p.out.rows = n; p.out.is_f32 = g->dw_f32;
       p.out.out = g->dw_f32 ? (void*)((float*)g->dw + v0 * g->dw_stride) : (void*)((T*)g->dw + v0 * g->dw_stride);
       p.out.prev = g->dw_add ? (const float*)p.out.out : nullptr;
@@ -708,6 +729,7 @@ int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int 
     if (g->dh) {
       const bool first = v0 == 0, last = v0 + n >= a->V;
       p.w = product_work(a->rows, a->d, n);
+      set_bytes(p, false);
       p.out.rows = a->rows;
       p.out.is_f32 = !last;
       p.out.out = last ? g->dh : (void*)g->dh_sum;
