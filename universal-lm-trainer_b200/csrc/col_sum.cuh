@@ -12,6 +12,7 @@ namespace {
 __global__ void __launch_bounds__(1024)
 col_sum_kernel(const float* __restrict__ partial, float* __restrict__ dw, int nparts, int d) {
   __shared__ float sub[32][33];
+  grid_dependency_wait();                                // at once where the launch is an ordinary one
   const int c = blockIdx.x * 32 + threadIdx.x;
   float t = 0.f;
   if (c < d)

@@ -29,6 +29,8 @@ __global__ void __launch_bounds__(kThreads)
 dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t nvec, int64_t n, const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsDrop<T>;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
+  grid_dependents_go();
+  grid_dependency_wait();
   uint4 rx[K];
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -73,6 +75,8 @@ gate_dropout_fwd_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __r
                         const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsGate;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
+  grid_dependents_go();
+  grid_dependency_wait();
   uint4 ra[K], rb[K];
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -108,6 +112,8 @@ gate_dropout_bwd_kernel(const T* __restrict__ a, const T* __restrict__ b, const 
                         int64_t nvec, int64_t n, const Rows rw, const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsGate;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
+  grid_dependents_go();
+  grid_dependency_wait();
   uint4 ra[K], rb[K], rg[K];
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -159,17 +165,15 @@ int check_drop(int dtype, int64_t n, double p, const char* who) {
 }
 
 template <typename T>
-void gate_launch(const ulm_swiglu_args* p, bool bwd, int64_t d, int64_t stride, const DropMask& mask) {
+int gate_launch(const ulm_swiglu_args* p, bool bwd, int64_t d, int64_t stride, const DropMask& mask, const char* who) {
   cudaStream_t st = (cudaStream_t)p->stream;
   const int64_t nvec = p->n / VecN<T>::N;
   const Rows rw{(uint32_t)(d / VecN<T>::N), stride / VecN<T>::N};
   const T *a = (const T*)p->a, *b = (const T*)p->b, *dy = (const T*)p->dy;
   T *y = (T*)p->y, *da = (T*)p->da, *db = (T*)p->db;
   const unsigned grid = grid_for(nvec, kVecsGate);
-  if (bwd && d) gate_dropout_bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a, b, dy, da, db, nvec, p->n, rw, mask);
-  else if (bwd) gate_dropout_bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a, b, dy, da, db, nvec, p->n, rw, mask);
-  else if (d) gate_dropout_fwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a, b, y, nvec, p->n, rw, mask);
-  else gate_dropout_fwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a, b, y, nvec, p->n, rw, mask);
+  if (bwd) return launch_dependent(who, d ? gate_dropout_bwd_kernel<T, true> : gate_dropout_bwd_kernel<T, false>, grid, kThreads, 0, st, a, b, dy, da, db, nvec, p->n, rw, mask);
+  return launch_dependent(who, d ? gate_dropout_fwd_kernel<T, true> : gate_dropout_fwd_kernel<T, false>, grid, kThreads, 0, st, a, b, y, nvec, p->n, rw, mask);
 }
 
 }  // namespace
@@ -186,10 +190,9 @@ extern "C" int ulm_dropout(const void* x, void* y, int64_t n, int32_t dtype, dou
   auto go = [&](auto t) {
     using T = decltype(t);
     const int64_t nvec = n / VecN<T>::N;
-    dropout_kernel<T><<<grid_for(nvec, kVecsDrop<T>), kThreads, 0, st>>>((const T*)x, (T*)y, nvec, n, mask);
+    return launch_dependent(who, dropout_kernel<T>, grid_for(nvec, kVecsDrop<T>), kThreads, 0, st, (const T*)x, (T*)y, nvec, n, mask);
   };
-  if (dtype == ULM_F16) go(__half()); else if (dtype == ULM_BF16) go(__nv_bfloat16()); else go(float());
-  return check_launch(who);
+  return dtype == ULM_F16 ? go(__half()) : dtype == ULM_BF16 ? go(__nv_bfloat16()) : go(float());
 }
 
 extern "C" int ulm_swiglu_dropout(const ulm_swiglu_args* a, int32_t backward, int64_t d, int64_t row_stride, double p, uint64_t seed) {
@@ -206,8 +209,7 @@ extern "C" int ulm_swiglu_dropout(const ulm_swiglu_args* a, int32_t backward, in
   if (!aligned16(a->a) || !aligned16(a->b) || (backward ? !aligned16(a->dy) || !aligned16(a->da) || !aligned16(a->db) : !aligned16(a->y)))
     return fail(ULM_ERR_ARG, "%s: %s must be non-null and 16-byte aligned", who, backward ? "a, b, dy, da, db" : "a, b, y");
   const DropMask mask = make_drop_mask(p, seed);
-  if (a->dtype == ULM_F16) gate_launch<__half>(a, backward, d, row_stride, mask);
-  else if (a->dtype == ULM_BF16) gate_launch<__nv_bfloat16>(a, backward, d, row_stride, mask);
-  else gate_launch<float>(a, backward, d, row_stride, mask);
-  return check_launch(who);
+  if (a->dtype == ULM_F16) return gate_launch<__half>(a, backward, d, row_stride, mask, who);
+  if (a->dtype == ULM_BF16) return gate_launch<__nv_bfloat16>(a, backward, d, row_stride, mask, who);
+  return gate_launch<float>(a, backward, d, row_stride, mask, who);
 }

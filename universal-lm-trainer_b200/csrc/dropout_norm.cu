@@ -84,6 +84,8 @@ template <typename TY, int E, int NV>
 __global__ void __launch_bounds__(kFwdWarps * 32, NV * E <= 24 ? 4 : 3)
 add_dropout_norm_fwd_kernel(const FwdParams p, const __grid_constant__ DropMask mask) {
   __shared__ float slots[2][kFwdWarps];
+  grid_dependents_go();
+  grid_dependency_wait();
   const TY* __restrict__ br = static_cast<const TY*>(p.branch);
   TY* __restrict__ y = static_cast<TY*>(p.y);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
@@ -146,6 +148,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == kBwdWideWarps ? 1 : 2)
 add_dropout_norm_bwd_kernel(const BwdParams p, const __grid_constant__ DropMask mask) {
   extern __shared__ float s_dw[];                        // [groups][d]
   __shared__ float slots[2][WARPS];
+  grid_dependents_go();
+  grid_dependency_wait();
   const TY* __restrict__ dy = static_cast<const TY*>(p.dy);
   TY* __restrict__ db = static_cast<TY*>(p.d_branch);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
@@ -268,46 +272,36 @@ int check_shape(const char* who, int x_dtype, int w_dtype, int kind, int d, int6
 }
 
 template <typename TY>
-void launch_fwd(FwdParams p, int E, const DropMask& mask, cudaStream_t st) {
+int launch_fwd(FwdParams p, int E, const DropMask& mask, cudaStream_t st, const char* who) {
   const int nvec = p.d / E, nv = fwd_nv(nvec, E);
   const Split s = split_rows(p.rows, nvec, nv, kFwdWarps);
   p.W = s.W;
   int64_t blocks = (p.rows + s.groups - 1) / s.groups;
   if (blocks > 64 * kNumSMs) blocks = 64 * kNumSMs;
   const int threads = s.W * s.groups * 32;
-  auto go = [&](auto kern) { kern<<<(unsigned)blocks, threads, 0, st>>>(p, mask); };
-  if (E == 8) {
-    if (nv == 1) go(add_dropout_norm_fwd_kernel<TY, 8, 1>);
-    else if (nv == 2) go(add_dropout_norm_fwd_kernel<TY, 8, 2>);
-    else if (nv == 3) go(add_dropout_norm_fwd_kernel<TY, 8, 3>);
-    else go(add_dropout_norm_fwd_kernel<TY, 8, 4>);
-  } else {
-    if (nv <= 2) go(add_dropout_norm_fwd_kernel<TY, 4, 2>);
-    else if (nv <= 4) go(add_dropout_norm_fwd_kernel<TY, 4, 4>);
-    else go(add_dropout_norm_fwd_kernel<TY, 4, 8>);
-  }
+  auto go = [&](auto kern) { return launch_dependent(who, kern, (unsigned)blocks, threads, 0, st, p, mask); };
+  if (E == 8)
+    return nv == 1 ? go(add_dropout_norm_fwd_kernel<TY, 8, 1>) : nv == 2 ? go(add_dropout_norm_fwd_kernel<TY, 8, 2>)
+         : nv == 3 ? go(add_dropout_norm_fwd_kernel<TY, 8, 3>) : go(add_dropout_norm_fwd_kernel<TY, 8, 4>);
+  return nv <= 2 ? go(add_dropout_norm_fwd_kernel<TY, 4, 2>) : nv <= 4 ? go(add_dropout_norm_fwd_kernel<TY, 4, 4>) : go(add_dropout_norm_fwd_kernel<TY, 4, 8>);
 }
 
 template <typename TY>
-int64_t launch_bwd(BwdParams p, int E, const DropMask& mask, cudaStream_t st) {
+int launch_bwd(BwdParams p, int E, const DropMask& mask, int64_t* parts, cudaStream_t st, const char* who) {
   const int nvec = p.d / E, nv = bwd_nv(p.d, E);
   const Split s = split_rows(p.rows, nvec, nv, kBwdWarps);
   p.W = s.W;
   const int64_t blocks = bwd_blocks(p.rows, s);
   const int threads = s.W * s.groups * 32;
   const size_t smem = (size_t)s.groups * p.d * sizeof(float);            // at most 12 x 512 floats: below 48 KB
-  auto go = [&](auto kern) { kern<<<(unsigned)blocks, threads, smem, st>>>(p, mask); };
+  *parts = blocks;
+  auto go = [&](auto kern) { return launch_dependent(who, kern, (unsigned)blocks, threads, smem, st, p, mask); };
   const bool wide = s.W > kBwdWarps;
-  if (E == 8) {
-    if (nv == 1) go(add_dropout_norm_bwd_kernel<TY, 8, 1, kBwdWarps>);
-    else if (wide) go(add_dropout_norm_bwd_kernel<TY, 8, 2, kBwdWideWarps>);
-    else go(add_dropout_norm_bwd_kernel<TY, 8, 2, kBwdWarps>);
-  } else {
-    if (nv == 2) go(add_dropout_norm_bwd_kernel<TY, 4, 2, kBwdWarps>);
-    else if (wide) go(add_dropout_norm_bwd_kernel<TY, 4, 4, kBwdWideWarps>);
-    else go(add_dropout_norm_bwd_kernel<TY, 4, 4, kBwdWarps>);
-  }
-  return blocks;
+  if (E == 8)
+    return nv == 1 ? go(add_dropout_norm_bwd_kernel<TY, 8, 1, kBwdWarps>)
+         : wide ? go(add_dropout_norm_bwd_kernel<TY, 8, 2, kBwdWideWarps>) : go(add_dropout_norm_bwd_kernel<TY, 8, 2, kBwdWarps>);
+  return nv == 2 ? go(add_dropout_norm_bwd_kernel<TY, 4, 2, kBwdWarps>)
+       : wide ? go(add_dropout_norm_bwd_kernel<TY, 4, 4, kBwdWideWarps>) : go(add_dropout_norm_bwd_kernel<TY, 4, 4, kBwdWarps>);
 }
 
 }  // namespace
@@ -326,9 +320,8 @@ extern "C" int ulm_add_dropout_norm_fwd(const ulm_rmsnorm_fwd_args* a, double p,
   const FwdParams q{(const float*)a->x, a->branch, (const float*)a->w, (float*)a->x_out, a->y, a->rstd,
                     a->x_stride, a->branch_stride, a->xout_stride, a->y_stride, a->rows, a->d, 1, a->eps};
   const DropMask mask = make_drop_mask(p, seed);
-  if (a->y_kind == ULM_Y_F16) launch_fwd<__half>(q, E, mask, (cudaStream_t)a->stream);
-  else launch_fwd<__nv_bfloat16>(q, E, mask, (cudaStream_t)a->stream);
-  return check_launch(who);
+  cudaStream_t st = (cudaStream_t)a->stream;
+  return a->y_kind == ULM_Y_F16 ? launch_fwd<__half>(q, E, mask, st, who) : launch_fwd<__nv_bfloat16>(q, E, mask, st, who);
 }
 
 // one CTA a row, or as many as run at a time
@@ -354,9 +347,7 @@ extern "C" int ulm_add_dropout_norm_bwd(const ulm_rmsnorm_bwd_args* a, double p,
     const BwdParams q{(const float*)a->x, (const float*)a->w, a->dy, a->rstd, (const float*)a->g_add, (float*)a->dx, a->d_branch, a->partial,
                       a->x_stride, a->dy_stride, a->gadd_stride, a->dx_stride, a->dbranch_stride, a->rows, a->d, 1};
     const DropMask mask = make_drop_mask(p, seed);
-    blocks = a->dy_kind == ULM_Y_F16 ? launch_bwd<__half>(q, E, mask, st) : launch_bwd<__nv_bfloat16>(q, E, mask, st);
-    if (int rc = check_launch(who)) return rc;
+    if (int rc = a->dy_kind == ULM_Y_F16 ? launch_bwd<__half>(q, E, mask, &blocks, st, who) : launch_bwd<__nv_bfloat16>(q, E, mask, &blocks, st, who)) return rc;
   }
-  col_sum_kernel<<<(a->d + 31) / 32, dim3(32, 32), 0, st>>>(a->partial, a->dw, (int)blocks, a->d);
-  return check_launch(who);
+  return launch_dependent(who, col_sum_kernel, (a->d + 31) / 32, dim3(32, 32), 0, st, a->partial, a->dw, (int)blocks, a->d);
 }
