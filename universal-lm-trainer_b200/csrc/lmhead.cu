@@ -51,6 +51,19 @@ static_assert(kLmSmem <= 227 * 1024, "shared memory");
 template <typename T> struct LmFmt { static constexpr int v = 0; };
 template <> struct LmFmt<__nv_bfloat16> { static constexpr int v = 1; };
 
+// Barrier over the 128 threads of one column half (ids 1, 2) whose OR-reduction tells every one of them
+// whether any of them (or another role of the CTA) has given up.
+__device__ __forceinline__ bool half_sync_any(int half, bool fail) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(any) : "r"((uint32_t)fail), "r"(half + 1) : "memory");
+  return any != 0;
+}
+
 // TOP1 (scoring): instead of storing the logits the epilogue picks out what a score needs of them, the target's logit
 // (into z_target) and the column of the largest one (part_i, the lowest on ties; ~column of the first NaN if there is one).
 struct LmTop1 {

@@ -9,7 +9,7 @@ namespace {
 constexpr int LM_BM = 128, LM_BN = 256, LM_BK = 64;
 constexpr int kLmGroupTiles = 25;                      // column tiles per work item (upper bound)
 
-// Column tiles per work item: the count whose rounds of items over the SMs take the fewest tile times, an item's own
+// Column tiles per work item: the count whose rounds of items over the workers (SMs, or pairs of them) take the fewest tile times, an item's own
 // cost (pipeline fill, statistics) being worth about a quarter of a tile.  At 32768 x 32000 that is 5 (220 tile times,
 // 216 ideal; the fixed 25 of before took 225); with 2048 rows x 4096 columns, 1 instead of 16: 256 items on 148 SMs
 // where 16 SMs had one each.

@@ -362,8 +362,10 @@ def streamed_cross_entropy(hidden, weight, target, ignore_index=0, compute_dtype
     if hidden.shape[0] == 0:
         return torch.zeros((), device=hidden.device, requires_grad=True)
     target = target.contiguous()
-    return _divided(lambda dev, host: N.ext().streamed_cross_entropy(hidden, weight, target, int(ignore_index), compute_dtype, dev, host, int(PIECE_BYTES)),
-                    denominator, hidden)
+
+    def loss_over(dev, host):
+        return N.ext().streamed_cross_entropy(hidden, weight, target, int(ignore_index), compute_dtype, dev, host, int(PIECE_BYTES))
+    return loss_over(None, 0.0) if denominator is None else _divided(loss_over, denominator, hidden)
 
 
 def token_targets(ids, labels, padded, ignore_index):
