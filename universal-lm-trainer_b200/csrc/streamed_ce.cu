@@ -495,8 +495,8 @@ streamed_ce_join_kernel(const Work w, const Out o) {
 
 // lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry): a
 // warp per row.  The target's logit is formed once more here, by fp32 fused multiply-adds, and takes the place of the tensor
-// core's in the sum and in the difference: their additions round towards zero, some 5e-6 of a logit of 8 at d = 1024, always the
-// same way, so that it stays in the mean (loss against 64 bits, d = 1024: 1.0e-6 -> 0.45e-6).  2 d bytes of H and W a row each.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
+// core's in the sum and in the difference: their additions round towards zero, 1e-6 of a logit at d = 1024 (-1.8e-5 +- 0.3e-5 at
+// 17, -0.3e-5 at d = 128), which stays in the mean (loss against 64 bits, d = 1024: 1.0e-6 -> 0.45e-6).  2 d bytes of H and W a row.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
 // n = *denom_dev, denom if that is positive, or the number of targets that are not ignore_index (at least 1).
 struct Mean {
   const float* denom_dev;
