@@ -80,7 +80,8 @@ def dropout(x, p, seed):
     """Inverted dropout of a CUDA fp16/bf16/fp32 tensor: each element is zero with probability ``p`` (in steps of 2^-16) and
     otherwise divided by the share that stays.  Which ones are dropped is a function of ``seed`` (any 64-bit integer) and of the
     element's row-major index alone (`Philox4x32`, include/ulm_b200.h says how), so nothing is kept for the backward: it forms
-    the mask again.  The same seed drops the same elements of another tensor of that size."""
+    the mask again.  The same seed drops the same elements of another tensor of that size; a captured graph replays the masks
+    of the seeds it was captured with."""
     return N.ext().dropout(x, float(p), _as_i64(seed))
 
 
