@@ -34,7 +34,8 @@ namespace {
 
 using namespace tc;
 
-enum Mode { kStats, kGrad, kRowGrad, kColGrad };         // statistics; G; dH = G W; dW = G^T H
+enum Mode { kStats, kGrad, kProducts };                  // statistics; G; dW = G^T H and dH = G W
+enum Product { kColGrad, kRowGrad, kNumProducts };       // dW, dH
 
 constexpr int kPairM = 2 * LM_BM;                         // rows of a pair's output tile
 constexpr int kPairs = kNumSMs / 2;
@@ -68,45 +69,16 @@ static_assert(smem_bytes(kGrad) <= 227 * 1024, "shared memory");
 // One launch's work.  Items are numbered and dealt round the CTAs.
 //   statistics: 128 rows x a group of column tiles, whose statistics stay in registers;
 //   G: one tile each, rows fastest, so that all CTAs read one stretch of W;
-//   products: `whole` tiles, then the `rest` tiles that would not fill a round of the SMs, cut into `split` stretches of the inner
-//   dimension each; every stretch leaves its fp32 tile in a slot, and a second kernel adds up a tile's slots in order.
+//   products: dW's and dH's `whole` tiles, then of each the `rest` that would not fill a round of the SMs, cut into `split`
+//   stretches of the inner dimension; every stretch leaves its fp32 tile in a slot, and a second kernel adds up a tile's slots
+//   in order.  Both products in one launch: one set-up and one drain less, and a launch or two of
+//   the host's time (forward and backward, replayed as a graph: 7 x 768 x 32000 72 -> 69.5 us, x 2560 40 -> 32; the largest calls 0.5 %
+//   slower).
 struct Work {
   int n_mt, n_nt, n_kb, group;
   int whole, rest, split;
 };
-struct Item { int mt, nt, count, kb0, kb1, slot; };
-
-template <int MODE>
-__host__ __device__ inline int n_items(const Work& w) {
-  if (MODE == kStats) return w.n_mt * ((w.n_nt + w.group - 1) / w.group);
-  if (MODE == kGrad) return w.n_mt * w.n_nt;
-  return w.whole + w.rest * w.split;
-}
-template <int MODE>
-__device__ __forceinline__ Item item_of(const Work& w, int q) {
-  Item it{0, 0, 1, 0, w.n_kb, -1};
-  if constexpr (MODE == kStats) {
-    const int g = q / w.n_mt;
-    it.mt = q - g * w.n_mt;
-    it.nt = g * w.group;
-    it.count = min(w.group, w.n_nt - it.nt);
-  } else if constexpr (MODE == kGrad) {
-    it.nt = q / w.n_mt;
-    it.mt = q - it.nt * w.n_mt;
-  } else {
-    int t = q;
-    if (q >= w.whole) {
-      const int part = q - w.whole, s = part / w.rest, j = part - s * w.rest;
-      t = w.whole + j;
-      it.kb0 = (int)((int64_t)w.n_kb * s / w.split);
-      it.kb1 = (int)((int64_t)w.n_kb * (s + 1) / w.split);
-      if (w.split > 1) it.slot = j * w.split + s;
-    }
-    it.mt = t / w.n_nt;                                  // the column tiles of one row tile side by side: they share its A panel in L2
-    it.nt = t - it.mt * w.n_nt;
-  }
-  return it;
-}
+struct Item { int mt, nt, count, kb0, kb1, slot, product; };
 
 // How the accumulators leave: out = factor * acc (+ prev).  A whole tile goes through shared memory and a TMA store, or where an
 // fp32 out is its own prev a TMA addition (one to each element: no order to depend on); where a 16-bit out adds an fp32 prev,
@@ -120,8 +92,25 @@ struct Out {
   int cols, is_f32;
   float* slots;
 };
+// Bytes of A that the CTAs of a pair load per k-block, and of B each; the K16 steps of a k-block.  Where all rows fit one CTA's
+// half tile, boxes end with them and the other CTA loads no A; an inner dimension of less than one k-block ends with its
+// last step.  Zeros past a tensor's end cost a load more than data does: 7 rows, forward 25 -> 21 us.
+struct Load {
+  uint32_t a_bytes[2], b_bytes;
+  int k_steps;
+};
+struct Products {
+  Work w[kNumProducts];
+  Out out[kNumProducts];
+  Load load[kNumProducts];
+  int slot0[kNumProducts];
+};
+// A and B, of the second product too; what is written; the slots
+struct alignas(64) Maps { CUtensorMap a[kNumProducts], b[kNumProducts], out[kNumProducts], slots; };
+
 struct Params {
-  Work w;
+  Work w;                                                // statistics and G
+  Load load;
   int64_t rows;
   int V, v0;                                             // vocabulary; first column of the piece
   const int64_t* target;
@@ -130,14 +119,55 @@ struct Params {
   uint32_t* done;
   const float* lse;                                      // G
   int g_cols;                                            // the workspace's columns
-  Out out;                                               // products
+  Products products;
   uint32_t* status;
-  // Bytes of A that the CTAs of a pair load per k-block, and of B each; the K16 steps of a k-block.  Where all rows fit one
-  // CTA's half tile, boxes end with them and the other CTA loads no A; an inner dimension of less than one
-  // k-block ends with its last step.  Zeros past a tensor's end cost a load more than data does: 7 rows, forward 25 -> 21 us.
-  uint32_t a_bytes[2], b_bytes;
-  int k_steps;
 };
+
+template <int MODE>
+__host__ __device__ inline int n_items(const Params& p) {
+  if (MODE == kStats) return p.w.n_mt * ((p.w.n_nt + p.w.group - 1) / p.w.group);
+  if (MODE == kGrad) return p.w.n_mt * p.w.n_nt;
+  const Work *c = &p.products.w[kColGrad], *r = &p.products.w[kRowGrad];
+  return c->whole + r->whole + c->rest * c->split + r->rest * r->split;
+}
+template <int MODE>
+__device__ __forceinline__ Item item_of(const Params& p, int q) {
+  Item it{0, 0, 1, 0, p.w.n_kb, -1, 0};
+  if constexpr (MODE == kStats) {
+    const int g = q / p.w.n_mt;
+    it.mt = q - g * p.w.n_mt;
+    it.nt = g * p.w.group;
+    it.count = min(p.w.group, p.w.n_nt - it.nt);
+  } else if constexpr (MODE == kGrad) {
+    it.nt = q / p.w.n_mt;
+    it.mt = q - it.nt * p.w.n_mt;
+  } else {
+    const Work *c = &p.products.w[kColGrad], *r = &p.products.w[kRowGrad];
+    int part = -1;
+    if (q >= c->whole) {
+      q -= c->whole;
+      it.product = kRowGrad;
+      if (q >= r->whole) {
+        part = q - r->whole;
+        if (part < c->rest * c->split) it.product = kColGrad;
+        else part -= c->rest * c->split;
+      }
+    }
+    const Work& w = p.products.w[it.product];
+    int t = q;
+    it.kb1 = w.n_kb;
+    if (part >= 0) {
+      const int s = part / w.rest, j = part - s * w.rest;
+      t = w.whole + j;
+      it.kb0 = (int)((int64_t)w.n_kb * s / w.split);
+      it.kb1 = (int)((int64_t)w.n_kb * (s + 1) / w.split);
+      if (w.split > 1) it.slot = p.products.slot0[it.product] + j * w.split + s;
+    }
+    it.mt = t / w.n_nt;                                  // the column tiles of one row tile side by side: they share its A panel in L2
+    it.nt = t - it.mt * w.n_nt;
+  }
+  return it;
+}
 
 __device__ __forceinline__ float out_factor(const Out& o) { return *o.factor_dev * (o.factor2_dev ? *o.factor2_dev : 1.f) * o.factor; }
 
@@ -191,9 +221,8 @@ __device__ __forceinline__ void add_and_round(const Out& o, float factor, int64_
 
 template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut,
-                   const __grid_constant__ CUtensorMap tmSlots, const __grid_constant__ Params p) {
-  constexpr bool kAmn = MODE == kColGrad, kBmn = MODE == kRowGrad || MODE == kColGrad;
+streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  constexpr bool kBmn = MODE == kProducts;               // and A too in dW
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stages = base;                                             // [stage][A tile | B tile]
@@ -202,7 +231,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   volatile int* abort_flag = &ctl->abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int items = n_items<MODE>(p.w);
+  const int items = n_items<MODE>(p);
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
@@ -228,11 +257,14 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == kEpiWarps) {
     // ---------------- TMA producer ----------------
     if (elect_one()) {
-      tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB);
+      for (int i = 0; i < (MODE == kProducts ? (int)kNumProducts : 1); ++i)
+        if (MODE != kProducts || p.products.w[i].n_kb) { tma_prefetch_desc(&maps.a[i]); tma_prefetch_desc(&maps.b[i]); }
       uint32_t it = 0;                                   // k-blocks issued so far, over all tiles
       bool ok = true;
       for (int q = pair; ok && q < items; q += pairs) {
-        const Item im = item_of<MODE>(p.w, q);
+        const Item im = item_of<MODE>(p, q);
+        const Load& load = MODE == kProducts ? p.products.load[im.product] : p.load;
+        const CUtensorMap *tmA = &maps.a[im.product], *tmB = &maps.b[im.product];
         for (int t = 0; ok && t < im.count; ++t) {
           const int m0 = im.mt * kPairM + (int)rank * LM_BM, n0 = (im.nt + t) * LM_BN + (int)rank * kBRows;
           for (int kb = im.kb0; kb < im.kb1; ++kb, ++it) {
@@ -245,21 +277,22 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             uint8_t* a = stages + (size_t)s * kStage;
             uint8_t* b = a + kATile;
             const int k0 = kb * LM_BK;
-            if (rank == 0) mbar_expect_tx(&ctl->full[s], p.a_bytes[0] + p.a_bytes[1] + 2 * p.b_bytes);
+            if (rank == 0) mbar_expect_tx(&ctl->full[s], load.a_bytes[0] + load.a_bytes[1] + 2 * load.b_bytes);
             const uint32_t full = peer_smem(&ctl->full[s], 0);
-            if constexpr (kAmn) {
+            // W's rows are vocabulary columns, counted from the piece's first; G's blocks of 64 columns are its third dimension
+            if constexpr (MODE == kProducts) {
+              if (im.product == kColGrad) {
 #pragma unroll
-              for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, &tmA, full, 0, k0, (m0 >> 6) + i, 0);
-            } else if (p.a_bytes[rank]) {
-              if constexpr (MODE == kRowGrad) tma_load_4d_pair(a, &tmA, full, 0, m0, kb, 0);
-              else tma_load_4d_pair(a, &tmA, full, k0, m0, 0, 0);
-            }
-            // W's rows are vocabulary columns, counted from the piece's first
-            if constexpr (kBmn) {
+                for (int i = 0; i < LM_BM / 64; ++i) tma_load_4d_pair(a + i * kAtom, tmA, full, 0, k0, (m0 >> 6) + i, 0);
+              } else if (load.a_bytes[rank]) {
+                tma_load_4d_pair(a, tmA, full, 0, m0, kb, 0);
+              }
+              const int row = im.product == kColGrad ? k0 : p.v0 + k0;
 #pragma unroll
-              for (int i = 0; i < kBRows / 64; ++i) tma_load_4d_pair(b + i * kAtom, &tmB, full, n0 + 64 * i, MODE == kRowGrad ? p.v0 + k0 : k0, 0, 0);
+              for (int i = 0; i < kBRows / 64; ++i) tma_load_4d_pair(b + i * kAtom, tmB, full, n0 + 64 * i, row, 0, 0);
             } else {
-              tma_load_4d_pair(b, &tmB, full, k0, p.v0 + n0, 0, 0);
+              if (load.a_bytes[rank]) tma_load_4d_pair(a, tmA, full, k0, m0, 0, 0);
+              tma_load_4d_pair(b, tmB, full, k0, p.v0 + n0, 0, 0);
             }
           }
         }
@@ -274,12 +307,15 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   } else if (warp == kEpiWarps + 1) {
     // ---------------- MMA issuer: rank 0 for both ----------------
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = make_idesc(Fmt<T>::idesc, kPairM, LM_BN, kBmn, kAmn);
-      constexpr uint64_t kStepA = kAmn ? 2048 >> 4 : 32 >> 4, kStepB = kBmn ? 2048 >> 4 : 32 >> 4;      // 16 elements of the inner dimension on
+      constexpr uint64_t kStepK = 32 >> 4, kStepMN = 2048 >> 4;      // 16 elements of the inner dimension on
       uint32_t it = 0, tt = 0;                           // k-blocks / tiles so far
       bool ok = true;
       for (int q = pair; ok && q < items; q += pairs) {
-        const Item im = item_of<MODE>(p.w, q);
+        const Item im = item_of<MODE>(p, q);
+        const bool a_mn = MODE == kProducts && im.product == kColGrad;
+        const uint32_t idesc = a_mn ? make_idesc(Fmt<T>::idesc, kPairM, LM_BN, kBmn, 1) : make_idesc(Fmt<T>::idesc, kPairM, LM_BN, kBmn, 0);
+        const uint64_t step_a = a_mn ? kStepMN : kStepK;
+        const int k_steps = a_mn ? p.products.load[kColGrad].k_steps : LM_BK / 16;
         for (int t = 0; ok && t < im.count; ++t, ++tt) {
           const uint32_t b = tt & 1;
           // the accumulator still holds tile tt-2 until the epilogue warps have read it
@@ -290,11 +326,11 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             if (!mbar_wait(&ctl->full[s], (it / kStages) & 1, abort_flag)) { atomicOr(&ctl->fail_bits, (uint32_t)ULM_STATUS_TIMEOUT_LOAD); ok = false; break; }
             fence_after_sync();
             const uint32_t sa = smem_u32(stages + (size_t)s * kStage);
-            const uint64_t da = kAmn ? make_sdesc_sw128_mn(sa, kAtom) : make_sdesc_sw128(sa);
+            const uint64_t da = a_mn ? make_sdesc_sw128_mn(sa, kAtom) : make_sdesc_sw128(sa);
             const uint64_t db = kBmn ? make_sdesc_sw128_mn(sa + kATile, kAtom) : make_sdesc_sw128(sa + kATile);
 #pragma unroll
             for (int kk = 0; kk < LM_BK / 16; ++kk)
-              if (MODE != kColGrad || kk < p.k_steps) mma_ss_pair(tmem_base + b * LM_BN, da + kk * kStepA, db + kk * kStepB, idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
+              if (MODE != kProducts || kk < k_steps) mma_ss_pair(tmem_base + b * LM_BN, da + kk * step_a, db + kk * (kBmn ? kStepMN : kStepK), idesc, (kb > im.kb0 || kk > 0) ? 1u : 0u);
             mma_commit_pair(&ctl->empty[s]);             // the stage is free in both CTAs once these MMAs have read it
           }
           if (ok) mma_commit_pair(&ctl->acc_full[b]);
@@ -308,7 +344,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     [[maybe_unused]] uint8_t* my_staging = staging + (size_t)warp * kStaging;
     [[maybe_unused]] float factor = 0.f;
-    if constexpr (MODE == kRowGrad || MODE == kColGrad) factor = out_factor(p.out);
+    if constexpr (MODE == kProducts) factor = out_factor(p.products.out[kColGrad]);         // the same for both
     uint32_t tt = 0;
     bool ok = true;
     // the row's target column and, for G, its shift of the exponent 2^(z log2e + shift); asked for an item ahead
@@ -316,7 +352,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     auto row_of = [&](int q) {
       Row w{-1, 0.f};
       if constexpr (MODE == kStats || MODE == kGrad) {
-        const int64_t row = (int64_t)item_of<MODE>(p.w, q < items ? q : pair).mt * kPairM + rank * LM_BM + r;
+        const int64_t row = (int64_t)item_of<MODE>(p, q < items ? q : pair).mt * kPairM + rank * LM_BM + r;
         if (row < p.rows) {
           w.target = p.target[row];
           if (w.target == p.ignore_index || w.target >= p.V) w.target = -1;
@@ -327,7 +363,7 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     };
     [[maybe_unused]] Row next = row_of(pair);
     for (int q = pair; ok && q < items; q += pairs) {
-      const Item im = item_of<MODE>(p.w, q);
+      const Item im = item_of<MODE>(p, q);
       const int64_t grow = (int64_t)im.mt * kPairM + rank * LM_BM + r;
       [[maybe_unused]] const int row0 = (int)grow - lane;                        // the warp's first row
       [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
@@ -416,23 +452,25 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 else if (col0 + c + 1 >= p.V) pk[c >> 1] &= 0xffffu;
               }
             }
-            if (col_tile + c_blk < p.g_cols && row0 < p.rows) store_block<false>(&tmOut, my_staging, lane, pk, 0, row0, (col_tile + c_blk) >> 6);
+            if (col_tile + c_blk < p.g_cols && row0 < p.rows) store_block<false>(&maps.out[0], my_staging, lane, pk, 0, row0, (col_tile + c_blk) >> 6);
           } else {
             const int col = col_tile + c_blk;
+            const Out& out = p.products.out[im.product];
+            const CUtensorMap* tmOut = &maps.out[im.product];
             if (im.slot >= 0) {
-              if (row0 < p.out.rows) store_f32<false>(&tmSlots, my_staging, lane, acc, 1.f, c_blk, LM_BN, im.slot * kPairM + (int)rank * LM_BM + (warp & 3) * 32);
-            } else if (col < p.out.cols && row0 < p.out.rows) {
-              if (p.out.is_f32 && p.out.prev) {
-                store_f32<true>(&tmOut, my_staging, lane, acc, factor, col, p.out.cols, row0);
-              } else if (p.out.is_f32) {
-                store_f32<false>(&tmOut, my_staging, lane, acc, factor, col, p.out.cols, row0);
-              } else if (p.out.prev) {
-                add_and_round<T>(p.out, factor, grow, col, acc);
+              if (row0 < out.rows) store_f32<false>(&maps.slots, my_staging, lane, acc, 1.f, c_blk, LM_BN, im.slot * kPairM + (int)rank * LM_BM + (warp & 3) * 32);
+            } else if (col < out.cols && row0 < out.rows) {
+              if (out.is_f32 && out.prev) {
+                store_f32<true>(tmOut, my_staging, lane, acc, factor, col, out.cols, row0);
+              } else if (out.is_f32) {
+                store_f32<false>(tmOut, my_staging, lane, acc, factor, col, out.cols, row0);
+              } else if (out.prev) {
+                add_and_round<T>(out, factor, grow, col, acc);
               } else {
                 uint32_t pk[32];
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) pk[c >> 1] = Cvt<T>::pack2(factor * __uint_as_float(acc[c]), factor * __uint_as_float(acc[c + 1]));
-                store_block<false>(&tmOut, my_staging, lane, pk, col, row0);
+                store_block<false>(tmOut, my_staging, lane, pk, col, row0);
               }
             }
           }
@@ -461,15 +499,19 @@ streamed_ce_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 // thread eight columns.
 template <typename T>
 __global__ void __launch_bounds__(256)
-streamed_ce_join_kernel(const Work w, const Out o) {
+streamed_ce_join_kernel(const Products p) {
   grid_dependents_go();
   grid_dependency_wait();
-  const int j = blockIdx.x, t = w.whole + j, mt = t / w.n_nt, nt = t - mt * w.n_nt;
+  const int of_dw = p.w[kColGrad].split > 1 ? p.w[kColGrad].rest : 0;
+  const int which = (int)blockIdx.x < of_dw ? kColGrad : kRowGrad, j = (int)blockIdx.x - (which == kColGrad ? 0 : of_dw);
+  const Work& w = p.w[which];
+  const Out& o = p.out[which];
+  const int t = w.whole + j, mt = t / w.n_nt, nt = t - mt * w.n_nt;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 8;
   const int64_t row = (int64_t)mt * kPairM + r;
   const int col = nt * LM_BN + c;
   if (row >= o.rows || col >= o.cols) return;
-  const float* s = o.slots + (int64_t)j * w.split * kSlot + r * LM_BN + c;
+  const float* s = o.slots + (p.slot0[which] + (int64_t)j * w.split) * kSlot + r * LM_BN + c;
   const float factor = out_factor(o);
   float v[8];
 #pragma unroll
@@ -601,31 +643,38 @@ Work product_work(int64_t m, int64_t n, int64_t k) {
   }
   return w;
 }
-int64_t slot_floats(const Work& w) { return w.split > 1 ? (int64_t)w.rest * w.split * kSlot : 0; }
+int n_slots(const Work& w) { return w.split > 1 ? w.rest * w.split : 0; }
 
 template <typename T, int MODE>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Params& p, int device, cudaStream_t st, const char* who) {
+int launch(const Maps& maps, const Params& p, int device, cudaStream_t st, const char* who) {
   static std::atomic<bool> attr_set[kMaxDevices];
   auto kern = streamed_ce_kernel<T, MODE>;
   if (int rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who)) return rc;
-  const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
-  return launch_dependent(who, kern, grid, kThreads, smem_bytes(MODE), st, ma, mb, mo, mo, p);
+  const int items = n_items<MODE>(p), grid = 2 * (items < kPairs ? items : kPairs);
+  return launch_dependent(who, kern, grid, kThreads, smem_bytes(MODE), st, maps, p);
 }
-// A product and, where tiles were cut, their sum
-template <typename T, int MODE>
-int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int dtype, int device, cudaStream_t st, const char* who) {
-  static std::atomic<bool> attr_set[kMaxDevices];
-  auto kern = streamed_ce_kernel<T, MODE>;
-  CUtensorMap mo, ms;
-  int rc;
-  if ((rc = ensure_smem_attr(kern, smem_bytes(MODE), device, attr_set, who))) return rc;
-  if ((rc = encode_matrix_map(&mo, p.out.out, p.out.is_f32 ? (int)ULM_F32 : dtype, p.out.rows, p.out.cols, p.out.ld, 32, who))) return rc;
-  ms = mo;
-  if (p.w.split > 1 && (rc = encode_matrix_map(&ms, p.out.slots, ULM_F32, (int64_t)p.w.rest * p.w.split * kPairM, LM_BN, LM_BN, 32, who))) return rc;
-  const int items = n_items<MODE>(p.w), grid = 2 * (items < kPairs ? items : kPairs);
-  rc = launch_dependent(who, kern, grid, kThreads, smem_bytes(MODE), st, ma, mb, mo, ms, p);
-  if (rc || p.w.split == 1) return rc;
-  return launch_dependent(who, streamed_ce_join_kernel<T>, dim3(p.w.rest, (unsigned)((p.out.rows < kPairM ? p.out.rows : kPairM) + 7) / 8), 256, 0, st, p.w, p.out);
+// Both products and, where tiles were cut, their sums
+template <typename T>
+int launch_products(Maps& maps, Params& p, float* slots, int dtype, int device, cudaStream_t st, const char* who) {
+  Products& m = p.products;
+  int rc, joined = 0, n = 0;
+  int64_t most_rows = 0;
+  for (int i = 0; i < kNumProducts; ++i) {
+    Out& o = m.out[i];
+    m.slot0[i] = n;
+    o.slots = slots;
+    if (!o.out) continue;
+    if ((rc = encode_matrix_map(&maps.out[i], o.out, o.is_f32 ? (int)ULM_F32 : dtype, o.rows, o.cols, o.ld, 32, who))) return rc;
+    if (m.w[i].split > 1) {
+      n += n_slots(m.w[i]);
+      joined += m.w[i].rest;
+      if (o.rows > most_rows) most_rows = o.rows;
+    }
+  }
+  if (n && (rc = encode_matrix_map(&maps.slots, slots, ULM_F32, (int64_t)n * kPairM, LM_BN, LM_BN, 32, who))) return rc;
+  rc = launch<T, kProducts>(maps, p, device, st, who);
+  if (rc || !joined) return rc;
+  return launch_dependent(who, streamed_ce_join_kernel<T>, dim3(joined, (unsigned)((most_rows < kPairM ? most_rows : kPairM) + 7) / 8), 256, 0, st, m);
 }
 
 int check_args(const ulm_streamed_ce_args* a, const char* who) {
@@ -645,16 +694,19 @@ bool ok_out(const void* p, int64_t stride, int d) { return !(reinterpret_cast<ui
 int a_box(int64_t rows) { return rows < LM_BM ? (int)(rows + 7) / 8 * 8 : LM_BM; }
 // K16 steps of dW's k-blocks, which go over the rows
 int col_steps(int64_t rows) { return rows < LM_BK ? (int)(rows + 15) / 16 : LM_BK / 16; }
-void set_bytes(Params& p, bool col_grad) {
-  p.k_steps = col_grad ? col_steps(p.rows) : LM_BK / 16;
-  p.a_bytes[0] = col_grad ? kATile / 4 * p.k_steps : (uint32_t)a_box(p.rows) * LM_BK * 2;
-  p.a_bytes[1] = !col_grad && p.rows <= LM_BM ? 0u : p.a_bytes[0];
-  p.b_bytes = col_grad ? kBTile / 4 * p.k_steps : kBTile;
+Load load_of(int64_t rows, bool col_grad) {
+  Load l;
+  l.k_steps = col_grad ? col_steps(rows) : LM_BK / 16;
+  l.a_bytes[0] = col_grad ? kATile / 4 * l.k_steps : (uint32_t)a_box(rows) * LM_BK * 2;
+  l.a_bytes[1] = !col_grad && rows <= LM_BM ? 0u : l.a_bytes[0];
+  l.b_bytes = col_grad ? kBTile / 4 * l.k_steps : kBTile;
+  return l;
 }
 
 Params common_params(const ulm_streamed_ce_args* a) {
   Params p{};
   p.rows = a->rows; p.V = a->V; p.target = a->target; p.ignore_index = a->ignore_index; p.status = a->status_dev;
+  p.load = load_of(a->rows, false);
   return p;
 }
 
@@ -669,17 +721,16 @@ Work stats_work(int64_t rows, int V, int d) {
 
 template <typename T>
 int forward(const ulm_streamed_ce_args* a, int device, const char* who) {
-  CUtensorMap mh, mw;
-  if (int rc = encode_matrix_map(&mh, a->h, a->dtype, a->rows, a->d, a->h_stride, a_box(a->rows), who)) return rc;
-  if (int rc = encode_matrix_map(&mw, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who)) return rc;
+  Maps maps{};
+  if (int rc = encode_matrix_map(&maps.a[0], a->h, a->dtype, a->rows, a->d, a->h_stride, a_box(a->rows), who)) return rc;
+  if (int rc = encode_matrix_map(&maps.b[0], a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who)) return rc;
   Params p = common_params(a);
-  set_bytes(p, false);
   p.w = stats_work(a->rows, a->V, a->d);
   const int parts = 2 * ((p.w.n_nt + p.w.group - 1) / p.w.group);
   p.part_m = a->scratch; p.part_s = a->scratch + a->rows * parts; p.z_target = a->loss;
   p.done = reinterpret_cast<uint32_t*>(a->scratch + 2 * a->rows * parts);
   cudaStream_t st = (cudaStream_t)a->stream;
-  if (int rc = launch<T, kStats>(mh, mw, mh, p, device, st, who)) return rc;
+  if (int rc = launch<T, kStats>(maps, p, device, st, who)) return rc;
   const Mean mean{a->denom_dev, a->denom, a->mean, a->inv, p.done};
   const Operands op{a->h, a->w, a->h_stride, a->w_stride, a->d};
   return launch_dependent(who, streamed_ce_finish_kernel<T>, (unsigned)((a->rows + 7) / 8), 256, 0, st, p.part_m, p.part_s, parts, a->target, a->ignore_index, a->V,
@@ -693,50 +744,50 @@ int64_t g_blocks(int64_t piece) { return (piece + 63) / 64; }
 template <typename T>
 int backward(const ulm_streamed_ce_args* a, const ulm_streamed_ce_grads* g, int device, const char* who) {
   cudaStream_t st = (cudaStream_t)a->stream;
-  CUtensorMap h_rows, h_mn, w_rows, w_mn;                // K-major and MN-major boxes of both
+  Maps logits{}, products{};                             // H and W for z; G and H, G and W for the products: K-major and MN-major boxes
   int rc;
-  if ((rc = encode_matrix_map(&h_rows, a->h, a->dtype, a->rows, a->d, a->h_stride, a_box(a->rows), who))) return rc;
-  if ((rc = encode_matrix_map(&h_mn, a->h, a->dtype, a->rows, a->d, a->h_stride, 16 * col_steps(a->rows), who))) return rc;
-  if ((rc = encode_matrix_map(&w_rows, a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who))) return rc;
-  if ((rc = encode_matrix_map(&w_mn, a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
+  const int steps = 16 * col_steps(a->rows), box = a_box(a->rows);
+  if ((rc = encode_matrix_map(&logits.a[0], a->h, a->dtype, a->rows, a->d, a->h_stride, box, who))) return rc;
+  if ((rc = encode_matrix_map(&logits.b[0], a->w, a->dtype, a->V, a->d, a->w_stride, kBRows, who))) return rc;
+  if ((rc = encode_matrix_map(&products.b[kColGrad], a->h, a->dtype, a->rows, a->d, a->h_stride, steps, who))) return rc;
+  if ((rc = encode_matrix_map(&products.b[kRowGrad], a->w, a->dtype, a->V, a->d, a->w_stride, 64, who))) return rc;
   for (int64_t v0 = 0; v0 < a->V; v0 += g->piece) {
     const int64_t n = a->V - v0 < g->piece ? a->V - v0 : g->piece;
-    CUtensorMap g_rows, g_mn, g_out;
     auto g_map = [&](CUtensorMap* m, int box_rows) {
       return encode_bhsd_map(m, g->workspace, a->dtype, 1, (int)g_blocks(n), (int)a->rows, 0, a->rows * 64, 64, box_rows, who);
     };
-    if ((rc = g_map(&g_rows, a_box(a->rows))) || (rc = g_map(&g_mn, 16 * col_steps(a->rows))) || (rc = g_map(&g_out, 32))) return rc;
+    if ((rc = g_map(&logits.out[0], 32)) || (rc = g_map(&products.a[kColGrad], steps)) || (rc = g_map(&products.a[kRowGrad], box))) return rc;
     Params p = common_params(a);
     p.v0 = (int)v0;
-    set_bytes(p, false);
     p.lse = a->lse;
     p.g_cols = (int)g_blocks(n) * 64;
     p.w = stats_work(a->rows, (int)n, a->d);
-    if ((rc = launch<T, kGrad>(h_rows, w_rows, g_out, p, device, st, who))) return rc;
-    p.out.factor_dev = g->factor_dev;
-    p.out.factor2_dev = g->factor2_dev;
-    p.out.factor = 1.f / (float)(1 << Fmt<T>::g_shift);
-    p.out.slots = g->slots;
-    p.out.cols = a->d;
+    if ((rc = launch<T, kGrad>(logits, p, device, st, who))) return rc;
+    Products& m = p.products;
+    for (Out& o : m.out) {
+      o.factor_dev = g->factor_dev;
+      o.factor2_dev = g->factor2_dev;
+      o.factor = 1.f / (float)(1 << Fmt<T>::g_shift);
+      o.cols = a->d;
+    }
     if (g->dw) {
-      p.w = product_work(n, a->d, a->rows);
-      set_bytes(p, true);
-      p.out.ld = g->dw_stride; p.out.rows = n; p.out.is_f32 = g->dw_f32;
-      p.out.out = g->dw_f32 ? (void*)((float*)g->dw + v0 * g->dw_stride) : (void*)((T*)g->dw + v0 * g->dw_stride);
-      p.out.prev = g->dw_add ? (const float*)p.out.out : nullptr;
-      if ((rc = launch_product<T, kColGrad>(g_mn, h_mn, p, a->dtype, device, st, who))) return rc;
+      m.w[kColGrad] = product_work(n, a->d, a->rows);
+      m.load[kColGrad] = load_of(a->rows, true);
+      Out& o = m.out[kColGrad];
+      o.ld = g->dw_stride; o.rows = n; o.is_f32 = g->dw_f32;
+      o.out = g->dw_f32 ? (void*)((float*)g->dw + v0 * g->dw_stride) : (void*)((T*)g->dw + v0 * g->dw_stride);
+      o.prev = g->dw_add ? (const float*)o.out : nullptr;
     }
     if (g->dh) {
       const bool first = v0 == 0, last = v0 + n >= a->V;
-      p.w = product_work(a->rows, a->d, n);
-      set_bytes(p, false);
-      p.out.rows = a->rows;
-      p.out.is_f32 = !last;
-      p.out.out = last ? g->dh : (void*)g->dh_sum;
-      p.out.prev = first ? nullptr : g->dh_sum;
-      p.out.ld = a->d;                                   // dh and dh_sum are dense
-      if ((rc = launch_product<T, kRowGrad>(g_rows, w_mn, p, a->dtype, device, st, who))) return rc;
+      m.w[kRowGrad] = product_work(a->rows, a->d, n);
+      m.load[kRowGrad] = load_of(a->rows, false);
+      Out& o = m.out[kRowGrad];
+      o.ld = a->d; o.rows = a->rows; o.is_f32 = !last;   // dh and dh_sum are dense
+      o.out = last ? g->dh : (void*)g->dh_sum;
+      o.prev = first ? nullptr : g->dh_sum;
     }
+    if ((rc = launch_products<T>(products, p, g->slots, a->dtype, device, st, who))) return rc;
   }
   return ULM_OK;
 }
@@ -759,11 +810,9 @@ extern "C" int64_t ulm_streamed_ce_slots(int64_t rows, int32_t V, int32_t d, int
   if (rows <= 0 || V <= 0 || d <= 0 || piece <= 0) return 0;
   int64_t most = 0;
   const int64_t tail = V % piece ? V % piece : piece;    // the pieces have two sizes at most
-  for (int64_t n : {piece < V ? piece : (int64_t)V, tail < V ? tail : (int64_t)V}) {
-    if (want_dw) most = std::max(most, slot_floats(product_work(n, d, rows)));
-    if (want_dh) most = std::max(most, slot_floats(product_work(rows, d, n)));
-  }
-  return most;
+  for (int64_t n : {piece < V ? piece : (int64_t)V, tail < V ? tail : (int64_t)V})
+    most = std::max<int64_t>(most, (want_dw ? n_slots(product_work(n, d, rows)) : 0) + (want_dh ? n_slots(product_work(rows, d, n)) : 0));
+  return most * kSlot;
 }
 
 extern "C" int ulm_streamed_ce_fwd(const ulm_streamed_ce_args* a) {
