@@ -19,7 +19,7 @@
 // N256 x K16 instructions over both CTAs, six stages of 128x64 + 128x64 operands a CTA in 128-byte-swizzled shared memory, two
 // accumulators of 256 TMEM columns so that a tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
 // contiguous, so dH reads W, and dW reads both G and H, as MN-major operands: rows of 64-element atoms, no transposed copies.
-// What bounds it from widths of 512 on: the tensor pipe, active 88-91 % of the cycles, and the clock that the power limit leaves.
+// What bounds it from widths of 512 on: the tensor pipe, active 87-94 % of the cycles, and the clock that the power limit leaves.
 // 32768 x 768 x 32000 bf16, forward and backward: 4.4 ms in short runs, 5.0-5.2 ms under lasting load (1250 TFLOP/s of the
 // products that are formed; library GEMMs of the same shapes 1120-1190).  One CTA a product instead of a pair: 5.69 ms where the pair
 // took 5.48.  Narrower: the exponentials, 256 x 128 of them a CTA and tile; 32768 x 64 x 32000 2.3 ms.
