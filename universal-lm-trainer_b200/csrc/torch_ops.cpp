@@ -832,8 +832,8 @@ struct SwigluBwd : OpNode {
 };
 
 Tensor gate(const Tensor& a_in, const Tensor& b_in, const Drop& drop) {
-  TORCH_CHECK_VALUE(a_in.is_cuda() && known(a_in.scalar_type()) && b_in.scalar_type() == a_in.scalar_type() && b_in.sizes() == a_in.sizes(),
-                    "swiglu needs two CUDA tensors of one shape and one of fp16/bf16/fp32");
+  TORCH_CHECK_VALUE(a_in.is_cuda() && known(a_in.scalar_type()) && b_in.scalar_type() == a_in.scalar_type() && b_in.sizes() == a_in.sizes() && b_in.device() == a_in.device(),
+                    "swiglu needs two tensors of one CUDA device, of one shape and one of fp16/bf16/fp32");
   Tensor a, b, y;
   {
     OpScope scope;
