@@ -22,3 +22,15 @@ def test_gate_refuses_operands_of_two_devices(op, elsewhere):
         op(a, torch.ones(4, 64, device=elsewhere))
     with pytest.raises(ValueError, match='one CUDA device'):
         op(torch.ones(4, 64, device=elsewhere), a)
+
+
+@pytest.mark.parametrize('bad', ['weight on the host', 'short weight', 'long weight', 'branch on the host'])
+def test_norms_refuse_what_they_cannot_read(bad):
+    x, b = torch.ones(4, 64, device='cuda'), torch.ones(4, 64, dtype=F16, device='cpu' if bad == 'branch on the host' else 'cuda')
+    w = torch.ones({'short weight': 32, 'long weight': 65}.get(bad, 64), device='cpu' if bad == 'weight on the host' else 'cuda')
+    with pytest.raises(ValueError):
+        ulm_ops.add_rms_norm(x, b, w)
+    if bad != 'branch on the host':
+        for dtype in (F16, BF16, F32):
+            with pytest.raises(ValueError, match='one weight per column'):
+                ulm_ops.rms_norm(x.to(dtype), w)

@@ -594,6 +594,9 @@ Tensor rows_of(const Tensor& x) {
   const bool ok = x2.stride(1) == 1 && !(reinterpret_cast<uintptr_t>(x2.data_ptr()) & 15) && (x2.stride(0) * x2.element_size()) % 16 == 0;
   return ok ? x2 : x2.contiguous();
 }
+void check_norm_weight(const Tensor& w, const Tensor& x, const char* who) {
+  TORCH_CHECK_VALUE(w.device() == x.device() && x.dim() >= 1 && w.numel() == x.size(-1), who, " needs one weight per column, on the device of x");
+}
 int y_kind(at::ScalarType y, at::ScalarType x) { return y == x ? ULM_Y_SAME : y == at::kHalf ? ULM_Y_F16 : ULM_Y_BF16; }
 
 // dx (and d_branch) and dw of one norm; ga: the gradient reaching the normalised tensor from elsewhere
@@ -628,6 +631,7 @@ struct NormBwd : OpNode {
 
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps, std::optional<at::ScalarType> out_dtype) {
   TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()), "rms_norm needs a CUDA fp16/bf16/fp32 tensor");
+  check_norm_weight(weight, x, "rms_norm");
   at::ScalarType yt = x.scalar_type();
   if (out_dtype) yt = *out_dtype;
   else if (yt == at::kFloat && at::autocast::is_autocast_enabled(at::kCUDA)) yt = at::autocast::get_autocast_dtype(at::kCUDA);
@@ -675,8 +679,9 @@ struct AddNormBwd : OpNode {
 };
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& branch, const Tensor& weight, double eps) {
-  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kFloat && is_16bit(branch.scalar_type()) && branch.sizes() == x.sizes(),
-                    "add_rms_norm needs an fp32 CUDA x and a 16-bit branch of the same shape");
+  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kFloat && is_16bit(branch.scalar_type()) && branch.device() == x.device() && branch.sizes() == x.sizes(),
+                    "add_rms_norm needs an fp32 CUDA x and a 16-bit branch of the same shape and device");
+  check_norm_weight(weight, x, "add_rms_norm");
   TORCH_CHECK_VALUE(x.size(-1) <= 1024 && x.size(-1) % 4 == 0, "add_rms_norm takes rows of at most 1024 elements, a multiple of 4");
   Tensor x_new, y, w, rstd;
   {
