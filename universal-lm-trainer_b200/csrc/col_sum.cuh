@@ -10,7 +10,7 @@ namespace {
 // every 32nd partial row of one column (coalesced 128-byte reads, short independent chains), and the 32
 // sub-sums of a column are added in index order.
 __global__ void __launch_bounds__(1024)
-col_sum_kernel(const float* __restrict__ partial, float* __restrict__ dw, int nparts, int d) {
+col_sum_kernel(const float* partial, float* dw, int nparts, int d) {
   __shared__ float sub[32][33];
   grid_dependency_wait();                                // at once where the launch is an ordinary one
   const int c = blockIdx.x * 32 + threadIdx.x;

@@ -28,6 +28,8 @@ inline int check_launch(const char* what) {
 // Programmatic dependent launch: a kernel launched by launch_dependent may be set up, and its blocks started on SMs that are
 // free, while the one before it in the stream still runs.  Such a kernel calls grid_dependency_wait before it touches
 // anything another kernel writes or reads; that returns once all kernels before it have ended and their writes can be seen.
+// "Seen" holds for ordinary loads.  __ldg and const __restrict__ promise that the data stay as they are for the whole kernel,
+// which began before they were written: such a kernel has neither.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next such launch begin.
 __device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

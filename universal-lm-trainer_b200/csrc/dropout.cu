@@ -26,7 +26,7 @@ constexpr int kVecsGate = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t nvec, int64_t n, const __grid_constant__ DropMask mask) {
+dropout_kernel(const T* x, T* y, int64_t nvec, int64_t n, const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsDrop<T>;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
   grid_dependents_go();
@@ -34,7 +34,7 @@ dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t nvec, int64_t
   uint4 rx[K];
 #pragma unroll
   for (int k = 0; k < K; ++k)
-    if (v0 + k * kThreads < nvec) rx[k] = __ldg(reinterpret_cast<const uint4*>(x) + v0 + k * kThreads);
+    if (v0 + k * kThreads < nvec) rx[k] = *(reinterpret_cast<const uint4*>(x) + v0 + k * kThreads);
   Keep<N> keep[K];                                       // while the loads are on their way
 #pragma unroll
   for (int k = 0; k < K; ++k) keep[k] = keep_of<N>(mask, (uint64_t)(v0 + k * kThreads));
@@ -71,7 +71,7 @@ __device__ __forceinline__ void gate_bwd_one(const DropMask& m, bool stays, floa
 
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(kThreads)
-gate_dropout_fwd_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __restrict__ y, int64_t nvec, int64_t n, const Rows rw,
+gate_dropout_fwd_kernel(const T* a, const T* b, T* y, int64_t nvec, int64_t n, const Rows rw,
                         const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsGate;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
@@ -82,8 +82,8 @@ gate_dropout_fwd_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __r
   for (int k = 0; k < K; ++k)
     if (v0 + k * kThreads < nvec) {
       const int64_t o = operand_vec<ROWS>(v0 + k * kThreads, rw);
-      ra[k] = __ldg(reinterpret_cast<const uint4*>(a) + o);
-      rb[k] = __ldg(reinterpret_cast<const uint4*>(b) + o);
+      ra[k] = *(reinterpret_cast<const uint4*>(a) + o);
+      rb[k] = *(reinterpret_cast<const uint4*>(b) + o);
     }
   Keep<N> keep[K];                                       // while the loads are on their way
 #pragma unroll
@@ -108,7 +108,7 @@ gate_dropout_fwd_kernel(const T* __restrict__ a, const T* __restrict__ b, T* __r
 
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(kThreads)
-gate_dropout_bwd_kernel(const T* __restrict__ a, const T* __restrict__ b, const T* __restrict__ dy, T* __restrict__ da, T* __restrict__ db,
+gate_dropout_bwd_kernel(const T* a, const T* b, const T* dy, T* da, T* db,
                         int64_t nvec, int64_t n, const Rows rw, const __grid_constant__ DropMask mask) {
   constexpr int N = VecN<T>::N, K = kVecsGate;
   const int64_t v0 = (int64_t)blockIdx.x * (kThreads * K) + threadIdx.x;
@@ -119,9 +119,9 @@ gate_dropout_bwd_kernel(const T* __restrict__ a, const T* __restrict__ b, const 
   for (int k = 0; k < K; ++k)
     if (v0 + k * kThreads < nvec) {
       const int64_t o = operand_vec<ROWS>(v0 + k * kThreads, rw);
-      ra[k] = __ldg(reinterpret_cast<const uint4*>(a) + o);
-      rb[k] = __ldg(reinterpret_cast<const uint4*>(b) + o);
-      rg[k] = __ldg(reinterpret_cast<const uint4*>(dy) + v0 + k * kThreads);
+      ra[k] = *(reinterpret_cast<const uint4*>(a) + o);
+      rb[k] = *(reinterpret_cast<const uint4*>(b) + o);
+      rg[k] = *(reinterpret_cast<const uint4*>(dy) + v0 + k * kThreads);
     }
   Keep<N> keep[K];                                       // while the loads are on their way
 #pragma unroll

@@ -86,8 +86,8 @@ add_dropout_norm_fwd_kernel(const FwdParams p, const __grid_constant__ DropMask 
   __shared__ float slots[2][kFwdWarps];
   grid_dependents_go();
   grid_dependency_wait();
-  const TY* __restrict__ br = static_cast<const TY*>(p.branch);
-  TY* __restrict__ y = static_cast<TY*>(p.y);
+  const TY* br = static_cast<const TY*>(p.branch);
+  TY* y = static_cast<TY*>(p.y);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
   const int group = warp / W, part = warp - group * W, groups = (int)(blockDim.x >> 5) / W;
   const int nvec = p.d / E, first = part * 32 + lane, hop = W * 32;
@@ -150,8 +150,8 @@ add_dropout_norm_bwd_kernel(const BwdParams p, const __grid_constant__ DropMask 
   __shared__ float slots[2][WARPS];
   grid_dependents_go();
   grid_dependency_wait();
-  const TY* __restrict__ dy = static_cast<const TY*>(p.dy);
-  TY* __restrict__ db = static_cast<TY*>(p.d_branch);
+  const TY* dy = static_cast<const TY*>(p.dy);
+  TY* db = static_cast<TY*>(p.d_branch);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
   const int group = warp / W, part = warp - group * W, groups = (int)(blockDim.x >> 5) / W;
   const int nvec = p.d / E, first = part * 32 + lane, hop = W * 32;

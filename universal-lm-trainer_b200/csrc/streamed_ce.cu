@@ -549,8 +549,8 @@ struct Mean {
 struct Operands { const void *h, *w; int64_t h_stride, w_stride; int d; };
 template <typename T>
 __global__ void __launch_bounds__(256)
-streamed_ce_finish_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int n_parts, const int64_t* __restrict__ target,
-                          int64_t ignore_index, int V, float* __restrict__ lse, float* loss, int64_t rows, const Operands op, const Mean mean) {
+streamed_ce_finish_kernel(const float* part_m, const float* part_s, int n_parts, const int64_t* target,
+                          int64_t ignore_index, int V, float* lse, float* loss, int64_t rows, const Operands op, const Mean mean) {
   __shared__ double s_sum[8];
   __shared__ int s_n[8];
   __shared__ uint32_t s_before;
