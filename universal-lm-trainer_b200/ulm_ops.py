@@ -109,7 +109,7 @@ def _as_i64(seed):
 def next_dropout_seed():
     """A seed from torch's default CPU generator: `torch.manual_seed` fixes the sequence, and a checkpointed forward that is run
     again draws the same ones.  No device is asked."""
-    return int(torch.randint(0, 1 << 62, ()))
+    return int(torch.randint(0, 1 << 62, (), device='cpu'))         # whatever torch's default device is
 
 
 class Dropout(nn.Module):
