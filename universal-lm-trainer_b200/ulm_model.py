@@ -35,6 +35,11 @@ class ModelConfig:  # train.py:725-737
     streamed_loss: bool = False     # ulm_ops.streamed_cross_entropy: no logits
 
 
+def _option(config, name):
+    """A field that is not the reference's; off in the reference's own configuration object, which does not have it."""
+    return getattr(config, name, False)
+
+
 # compute_loss pads the flattened token dimension to a multiple of this (see DecoderOnlyTransformer._forward_flat)
 TOKEN_QUANTUM = 1024
 
@@ -171,10 +176,11 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
     def __init__(self, config: ModelConfig):
         super().__init__()
         self.self_attn = MultiHeadAttention(config)
-        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout, config.counter_dropout)
+        counter = _option(config, 'counter_dropout')
+        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout, counter)
         self.norm1 = FusedRMSNorm(config.d_model)
         self.norm2 = FusedRMSNorm(config.d_model)
-        self.dropout = _make_dropout(config.dropout, config.counter_dropout)
+        self.dropout = _make_dropout(config.dropout, counter)
 
     def forward(self, x, pending=None, cos=None, sin=None, shape=None):
         if pending is None:
@@ -257,7 +263,7 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
         Tp = n * L if TOKEN_QUANTUM <= 1 else -(-n * L // TOKEN_QUANTUM) * TOKEN_QUANTUM
         flat_ids, target = ulm_ops.token_targets(input_ids.contiguous(), labels.contiguous(), Tp, ignore_index)
         hidden, _ = self._forward_flat(input_ids, TOKEN_QUANTUM, flat_ids)
-        if self.config.streamed_loss:
+        if _option(self.config, 'streamed_loss'):
             return ulm_ops.streamed_cross_entropy(hidden, self.fc_out.weight, target, ignore_index=ignore_index, denominator=denominator)
         return ulm_ops.chunked_cross_entropy(hidden, self.fc_out.weight, target, ignore_index=ignore_index,
                                              chunk_rows=chunk_rows, denominator=denominator)
