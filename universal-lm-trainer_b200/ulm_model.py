@@ -131,18 +131,24 @@ class MultiHeadAttention(nn.Module):  # train.py:1920-1964
         return out if flat else out.view(n, L, out.shape[-1])
 
 
+def _plain(module, kind):
+    """Whether calling ``module`` does what ``kind`` does and nothing else: nobody has derived from it, patched it or hooked it."""
+    if type(module) is not kind or 'forward' in module.__dict__ or nn.modules.module._has_any_global_hook():
+        return False
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+
+
 def _drop(dropout, x):
     """``dropout(x)`` without the module call (6 us of host time, twice a block) where that is known to change nothing:
-    a plain ``nn.Dropout`` that nobody has hooked.  Anything else put in its place is called."""
-    idle = type(dropout) is nn.Dropout and not (dropout.training and dropout.p > 0.0) and not (dropout._forward_hooks or dropout._forward_pre_hooks)
+    a plain ``nn.Dropout``, idle.  Anything else put in its place is called."""
+    idle = _plain(dropout, nn.Dropout) and not (dropout.training and dropout.p > 0.0)
     return x if idle else dropout(x)
 
 
 def _mask_of(dropout):
     """(p, seed) where ``dropout`` is a plain `ulm_ops.Dropout` at work, for the kernel that works in its place; None where it has
     to be called (or is idle)."""
-    plain = type(dropout) is ulm_ops.Dropout and not (dropout._forward_hooks or dropout._forward_pre_hooks)
-    return (dropout.p, ulm_ops.next_dropout_seed()) if plain and dropout.active() else None
+    return (dropout.p, ulm_ops.next_dropout_seed()) if _plain(dropout, ulm_ops.Dropout) and dropout.active() else None
 
 
 def _make_dropout(p, counter):
