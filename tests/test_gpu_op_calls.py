@@ -34,3 +34,50 @@ def test_norms_refuse_what_they_cannot_read(bad):
         for dtype in (F16, BF16, F32):
             with pytest.raises(ValueError, match='one weight per column'):
                 ulm_ops.rms_norm(x.to(dtype), w)
+
+
+def shifted(t):
+    """The same values, contiguous, one element past an aligned address."""
+    v = torch.empty(t.numel() + 1, device='cuda', dtype=t.dtype)[1:].view_as(t)
+    return v.copy_(t)
+
+
+OPS = {
+    'swiglu': lambda dt: (ulm_ops.swiglu, [randn((5, 64), dt, 1), randn((5, 64), dt, 2)]),
+    'swiglu_dropout': lambda dt: (lambda a, b: ulm_ops.swiglu_dropout(a, b, 0.5, 1), [randn((5, 64), dt, 1), randn((5, 64), dt, 2)]),
+    'dropout': lambda dt: (lambda a: ulm_ops.dropout(a, 0.5, 1), [randn((5, 64), dt, 1)]),
+    'rms_norm': lambda dt: (ulm_ops.rms_norm, [randn((5, 64), dt, 1), randn(64, F32, 2)]),
+    'rms_norm, wide rows': lambda dt: (ulm_ops.rms_norm, [randn((5, 1000), dt, 1), randn(1000, F32, 2)]),
+    'add_rms_norm': lambda dt: (ulm_ops.add_rms_norm, [randn((5, 64), F32, 1), randn((5, 64), BF16 if dt is F32 else dt, 2), randn(64, F32, 3)]),
+    'dropout_add_rms_norm': lambda dt: (lambda x, b, w: ulm_ops.dropout_add_rms_norm(x, b, w, 0.5, 1),
+                                        [randn((5, 64), F32, 1), randn((5, 64), BF16 if dt is F32 else dt, 2), randn(64, F32, 3)]),
+}
+# the operands of these go to library products, which may take another kernel for another alignment
+PROJECTED = {
+    'gated_linear': lambda dt: (ulm_ops.gated_linear, [randn((5, 64), dt, 1), randn((32, 64), dt, 2), randn((32, 64), dt, 3)]),
+    'gated_linear with dropout': lambda dt: (lambda x, w, v: ulm_ops.gated_linear(x, w, v, 0.5, 1), [randn((5, 64), dt, 1), randn((32, 64), dt, 2), randn((32, 64), dt, 3)]),
+}
+
+
+def outputs_and_gradients(op, ins, of_input=lambda t: t, of_grad=lambda t: t):
+    ins = [of_input(t).detach().requires_grad_() for t in ins]
+    out = op(*ins)
+    out = list(out) if isinstance(out, tuple) else [out]
+    grads = torch.autograd.grad(out, ins, [of_grad(randn(o.shape, o.dtype, 9 + i)) for i, o in enumerate(out)])
+    return [*out, *grads]
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+@pytest.mark.parametrize('name', [*OPS, *PROJECTED])
+def test_gradients_of_any_alignment(name, dtype):
+    op, ins = {**OPS, **PROJECTED}[name](dtype)
+    for got, want in zip(outputs_and_gradients(op, ins, of_grad=shifted), outputs_and_gradients(op, ins)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+@pytest.mark.parametrize('name', list(OPS))
+def test_operands_of_any_alignment(name, dtype):
+    op, ins = OPS[name](dtype)
+    for got, want in zip(outputs_and_gradients(op, ins, of_input=shifted), outputs_and_gradients(op, ins)):
+        assert torch.equal(got, want)

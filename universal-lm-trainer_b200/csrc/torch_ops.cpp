@@ -588,11 +588,17 @@ std::array<Tensor, 3> single_rope_backward(const Tensor& q, const Tensor& k, con
 // ---------------------------------------------------------------------------
 // RMSNorm, SwiGLU
 // ---------------------------------------------------------------------------
+bool aligned_to(const Tensor& t, int64_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
+// contiguous and 16-byte aligned
+Tensor dense16(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return aligned_to(c, 16) ? c : c.clone();
+}
 // [.., d] as [rows, d] with contiguous 16-byte aligned rows
 Tensor rows_of(const Tensor& x) {
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  const bool ok = x2.stride(1) == 1 && !(reinterpret_cast<uintptr_t>(x2.data_ptr()) & 15) && (x2.stride(0) * x2.element_size()) % 16 == 0;
-  return ok ? x2 : x2.contiguous();
+  const bool ok = x2.stride(1) == 1 && aligned_to(x2, 16) && (x2.stride(0) * x2.element_size()) % 16 == 0;
+  return ok ? x2 : dense16(x2);
 }
 void check_norm_weight(const Tensor& w, const Tensor& x, const char* who) {
   TORCH_CHECK_VALUE(w.device() == x.device() && x.dim() >= 1 && w.numel() == x.size(-1), who, " needs one weight per column, on the device of x");
@@ -646,7 +652,7 @@ Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps, std::optional
     y = empty_cuda(x.sizes(), yt, x);
     rstd = empty_cuda({rows}, at::kFloat, x);
     w = weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat ? weight : weight.to(at::kFloat);
-    w = w.contiguous();
+    w = dense16(w);
     ulm_rmsnorm_fwd_args a{};
     a.x = x2.data_ptr(); a.w = w.data_ptr(); a.y = y.data_ptr(); a.rstd = rstd.data_ptr<float>();
     a.x_stride = x2.stride(0); a.y_stride = d; a.rows = rows; a.d = (int32_t)d;
@@ -692,7 +698,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& branch, c
     x_new = empty_cuda(x.sizes(), at::kFloat, x);
     y = empty_cuda(x.sizes(), branch.scalar_type(), x);
     rstd = empty_cuda({rows}, at::kFloat, x);
-    w = weight.to(at::kFloat).contiguous();
+    w = dense16(weight.to(at::kFloat));
     ulm_rmsnorm_fwd_args a{};
     a.x = x2.data_ptr(); a.w = w.data_ptr(); a.y = y.data_ptr(); a.rstd = rstd.data_ptr<float>();
     a.x_stride = x2.stride(0); a.y_stride = d; a.rows = rows; a.d = (int32_t)d;
@@ -720,14 +726,8 @@ struct Drop {
   bool none() const { return p == 0; }
 };
 void check_drop(double p, const char* who) { TORCH_CHECK_VALUE(p >= 0 && p <= 1, who, ": p must lie between 0 and 1, got ", p); }
-bool aligned_to(const Tensor& t, int64_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 // t.to(type) without a way through the dispatcher where nothing is to be done
 Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
-// contiguous and 16-byte aligned
-Tensor dense16(const Tensor& t) {
-  const Tensor c = t.contiguous();
-  return aligned_to(c, 16) ? c : c.clone();
-}
 // [.., d] as [rows, d] with contiguous rows that all start on a multiple of `bytes`
 Tensor rows_on(const Tensor& x, int64_t bytes) {
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
@@ -828,7 +828,7 @@ std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& b
 struct SwigluBwd : OpNode {
   Drop drop;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor a = kept[0], b = kept[1], gy = as_type(g[0], a.scalar_type()), dy = drop.none() ? gy.contiguous() : dense16(gy);
+    const Tensor a = kept[0], b = kept[1], dy = dense16(as_type(g[0], a.scalar_type()));
     const Tensor da = empty_cuda(a.sizes(), a.scalar_type(), a), db = empty_cuda(a.sizes(), a.scalar_type(), a);
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), nullptr, dy.data_ptr(), da.data_ptr(), db.data_ptr(), a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
     check(drop.none() ? ulm_swiglu_bwd(&p) : ulm_swiglu_dropout(&p, true, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu backward");
@@ -843,8 +843,8 @@ Tensor gate(const Tensor& a_in, const Tensor& b_in, const Drop& drop) {
   {
     OpScope scope;
     c10::cuda::CUDAGuard dev(a_in.device());
-    a = drop.none() ? a_in.contiguous() : dense16(a_in);
-    b = drop.none() ? b_in.contiguous() : dense16(b_in);
+    a = dense16(a_in);
+    b = dense16(b_in);
     y = empty_cuda(a.sizes(), a.scalar_type(), a);
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), y.data_ptr(), nullptr, nullptr, nullptr, a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
     check(drop.none() ? ulm_swiglu_fwd(&p) : ulm_swiglu_dropout(&p, false, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu forward");
@@ -1061,7 +1061,7 @@ struct GatedBwd : OpNode {
   Drop drop;
   variable_list backward(variable_list& g, const variable_list& kept) override {
     const Tensor x = kept[0], w1 = kept[1], w3 = kept[2], ab = kept[3];
-    const Tensor dy = g[0].reshape({-1, g[0].size(-1)}).to(cd).contiguous(), x2 = x.reshape({-1, x.size(-1)});
+    const Tensor dy = dense16(g[0].reshape({-1, g[0].size(-1)}).to(cd)), x2 = x.reshape({-1, x.size(-1)});
     const Tensor dab = empty_cuda(ab.sizes(), cd, ab);
     swiglu_rows(ab, Tensor(), dy, dab, true, drop);
     const int64_t ff = w1.size(0);
