@@ -81,3 +81,22 @@ def test_operands_of_any_alignment(name, dtype):
     op, ins = OPS[name](dtype)
     for got, want in zip(outputs_and_gradients(op, ins, of_input=shifted), outputs_and_gradients(op, ins)):
         assert torch.equal(got, want)
+
+
+def odd_row(t):
+    """The same values; where there is one row, its stride is no multiple of anything (torch calls it contiguous all the same)."""
+    if t.dim() < 2:
+        return t
+    n = t.shape[-1]
+    v = torch.empty(n + 3, device='cuda', dtype=t.dtype).as_strided(t.shape, [n + 3] * (t.dim() - 1) + [1])
+    return v.copy_(t)
+
+
+@pytest.mark.parametrize('name', ['rms_norm', 'add_rms_norm', 'dropout_add_rms_norm'])
+def test_one_row_of_any_stride(name):
+    op, ins = OPS[name](F32)
+    ins = [t[:1] if t.dim() > 1 else t for t in ins]
+    assert odd_row(ins[0]).is_contiguous()
+    want = outputs_and_gradients(op, ins)
+    for got in (outputs_and_gradients(op, ins, of_input=odd_row), outputs_and_gradients(op, ins, of_grad=odd_row)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -594,11 +594,16 @@ Tensor dense16(const Tensor& t) {
   const Tensor c = t.contiguous();
   return aligned_to(c, 16) ? c : c.clone();
 }
+// the same of a matrix, its rows one behind the other: a single row is contiguous to torch whatever its stride
+Tensor dense_rows16(const Tensor& x2) {
+  const Tensor c = dense16(x2);
+  return c.stride(0) == c.size(1) ? c : c.as_strided(c.sizes(), {c.size(1), 1});
+}
 // [.., d] as [rows, d] with contiguous 16-byte aligned rows
 Tensor rows_of(const Tensor& x) {
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
   const bool ok = x2.stride(1) == 1 && aligned_to(x2, 16) && (x2.stride(0) * x2.element_size()) % 16 == 0;
-  return ok ? x2 : dense16(x2);
+  return ok ? x2 : dense_rows16(x2);
 }
 void check_norm_weight(const Tensor& w, const Tensor& x, const char* who) {
   TORCH_CHECK_VALUE(w.device() == x.device() && x.dim() >= 1 && w.numel() == x.size(-1), who, " needs one weight per column, on the device of x");
@@ -732,7 +737,7 @@ Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() ==
 Tensor rows_on(const Tensor& x, int64_t bytes) {
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
   const bool in_place = x2.stride(1) == 1 && (x2.size(0) <= 1 || x2.stride(0) >= x2.size(1)) && aligned_to(x2, bytes) && x2.stride(0) * x2.element_size() % bytes == 0;
-  return in_place ? x2 : dense16(x2);                     // a broadcast row among others
+  return in_place ? x2 : dense_rows16(x2);                // a broadcast row among others
 }
 
 Tensor dropout_launch(const Tensor& x_in, const Drop& drop) {
