@@ -100,3 +100,16 @@ def test_one_row_of_any_stride(name):
     want = outputs_and_gradients(op, ins)
     for got in (outputs_and_gradients(op, ins, of_input=odd_row), outputs_and_gradients(op, ins, of_grad=odd_row)):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('shape', [(2, 3, 64), (1, 1, 64), (64,), (2, 2, 2, 64)])
+@pytest.mark.parametrize('name', ['rms_norm', 'add_rms_norm', 'dropout_add_rms_norm'])
+def test_norms_of_any_number_of_dimensions(name, shape):
+    op, ins = OPS[name](F32)
+    rows = torch.Size(shape).numel() // 64
+    wide = [randn((rows, 64), t.dtype, 4 + i) if t.dim() > 1 else t for i, t in enumerate(ins)]
+    flat = outputs_and_gradients(op, wide)
+    shaped = outputs_and_gradients(lambda *a: op(*a), [t.view(shape) if t.dim() > 1 else t for t in wide])
+    for got, want in zip(shaped, flat):
+        assert torch.equal(got.reshape(want.shape), want)
+        assert got.shape == (shape if want.dim() > 1 else want.shape)

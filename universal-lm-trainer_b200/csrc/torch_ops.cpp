@@ -681,7 +681,7 @@ struct AddNormBwd : OpNode {
   variable_list backward(variable_list& g, const variable_list& kept) override {
     if (!g[1].defined()) return {g[0], g[0].to(bdtype), zero_grad(2)};      // the normalised output went unused
     const Tensor x = kept[0], w = kept[1], rstd = kept[2];
-    const int64_t rows = x.size(0), d = x.size(1);
+    const int64_t rows = rstd.size(0), d = w.numel();
     const Tensor dy = rows_of(g[1].to(bdtype)), ga = g[0].defined() ? rows_of(g[0].to(at::kFloat)) : Tensor();
     const Tensor dx = empty_cuda({rows, d}, at::kFloat, x), db = empty_cuda({rows, d}, bdtype, x);
     const Tensor dw = norm_backward(x.view({rows, d}), w, rstd, dy, eps, y_kind(bdtype, at::kFloat), dx, ga, db);
