@@ -113,3 +113,35 @@ def test_norms_of_any_number_of_dimensions(name, shape):
     for got, want in zip(shaped, flat):
         assert torch.equal(got.reshape(want.shape), want)
         assert got.shape == (shape if want.dim() > 1 else want.shape)
+
+
+ONCE = {
+    'swiglu_dropout': OPS['swiglu_dropout'],
+    'gated_linear with dropout': PROJECTED['gated_linear with dropout'],
+    'dropout_add_rms_norm': OPS['dropout_add_rms_norm'],
+    'streamed_cross_entropy': lambda dt: (lambda h, w: ulm_ops.streamed_cross_entropy(h, w, torch.tensor([3, 0, 8, 1, 8], device='cuda'), compute_dtype=BF16),
+                                          [randn((5, 64), dt, 1), randn((9, 64), dt, 2)]),
+}
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('name', list(ONCE))
+def test_second_derivatives_are_refused_and_not_left_out(name, dtype):
+    op, ins = ONCE[name](dtype)
+    ins = [t.requires_grad_() for t in ins]
+    out = op(*ins)
+    out = list(out) if isinstance(out, tuple) else [out]
+    ups = [torch.ones_like(o, requires_grad=True) for o in out]
+    want = torch.autograd.grad(out, ins, ups, retain_graph=True)
+    got = torch.autograd.grad(out, ins, ups, create_graph=True)
+    for g, w in zip(got, want):
+        assert g.requires_grad and torch.equal(g.detach(), w)
+    for i, x in enumerate(ins):
+        total = got[i].float().square().sum() + sum((t.float() ** 3).sum() for t in ins)
+        for wrt in (x, ups[0]):
+            with pytest.raises(RuntimeError, match='has no second derivative'):
+                torch.autograd.grad(total, wrt, retain_graph=True, allow_unused=True)
+        with pytest.raises(RuntimeError, match='has no second derivative'):
+            total.backward(retain_graph=True)
+    # what does not go through the gradients is not in the way
+    assert torch.autograd.grad(sum((t.float() ** 3).sum() for t in ins), ins[0])[0] is not None

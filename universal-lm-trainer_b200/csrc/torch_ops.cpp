@@ -78,6 +78,12 @@ struct OpScope {
   c10::impl::ExcludeDispatchKeyGuard no_autocast{c10::DispatchKeySet(c10::DispatchKey::AutocastCUDA)};
 };
 
+// Stands behind gradients that the kernels cannot differentiate, and raises when that is asked of it.
+struct NoSecondDerivative : torch::autograd::Node {
+  const char* op = "";
+  variable_list apply(variable_list&&) override { TORCH_CHECK(false, op, " has no second derivative: its gradient is a kernel's"); }
+};
+
 // Base of the ops' backward nodes: the tensors they keep, unpacked through autograd's own saved variables (version
 // checks, saved-tensor hooks, release after the backward).  All are unpacked BEFORE the op's scope opens: a hook may run
 // a checkpointed forward again, which has to record its graph and to autocast as it did the first time.
@@ -96,6 +102,24 @@ struct OpNode : torch::autograd::Node {
   virtual variable_list backward_recorded(variable_list& g, const variable_list& kept) {
     OpScope scope;
     return backward(g, kept);
+  }
+  // the same for an op that refuses to be differentiated twice: its gradients lead back to its inputs and to `g` through a node
+  // that raises, so that no part of a second derivative is left out without a word
+  variable_list backward_once(variable_list& g, const variable_list& kept, const char* op) {
+    variable_list out;
+    {
+      OpScope scope;
+      out = backward(g, kept);
+    }
+    std::shared_ptr<NoSecondDerivative> node(new NoSecondDerivative(), torch::autograd::deleteNode);
+    node->op = op;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(g);
+    for (const torch::autograd::Edge& e : next_edges())
+      if (e.is_valid()) edges.push_back(e);
+    node->set_next_edges(std::move(edges));
+    for (const Tensor& t : out)
+      if (t.defined()) torch::autograd::set_history(t, node);
+    return out;
   }
   variable_list apply(variable_list&& g) final {
     if (std::none_of(g.begin(), g.end(), [](const Tensor& t) { return t.defined(); })) {
@@ -792,6 +816,7 @@ struct DropNormBwd : OpNode {
     check(ulm_add_dropout_norm_bwd(&a, drop.p, (uint64_t)drop.seed), "dropout_add_rms_norm backward");
     return {dx, db, as_type(dw, wdtype)};
   }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "dropout_add_rms_norm"); }
 };
 
 std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& branch, const Tensor& weight, double p, int64_t seed, double eps) {
@@ -838,6 +863,9 @@ struct SwigluBwd : OpNode {
     ulm_swiglu_args p{a.data_ptr(), b.data_ptr(), nullptr, dy.data_ptr(), da.data_ptr(), db.data_ptr(), a.numel(), code_of(a.scalar_type()), 0, stream_of(a)};
     check(drop.none() ? ulm_swiglu_bwd(&p) : ulm_swiglu_dropout(&p, true, 0, 0, drop.p, (uint64_t)drop.seed), "swiglu backward");
     return {da, db};
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override {
+    return drop.none() ? OpNode::backward_recorded(g, kept) : backward_once(g, kept, "swiglu_dropout");
   }
 };
 
@@ -1095,6 +1123,9 @@ struct GatedBwd : OpNode {
     if (need3) dw3 = weight_grad(w3, db, x2);
     return {dx, dw1, dw3};
   }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override {
+    return drop.none() ? OpNode::backward_recorded(g, kept) : backward_once(g, kept, "gated_linear with dropout");
+  }
 };
 
 // Both projections write the two halves of one [rows, 2 ff] matrix: as one GEMM where the weights' 16-bit copies lie one
@@ -1330,6 +1361,7 @@ struct StreamedCeBwd : OpNode {
     else if (want_w && dw.scalar_type() != weight.scalar_type()) dw = dw.to(weight.scalar_type());
     return {dh, dw};
   }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "streamed_cross_entropy"); }
 };
 
 Tensor streamed_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t ignore_index, at::ScalarType cd,
