@@ -31,7 +31,7 @@ class ModelConfig:  # train.py:725-737
     tie_weights: bool = True
     use_gradient_checkpointing: bool = False
     # not the reference's: what a training step need not store between forward and backward
-    counter_dropout: bool = False   # feed-forward and residual dropout by ulm_ops.Dropout, inside the gate and the residual add + norm
+    counter_dropout: bool = False   # feed-forward and residual dropout by ulm_ops.Dropout, inside the gate and the residual add + norm; not to be captured in a CUDA graph
     streamed_loss: bool = False     # ulm_ops.streamed_cross_entropy: no logits
 
 

@@ -108,12 +108,18 @@ def _as_i64(seed):
 
 def next_dropout_seed():
     """A seed from torch's default CPU generator: `torch.manual_seed` fixes the sequence, and a checkpointed forward that is run
-    again draws the same ones.  No device is asked."""
+    again draws the same ones.  No device is asked.  Refused while a CUDA graph is captured or a module traced: the seed would be a
+    constant of the recording, which would drop the same elements at every run."""
+    if torch.jit.is_tracing() or (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()):
+        raise RuntimeError('a captured or traced step would drop the same elements at every run: give ulm_ops.dropout and its like a seed '
+                           'of your own where that is meant, or use nn.Dropout there')
     return int(torch.randint(0, 1 << 62, (), device='cpu'))         # whatever torch's default device is
 
 
 class Dropout(nn.Module):
-    """`nn.Dropout` on `dropout`: the same ``p`` and the same training switch, no stored mask, a mask of its own per call."""
+    """`nn.Dropout` on `dropout`, for CUDA fp16/bf16/fp32 tensors: the same ``p`` and the same training switch, no stored mask, a
+    mask of its own per call.  Where nn.Dropout would draw anew at each replay of a captured graph, this one, at work, refuses
+    the capture (`next_dropout_seed`)."""
 
     def __init__(self, p: float = 0.5):
         super().__init__()
