@@ -297,12 +297,6 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
           }
         }
       }
-      // Given up: our copies land before the pair's shared memory goes away.  Their barrier is rank 0's and may lack the other
-      // CTA's half, so it is time that is waited for: a thousand times what a load takes.
-      if (*abort_flag) {
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000ull) {}
-      }
     }
   } else if (warp == kEpiWarps + 1) {
     // ---------------- MMA issuer: rank 0 for both ----------------
@@ -490,6 +484,14 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
 
   fence_before_sync();
   __syncthreads();
+  // Some warp has given up: this CTA's copies and products in flight land before the pair's shared memory and TMEM go away.  The
+  // copies' barrier is rank 0's and may lack the other CTA's half, so it is time that is waited for: a thousand times what a load
+  // takes.  Here, where no warp can issue or give up any more: the producer may have issued its last copies before another warp gave up.
+  if (*abort_flag && threadIdx.x == 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {}
+  }
+  __syncwarp();
   cluster_sync();                                        // neither CTA leaves while the other's products or arrivals may reach it
   if (warp == kEpiWarps + 1) tmem_dealloc_pair(tmem_base, 512);
   if (threadIdx.x == 0 && ctl->fail_bits && p.status) atomicOr(p.status, ctl->fail_bits);
