@@ -3,6 +3,7 @@ rows of any stride, hooked modules, second derivatives, captured steps."""
 import pytest
 import torch
 
+import _native as N
 import ulm_ops
 
 pytestmark = pytest.mark.gpu
@@ -145,3 +146,23 @@ def test_second_derivatives_are_refused_and_not_left_out(name, dtype):
             total.backward(retain_graph=True)
     # what does not go through the gradients is not in the way
     assert torch.autograd.grad(sum((t.float() ** 3).sum() for t in ins), ins[0])[0] is not None
+
+
+@pytest.mark.parametrize('rows,d,piece_bytes', [(4096, 1024, 16 << 20), (16384, 256, 1 << 20), (300, 64, 1 << 16)])
+def test_memory_of_the_streamed_backward(rows, d, piece_bytes, monkeypatch):
+    """The softmax of a piece, hidden's fp32 sum, the parts of cut tiles; and the gradients."""
+    V = 32768
+    monkeypatch.setattr(ulm_ops, 'PIECE_BYTES', piece_bytes)
+    h, w = (randn(s, BF16, i).requires_grad_() for i, s in enumerate([(rows, d), (V, d)]))
+    loss = ulm_ops.streamed_cross_entropy(h, w, torch.randint(1, V, (rows,), device='cuda'))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    torch.autograd.grad(loss, [h, w])
+    peak = torch.cuda.max_memory_allocated() - before - 2 * (rows + V) * d
+    piece = max(256, piece_bytes // (2 * rows) // 256 * 256)
+    parts = N.lib().ulm_streamed_ce_slots(rows, V, d, piece, 1, 1) * 4
+    assert parts % (256 * 256 * 4) == 0
+    # what the allocator rounds each of four tensors up to: 2 MB at most
+    assert peak <= max(piece_bytes, 512 * rows) + 4 * rows * d + parts + (8 << 20)
+    assert peak >= 4 * rows * d

@@ -348,7 +348,8 @@ def chunked_cross_entropy(hidden, weight, target, ignore_index=0, chunk_rows=204
     return _ChunkedCE.apply(hidden, weight, target, int(ignore_index), int(chunk_rows), compute_dtype, denominator)
 
 
-# Largest workspace the backward of `streamed_cross_entropy` takes for one piece of the vocabulary: 16 bits per row and column.
+# Bytes that the backward of `streamed_cross_entropy` takes for the 16-bit softmax of one piece of the vocabulary (a piece has
+# at least 256 columns, so 512 bytes a row where that is more).  Not all it takes: see there.
 # At 32768 rows this is 16384 columns, two pieces of a vocabulary of 32000: 5.50 ms forward and backward against 5.67 with half
 # of it, 6.15 with a quarter and 5.48 in one piece (fewer passes over dh's fp32 sum, fewer launches).
 PIECE_BYTES = 1 << 30
@@ -358,12 +359,20 @@ def streamed_cross_entropy(hidden, weight, target, ignore_index=0, compute_dtype
     """`chunked_cross_entropy` without logits: hidden [rows, d], weight [V, d], target int64 [rows] -> the mean cross-entropy over the
     targets that are not ``ignore_index`` (or the sum over ``denominator``), for any number of rows and vocabulary columns and a
     width that is a multiple of 8.  The forward keeps one fp32 log-sum-exp per row; the backward forms the logits again, one piece
-    of the vocabulary at a time, in a workspace of at most about PIECE_BYTES, whatever the vocabulary.  The logits are never
-    rounded to 16 bits, so the loss is the fp32 loss of the 16-bit operands.  Gradients: in the operands' types; an fp32 weight's is
-    the fp32 sum, under `wgrad_in_place` added into its ``grad``.
+    of the vocabulary at a time.  The logits are never rounded to 16 bits, so the loss is the fp32 loss of the 16-bit operands.
+
+    Gradients: softmax - onehot is rounded once to the compute type, because the tensor cores multiply 16-bit numbers; the products'
+    sums are fp32.  hidden's gradient is rounded to the compute type (and widened for an fp32 hidden), a 16-bit weight's to its own;
+    an fp32 weight's is the fp32 sum of those rounded terms, under `wgrad_in_place` added into its ``grad``.  That is 2e-3 of a
+    gradient in bf16 and 2.6e-4 in fp16 (2-norm against 64 bits; fp32 arithmetic throughout, rounded at the end: 1.7e-3 and 2.1e-4), up to
+    4e-3 in bf16 with one to four rows, where one rounded number scales most of a gradient.
+
+    The backward's memory beside the gradients: PIECE_BYTES for the softmax of a piece (512 bytes a row if that is more), 4 rows d
+    bytes for hidden's fp32 sum where there is more than one piece, and 256 KB for each part of an output tile that is cut to fill
+    the SMs (290 parts at 32768 x 768 x 32000; `ulm_streamed_ce_slots` tells how many).
 
     Against the kept form: a quarter more arithmetic, none of its 2 rows V bytes between forward and backward, and the backward
-    may run more than once."""
+    may run more than once (but has no second derivative)."""
     if compute_dtype is None:
         compute_dtype = _loss_dtype(hidden)
     if hidden.shape[0] == 0:
