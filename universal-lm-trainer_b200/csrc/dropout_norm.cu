@@ -249,6 +249,10 @@ Split split_rows(int64_t rows, int nvec, int nv, int warps) {
 // with what is taken).
 int fwd_nv(int nvec, int E) { const int most = E == 8 || nvec <= 1024 ? 4 : 8, need = ceil_div(nvec, 32); return need < most ? need : most; }
 int bwd_nv(int d, int E) { return (d <= 2048 ? 8 : 16) / E; }
+// columns of a row that a warp of the backward has at most; a whole row fits the widest CTA, and a CTA's dw the 48 KB that need no opt-in
+constexpr int kBwdElems = 32 * 16;
+static_assert(kMaxRow <= kBwdWideWarps * kBwdElems, "rows");
+static_assert((kBwdWideWarps * kBwdElems + 2 * kBwdWideWarps) * sizeof(float) <= 48 * 1024, "shared memory");
 
 // A CTA of the backward per `groups` rows, 24 warps per SM at most (their registers fill it): each leaves one partial row
 constexpr int kBwdWarpsPerSm = 24, kMostBwdCtas = 3;
@@ -293,7 +297,8 @@ int launch_bwd(BwdParams p, int E, const DropMask& mask, int64_t* parts, cudaStr
   p.W = s.W;
   const int64_t blocks = bwd_blocks(p.rows, s);
   const int threads = s.W * s.groups * 32;
-  const size_t smem = (size_t)s.groups * p.d * sizeof(float);            // at most 12 x 512 floats: below 48 KB
+  // a warp has at most kBwdElems columns of a row, so groups x d is at most that for every warp of the CTA (32 KB)
+  const size_t smem = (size_t)s.groups * p.d * sizeof(float);
   *parts = blocks;
   auto go = [&](auto kern) { return launch_dependent(who, kern, (unsigned)blocks, threads, smem, st, p, mask); };
   const bool wide = s.W > kBwdWarps;
