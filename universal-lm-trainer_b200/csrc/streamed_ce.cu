@@ -67,7 +67,7 @@ constexpr size_t smem_bytes(int mode) { return 1024 + (size_t)kStages * kStage +
 static_assert(smem_bytes(kGrad) <= 227 * 1024, "shared memory");
 
 // One launch's work.  Items are numbered and dealt round the CTAs.
-//   statistics: 128 rows x a group of column tiles, whose statistics stay in registers;
+//   statistics: 256 rows x a group of column tiles, whose statistics stay in registers;
 //   G: one tile each, rows fastest, so that all CTAs read one stretch of W;
 //   products: dW's and dH's `whole` tiles, then of each the `rest` that would not fill a round of the SMs, cut into `split`
 //   stretches of the inner dimension; every stretch leaves its fp32 tile in a slot, and a second kernel adds up a tile's slots
