@@ -9,7 +9,8 @@
 // 3 us for dw's column sums.  A row belongs to W warps of a CTA (W = 1 up to 1024
 // elements forward) and is held in registers between its two uses; a lane owns vectors of E elements: eight where all
 // rows are whole 16-byte vectors of the 16-bit tensors, so that a vector is exactly one group of the mask, else four
-// (two lanes then form the same group, twice the generator's work: 20000 x 772 41 and 69 us).
+// (two lanes then form the same group, twice the generator's work: 20000 x 772 42 and 69 us, x 768 31 and 44).
+// From 2048 columns on the backward is at 4.6-5.0 TB/s (1024: 5.2): a row's loads, barrier and stores follow one another in its group.
 // dw: per-lane sums over a CTA's rows, added up over the CTA's groups in shared memory, one partial row per CTA, column
 // sums in a fixed order: no atomics.
 #include "col_sum.cuh"

@@ -20,9 +20,10 @@
 // accumulators of 256 TMEM columns so that a tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
 // contiguous, so dH reads W, and dW reads both G and H, as MN-major operands: rows of 64-element atoms, no transposed copies.
 // What bounds it from widths of 512 on: the tensor pipe, active 87-94 % of the cycles, and the clock that the power limit leaves.
-// 32768 x 768 x 32000 bf16, forward and backward: 4.4 ms in short runs, 5.0-5.2 ms under lasting load (1250 TFLOP/s of the
+// 32768 x 768 x 32000 bf16, forward and backward: 4.4 ms in short runs, 5.0-5.5 ms under lasting load, box by box (1160-1280 TFLOP/s of the
 // products that are formed; library GEMMs of the same shapes 1120-1190).  One CTA a product instead of a pair: 5.69 ms where the pair
-// took 5.48.  Narrower: the exponentials, 256 x 128 of them a CTA and tile; 32768 x 64 x 32000 2.3 ms.
+// took 5.48.  Narrower: the exponentials, 256 x 128 of them a CTA and tile, and G's way through memory (written once, read twice, at 6 TB/s);
+// the products' column tiles are 256 wide whatever the width, the rest zeros; 32768 x 64 x 32000 2.3 ms.
 // Waits are bounded (status bit and clean exit on expiry), like the attention kernels'.
 #include "lmhead_tiles.cuh"
 #include "tc.cuh"
