@@ -360,7 +360,8 @@ int ulm_lmhead_score(const ulm_lmhead_lse_args* a, uint8_t* hit, int32_t* part_i
  * The loss of train.py:2069-2082 over a vocabulary too large to keep [rows, V] logits for: the forward goes over the
  * vocabulary once with a running maximum and sum per row, the backward forms the logits again, `piece` columns at a time,
  * and keeps softmax - onehot of one piece in 16 bits.  z = h w^T stays in fp32 throughout (it is not rounded to the 16-bit type).
- * fwd: lse[r] and loss[r] = lse[r] - z[r, target[r]] in fp32; loss 0 where target[r] is ignore_index or no column; and the
+ * fwd: lse[r], of the logits as the backward forms them again, and loss[r] = -log softmax of the target in fp32, its logit
+ *      summed once more by fused multiply-adds (so loss[r] is not lse[r] minus a logit to the last bit); loss 0 where target[r] is ignore_index or no column; and the
  *      mean of the losses, *mean and *inv as ulm_loss_mean gives them.  scratch: ulm_streamed_ce_scratch(rows, V, d) floats.
  * bwd: with f = *factor_dev (times *factor2_dev; d total / d row loss) and G = softmax - onehot, 0 on the rows above:
  *      dh [rows, d] = f G w, dense, of the 16-bit type; dw [V, d] = f G^T h, 16-bit, or fp32 with dw_f32, or added to an fp32

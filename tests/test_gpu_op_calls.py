@@ -166,3 +166,29 @@ def test_memory_of_the_streamed_backward(rows, d, piece_bytes, monkeypatch):
     # what the allocator rounds each of four tensors up to: 2 MB at most
     assert peak <= max(piece_bytes, 512 * rows) + 4 * rows * d + parts + (8 << 20)
     assert peak >= 4 * rows * d
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('rows,V,d', [(300, 32000, 1024), (64, 4096, 768), (200, 1000, 128)])
+@pytest.mark.parametrize('logit', [10.0, 14.0, 17.0, 22.0])
+def test_gradient_of_rows_that_are_almost_certain(rows, V, d, dtype, logit):
+    """The target's probability p is close to 1; what is left of the gradient is as small as 1 - p."""
+    w = randn((V, d), F32, 1, d ** -0.5).to(dtype)
+    t = torch.randint(1, V, (rows,), generator=torch.Generator(device='cuda').manual_seed(2), device='cuda')
+    h, wt = randn((rows, d), F32, 3, 0.5), w[t].float()
+    h = (h + wt * ((logit - (h * wt).sum(1)) / wt.square().sum(1))[:, None]).to(dtype).requires_grad_()
+    up = 2.0 ** 12
+    dh, = torch.autograd.grad(ulm_ops.streamed_cross_entropy(h, w, t, denominator=1.0), [h], torch.tensor(up, device='cuda'))
+    z = h.detach().double() @ w.double().T
+    lse, at = torch.logsumexp(z, 1), torch.arange(rows, device='cuda')
+    g = torch.exp(z - lse[:, None])
+    rest = 1 - g[at, t]                                    # exact to 1e-16
+    g[at, t] = 0
+    others = g @ w.double()
+    want = up * (others - rest[:, None] * w[t].double())
+    unit = {F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    norm = w.double().norm(dim=1)
+    # the log-sum-exp's rounding to fp32, and 2^-22 for the sum behind it and its parts; one rounding of each probability and of
+    # p - 1; logits short by 2^-16 at most (1e-6 of 22); one rounding of the result
+    bound = up * ((2.0 ** -24 * lse.abs() + 2.0 ** -21) * norm[t] + (unit + 2.0 ** -16) * ((g * norm).sum(1) + rest * norm[t])) + unit * want.norm(dim=1)
+    assert bool(((dh.double() - want).norm(dim=1) <= bound).all())

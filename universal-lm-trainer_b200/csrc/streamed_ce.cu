@@ -342,7 +342,7 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
     if constexpr (MODE == kProducts) factor = out_factor(p.products.out[kColGrad]);         // the same for both
     uint32_t tt = 0;
     bool ok = true;
-    // the row's target column and, for G, its shift of the exponent 2^(z log2e + shift); asked for an item ahead
+    // the row's target column and, for G, its log-sum-exp; asked for an item ahead
     struct Row { int64_t target; float lse; };
     auto row_of = [&](int q) {
       Row w{-1, 0.f};
@@ -363,7 +363,7 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
       [[maybe_unused]] const int row0 = (int)grow - lane;                        // the warp's first row
       [[maybe_unused]] float m = -INFINITY, ssum = 0.f;  // base-2 domain: m = max(z) * log2e
       [[maybe_unused]] const int tgt = next.target >= 0 ? (int)next.target : -1;
-      [[maybe_unused]] const float shift = (float)Fmt<T>::g_shift - next.lse * kLog2e;
+      [[maybe_unused]] const float lse = next.lse;
       if constexpr (MODE == kStats || MODE == kGrad) next = row_of(q + pairs);
       for (int t = 0; ok && t < im.count; ++t, ++tt) {
         const uint32_t b = tt & 1;
@@ -424,8 +424,19 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
             }
           } else if constexpr (MODE == kGrad) {
             const int col0 = p.v0 + col_tile + c_blk;
+            const float shift = (float)Fmt<T>::g_shift - lse * kLog2e;           // of the exponent
             const uint64_t log2e2 = f2_pack(kLog2e, kLog2e), shift2 = f2_pack(shift, shift);
             uint32_t pk[32];
+            // p - 1 of the target, which may be far below an ulp of p: from the exponent by itself, without the rounding of lse log2e that
+            // the other columns' share, and not as a difference
+            float g_target = 0.f;
+            if ((unsigned)(tgt - col0) < 64u) {
+              float z = 0.f;
+#pragma unroll
+              for (int c = 0; c < 64; ++c) z = tgt - col0 == c ? __uint_as_float(acc[c]) : z;
+              const float hi = lse * kLog2e, lo = fmaf(lse, kLog2e, -hi);
+              g_target = (float)(1 << Fmt<T>::g_shift) * expm1f((fmaf(z, kLog2e, -hi) - lo) * kLn2);
+            }
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
               float g0, g1;
@@ -436,7 +447,7 @@ streamed_ce_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pa
             if ((unsigned)(tgt - col0) < 64u) {
 #pragma unroll
               for (int c = 0; c < 64; ++c)
-                if (tgt - col0 == c) acc[c] = __float_as_uint(__uint_as_float(acc[c]) - (float)(1 << Fmt<T>::g_shift));
+                if (tgt - col0 == c) acc[c] = __float_as_uint(g_target);
             }
 #pragma unroll
             for (int c = 0; c < 64; c += 2) pk[c >> 1] = tgt >= 0 ? Cvt<T>::pack2(__uint_as_float(acc[c]), __uint_as_float(acc[c + 1])) : 0u;
@@ -539,7 +550,7 @@ streamed_ce_join_kernel(const Products p) {
 }
 
 // lse[r] from the per-group (max, sum) pairs, loss[r] = lse[r] - z_target[r] (0 on ignored rows; loss holds z_target on entry): a
-// warp per row.  The target's logit is formed once more here, by fp32 fused multiply-adds, and takes the place of the tensor
+// warp per row.  For the loss the target's logit is formed once more here, by fp32 fused multiply-adds, and takes the place of the tensor
 // core's in the sum and in the difference: their additions round towards zero, 1e-6 of a logit at d = 1024 (-1.8e-5 +- 0.3e-5 at
 // 17, -0.3e-5 at d = 128), which stays in the mean (loss against 64 bits, d = 1024: 1.0e-6 -> 0.45e-6).  2 d bytes of H and W a row.  The CTA that finishes last adds up the rows' losses, in fp64 and a fixed order: mean = sum / n and inv = 1 / n,
 // n = *denom_dev, denom if that is positive, or the number of targets that are not ignore_index (at least 1).
@@ -593,9 +604,11 @@ streamed_ce_finish_kernel(const float* part_m, const float* part_s, int n_parts,
       z = warp_sum(z0 + z1);
     }
     if (lane == 0) {
+      // the log-sum-exp of the very logits that the backward forms again: the target's probability is their ratio, and what
+      // it lacks of 1 may be far below the two logits' difference.  In fp64 up to one rounding
+      lse[r] = (float)(((double)m + (double)log2f(s)) / (double)kLog2e);
       if (counts) s += exp2f(fmaf(z, kLog2e, -m)) - exp2f(fmaf(z_tensor, kLog2e, -m));
       const float log2_s = log2f(s);
-      lse[r] = (m + log2_s) * kLn2;
       // lse - z, with the large parts subtracted first and exactly: their difference is as small as the loss
       loss[r] = counts ? (fmaf(-z, kLog2e, m) + log2_s) * kLn2 : 0.f;
     }
