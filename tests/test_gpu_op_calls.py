@@ -192,3 +192,14 @@ def test_gradient_of_rows_that_are_almost_certain(rows, V, d, dtype, logit):
     # p - 1; logits short by 2^-16 at most (1e-6 of 22); one rounding of the result
     bound = up * ((2.0 ** -24 * lse.abs() + 2.0 ** -21) * norm[t] + (unit + 2.0 ** -16) * ((g * norm).sum(1) + rest * norm[t])) + unit * want.norm(dim=1)
     assert bool(((dh.double() - want).norm(dim=1) <= bound).all())
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('V,d', [(32000, 1024), (4096, 128), (1, 64)])
+def test_no_loss_is_negative(V, d, dtype):
+    w, h = randn((V, d), F32, 1, d ** -0.5).to(dtype), randn((256, d), F32, 2, 40.0).to(dtype)
+    t = (h.float() @ w.float().T).argmax(1)                # the most likely column of rows that are sharp: p = 1 for many
+    losses = torch.stack([ulm_ops.streamed_cross_entropy(h[i:i + 1], w, t[i:i + 1], ignore_index=-1) for i in range(256)])
+    assert bool((losses >= 0).all()) and bool((losses < 1e-6).any())
+    h[0, 0] = float('nan')
+    assert ulm_ops.streamed_cross_entropy(h[:1], w, t[:1], ignore_index=-1).isnan()

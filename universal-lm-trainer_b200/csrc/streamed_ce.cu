@@ -20,7 +20,7 @@
 // accumulators of 256 TMEM columns so that a tile's epilogue runs under the next one's products.  H and W are stored with d contiguous and G with the vocabulary
 // contiguous, so dH reads W, and dW reads both G and H, as MN-major operands: rows of 64-element atoms, no transposed copies.
 // What bounds it from widths of 512 on: the tensor pipe, active 87-94 % of the cycles, and the clock that the power limit leaves.
-// 32768 x 768 x 32000 bf16, forward and backward: 4.4 ms in short runs, 5.0-5.5 ms under lasting load, box by box (1160-1280 TFLOP/s of the
+// 32768 x 768 x 32000 bf16, forward and backward: 4.4 ms in short runs, 5.0-5.5 ms under lasting load, by the GPU (1160-1280 TFLOP/s of the
 // products that are formed; library GEMMs of the same shapes 1120-1190).  One CTA a product instead of a pair: 5.69 ms where the pair
 // took 5.48.  Narrower: the exponentials, 256 x 128 of them a CTA and tile, and G's way through memory (written once, read twice, at 6 TB/s);
 // the products' column tiles are 256 wide whatever the width, the rest zeros; 32768 x 64 x 32000 2.3 ms.
@@ -610,7 +610,8 @@ streamed_ce_finish_kernel(const float* part_m, const float* part_s, int n_parts,
       if (counts) s += exp2f(fmaf(z, kLog2e, -m)) - exp2f(fmaf(z_tensor, kLog2e, -m));
       const float log2_s = log2f(s);
       // lse - z, with the large parts subtracted first and exactly: their difference is as small as the loss
-      loss[r] = counts ? (fmaf(-z, kLog2e, m) + log2_s) * kLn2 : 0.f;
+      const float l = (fmaf(-z, kLog2e, m) + log2_s) * kLn2;
+      loss[r] = !counts || l < 0.f ? 0.f : l;             // the sum may round below its largest term; NaN stays
     }
   }
   __threadfence();
