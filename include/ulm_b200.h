@@ -85,6 +85,32 @@ typedef struct {
 } ulm_rope_args;
 int ulm_rope(const ulm_rope_args* a);
 
+/* ---- rotary positions of any width, pairing and frequency ------------------
+ * Beyond the reference, whose RoPE (above) has one form.  q: (B,Hq,S,D), k: (B,Hk,S,D) views of one dtype, any b/h/s strides,
+ * innermost contiguous; Hq = 0 or Hk = 0 leaves that tensor out.  The first R columns of a head are R/2 pairs, column i with
+ * i + R/2 or, interleaved, 2i with 2i + 1; the others are copied.  Pair i is turned by position * turns[i] / 2^64 full turns (the
+ * product modulo 2^64; turns and positions may be negative) and multiplied by `factor`; backward != 0 turns the other way (the
+ * adjoint; inputs are the output gradients).  fp32 arithmetic, one rounding to the dtype.
+ * positions: pos_kind 0: 0, 1, 2, .. along S; 1: int32, 2: int64, element (b, s) at positions[b * pos_sb + s * pos_ss].
+ * Outputs may be the inputs, with the same strides. */
+typedef struct {
+  const void* q; const void* k;
+  void* qo; void* ko;
+  const int64_t* turns;
+  const void* positions;
+  int64_t q_sb, q_sh, q_ss;
+  int64_t k_sb, k_sh, k_ss;
+  int64_t qo_sb, qo_sh, qo_ss;
+  int64_t ko_sb, ko_sh, ko_ss;
+  int64_t pos_sb, pos_ss;
+  int32_t B, Hq, Hk, S, D, R;
+  int32_t dtype;                       /* ULM_F16, ULM_BF16 or ULM_F32        */
+  int32_t interleaved, backward, pos_kind;
+  float factor; int32_t reserved;
+  void* stream;
+} ulm_rotary_args;
+int ulm_rotary(const ulm_rotary_args* a);
+
 /* ---- attention forward ---------------------------------------------------
  * Replaces fa_fwd (csrc/flash_attn_v100/flash_attn_v100.cu:337-364, kernel
  * fa_fwd_kernel :40-309), called from flash_attn_v100_cuda.py:76.

@@ -1,0 +1,72 @@
+"""Frequencies of the rotary positions, and which calls are refused on the host."""
+import math
+from fractions import Fraction
+
+import pytest
+import torch
+
+import ulm_ops
+
+
+def radians(turns):
+    return [Fraction(int(t), 1 << 64) * 2 * Fraction(math.pi) for t in turns]
+
+
+@pytest.mark.parametrize('dim', [2, 6, 20, 64, 128, 256])
+@pytest.mark.parametrize('base', [10000.0, 500000.0, 2.0])
+def test_frequencies_are_powers_of_the_base(dim, base):
+    turns, factor = ulm_ops.rotary_turns(dim, base)
+    assert turns.dtype == torch.int64 and turns.shape == (dim // 2,) and factor == 1.0
+    for i, w in enumerate(radians(turns)):
+        # a power, a quotient by 2 pi and its rounding to 64 bits
+        assert abs(float(w) - base ** (-2 * i / dim)) <= 2.0 ** -50 * base ** (-2 * i / dim) + 2.0 ** -61
+
+
+@pytest.mark.parametrize('dim', [2, 64, 96])
+def test_stretched_frequencies(dim):
+    plain = [float(w) for w in radians(ulm_ops.rotary_turns(dim)[0])]
+    get = lambda **kw: ulm_ops.rotary_turns(dim, scaling=kw)       # noqa: E731
+    close = lambda a, b: abs(a - b) <= 2.0 ** -48 * abs(b)         # noqa: E731
+    lin, f = get(kind='linear', factor=4.0)
+    assert f == 1.0 and all(close(float(w), p / 4) for w, p in zip(radians(lin), plain))
+    ntk, f = get(kind='ntk', factor=4.0)
+    ntk = [float(w) for w in radians(ntk)]
+    assert f == 1.0 and close(ntk[0], 1.0) and (dim == 2 or close(ntk[-1], plain[-1] / 4))
+    for kind, fast in (('parts', 4.0), ('yarn', 32.0)):
+        got, f = get(kind=kind, factor=4.0, original_length=4096, slow=1.0, fast=fast)
+        assert close(f, 0.1 * math.log(4.0) + 1.0) if kind == 'yarn' else f == 1.0
+        for w, p in zip(radians(got), plain):
+            turned = 4096 * p / (2 * math.pi)
+            keep = min(1.0, max(0.0, (turned - 1.0) / (fast - 1.0)))
+            assert close(float(w), p * keep + p / 4 * (1 - keep))
+            assert (turned < fast or close(float(w), p)) and (turned > 1 or close(float(w), p / 4))
+    assert torch.equal(get(kind='yarn', factor=4.0, original_length=4096)[0], get(kind='yarn', factor=4.0, original_length=4096, slow=1.0, fast=32.0)[0])
+    assert get(kind='yarn', factor=4.0, original_length=4096, attention_factor=1.25)[1] == 1.25
+    assert get(kind='linear', factor=1.0)[0].equal(ulm_ops.rotary_turns(dim)[0])
+
+
+@pytest.mark.parametrize('args', [
+    dict(rotary_dim=0), dict(rotary_dim=-2), dict(rotary_dim=7), dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, base=float('nan')),
+    dict(rotary_dim=8, base=float('inf')), dict(rotary_dim=8, scaling=dict(factor=2.0)), dict(rotary_dim=8, scaling=dict(kind='longer', factor=2.0)),
+    dict(rotary_dim=8, scaling=dict(kind='linear')), dict(rotary_dim=8, scaling=dict(kind='linear', factor=-1.0)), dict(rotary_dim=8, scaling=dict(kind='linear', factor=2.0, slow=1.0)),
+    dict(rotary_dim=8, scaling=dict(kind='parts', factor=2.0)), dict(rotary_dim=8, scaling=dict(kind='parts', factor=2.0, original_length=64, slow=4.0, fast=4.0)),
+    dict(rotary_dim=8, scaling=dict(kind='linear', factor=2.0, attention_factor=-1.0)),
+])
+def test_refused_frequencies(args):
+    with pytest.raises(ValueError):
+        ulm_ops.rotary_turns(**args)
+
+
+def test_the_module_keeps_nothing_in_a_state_dict_and_survives_casts():
+    m = ulm_ops.Rotary(64, scaling=dict(kind='linear', factor=2.0))
+    assert not m.state_dict() and m.half().turns.dtype == torch.int64
+    assert torch.equal(m.turns, ulm_ops.rotary_turns(64, scaling=dict(kind='linear', factor=2.0))[0])
+
+
+@pytest.mark.parametrize('where', ['cpu', 'meta'])
+def test_tensors_elsewhere_are_refused(where):
+    x = torch.zeros(1, 2, 3, 8, device=where)
+    with pytest.raises(ValueError, match='CUDA'):
+        ulm_ops.rotary(x, x, ulm_ops.rotary_turns(8)[0])
+    with pytest.raises(ValueError, match='CUDA'):
+        ulm_ops.rotary(x, None, ulm_ops.rotary_turns(8)[0])

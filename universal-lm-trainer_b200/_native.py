@@ -23,7 +23,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
-            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu']          # slowest first: they are compiled in parallel
+            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'rotary.cu']          # slowest first: they are compiled in parallel
 _HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
@@ -48,6 +48,14 @@ class RopeArgs(C.Structure):
                                     'qo_sb', 'qo_sh', 'qo_ss', 'ko_sb', 'ko_sh', 'ko_ss',
                                     'cos_stride', 'sin_stride')] +
                 [(n, i32) for n in ('B', 'H', 'S', 'dtype', 'backward')] + [('stream', vp)])
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = ([(n, vp) for n in ('q', 'k', 'qo', 'ko', 'turns', 'positions')] +
+                [(n, i64) for n in ('q_sb', 'q_sh', 'q_ss', 'k_sb', 'k_sh', 'k_ss', 'qo_sb', 'qo_sh', 'qo_ss',
+                                    'ko_sb', 'ko_sh', 'ko_ss', 'pos_sb', 'pos_ss')] +
+                [(n, i32) for n in ('B', 'Hq', 'Hk', 'S', 'D', 'R', 'dtype', 'interleaved', 'backward', 'pos_kind')] +
+                [('factor', f32), ('reserved', i32), ('stream', vp)])
 
 
 class AttnFwdArgs(C.Structure):
@@ -128,6 +136,7 @@ EXPORTS = {
     'ulm_device_ok': (C.c_int, [C.c_int]),
     'ulm_launch_count': (C.c_uint64, []),
     'ulm_rope': (C.c_int, [C.POINTER(RopeArgs)]),
+    'ulm_rotary': (C.c_int, [C.POINTER(RotaryArgs)]),
     'ulm_attn_fwd': (C.c_int, [C.POINTER(AttnFwdArgs)]),
     'ulm_attn_fwd_rope_qk': (C.c_int, [C.POINTER(AttnFwdArgs), vp, i64, i64, i64]),
     'ulm_attn_bwd': (C.c_int, [C.POINTER(AttnBwdArgs)]),

@@ -897,6 +897,142 @@ Tensor swiglu_dropout(const Tensor& a, const Tensor& b, double p, int64_t seed) 
 }
 
 // ---------------------------------------------------------------------------
+// rotary positions of any form, and the attention behind them
+// ---------------------------------------------------------------------------
+struct Turning {
+  bool interleaved = false, inverse = false;
+  double factor = 1.0;
+};
+// Each head's columns contiguous and on 16-byte boundaries where its width allows: read in place.  Others are copied.
+Tensor rotary_ready(const Tensor& t) {
+  bool ok = t.stride(3) == 1 || t.size(3) == 1;
+  int64_t bytes = 16;
+  while (t.size(3) * t.element_size() % bytes) bytes /= 2;
+  ok = ok && !(reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes);
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) * t.element_size() % bytes == 0));
+  if (ok) return t;
+  const Tensor c = t.contiguous();
+  return c.unsafeGetTensorImpl() == t.unsafeGetTensorImpl() ? c.clone() : c;
+}
+// A dense tensor in the input's memory order: heads beside one another within a position, or positions within a head
+Tensor rotary_out_like(const Tensor& t) {
+  if (t.is_non_overlapping_and_dense()) return empty_strided(t.sizes(), t.strides(), t.scalar_type(), t);
+  const int64_t B = t.size(0), H = t.size(1), S = t.size(2), D = t.size(3);
+  if (t.stride(2) >= t.stride(1)) return empty_strided({B, H, S, D}, {S * H * D, D, H * D, 1}, t.scalar_type(), t);
+  return empty_cuda(t.sizes(), t.scalar_type(), t);
+}
+
+// q or k may be undefined; positions: undefined, [S], or [B or 1, S]
+void rotary_launch(const Tensor& q, const Tensor& k, const Tensor& qo, const Tensor& ko, const Tensor& turns, const Tensor& positions, const Turning& how) {
+  const Tensor& any = q.defined() ? q : k;
+  ulm_rotary_args a{};
+  // a dimension of one element is never stepped along: its stride, which may be anything, does not count
+  auto step = [](const Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); };
+  if (q.defined()) {
+    a.q = q.data_ptr(); a.qo = qo.data_ptr(); a.Hq = (int32_t)q.size(1);
+    a.q_sb = step(q, 0); a.q_sh = step(q, 1); a.q_ss = step(q, 2);
+    a.qo_sb = step(qo, 0); a.qo_sh = step(qo, 1); a.qo_ss = step(qo, 2);
+  }
+  if (k.defined()) {
+    a.k = k.data_ptr(); a.ko = ko.data_ptr(); a.Hk = (int32_t)k.size(1);
+    a.k_sb = step(k, 0); a.k_sh = step(k, 1); a.k_ss = step(k, 2);
+    a.ko_sb = step(ko, 0); a.ko_sh = step(ko, 1); a.ko_ss = step(ko, 2);
+  }
+  a.turns = turns.data_ptr<int64_t>();
+  if (positions.defined()) {
+    a.positions = positions.data_ptr(); a.pos_kind = positions.scalar_type() == at::kInt ? 1 : 2;
+    a.pos_ss = positions.size(-1) == 1 ? 0 : positions.stride(-1);
+    a.pos_sb = positions.dim() == 1 || positions.size(0) == 1 ? 0 : positions.stride(0);
+  }
+  a.B = (int32_t)any.size(0); a.S = (int32_t)any.size(2); a.D = (int32_t)any.size(3); a.R = (int32_t)(2 * turns.numel());
+  a.dtype = code_of(any.scalar_type()); a.interleaved = how.interleaved; a.backward = how.inverse; a.factor = (float)how.factor;
+  a.stream = stream_of(any);
+  check(ulm_rotary(&a), "rotary");
+}
+
+void check_turns(const Tensor& turns, const Tensor& positions, const Tensor& like, int64_t B, int64_t S, int64_t D, const char* who) {
+  TORCH_CHECK_VALUE(turns.device() == like.device() && turns.scalar_type() == at::kLong && turns.dim() == 1 && turns.is_contiguous() && turns.numel() >= 1 &&
+                        2 * turns.numel() <= D,
+                    who, " needs one int64 number of turns for each pair of columns (rotary_turns), on the device of the tensors and for no more columns than a head has");
+  if (!positions.defined()) return;
+  TORCH_CHECK_VALUE(positions.device() == like.device() && (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) &&
+                        ((positions.dim() == 1 && positions.size(0) == S) ||
+                         (positions.dim() == 2 && positions.size(1) == S && (positions.size(0) == B || positions.size(0) == 1))),
+                    who, " takes int32 or int64 positions [S], [1, S] or [B, S], on the device of the tensors");
+}
+
+Tensor rotary_one(const Tensor& x, const Tensor& turns, const OptTensor& positions, bool interleaved, double factor, bool inverse);
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& turns, const OptTensor& positions, bool interleaved, double factor, bool inverse);
+
+// The gradient of a rotation is the rotation back; linear in its input, it can be differentiated again.
+struct RotaryBwd : OpNode {
+  Turning how;                                             // of the gradient
+  at::ScalarType dtype;
+  Tensor positions(const variable_list& kept) { return kept.size() > 1 ? kept[1] : Tensor(); }
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    Tensor in[2], out[2];
+    for (size_t i = 0; i < num_outputs(); ++i)
+      if (g[i].defined()) {
+        in[i] = rotary_ready(as_type(g[i], dtype));
+        out[i] = rotary_out_like(in[i]);
+      }
+    rotary_launch(in[0], in[1], out[0], out[1], kept[0], positions(kept), how);
+    variable_list r;
+    for (size_t i = 0; i < num_outputs(); ++i) r.push_back(out[i].defined() ? out[i] : zero_grad(i));
+    return r;
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override {
+    const Tensor at = positions(kept);
+    const OptTensor pos = at.defined() ? OptTensor(at) : std::nullopt;
+    variable_list r;
+    for (size_t i = 0; i < num_outputs(); ++i)
+      r.push_back(g[i].defined() ? ::rotary_one(g[i].to(dtype), kept[0], pos, how.interleaved, how.factor, how.inverse) : zero_grad(i));
+    return r;
+  }
+};
+
+void check_rotary(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()) && x.dim() == 4, "rotary needs CUDA fp16/bf16/fp32 (B,H,S,D) tensors: ", name, " is not one");
+  for (int i = 0; i < 4; ++i) TORCH_CHECK_VALUE(x.size(i) <= INT32_MAX, "rotary: ", name, " is too large");
+}
+
+// one or two tensors; k undefined: one
+std::array<Tensor, 2> rotate(const Tensor& q_in, const Tensor& k_in, const Tensor& turns, const OptTensor& positions_o, const Turning& how) {
+  const Tensor positions = positions_o.value_or(Tensor());
+  check_turns(turns, positions, q_in, q_in.size(0), q_in.size(2), q_in.size(3), "rotary");
+  std::array<Tensor, 2> out;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(q_in.device());
+    const Tensor q = rotary_ready(q_in), k = k_in.defined() ? rotary_ready(k_in) : Tensor();
+    out[0] = rotary_out_like(q);
+    if (k.defined()) out[1] = rotary_out_like(k);
+    rotary_launch(q, k, out[0], out[1], turns, positions, how);
+  }
+  if (k_in.defined() ? !no_graph(q_in, k_in) : !no_graph(q_in)) {
+    auto node = k_in.defined() ? make_node<RotaryBwd>(q_in, k_in) : make_node<RotaryBwd>(q_in);
+    node->how = {how.interleaved, !how.inverse, how.factor}; node->dtype = q_in.scalar_type();
+    node->keep(turns);
+    if (positions.defined()) node->keep(positions);
+    for (const Tensor& t : out)
+      if (t.defined()) torch::autograd::set_history(t, node);
+  }
+  return out;
+}
+Tensor rotary_one(const Tensor& x, const Tensor& turns, const OptTensor& positions, bool interleaved, double factor, bool inverse) {
+  check_rotary(x, "x");
+  return rotate(x, Tensor(), turns, positions, {interleaved, inverse, factor})[0];
+}
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& turns, const OptTensor& positions, bool interleaved, double factor, bool inverse) {
+  check_rotary(q, "q");
+  check_rotary(k, "k");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.device() == q.device() && k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3),
+                    "rotary needs q and k of one type, device, batch, length and head width");
+  const std::array<Tensor, 2> out = rotate(q, k, turns, positions, {interleaved, inverse, factor});
+  return {out[0], out[1]};
+}
+
+// ---------------------------------------------------------------------------
 // linear layers
 // ---------------------------------------------------------------------------
 // What `wgrad_in_place` and `weight_cast_scope` switch on belongs to the thread that entered them and to the backward
@@ -1445,6 +1581,8 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "add_rms_norm", &::add_rms_norm);
   def_op(m, "swiglu", &::swiglu);
   def_op(m, "swiglu_dropout", &::swiglu_dropout);
+  def_op(m, "rotary", &::rotary);
+  def_op(m, "rotary_one", &::rotary_one);
   def_op(m, "dropout", &::dropout);
   def_op(m, "dropout_add_rms_norm", &::dropout_add_rms_norm);
   py::class_<ContextToken>(m, "ContextToken").def("leave", &leave_context);

@@ -1,4 +1,4 @@
-"""RMSNorm, the SwiGLU gate, dropout and the cross-entropy on the sm_100a library, as autograd ops.
+"""RMSNorm, the SwiGLU gate, dropout, rotary positions and the cross-entropy on the sm_100a library, as autograd ops.
 
 The reference has no custom kernels for these: ``FusedRMSNorm`` calls
 F.rms_norm (train.py:1862-1875), dropout is nn.Dropout and ``compute_loss`` loops fc_out +
@@ -7,6 +7,7 @@ below keep those names and argument meanings.
 """
 import contextlib
 import ctypes as C
+import math
 
 import torch
 import torch.nn as nn
@@ -135,6 +136,87 @@ class Dropout(nn.Module):
 
     def extra_repr(self):
         return f'p={self.p}'
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions of any width, pairing and frequency
+# ---------------------------------------------------------------------------
+def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
+    """``(turns, factor)`` for `rotary`: how far each of the rotary_dim / 2 pairs turns per position, as an int64 tensor of 2^-64 turns,
+    and what the turned vectors are multiplied by.  Pair i turns by w_i = base^(-2i / rotary_dim) radians; ``scaling`` stretches that:
+
+      None                              as it is
+      dict(kind='linear', factor=f)     w_i / f: positions f times closer together
+      dict(kind='ntk', factor=f)        base * f^(rotary_dim / (rotary_dim - 2)): the slowest pair f times slower, the fastest as it is
+      dict(kind='parts', factor=f, original_length=L, slow=a, fast=b)
+                                        pairs that turn at least b times within L positions stay, those that turn at most a times
+                                        are f times slower, those between in proportion
+      dict(kind='yarn', ...)            'parts' (a = 1, b = 32 by default), and q and k multiplied by 0.1 ln f + 1 each (Peng, Quesnelle, Fan
+                                        and Shippole, "YaRN: efficient context window extension of large language models", 2023)
+
+    ``attention_factor=`` beside any of them replaces the multiplier.  Computed on the host in 64 bits."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f'rotary_dim has to be a positive even number, but got {rotary_dim}')
+    if not base > 1.0 or not math.isfinite(base):
+        raise ValueError(f'base has to be a finite number above 1, but got {base}')
+    spec = dict(scaling or {})
+    kind = spec.pop('kind', None)
+    if scaling is not None and kind not in ('linear', 'ntk', 'parts', 'yarn'):
+        raise ValueError(f"scaling is one of kind 'linear', 'ntk', 'parts' and 'yarn', but got {scaling}")
+    multiplier = float(spec.pop('attention_factor', 0.0))
+    w = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if kind is not None:
+        f = float(spec.pop('factor', 0.0))
+        if not f > 0.0 or not math.isfinite(f):
+            raise ValueError(f'scaling needs a positive factor, but got {scaling}')
+        if kind == 'linear':
+            w = [x / f for x in w]
+        elif kind == 'ntk':
+            if rotary_dim > 2:
+                w = [(base * f ** (rotary_dim / (rotary_dim - 2.0))) ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        else:
+            length, slow, fast = (float(spec.pop(n, d)) for n, d in (('original_length', 0.0), ('slow', 1.0), ('fast', 32.0)))
+            if not length > 0.0 or not fast > slow:
+                raise ValueError(f"scaling of kind '{kind}' needs an original_length and slow < fast, but got {scaling}")
+            keep = [min(1.0, max(0.0, (length * x / (2.0 * math.pi) - slow) / (fast - slow))) for x in w]
+            w = [x * k + x / f * (1.0 - k) for x, k in zip(w, keep)]
+            if kind == 'yarn' and not multiplier:
+                multiplier = 0.1 * math.log(f) + 1.0
+    if spec:
+        raise ValueError(f'scaling does not know {sorted(spec)}')
+    if not math.isfinite(multiplier) or multiplier < 0.0:
+        raise ValueError(f'the attention factor has to be a positive number, but got {multiplier}')
+    # w / 2 pi of 2^64, as a signed number of the same bits: a float has 53 of them, so that an angle is off by 2^-54 of itself
+    turns = [round(math.ldexp(x / (2.0 * math.pi), 64)) % (1 << 64) for x in w]
+    return torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device), multiplier or 1.0
+
+
+def rotary(q, k, turns, positions=None, interleaved=False, factor=1.0, inverse=False):
+    """The first columns of each head, turned by an angle that grows with the position: q (B,Hq,S,D) and k (B,Hk,S,D), fp16, bf16 or fp32
+    views of any stride, of one type -> both turned, in the memory order they came in; ``k`` may be None (None comes back).
+    ``turns`` (`rotary_turns`) has one number for each pair of columns: i with i + len(turns), or with ``interleaved`` 2i with 2i + 1;
+    columns beyond 2 len(turns) pass through.  ``positions``: int32 or int64 [S] or [B, S] (packed sequences, single tokens of a cached
+    context; negative ones turn the other way), 0, 1, 2, .. without.  Exact at any distance: the angle is a 64-bit fraction of a turn.
+    fp32 arithmetic, one rounding.  ``inverse`` turns the other way (times the same ``factor``), which is also the gradient."""
+    if k is None:
+        return N.ext().rotary_one(q, turns, positions, bool(interleaved), float(factor), bool(inverse)), None
+    return N.ext().rotary(q, k, turns, positions, bool(interleaved), float(factor), bool(inverse))
+
+
+class Rotary(nn.Module):
+    """`rotary` with the frequencies of `rotary_turns`, which are no parameters and not part of a state dict."""
+
+    def __init__(self, rotary_dim, base=10000.0, interleaved=False, scaling=None):
+        super().__init__()
+        self.rotary_dim, self.base, self.interleaved, self.scaling = rotary_dim, base, interleaved, scaling
+        turns, self.factor = rotary_turns(rotary_dim, base, scaling, device='cpu')
+        self.register_buffer('turns', turns, persistent=False)
+
+    def forward(self, q, k, positions=None):
+        return rotary(q, k, self.turns, positions, self.interleaved, self.factor)
+
+    def extra_repr(self):
+        return f'{self.rotary_dim}, base={self.base}, interleaved={self.interleaved}, scaling={self.scaling}'
 
 
 # ---------------------------------------------------------------------------
