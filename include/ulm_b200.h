@@ -309,6 +309,43 @@ int ulm_add_dropout_norm_fwd(const ulm_rmsnorm_fwd_args* a, double p, uint64_t s
 int ulm_add_dropout_norm_bwd(const ulm_rmsnorm_bwd_args* a, double p, uint64_t seed);
 int64_t ulm_add_dropout_norm_partial_rows(int64_t rows);
 
+/* ---- the norms behind and in front of a block, with the residual add between them ----
+ * No counterpart in the reference, whose blocks have the second norm alone (train.py:1989-1993).
+ * fwd: u = branch rstd_branch, rstd_branch = rsqrt(mean(branch^2) + eps); x_out = x + s sigmoid(gate) v u; y = w x_out rstd,
+ *      rstd = rsqrt(mean(x_out^2) + eps).  x, x_out: fp32 [rows, d]; branch, gate (NULL: no gate, its factor is 1), y: [rows, d] of
+ *      dtype (16 bits); v, w: fp32 [d]; rstd_branch, rstd: fp32 [rows], kept for the backward.  s: with scale_channels fp32 [d] at
+ *      `scale`, otherwise one number, at `scale`, or scale_value where that is NULL.
+ * bwd: x is the forward's x_out, dy the gradient of y, g_add (fp32, may be NULL) the one that reaches x_out from elsewhere.  dx: the whole
+ *      gradient of x_out, which is x's; d_branch, d_gate (NULL without a gate); dw, dv: fp32 [d], dscale (may be NULL): fp32 [d] or [1],
+ *      all three OVERWRITTEN.  partial: ulm_norm_add_norm_partial(rows, d) floats.
+ * Rows of at most 8192 elements, a multiple of 4; fp32 rows 16-byte aligned, 16-bit rows 8-byte aligned or better.  All sums run in a
+ * fixed order. */
+typedef struct {
+  const float* x; const void* branch; const void* gate;
+  const float* v; const float* w; const float* scale;
+  float* x_out; void* y; float* rstd_branch; float* rstd;
+  int64_t x_stride, branch_stride, gate_stride, xout_stride, y_stride;
+  int64_t rows; int32_t d;
+  int32_t dtype, scale_channels;
+  float scale_value, eps; int32_t reserved;
+  void* stream;
+} ulm_norm_add_norm_fwd_args;
+typedef struct {
+  const float* x; const void* branch; const void* gate;
+  const float* v; const float* w; const float* scale;
+  const void* dy; const float* g_add; const float* rstd_branch; const float* rstd;
+  float* dx; void* d_branch; void* d_gate;
+  float* dw; float* dv; float* dscale; float* partial;
+  int64_t x_stride, branch_stride, gate_stride, dy_stride, gadd_stride, dx_stride, dbranch_stride, dgate_stride;
+  int64_t rows; int32_t d;
+  int32_t dtype, scale_channels;
+  float scale_value;
+  void* stream;
+} ulm_norm_add_norm_bwd_args;
+int ulm_norm_add_norm_fwd(const ulm_norm_add_norm_fwd_args* a);
+int ulm_norm_add_norm_bwd(const ulm_norm_add_norm_bwd_args* a);
+int64_t ulm_norm_add_norm_partial(int64_t rows, int32_t d);
+
 /* ---- chunked cross-entropy row kernels -----------------------------------
  * The reference loops fc_out + F.cross_entropy(reduction='sum') over chunks of
  * rows (train.py:2075-2079).  These kernels are the softmax part over one

@@ -23,8 +23,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
-            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'rotary.cu']          # slowest first: they are compiled in parallel
-_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
+            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'norm_add_norm.cu', 'rotary.cu']          # slowest first: they are compiled in parallel
+_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'norm_rows.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
 _EXT_SOURCE = 'torch_ops.cpp'
@@ -94,6 +94,19 @@ class RmsBwdArgs(C.Structure):
                 ('g_add', vp), ('d_branch', vp), ('gadd_stride', i64), ('dbranch_stride', i64)]
 
 
+class NormAddNormFwdArgs(C.Structure):
+    _fields_ = ([(n, vp) for n in ('x', 'branch', 'gate', 'v', 'w', 'scale', 'x_out', 'y', 'rstd_branch', 'rstd')] +
+                [(n, i64) for n in ('x_stride', 'branch_stride', 'gate_stride', 'xout_stride', 'y_stride', 'rows')] +
+                [(n, i32) for n in ('d', 'dtype', 'scale_channels')] + [('scale_value', f32), ('eps', f32), ('reserved', i32), ('stream', vp)])
+
+
+class NormAddNormBwdArgs(C.Structure):
+    _fields_ = ([(n, vp) for n in ('x', 'branch', 'gate', 'v', 'w', 'scale', 'dy', 'g_add', 'rstd_branch', 'rstd', 'dx', 'd_branch', 'd_gate',
+                                   'dw', 'dv', 'dscale', 'partial')] +
+                [(n, i64) for n in ('x_stride', 'branch_stride', 'gate_stride', 'dy_stride', 'gadd_stride', 'dx_stride', 'dbranch_stride', 'dgate_stride', 'rows')] +
+                [(n, i32) for n in ('d', 'dtype', 'scale_channels')] + [('scale_value', f32), ('stream', vp)])
+
+
 class SwigluArgs(C.Structure):
     _fields_ = [('a', vp), ('b', vp), ('y', vp), ('dy', vp), ('da', vp), ('db', vp), ('n', i64),
                 ('dtype', i32), ('reserved', i32), ('stream', vp)]
@@ -159,6 +172,9 @@ EXPORTS = {
     'ulm_add_dropout_norm_fwd': (C.c_int, [C.POINTER(RmsFwdArgs), f64, u64]),
     'ulm_add_dropout_norm_bwd': (C.c_int, [C.POINTER(RmsBwdArgs), f64, u64]),
     'ulm_add_dropout_norm_partial_rows': (i64, [i64]),
+    'ulm_norm_add_norm_fwd': (C.c_int, [C.POINTER(NormAddNormFwdArgs)]),
+    'ulm_norm_add_norm_bwd': (C.c_int, [C.POINTER(NormAddNormBwdArgs)]),
+    'ulm_norm_add_norm_partial': (i64, [i64, i32]),
     'ulm_streamed_ce_fwd': (C.c_int, [C.POINTER(StreamedCeArgs)]),
     'ulm_streamed_ce_bwd': (C.c_int, [C.POINTER(StreamedCeArgs), C.POINTER(StreamedCeGrads)]),
     'ulm_streamed_ce_scratch': (i64, [i64, i32, i32]),

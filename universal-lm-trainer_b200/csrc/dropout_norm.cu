@@ -14,6 +14,7 @@
 // dw: per-lane sums over a CTA's rows, added up over the CTA's groups in shared memory, one partial row per CTA, column
 // sums in a fixed order: no atomics.
 #include "col_sum.cuh"
+#include "norm_rows.cuh"
 #include "philox.cuh"
 
 namespace ulm {
@@ -21,59 +22,6 @@ namespace {
 
 constexpr int kMaxRow = 8192;
 constexpr int kFwdWarps = 8, kBwdWarps = 12, kBwdWideWarps = 16;
-
-template <int E>
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[E]) {
-#pragma unroll
-  for (int j = 0; j < E; j += 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p + j);
-    v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
-  }
-}
-template <int E>
-__device__ __forceinline__ void store_f32(float* p, const float (&v)[E]) {
-#pragma unroll
-  for (int j = 0; j < E; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-}
-// E 16-bit elements as they lie in memory
-template <int E> struct Raw { uint32_t u[E / 2]; };
-template <typename TY, int E>
-__device__ __forceinline__ Raw<E> load_raw(const TY* p) {
-  Raw<E> r;
-  if constexpr (E == 8) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    r.u[0] = q.x; r.u[1] = q.y; r.u[2] = q.z; r.u[3] = q.w;
-  } else {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
-    r.u[0] = q.x; r.u[1] = q.y;
-  }
-  return r;
-}
-template <typename TY, int E>
-__device__ __forceinline__ void unpack_raw(const Raw<E>& r, float (&v)[E]) {
-#pragma unroll
-  for (int j = 0; j < E / 2; ++j) { const float2 f = Cvt<TY>::unpack2(r.u[j]); v[2 * j] = f.x; v[2 * j + 1] = f.y; }
-}
-template <typename TY, int E>
-__device__ __forceinline__ void store_16(TY* p, const float (&v)[E]) {
-  uint32_t u[E / 2];
-#pragma unroll
-  for (int j = 0; j < E / 2; ++j) u[j] = Cvt<TY>::pack2(v[2 * j], v[2 * j + 1]);
-  if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-  else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-}
-
-// Sum over the W warps of a row.  `slots`: this call's own kMaxWarps floats; consecutive calls of a warp alternate between two
-// sets, so that one barrier a call is enough.
-__device__ __forceinline__ float row_sum(float v, int W, int group, int warp, int lane, float* slots) {
-  v = warp_sum(v);
-  if (W == 1) return v;
-  if (lane == 0) slots[warp] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * W) : "memory");
-  float t = 0.f;
-  for (int i = 0; i < W; ++i) t += slots[group * W + i];
-  return t;
-}
 
 struct FwdParams {
   const float* x; const void* branch; const float* w; float* x_out; void* y; float* rstd;
@@ -231,18 +179,6 @@ add_dropout_norm_bwd_kernel(const BwdParams p, const __grid_constant__ DropMask 
   }
 }
 
-int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// Warps a row and rows a CTA.  Few rows (less than the SMs take at full CTAs) are spread over more, smaller CTAs.
-struct Split { int W, groups; };
-Split split_rows(int64_t rows, int nvec, int nv, int warps) {
-  Split s;
-  s.W = ceil_div(nvec, 32 * nv);
-  s.groups = warps / s.W > 0 ? warps / s.W : 1;
-  const int64_t spread = (rows + kNumSMs - 1) / kNumSMs;
-  if (spread < s.groups) s.groups = spread < 1 ? 1 : (int)spread;
-  return s;
-}
 // Elements a lane holds.  Forward 32 with vectors of eight (one warp a row up to 1024), with vectors of four 16 up to rows of
 // 4096 and 32 beyond.  Backward, where a
 // row's z, dy, g and dw are alive together, 8 up to rows of 2048 and 16 beyond: us with 8 / 16, bf16,
@@ -263,9 +199,6 @@ int64_t bwd_blocks(int64_t rows, const Split& s) {
   per_sm = per_sm < 1 ? 1 : per_sm > kMostBwdCtas ? kMostBwdCtas : per_sm;
   return want < per_sm * kNumSMs ? want : per_sm * kNumSMs;
 }
-
-bool ok16(const void* p, int64_t stride, int E) { return !(reinterpret_cast<uintptr_t>(p) & (2 * E - 1)) && stride % E == 0; }
-bool ok32(const void* p, int64_t stride) { return !(reinterpret_cast<uintptr_t>(p) & 15) && stride % 4 == 0; }
 
 int check_shape(const char* who, int x_dtype, int w_dtype, int kind, int d, int64_t rows, double p) {
   if (x_dtype != ULM_F32 || w_dtype != ULM_F32 || (kind != ULM_Y_F16 && kind != ULM_Y_BF16))

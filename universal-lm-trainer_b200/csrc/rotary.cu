@@ -16,6 +16,7 @@ namespace ulm {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr unsigned kGroup = kThreads;                    // positions; a multiple of kThreads
 
 // V elements that lie on a multiple of A
 template <typename T, int V, int A> struct alignas(sizeof(T) * A) Vec { T v[V]; };
@@ -26,9 +27,9 @@ struct RotaryParams {
   const uint64_t* turns;
   const void* positions;                                 // null: 0, 1, 2, ..
   int64_t pos_sb, pos_ss;
-  int S, R, D, turning, units, per_position;             // units: of a head, `turning` of them turn; per_position: threads
-  unsigned tasks;
-  int pos_32;
+  unsigned turning, passing, chunks;                     // units of a head that turn and that pass through; groups of heads of both tensors
+  unsigned turn_tasks, per_group, count;                 // threads of a group of positions: for what turns, in all; positions
+  int S, R, D, pos_32, pass_wide;                        // pass_wide: whole 16-byte vectors whatever V is
   float factor, sign;                                    // sign: -1 backward
 };
 
@@ -53,46 +54,54 @@ __device__ __forceinline__ void turn(uint64_t share, float f, float sign, float&
   s = quarter & 2 ? -f * sign * b : f * sign * b;        // 2 and 3: the sine
 }
 
+// Heads a thread: 8 vectors of 16 bytes in flight where pairs lie apart, 4 where they are neighbours.  8x12x4096x64 bf16, 2 / 4 / 6 heads:
+// apart 40.1 / 32.8 / 32.5 us (floor 30.7), neighbours 31.9 with 4, 33.1 with 6, 35.8 with 8; 12 heads leave a thread of 8 heads half empty.
+// CTAs of 256 threads: 37.7 and 33.7.  What passes through in warps of its own: 1x(16+4)x32001x128 fp16, half of it turning, 64 -> 50.1 us
+// (floor 50.0), as against both in one warp, which waited for memory twice.
+constexpr int kHeads = 4;
+
 template <typename T, int V, int A, bool INTER>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int kHeads = INTER ? 8 : 4;                  // 8 vectors a thread either way
-  const unsigned task = blockIdx.x * kThreads + threadIdx.x;
+  constexpr int H = kHeads;
   grid_dependents_go();
   grid_dependency_wait();
-  if (task >= p.tasks) return;
-  const unsigned at = task / (unsigned)p.per_position, r = task - at * (unsigned)p.per_position;
-  const int chunk = (int)(r / (unsigned)p.units), unit = (int)(r - (unsigned)chunk * (unsigned)p.units);
+  // of every kGroup positions first all that turns, then all that passes through: no warp has both, and the two halves of a
+  // row of memory are asked for within a short time
+  const unsigned task = blockIdx.x * kThreads + threadIdx.x, group = task / p.per_group, rest = task - group * p.per_group;
+  const bool turns = rest < p.turn_tasks;
+  const unsigned units = turns ? p.turning : p.passing, per_position = units * p.chunks, local = turns ? rest : rest - p.turn_tasks;
+  const unsigned in_group = local / per_position, at = group * kGroup + in_group, r = local - in_group * per_position;
+  if (at >= p.count) return;
+  const int chunk = (int)(r / units), unit = (int)(r - (unsigned)chunk * units);
   const int b = (int)(at / (unsigned)p.S), s = (int)(at - (unsigned)b * (unsigned)p.S);
   const bool second = chunk >= p.side[0].chunks;
   const Side& d = p.side[second];
-  const int h0 = (second ? chunk - p.side[0].chunks : chunk) * kHeads, nh = d.heads - h0;
+  const int h0 = (second ? chunk - p.side[0].chunks : chunk) * H, nh = d.heads - h0;
   const T* in = static_cast<const T*>(d.in) + b * d.in_sb + s * d.in_ss + h0 * d.in_sh;
   T* out = static_cast<T*>(d.out) + b * d.out_sb + s * d.out_ss + h0 * d.out_sh;
   using W = Vec<T, V, A>;
-  if (unit >= p.turning) {                               // columns that pass through
-    const int col = p.R + (unit - p.turning) * V;
-    if constexpr (A < V) {                               // a head of an odd number of columns ends inside the last unit
+  if (!turns) {
+    auto copy = [&](auto w0, int col) {
+      using C = decltype(w0);
+      C w[H];
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i)
+      for (int i = 0; i < H; ++i)
+        if (i < nh) w[i] = *reinterpret_cast<const C*>(in + i * d.in_sh + col);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (i < nh && col + j < p.D) out[i * d.out_sh + col + j] = in[i * d.in_sh + col + j];
-      return;
-    }
-    W w[kHeads];
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (i < nh) w[i] = *reinterpret_cast<const W*>(in + i * d.in_sh + col);
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i)
-      if (i < nh) *reinterpret_cast<W*>(out + i * d.out_sh + col) = w[i];
+      for (int i = 0; i < H; ++i)
+        if (i < nh) *reinterpret_cast<C*>(out + i * d.out_sh + col) = w[i];
+    };
+    const int col = p.R + unit * V;
+    if (p.pass_wide) copy(uint4(), p.R + unit * (int)(16 / sizeof(T)));
+    else if (A == V || col + V <= p.D) copy(W(), col);
+    else copy(T(), col);                                 // a head of an odd number of columns ends inside its last unit
     return;
   }
   const int col = unit * V, half = p.R >> 1;
-  W lo[kHeads], hi[INTER ? 1 : kHeads];
+  W lo[H], hi[INTER ? 1 : H];
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i)
+  for (int i = 0; i < H; ++i)
     if (i < nh) {
       lo[i] = *reinterpret_cast<const W*>(in + i * d.in_sh + col);
       if constexpr (!INTER) hi[i] = *reinterpret_cast<const W*>(in + i * d.in_sh + col + half);
@@ -107,7 +116,7 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) turn(position * p.turns[unit * kPairs + j], p.factor, p.sign, cs[j], sn[j]);
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i)
+  for (int i = 0; i < H; ++i)
     if (i < nh) {
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
@@ -124,7 +133,7 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
 
 template <typename T, bool INTER>
 int launch(const RotaryParams& p, int V, cudaStream_t st, const char* who) {
-  const unsigned grid = (p.tasks + kThreads - 1) / kThreads;
+  const unsigned grid = (p.count + kGroup - 1) / kGroup * (p.per_group / kThreads);
   auto go = [&](auto kern) { return launch_dependent(who, kern, grid, kThreads, 0, st, p); };
   if constexpr (sizeof(T) == 2)
     if (V == 8) return go(rotary_kernel<T, 8, 8, INTER>);
@@ -148,24 +157,26 @@ extern "C" int ulm_rotary(const ulm_rotary_args* a) {
   if (a->B == 0 || a->S == 0 || (a->Hq == 0 && a->Hk == 0)) return ULM_OK;
   if ((a->Hq && (!a->q || !a->qo)) || (a->Hk && (!a->k || !a->ko)) || !a->turns || (a->pos_kind && !a->positions)) return fail(ULM_ERR_ARG, "%s: null tensor", who);
   const int es = a->dtype == ULM_F32 ? 4 : 2;
-  // elements a vector: they divide what turns and what does not, and every head of every tensor starts on a whole one
-  int V = 16 / es;
-  auto fits = [&](int v) {
+  const int wide = 16 / es;
+  auto starts_on = [&](int v) {                          // every head of every tensor on a whole vector
     const int64_t t[12] = {a->q_sb, a->q_sh, a->q_ss, a->qo_sb, a->qo_sh, a->qo_ss, a->k_sb, a->k_sh, a->k_ss, a->ko_sb, a->ko_sh, a->ko_ss};
     const void* ptr[4] = {a->q, a->qo, a->k, a->ko};
-    if ((a->interleaved ? a->R : a->R / 2) % v || (a->D - a->R) % v) return false;
     for (int i = 0; i < 12; ++i)
       if ((i < 6 ? a->Hq : a->Hk) && t[i] % v) return false;
     for (int i = 0; i < 4; ++i)
       if ((i < 2 ? a->Hq : a->Hk) && reinterpret_cast<uintptr_t>(ptr[i]) % (uintptr_t)(v * es)) return false;
     return true;
   };
+  if (!starts_on(1)) return fail(ULM_ERR_ARG, "%s: tensors must lie on whole elements", who);
+  // elements a vector: they divide what turns, and what does not
+  const bool pass_wide = a->R % wide == 0 && (a->D - a->R) % wide == 0 && starts_on(wide);
+  auto fits = [&](int v) { return (a->interleaved ? a->R : a->R / 2) % v == 0 && (pass_wide || (a->D - a->R) % v == 0) && starts_on(v); };
+  int V = wide;
   while (V > 1 && !fits(V)) V /= 2;
-  if (!fits(V)) return fail(ULM_ERR_ARG, "%s: tensors must lie on whole elements", who);
   if (reinterpret_cast<uintptr_t>(a->turns) % 8 || (a->pos_kind && reinterpret_cast<uintptr_t>(a->positions) % (a->pos_kind == 1 ? 4 : 8)))
     return fail(ULM_ERR_ARG, "%s: turns and positions must lie on whole elements", who);
   RotaryParams p{};
-  const int per = a->interleaved ? 8 : 4;
+  const int per = kHeads;
   p.side[0] = {a->q, a->qo, a->q_sb, a->q_sh, a->q_ss, a->qo_sb, a->qo_sh, a->qo_ss, a->Hq, (a->Hq + per - 1) / per};
   p.side[1] = {a->k, a->ko, a->k_sb, a->k_sh, a->k_ss, a->ko_sb, a->ko_sh, a->ko_ss, a->Hk, (a->Hk + per - 1) / per};
   p.turns = reinterpret_cast<const uint64_t*>(a->turns);
@@ -173,13 +184,18 @@ extern "C" int ulm_rotary(const ulm_rotary_args* a) {
   p.pos_sb = a->pos_sb; p.pos_ss = a->pos_ss; p.pos_32 = a->pos_kind == 1;
   p.S = a->S; p.R = a->R; p.D = a->D;
   const int step = a->interleaved && V == 1 ? 2 : V;     // a thread has whole pairs
-  p.turning = (a->interleaved ? a->R : a->R / 2) / step;
-  p.units = p.turning + (a->D - a->R + step - 1) / step;
-  const int64_t per_position = (int64_t)p.units * (p.side[0].chunks + p.side[1].chunks);
-  const int64_t positions = (int64_t)a->B * a->S;
-  if (per_position > 0x7fffffffLL || positions > 0xfffffff0LL / per_position) return fail(ULM_ERR_TOO_LARGE, "%s: too many elements", who);
-  p.per_position = (int)per_position;
-  p.tasks = (unsigned)(positions * per_position);
+  p.turning = (unsigned)((a->interleaved ? a->R : a->R / 2) / step);
+  p.pass_wide = pass_wide;
+  p.passing = (unsigned)(pass_wide ? (a->D - a->R) / wide : (a->D - a->R + step - 1) / step);
+  p.chunks = (unsigned)(p.side[0].chunks + p.side[1].chunks);
+  // what passes through is where it belongs already
+  if ((!a->Hq || a->q == a->qo) && (!a->Hk || a->k == a->ko)) p.passing = 0;
+  const int64_t positions = (int64_t)a->B * a->S, per_position = (int64_t)(p.turning + p.passing) * p.chunks;
+  if (per_position * kGroup > 0x7fffffffLL || positions > 0x7fffff00LL || (positions + kGroup) * per_position > 0xffffffffLL)
+    return fail(ULM_ERR_TOO_LARGE, "%s: too many elements", who);
+  p.count = (unsigned)positions;
+  p.turn_tasks = (unsigned)(kGroup * p.turning * p.chunks);
+  p.per_group = (unsigned)(kGroup * per_position);
   p.factor = a->factor; p.sign = a->backward ? -1.f : 1.f;
   cudaStream_t st = (cudaStream_t)a->stream;
   auto go = [&](auto t) {

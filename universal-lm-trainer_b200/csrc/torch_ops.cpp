@@ -855,6 +855,106 @@ std::tuple<Tensor, Tensor> dropout_add_rms_norm(const Tensor& x, const Tensor& b
   return {x_new, y};
 }
 
+// ---------------------------------------------------------------------------
+// the norms behind and in front of a block, with the residual add between them
+// ---------------------------------------------------------------------------
+struct NormAddNormBwd : OpNode {
+  at::ScalarType vdtype, wdtype, sdtype, bdtype;
+  bool has_gate = false, has_scale = false, channels = false;
+  double scale_value = 1.0;
+  std::vector<int64_t> scale_shape;
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    // the inputs themselves are kept, so that a change in place is noticed, and brought into the kernel's form again
+    const Tensor x = kept[0], b = rows_on(kept[1], 8), v = dense16(as_type(kept[2], at::kFloat)), w = dense16(as_type(kept[3], at::kFloat)), rstd1 = kept[4], rstd2 = kept[5],
+                 gate = has_gate ? rows_on(kept[6], 8) : Tensor(), scale = has_scale ? dense16(as_type(kept[has_gate ? 7 : 6], at::kFloat)) : Tensor();
+    const int64_t rows = rstd1.size(0), d = w.size(0);
+    // a y that nobody used has the gradient zero
+    const Tensor dy = g[1].defined() ? rows_on(as_type(g[1], bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
+    const Tensor ga = g[0].defined() ? rows_on(as_type(g[0], at::kFloat), 16) : Tensor();
+    const Tensor dx = empty_cuda(x.sizes(), at::kFloat, x), db = empty_cuda(x.sizes(), bdtype, x), dg = has_gate ? empty_cuda(x.sizes(), bdtype, x) : Tensor();
+    // dw, dv, dscale, then the CTAs' partial rows
+    const int64_t n_scale = !has_scale ? 0 : channels ? d : 4;
+    const Tensor sums = empty_cuda({2 * d + n_scale}, at::kFloat, x), partial = empty_cuda({ulm_norm_add_norm_partial(rows, (int32_t)d)}, at::kFloat, x);
+    ulm_norm_add_norm_bwd_args a{};
+    a.x = x.data_ptr<float>(); a.branch = b.data_ptr(); a.gate = has_gate ? gate.data_ptr() : nullptr;
+    a.v = v.data_ptr<float>(); a.w = w.data_ptr<float>(); a.scale = has_scale ? scale.data_ptr<float>() : nullptr;
+    a.dy = dy.data_ptr(); a.g_add = ga.defined() ? ga.data_ptr<float>() : nullptr; a.rstd_branch = rstd1.data_ptr<float>(); a.rstd = rstd2.data_ptr<float>();
+    a.dx = dx.data_ptr<float>(); a.d_branch = db.data_ptr(); a.d_gate = has_gate ? dg.data_ptr() : nullptr;
+    a.dw = sums.data_ptr<float>(); a.dv = a.dw + d; a.dscale = has_scale ? a.dv + d : nullptr; a.partial = partial.data_ptr<float>();
+    a.x_stride = a.dx_stride = a.dbranch_stride = a.dgate_stride = d;
+    a.branch_stride = b.stride(0); a.gate_stride = has_gate ? gate.stride(0) : d; a.dy_stride = dy.stride(0); a.gadd_stride = ga.defined() ? ga.stride(0) : d;
+    a.rows = rows; a.d = (int32_t)d; a.dtype = code_of(bdtype); a.scale_channels = channels; a.scale_value = (float)scale_value; a.stream = stream_of(x);
+    check(ulm_norm_add_norm_bwd(&a), "norm_add_norm backward");
+    variable_list r{dx, db, as_type(sums.narrow(0, d, d), vdtype), as_type(sums.narrow(0, 0, d), wdtype)};
+    if (has_gate) r.push_back(dg);
+    if (has_scale) r.push_back(as_type(sums.narrow(0, 2 * d, channels ? d : 1), sdtype).view(scale_shape));
+    return r;
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "norm_add_norm"); }
+};
+
+std::tuple<Tensor, Tensor> norm_add_norm(const Tensor& x, const Tensor& branch, const Tensor& post_weight, const Tensor& weight, const Tensor& gate_in, const Tensor& scale_in,
+                                         double scale_value, double eps) {
+  const char* who = "norm_add_norm";
+  const bool has_gate = gate_in.defined(), has_scale = scale_in.defined();
+  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kFloat && is_16bit(branch.scalar_type()) && branch.device() == x.device() && branch.sizes() == x.sizes(),
+                    who, " needs an fp32 CUDA x and a 16-bit branch of the same shape and device");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) <= 8192 && x.size(-1) % 4 == 0, who, " takes rows of at most 8192 elements, a multiple of 4");
+  for (const Tensor& w : {post_weight, weight})
+    TORCH_CHECK_VALUE(w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(-1) && w.is_floating_point(), who, " needs one weight per column for each norm, on the device of x");
+  TORCH_CHECK_VALUE(!has_gate || (gate_in.device() == x.device() && gate_in.scalar_type() == branch.scalar_type() && gate_in.sizes() == x.sizes()),
+                    who, " takes a gate of the branch's type, shape and device");
+  TORCH_CHECK_VALUE(!has_scale || (scale_in.device() == x.device() && scale_in.is_floating_point() &&
+                                   (scale_in.numel() == 1 ? scale_in.dim() <= 1 : scale_in.dim() == 1 && scale_in.size(0) == x.size(-1))),
+                    who, " takes a number, a tensor of one element or one of one element per column as its scale, on the device of x");
+  Tensor x_new, y, b2, g2, v, w, s, rstd1, rstd2;
+  const int64_t d = x.size(-1);
+  const bool channels = has_scale && scale_in.numel() != 1;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(x.device());
+    const Tensor x2 = rows_on(x, 16);
+    b2 = rows_on(branch, 8);
+    if (has_gate) g2 = rows_on(gate_in, 8);
+    x_new = empty_cuda(x.sizes(), at::kFloat, x);
+    y = empty_cuda(x.sizes(), branch.scalar_type(), x);
+    rstd1 = empty_cuda({x2.size(0)}, at::kFloat, x);
+    rstd2 = empty_cuda({x2.size(0)}, at::kFloat, x);
+    v = dense16(as_type(post_weight, at::kFloat));
+    w = dense16(as_type(weight, at::kFloat));
+    if (has_scale) s = dense16(as_type(scale_in, at::kFloat));
+    ulm_norm_add_norm_fwd_args a{};
+    a.x = x2.data_ptr<float>(); a.branch = b2.data_ptr(); a.gate = has_gate ? g2.data_ptr() : nullptr;
+    a.v = v.data_ptr<float>(); a.w = w.data_ptr<float>(); a.scale = has_scale ? s.data_ptr<float>() : nullptr;
+    a.x_out = x_new.data_ptr<float>(); a.y = y.data_ptr(); a.rstd_branch = rstd1.data_ptr<float>(); a.rstd = rstd2.data_ptr<float>();
+    a.x_stride = x2.stride(0); a.branch_stride = b2.stride(0); a.gate_stride = has_gate ? g2.stride(0) : d; a.xout_stride = a.y_stride = d;
+    a.rows = x2.size(0); a.d = (int32_t)d; a.dtype = code_of(branch.scalar_type()); a.scale_channels = channels; a.scale_value = (float)scale_value; a.eps = (float)eps;
+    a.stream = stream_of(x);
+    check(ulm_norm_add_norm_fwd(&a), who);
+  }
+  auto finish = [&](std::shared_ptr<NormAddNormBwd> node) {
+    node->vdtype = post_weight.scalar_type(); node->wdtype = weight.scalar_type(); node->bdtype = branch.scalar_type();
+    node->has_gate = has_gate; node->has_scale = has_scale; node->channels = channels; node->scale_value = scale_value;
+    if (has_scale) { node->sdtype = scale_in.scalar_type(); node->scale_shape = scale_in.sizes().vec(); }
+    // an alias of x_new, so that the node does not hold its own output; it shares the version counter
+    node->keep(x_new.detach()); node->keep(branch); node->keep(post_weight); node->keep(weight); node->keep(rstd1); node->keep(rstd2);
+    if (has_gate) node->keep(gate_in);
+    if (has_scale) node->keep(scale_in);
+    torch::autograd::set_history(x_new, node);
+    torch::autograd::set_history(y, node);
+  };
+  if (has_gate && has_scale) { if (!no_graph(x, branch, post_weight, weight, gate_in, scale_in)) finish(make_node<NormAddNormBwd>(x, branch, post_weight, weight, gate_in, scale_in)); }
+  else if (has_gate) { if (!no_graph(x, branch, post_weight, weight, gate_in)) finish(make_node<NormAddNormBwd>(x, branch, post_weight, weight, gate_in)); }
+  else if (has_scale) { if (!no_graph(x, branch, post_weight, weight, scale_in)) finish(make_node<NormAddNormBwd>(x, branch, post_weight, weight, scale_in)); }
+  else if (!no_graph(x, branch, post_weight, weight)) finish(make_node<NormAddNormBwd>(x, branch, post_weight, weight));
+  return {x_new, y};
+}
+// the forms that are bound: every tensor that may have a gradient is an argument of its own
+std::tuple<Tensor, Tensor> norm_add_norm_plain(const Tensor& x, const Tensor& b, const Tensor& v, const Tensor& w, double s, double eps) { return norm_add_norm(x, b, v, w, Tensor(), Tensor(), s, eps); }
+std::tuple<Tensor, Tensor> norm_add_norm_gate(const Tensor& x, const Tensor& b, const Tensor& v, const Tensor& w, const Tensor& gate, double s, double eps) { return norm_add_norm(x, b, v, w, gate, Tensor(), s, eps); }
+std::tuple<Tensor, Tensor> norm_add_norm_scale(const Tensor& x, const Tensor& b, const Tensor& v, const Tensor& w, const Tensor& s, double eps) { return norm_add_norm(x, b, v, w, Tensor(), s, 1.0, eps); }
+std::tuple<Tensor, Tensor> norm_add_norm_gate_scale(const Tensor& x, const Tensor& b, const Tensor& v, const Tensor& w, const Tensor& gate, const Tensor& s, double eps) { return norm_add_norm(x, b, v, w, gate, s, 1.0, eps); }
+
 struct SwigluBwd : OpNode {
   Drop drop;
   variable_list backward(variable_list& g, const variable_list& kept) override {
@@ -1581,6 +1681,10 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "add_rms_norm", &::add_rms_norm);
   def_op(m, "swiglu", &::swiglu);
   def_op(m, "swiglu_dropout", &::swiglu_dropout);
+  def_op(m, "norm_add_norm_plain", &::norm_add_norm_plain);
+  def_op(m, "norm_add_norm_gate", &::norm_add_norm_gate);
+  def_op(m, "norm_add_norm_scale", &::norm_add_norm_scale);
+  def_op(m, "norm_add_norm_gate_scale", &::norm_add_norm_gate_scale);
   def_op(m, "rotary", &::rotary);
   def_op(m, "rotary_one", &::rotary_one);
   def_op(m, "dropout", &::dropout);

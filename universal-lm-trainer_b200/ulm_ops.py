@@ -99,6 +99,23 @@ def dropout_add_rms_norm(x, branch, weight, p, seed, eps: float = 1e-6):
     return N.ext().dropout_add_rms_norm(x, branch, weight, float(p), _as_i64(seed), float(eps))
 
 
+def norm_add_norm(x, branch, post_weight, weight, gate=None, scale=None, eps: float = 1e-6):
+    """The norms behind and in front of a block, with the residual add between them, in one pass each way:
+    ``x_new = x + scale * sigmoid(gate) * rms_norm(branch, post_weight)`` and ``y = rms_norm(x_new, weight)``; returns ``(x_new, y)``.
+    x and x_new fp32 (the residual stream), branch, gate and y of one 16-bit type, rows of at most 8192 elements, a multiple of 4.
+    ``gate``: a tensor of branch's shape, before its sigmoid; None: no gate.  ``scale``: None, a number, or a floating tensor on x's device of one
+    element or of one per column, which then has a gradient.  Statistics, sums and x_new are fp32, y and the gradients of branch and
+    gate are rounded once.  The gradient of a 16-bit weight or scale is the fp32 sum, rounded."""
+    if isinstance(scale, torch.Tensor):
+        if gate is None:
+            return N.ext().norm_add_norm_scale(x, branch, post_weight, weight, scale, float(eps))
+        return N.ext().norm_add_norm_gate_scale(x, branch, post_weight, weight, gate, scale, float(eps))
+    value = 1.0 if scale is None else float(scale)
+    if gate is None:
+        return N.ext().norm_add_norm_plain(x, branch, post_weight, weight, value, float(eps))
+    return N.ext().norm_add_norm_gate(x, branch, post_weight, weight, gate, value, float(eps))
+
+
 def _as_i64(seed):
     """The 64 bits of ``seed`` as the signed integer the extension takes."""
     seed = int(seed)
