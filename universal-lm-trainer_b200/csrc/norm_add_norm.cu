@@ -8,11 +8,13 @@
 // x, z and their gradients fp32; b, g, y and theirs 16-bit; s one number or one a column, g may be left out.  Statistics and sums fp32,
 // one rounding to 16 bits; exponent and division of the sigmoid in full, because z keeps what they leave.
 //
-// What bounds it: HBM, 12 bytes an element forward and 18 backward, 2 and 4 more with a gate.  A row belongs to W warps of a CTA and stays
-// in registers between its uses; a lane owns vectors of E elements.  The backward's second mean needs dz and so the first one:
+// What bounds it: HBM, 12 bytes an element forward and 18 backward, 2 and 4 more with a gate.  A row belongs to L lanes of a CTA (half a warp, or
+// whole ones) and stays in registers between its uses; a lane owns vectors of E elements.  The backward's second mean needs dz and so the first one:
 // with dz = p - m q (p = r2 G + gz, q = r2 h, m = mean(G h)), sum(n u) = sum(t p u) - m sum(t q u) for t = s sig(g) v, so that all three
 // sums of a row are formed before one barrier.  Column sums: per lane over a CTA's rows, added up over its groups in shared memory, a partial
 // row per CTA, joined in a fixed order: no atomics.
+#include <type_traits>
+
 #include "common.cuh"
 #include "norm_rows.cuh"
 
@@ -20,15 +22,74 @@ namespace ulm {
 namespace {
 
 constexpr int kMaxRow = 8192;
-constexpr int kFwdWarps = 8, kBwdWarps = 12, kBwdWideWarps = 16;
 
-// sig(g), and sig(g) (1 - sig(g)) without a difference
-__device__ __forceinline__ float opened(float g, float& slope) {
-  const float e = expf(-fabsf(g)), q = 1.f / (1.f + e);
-  slope = e * q * q;
-  return g >= 0.f ? q : e * q;                           // a NaN is not, and stays one
+// Two fp32 values at a time: half the instructions of the multiply-add pipe, which had 37 of the backward's 82 an element.
+__device__ __forceinline__ uint64_t bits(const float2& v) { return reinterpret_cast<const uint64_t&>(v); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return reinterpret_cast<float2&>(r);
 }
-__device__ __forceinline__ float opened(float g) { float slope; return opened(g, slope); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// The sigmoid as its smaller side s = sig(-|g|) with the sign of g: sig(g) is s or 1 - s, its slope s (1 - s) without a difference that cancels.
+// 2^x and the reciprocal are the special-function unit's, within 2^-22 and 2^-23; with the exponent's rounding s is within 2^-21 + |g| 2^-24 of
+// itself, its other side within 2^-23.  With expf and an IEEE division, evaluated at both uses, 12011 x 1024 took 50 + 91 us.
+__device__ __forceinline__ float2 shut(float2 g) {
+  const float2 t = mul2(make_float2(fabsf(g.x), fabsf(g.y)), both(-1.44269504f));
+  float2 e, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 d = add2(e, both(1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(d.y));
+  const float2 s = mul2(e, q);
+  return make_float2(copysignf(s.x, g.x), copysignf(s.y, g.y));
+}
+// by its sign bit: s may be a zero; a NaN stays one
+__device__ __forceinline__ float opened(float s) { return __float_as_int(s) < 0 ? -s : 1.f - s; }
+__device__ __forceinline__ float2 opened(float2 s) { return make_float2(opened(s.x), opened(s.y)); }
+// sig (1 - sig) = |s| - s^2
+__device__ __forceinline__ float2 slope(float2 s) { return fma2(s, make_float2(-s.x, -s.y), make_float2(fabsf(s.x), fabsf(s.y))); }
+
+// E fp32 columns: with E = 8 a lane takes 32 bytes in one access, so that a warp's is a kilobyte without gaps.  As two accesses of 16 bytes each
+// would touch the same eight lines, and L1 was 72 % busy.  p on a multiple of 4 E bytes.
+template <int E> __device__ __forceinline__ void load_row(const float* p, float2 (&v)[E / 2]) {
+  if constexpr (E == 8) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y) : "l"(p));
+  } else {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = make_float2(f.x, f.y); v[1] = make_float2(f.z, f.w);
+  }
+}
+template <int E> __device__ __forceinline__ void store_row(float* p, const float2 (&v)[E / 2]) {
+  if constexpr (E == 8)
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(p), "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y) : "memory");
+  else *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+}
+template <typename TY, int E> __device__ __forceinline__ void unpack_row(const Raw<E>& r, float2 (&v)[E / 2]) {
+#pragma unroll
+  for (int j = 0; j < E / 2; ++j) v[j] = Cvt<TY>::unpack2(r.u[j]);
+}
+template <typename TY, int E> __device__ __forceinline__ void store_row16(TY* p, const float2 (&v)[E / 2]) {
+  uint32_t u[E / 2];
+#pragma unroll
+  for (int j = 0; j < E / 2; ++j) u[j] = Cvt<TY>::pack2(v[j].x, v[j].y);
+  if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+}
 
 // the branch's factor: one number (on the device, or from the host) or one a column
 struct Scale { const float* dev; float value; int channels; };
@@ -36,81 +97,99 @@ __device__ __forceinline__ float whole_scale(const Scale& s) { return s.channels
 // v, times s where it is one a column: of E columns.  One s for all is applied by whoever calls, because its gradient, which may not
 // be divided by it, is the sum without it.
 template <int E>
-__device__ __forceinline__ void load_tv(const float* v, const Scale& s, int col, float (&t)[E]) {
-  load_f32<E>(v + col, t);
+__device__ __forceinline__ void load_tv(const float* v, const Scale& s, int col, float2 (&t)[E / 2]) {
+  load_row<E>(v + col, t);
   if (s.channels) {
-    float c[E];
-    load_f32<E>(s.dev + col, c);
+    float2 c[E / 2];
+    load_row<E>(s.dev + col, c);
 #pragma unroll
-    for (int j = 0; j < E; ++j) t[j] *= c[j];
+    for (int j = 0; j < E / 2; ++j) t[j] = mul2(t[j], c[j]);
   }
+}
+
+// A row belongs to L lanes: half a warp, or whole warps.
+__device__ __forceinline__ uint32_t row_mask(int L, int lane) { return L == 16 ? 0xffffu << (lane & 16) : 0xffffffffu; }
+// Sum over them.  `slots`: this call's own float a warp; consecutive calls of a warp alternate between two sets, so that one barrier a
+// call is enough.
+__device__ __forceinline__ float row_sum(float v, int L, int group, float* slots) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t mask = row_mask(L, lane);
+  if (L != 16) v += __shfl_xor_sync(mask, v, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+  if (L <= 32) return v;
+  const int warp = threadIdx.x >> 5, W = L >> 5;
+  if (lane == 0) slots[warp] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(L) : "memory");
+  float t = 0.f;
+  for (int i = 0; i < W; ++i) t += slots[group * W + i];
+  return t;
 }
 
 struct FwdParams {
   const float* x; const void* branch; const void* gate; const float* v; const float* w; Scale scale;
   float* x_out; void* y; float* rstd1; float* rstd2;
   int64_t x_stride, branch_stride, gate_stride, xout_stride, y_stride, rows;
-  int d, W; float eps;
+  int d, L; float eps;
 };
 
-template <typename TY, int E, int NV, bool GATE>
-__global__ void __launch_bounds__(kFwdWarps * 32, 3)
+template <typename TY, int E, int NV, int WARPS, int CTAS, bool GATE>
+__global__ void __launch_bounds__(WARPS * 32, CTAS)
 norm_add_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
-  __shared__ float slots[2][kFwdWarps];
+  __shared__ float slots[2][WARPS];
   grid_dependents_go();
   grid_dependency_wait();
   const TY* br = static_cast<const TY*>(p.branch);
   const TY* gt = static_cast<const TY*>(p.gate);
   TY* y = static_cast<TY*>(p.y);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
-  const int group = warp / W, part = warp - group * W, groups = (int)(blockDim.x >> 5) / W;
-  const int nvec = p.d / E, first = part * 32 + lane, hop = W * 32;
+  const int L = p.L, group = threadIdx.x / L, groups = blockDim.x / L, nvec = p.d / E, first = threadIdx.x - group * L, hop = L;
   const float inv_d = 1.f / (float)p.d, whole = whole_scale(p.scale);
   for (int64_t r = (int64_t)blockIdx.x * groups + group; r < p.rows; r += (int64_t)gridDim.x * groups) {
-    float z[NV][E];
+    float2 z[NV][E / 2];
     Raw<E> b[NV], g[GATE ? NV : 1];
 #pragma unroll
     for (int it = 0; it < NV; ++it) {                    // the whole row is requested before any of it is used
       const int vi = first + it * hop;
       if (vi < nvec) {
         b[it] = load_raw<TY, E>(br + r * p.branch_stride + vi * E);
-        load_f32<E>(p.x + r * p.x_stride + vi * E, z[it]);
+        load_row<E>(p.x + r * p.x_stride + vi * E, z[it]);
         if constexpr (GATE) g[it] = load_raw<TY, E>(gt + r * p.gate_stride + vi * E);
       }
     }
-    float sum = 0.f;
+    float2 sum = both(0.f);
 #pragma unroll
     for (int it = 0; it < NV; ++it)
       if (first + it * hop < nvec) {
-        float f[E];
-        unpack_raw<TY, E>(b[it], f);
+        float2 f[E / 2];
+        unpack_row<TY, E>(b[it], f);
 #pragma unroll
-        for (int j = 0; j < E; ++j) sum += f[j] * f[j];
+        for (int j = 0; j < E / 2; ++j) sum = fma2(f[j], f[j], sum);
       }
-    const float r1 = rsqrtf(row_sum(sum, W, group, warp, lane, slots[0]) * inv_d + p.eps), r1s = r1 * whole;
-    sum = 0.f;
+    const float r1 = rsqrtf(row_sum(sum.x + sum.y, L, group, slots[0]) * inv_d + p.eps);
+    const float2 r1s = both(r1 * whole);
+    sum = both(0.f);
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
       const int vi = first + it * hop;
       if (vi < nvec) {
-        float f[E], t[E];
-        unpack_raw<TY, E>(b[it], f);
+        float2 f[E / 2], t[E / 2];
+        unpack_row<TY, E>(b[it], f);
         load_tv<E>(p.v, p.scale, vi * E, t);
         if constexpr (GATE) {
-          float o[E];
-          unpack_raw<TY, E>(g[it], o);
+          float2 o[E / 2];
+          unpack_row<TY, E>(g[it], o);
 #pragma unroll
-          for (int j = 0; j < E; ++j) t[j] *= opened(o[j]);
+          for (int j = 0; j < E / 2; ++j) t[j] = mul2(t[j], opened(shut(o[j])));
         }
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          z[it][j] = fmaf(f[j] * r1s, t[j], z[it][j]);
-          sum += z[it][j] * z[it][j];
+        for (int j = 0; j < E / 2; ++j) {
+          z[it][j] = fma2(mul2(f[j], r1s), t[j], z[it][j]);
+          sum = fma2(z[it][j], z[it][j], sum);
         }
-        store_f32<E>(p.x_out + r * p.xout_stride + vi * E, z[it]);
+        store_row<E>(p.x_out + r * p.xout_stride + vi * E, z[it]);
       }
     }
-    const float r2 = rsqrtf(row_sum(sum, W, group, warp, lane, slots[1]) * inv_d + p.eps);
+    const float r2 = rsqrtf(row_sum(sum.x + sum.y, L, group, slots[1]) * inv_d + p.eps);
     if (first == 0) {
       p.rstd1[r] = r1;
       p.rstd2[r] = r2;
@@ -119,11 +198,11 @@ norm_add_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
     for (int it = 0; it < NV; ++it) {
       const int vi = first + it * hop;
       if (vi < nvec) {
-        float wv[E], o[E];
-        load_f32<E>(p.w + vi * E, wv);
+        float2 wv[E / 2];
+        load_row<E>(p.w + vi * E, wv);
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] = z[it][j] * r2 * wv[j];
-        store_16<TY, E>(y + r * p.y_stride + vi * E, o);
+        for (int j = 0; j < E / 2; ++j) wv[j] = mul2(mul2(z[it][j], both(r2)), wv[j]);
+        store_row16<TY, E>(y + r * p.y_stride + vi * E, wv);
       }
     }
   }
@@ -134,29 +213,45 @@ struct BwdParams {
   const void* dy; const float* gz; const float* rstd1; const float* rstd2;
   float* dx; void* db; void* dg; float* partial;
   int64_t z_stride, branch_stride, gate_stride, dy_stride, gz_stride, dx_stride, db_stride, dg_stride, rows;
-  int d, W;
+  int d, L;
 };
 
-// Three sums over the W warps of a row, one barrier; `slots` as for row_sum, three floats a warp.
-template <int WARPS>
-__device__ __forceinline__ void row_sums(float (&v)[3], int W, int group, int warp, int lane, float (*slots)[WARPS]) {
-#pragma unroll
-  for (int i = 0; i < 3; ++i) v[i] = warp_sum(v[i]);
-  if (W == 1) return;
-  if (lane < 3) slots[lane][warp] = lane == 0 ? v[0] : lane == 1 ? v[1] : v[2];
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * W) : "memory");
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    v[i] = 0.f;
-    for (int k = 0; k < W; ++k) v[i] += slots[i][group * W + k];
+// Three sums over the L lanes of a row, one barrier where they are more than a warp.  Every exchange between lanes halves the number of sums
+// that a lane carries: six of them instead of fifteen.  `slots` as for row_sum, a float4 a warp.
+__device__ __forceinline__ void row_sums(float& a, float& b, float& c, int L, int group, float4* slots) {
+  const int lane = threadIdx.x & 31, top = L == 16 ? 8 : 16;
+  const uint32_t mask = row_mask(L, lane);
+  const bool up = lane & top, right = lane & (top >> 1);
+  float s0 = up ? c : a, s1 = up ? 0.f : b;              // the lower half of the lanes goes on with a and b, the upper with c
+  s0 += __shfl_xor_sync(mask, up ? a : c, top);
+  s1 += __shfl_xor_sync(mask, up ? b : 0.f, top);
+  float t = right ? s1 : s0;
+  t += __shfl_xor_sync(mask, right ? s0 : s1, top >> 1);
+  if (L != 16) t += __shfl_xor_sync(mask, t, 4);
+  t += __shfl_xor_sync(mask, t, 2);
+  t += __shfl_xor_sync(mask, t, 1);
+  if (L <= 32) {
+    const int base = L == 16 ? lane & 16 : 0;
+    a = __shfl_sync(mask, t, base);
+    b = __shfl_sync(mask, t, base + (top >> 1));
+    c = __shfl_sync(mask, t, base + top);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, W = L >> 5;
+  if ((lane & 7) == 0) reinterpret_cast<float*>(slots + warp)[lane >> 3] = t;
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(L) : "memory");
+  a = b = c = 0.f;
+  for (int k = 0; k < W; ++k) {
+    const float4 q = slots[group * W + k];
+    a += q.x; b += q.y; c += q.z;
   }
 }
 
-template <typename TY, int E, int NV, int WARPS, bool GATE>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == kBwdWideWarps ? 1 : 2)
+template <typename TY, int E, int NV, int WARPS, int CTAS, bool GATE>
+__global__ void __launch_bounds__(WARPS * 32, CTAS)
 norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
   extern __shared__ float s_sum[];                       // [groups][d]
-  __shared__ float slots[2][3][WARPS];
+  __shared__ float4 slots[2][WARPS];
   grid_dependents_go();
   grid_dependency_wait();
   const TY* br = static_cast<const TY*>(p.branch);
@@ -164,101 +259,94 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
   const TY* dy = static_cast<const TY*>(p.dy);
   TY* db = static_cast<TY*>(p.db);
   TY* dg = static_cast<TY*>(p.dg);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = p.W;
-  const int group = warp / W, part = warp - group * W, groups = (int)(blockDim.x >> 5) / W;
-  const int nvec = p.d / E, first = part * 32 + lane, hop = W * 32;
+  const int L = p.L, group = threadIdx.x / L, groups = blockDim.x / L, nvec = p.d / E, first = threadIdx.x - group * L, hop = L;
   const float inv_d = 1.f / (float)p.d, whole = whole_scale(p.scale);
-  float acc_w[NV][E], acc_c[NV][E], acc_s = 0.f;
+  // a lane has the same columns of every row: their weights stay in registers where there are few
+  constexpr bool kHold = NV * E <= 16;
+  float2 wv[kHold ? NV : 1][E / 2], tv[kHold ? NV : 1][E / 2], acc_w[NV][E / 2], acc_c[NV][E / 2];
+  float acc_s = 0.f;
 #pragma unroll
-  for (int it = 0; it < NV; ++it)
+  for (int it = 0; it < NV; ++it) {
+    if (kHold && first + it * hop < nvec) {
+      load_row<E>(p.w + (first + it * hop) * E, wv[it]);
+      load_tv<E>(p.v, p.scale, (first + it * hop) * E, tv[it]);
+    }
 #pragma unroll
-    for (int j = 0; j < E; ++j) acc_w[it][j] = acc_c[it][j] = 0.f;
+    for (int j = 0; j < E / 2; ++j) acc_w[it][j] = acc_c[it][j] = both(0.f);
+  }
   int phase = 0;
   for (int64_t r = (int64_t)blockIdx.x * groups + group; r < p.rows; r += (int64_t)gridDim.x * groups, phase ^= 1) {
-    float z[NV][E], gz[NV][E];
+    float2 z[NV][E / 2], gz[NV][E / 2], shuts[GATE ? NV : 1][E / 2];
     Raw<E> b[NV], q[NV], g[GATE ? NV : 1];
 #pragma unroll
-    for (int it = 0; it < NV; ++it) {
+    for (int it = 0; it < NV; ++it) {                    // the whole row is requested before any of it is used
       const int vi = first + it * hop;
       if (vi < nvec) {
-        load_f32<E>(p.z + r * p.z_stride + vi * E, z[it]);
+        load_row<E>(p.z + r * p.z_stride + vi * E, z[it]);
         q[it] = load_raw<TY, E>(dy + r * p.dy_stride + vi * E);
         b[it] = load_raw<TY, E>(br + r * p.branch_stride + vi * E);
         if constexpr (GATE) g[it] = load_raw<TY, E>(gt + r * p.gate_stride + vi * E);
         if (p.gz) {
-          load_f32<E>(p.gz + r * p.gz_stride + vi * E, gz[it]);
+          load_row<E>(p.gz + r * p.gz_stride + vi * E, gz[it]);
         } else {
 #pragma unroll
-          for (int j = 0; j < E; ++j) gz[it][j] = 0.f;
+          for (int j = 0; j < E / 2; ++j) gz[it][j] = both(0.f);
         }
       }
     }
     const float r1 = p.rstd1[r], r2 = p.rstd2[r];
-    float sums[3] = {0.f, 0.f, 0.f};
+    float2 gh2 = both(0.f), pt2 = gh2, ht2 = gh2;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      const int vi = first + it * hop;
+      const int vi = first + it * hop, at = kHold ? it : 0;
       if (vi < nvec) {
-        float G[E], u[E], wv[E], t[E];
-        unpack_raw<TY, E>(q[it], G);
-        unpack_raw<TY, E>(b[it], u);
-        load_f32<E>(p.w + vi * E, wv);
-        load_tv<E>(p.v, p.scale, vi * E, t);
+        float2 G[E / 2], u[E / 2];
+        if constexpr (!kHold) {
+          load_row<E>(p.w + vi * E, wv[0]);
+          load_tv<E>(p.v, p.scale, vi * E, tv[0]);
+        }
+        unpack_row<TY, E>(q[it], G);
+        unpack_row<TY, E>(b[it], u);
         if constexpr (GATE) {
-          float o[E];
-          unpack_raw<TY, E>(g[it], o);
+          unpack_row<TY, E>(g[it], shuts[it]);
 #pragma unroll
-          for (int j = 0; j < E; ++j) t[j] *= opened(o[j]);
+          for (int j = 0; j < E / 2; ++j) shuts[it][j] = shut(shuts[it][j]);
         }
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          z[it][j] *= r2;                                // h from here on
-          acc_w[it][j] += G[j] * z[it][j];
-          G[j] *= wv[j];
-          gz[it][j] += r2 * G[j];                        // p from here on
-          const float tu = t[j] * u[j] * r1;
-          sums[0] += G[j] * z[it][j];
-          sums[1] += gz[it][j] * tu;
-          sums[2] += z[it][j] * tu;
+        for (int j = 0; j < E / 2; ++j) {
+          z[it][j] = mul2(z[it][j], both(r2));           // h from here on
+          const float2 tu = mul2(GATE ? mul2(tv[at][j], opened(shuts[it][j])) : tv[at][j], mul2(u[j], both(r1))), a = mul2(G[j], z[it][j]);
+          acc_w[it][j] = add2(acc_w[it][j], a);
+          gh2 = fma2(a, wv[at][j], gh2);
+          gz[it][j] = fma2(mul2(G[j], wv[at][j]), both(r2), gz[it][j]);      // p from here on
+          pt2 = fma2(gz[it][j], tu, pt2);
+          ht2 = fma2(z[it][j], tu, ht2);
         }
       }
     }
-    row_sums<WARPS>(sums, W, group, warp, lane, slots[phase]);
-    const float m = sums[0] * inv_d * r2, nu = sums[1] - m * sums[2], k = nu * inv_d, rs = r1 * whole;      // dz = p - m h
+    float gh = gh2.x + gh2.y, pt = pt2.x + pt2.y, ht = ht2.x + ht2.y;
+    row_sums(gh, pt, ht, L, group, slots[phase]);
+    const float m = gh * inv_d * r2, nu = pt - m * ht, rs = r1 * whole, k = nu * inv_d * rs * r1;      // dz = p - m h
     acc_s += nu;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      const int vi = first + it * hop;
+      const int vi = first + it * hop, at = kHold ? it : 0;
       if (vi < nvec) {
-        float u[E], t[E], o[E];
-        unpack_raw<TY, E>(b[it], u);
-        load_tv<E>(p.v, p.scale, vi * E, t);
+        float2 u[E / 2], o[E / 2];
+        unpack_row<TY, E>(b[it], u);
+        if constexpr (!kHold) load_tv<E>(p.v, p.scale, vi * E, tv[0]);
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          gz[it][j] -= m * z[it][j];                     // dz from here on
-          u[j] *= r1;
+        for (int j = 0; j < E / 2; ++j) gz[it][j] = fma2(both(-m), z[it][j], gz[it][j]);      // dz from here on
+        store_row<E>(p.dx + r * p.dx_stride + vi * E, gz[it]);
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+          const float2 ds = GATE ? mul2(gz[it][j], opened(shuts[it][j])) : gz[it][j];
+          acc_c[it][j] = fma2(ds, mul2(u[j], both(r1)), acc_c[it][j]);
+          o[j] = fma2(mul2(ds, both(rs)), tv[at][j], mul2(u[j], both(-k)));
+          if constexpr (GATE) gz[it][j] = mul2(mul2(gz[it][j], slope(shuts[it][j])), mul2(mul2(u[j], both(rs)), tv[at][j]));
         }
-        store_f32<E>(p.dx + r * p.dx_stride + vi * E, gz[it]);
-        if constexpr (GATE) {
-          float a[E];
-          unpack_raw<TY, E>(g[it], a);
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            float slope;
-            const float sig = opened(a[j], slope), n = gz[it][j] * t[j];
-            o[j] = rs * (n * sig - u[j] * k);
-            acc_c[it][j] += gz[it][j] * sig * u[j];
-            a[j] = whole * (n * u[j] * slope);
-          }
-          store_16<TY, E>(dg + r * p.dg_stride + vi * E, a);
-        } else {
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            o[j] = rs * (gz[it][j] * t[j] - u[j] * k);
-            acc_c[it][j] += gz[it][j] * u[j];
-          }
-        }
-        store_16<TY, E>(db + r * p.db_stride + vi * E, o);
+        store_row16<TY, E>(db + r * p.db_stride + vi * E, o);
+        if constexpr (GATE) store_row16<TY, E>(dg + r * p.dg_stride + vi * E, gz[it]);
       }
     }
   }
@@ -272,7 +360,7 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
       const int vi = first + it * hop;
       if (vi < nvec) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) s_sum[group * p.d + vi * E + j] = set ? acc_c[it][j] : acc_w[it][j];
+        for (int j = 0; j < E / 2; ++j) *reinterpret_cast<float2*>(s_sum + group * p.d + vi * E + 2 * j) = set ? acc_c[it][j] : acc_w[it][j];
       }
     }
     __syncthreads();
@@ -283,7 +371,7 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
     }
   }
   __syncthreads();
-  if (lane == 0 && part == 0) s_sum[group] = acc_s;
+  if (first == 0) s_sum[group] = acc_s;
   __syncthreads();
   if (threadIdx.x == 0) {
     float t = 0.f;
@@ -318,6 +406,9 @@ norm_add_norm_finish_kernel(const float* partial, const float* v, const Scale sc
   }
 }
 
+// fp32 rows that vectors of eight may be read from
+bool ok256(const void* p, int64_t stride) { return !(reinterpret_cast<uintptr_t>(p) & 31) && stride % 8 == 0; }
+
 int check_shape(const char* who, int dtype, int d, int64_t rows) {
   if (dtype != ULM_F16 && dtype != ULM_BF16) return fail(ULM_ERR_ARG, "%s: branch, gate and y are fp16 or bf16", who);
   if (d <= 0 || d % 4 || rows < 0) return fail(ULM_ERR_ARG, "%s: need rows >= 0 and d a positive multiple of 4", who);
@@ -325,51 +416,72 @@ int check_shape(const char* who, int dtype, int d, int64_t rows) {
   return ULM_OK;
 }
 
-// vectors of a lane
-int fwd_nv(int nvec, int E) { const int most = E == 8 || nvec <= 1024 ? 4 : 8, need = ceil_div(nvec, 32); return need < most ? need : most; }
-int bwd_nv(int d, int E) { return (d <= 2048 ? 8 : 16) / E; }
-constexpr int kBwdElems = 32 * 16;                       // columns a warp of the backward has at most
-static_assert(kMaxRow <= kBwdWideWarps * kBwdElems, "rows");
-static_assert((kBwdWideWarps * kBwdElems + 6 * kBwdWideWarps) * sizeof(float) <= 48 * 1024, "shared memory");
+// A kernel's form: vectors of E columns a lane, warps of a CTA, CTAs on an SM, rows that a full CTA has at least; the columns that this allows.
+template <int E_, int NV_, int WARPS_, int CTAS_, int ROWS> struct Form {
+  static constexpr int E = E_, NV = NV_, WARPS = WARPS_, CTAS = CTAS_, kMost = E * NV * 32 * (WARPS / ROWS);
+};
+template <typename...> struct Forms {};
+// The first form whose columns suffice.  us at us of the bytes alone (bf16, without a gate, then with one):
+//   forward   32768 x 768 47.2 (46.1), x 1024 63.1 (61.4), 16396 x 4096 125 (123); 48044 x 1024 105 (105), 16396 x 4096 145 (144).  One warp a row up to
+//             1024 columns: with eight columns a lane, and so three warps and two barriers for 768, 32768 x 768 took 65
+//   backward  32768 x 768 78 (69), x 1024 102 (92), 16396 x 4096 208 (184); 48044 x 1024 181 (165), 16396 x 4096 300 (225).  Eight columns a lane and
+//             24 warps an SM without a gate up to 1024 (sixteen a lane: 87 at 768); the gate's values do not fit the 80 registers of that,
+//             and with sixteen a lane 48044 x 1024 went from 204 to 181.  Thirty-two from where two rows no longer fit a CTA: 16396 x 4096
+//             with a gate 340 -> 300.  There one or two rows are on an SM's way through load, sums, barrier and stores at a time, which is what bounds it
+using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 1>>;
+using Bwd8 = Forms<Form<8, 1, 12, 2, 3>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
+using Bwd8Gate = Forms<Form<8, 1, 20, 1, 6>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
+// widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only
+using Fwd4 = Forms<Form<4, 1, 8, 4, 8>, Form<4, 8, 8, 2, 1>>;
+using Bwd4 = Forms<Form<4, 1, 16, 2, 16>, Form<4, 2, 12, 2, 4>, Form<4, 4, 12, 1, 2>, Form<4, 8, 8, 1, 1>>;
 
-constexpr int kBwdWarpsPerSm = 24, kMostBwdCtas = 3;
-int64_t bwd_blocks(int64_t rows, const Split& s) {
-  const int64_t want = (rows + s.groups - 1) / s.groups;
-  int per_sm = kBwdWarpsPerSm / (s.W * s.groups);
-  per_sm = per_sm < 1 ? 1 : per_sm > kMostBwdCtas ? kMostBwdCtas : per_sm;
-  return want < per_sm * kNumSMs ? want : per_sm * kNumSMs;
+// Lanes a row and rows a CTA.  Few rows (less than the SMs take at full CTAs) are spread over more, smaller CTAs.
+struct Deal { int L, groups, threads; };
+template <typename F> Deal deal(int64_t rows, int d) {
+  Deal s;
+  const int nvec = d / F::E;
+  s.L = nvec <= 16 ? 16 : 32 * ceil_div(nvec, 32 * F::NV);
+  s.groups = F::WARPS * 32 / s.L;
+  const int64_t spread = (rows + kNumSMs - 1) / kNumSMs;
+  if (spread < s.groups) s.groups = spread < 1 ? 1 : (int)spread;
+  s.threads = ceil_div(s.groups * s.L, 32) * 32;
+  s.groups = s.threads / s.L;
+  return s;
+}
+constexpr int kMostCtas = 2;                             // on an SM, of all forms of the backward
+
+template <typename TY, bool GATE, typename F, typename... Rest>
+int launch_fwd(Forms<F, Rest...>, FwdParams p, cudaStream_t st, const char* who) {
+  if constexpr (sizeof...(Rest) > 0)
+    if (p.d > F::kMost) return launch_fwd<TY, GATE>(Forms<Rest...>(), p, st, who);
+  const Deal s = deal<F>(p.rows, p.d);
+  p.L = s.L;
+  const int64_t blocks = (p.rows + s.groups - 1) / s.groups;
+  auto kern = norm_add_norm_fwd_kernel<TY, F::E, F::NV, F::WARPS, F::CTAS, GATE>;
+  return launch_dependent(who, kern, (unsigned)(blocks < 64 * kNumSMs ? blocks : 64 * kNumSMs), s.threads, 0, st, p);
 }
 
-template <typename TY, bool GATE>
-int launch_fwd(FwdParams p, int E, cudaStream_t st, const char* who) {
-  const int nvec = p.d / E, nv = fwd_nv(nvec, E);
-  const Split s = split_rows(p.rows, nvec, nv, kFwdWarps);
-  p.W = s.W;
-  int64_t blocks = (p.rows + s.groups - 1) / s.groups;
-  if (blocks > 64 * kNumSMs) blocks = 64 * kNumSMs;
-  auto go = [&](auto kern) { return launch_dependent(who, kern, (unsigned)blocks, s.W * s.groups * 32, 0, st, p); };
-  if (E == 8)
-    return nv == 1 ? go(norm_add_norm_fwd_kernel<TY, 8, 1, GATE>) : nv == 2 ? go(norm_add_norm_fwd_kernel<TY, 8, 2, GATE>)
-         : nv == 3 ? go(norm_add_norm_fwd_kernel<TY, 8, 3, GATE>) : go(norm_add_norm_fwd_kernel<TY, 8, 4, GATE>);
-  return nv <= 2 ? go(norm_add_norm_fwd_kernel<TY, 4, 2, GATE>) : nv <= 4 ? go(norm_add_norm_fwd_kernel<TY, 4, 4, GATE>) : go(norm_add_norm_fwd_kernel<TY, 4, 8, GATE>);
+template <typename TY, bool GATE, typename F, typename... Rest>
+int launch_bwd(Forms<F, Rest...>, BwdParams p, int64_t* parts, cudaStream_t st, const char* who) {
+  if constexpr (sizeof...(Rest) > 0)
+    if (p.d > F::kMost) return launch_bwd<TY, GATE>(Forms<Rest...>(), p, parts, st, who);
+  const Deal s = deal<F>(p.rows, p.d);
+  p.L = s.L;
+  const size_t smem = (size_t)s.groups * p.d * sizeof(float);       // a warp has E NV 32 columns at most
+  static_assert(F::CTAS <= kMostCtas && (F::E * F::NV * F::WARPS * 32 + 8 * F::WARPS) * sizeof(float) <= 48 * 1024, "partial rows; shared memory without an opt-in");
+  auto kern = norm_add_norm_bwd_kernel<TY, F::E, F::NV, F::WARPS, F::CTAS, GATE>;
+  const int64_t want = (p.rows + s.groups - 1) / s.groups;
+  *parts = want < F::CTAS * kNumSMs ? want : F::CTAS * kNumSMs;
+  return launch_dependent(who, kern, (unsigned)*parts, s.threads, smem, st, p);
 }
-
 template <typename TY, bool GATE>
-int launch_bwd(BwdParams p, int E, int64_t* parts, cudaStream_t st, const char* who) {
-  const int nvec = p.d / E, nv = bwd_nv(p.d, E);
-  const Split s = split_rows(p.rows, nvec, nv, kBwdWarps);
-  p.W = s.W;
-  const int64_t blocks = bwd_blocks(p.rows, s);
-  // a warp has at most kBwdElems columns of a row, so groups x d is at most that for every warp of the CTA (32 KB)
-  const size_t smem = (size_t)s.groups * p.d * sizeof(float);
-  *parts = blocks;
-  auto go = [&](auto kern) { return launch_dependent(who, kern, (unsigned)blocks, s.W * s.groups * 32, smem, st, p); };
-  const bool wide = s.W > kBwdWarps;
-  if (E == 8)
-    return nv == 1 ? go(norm_add_norm_bwd_kernel<TY, 8, 1, kBwdWarps, GATE>)
-         : wide ? go(norm_add_norm_bwd_kernel<TY, 8, 2, kBwdWideWarps, GATE>) : go(norm_add_norm_bwd_kernel<TY, 8, 2, kBwdWarps, GATE>);
-  return nv == 2 ? go(norm_add_norm_bwd_kernel<TY, 4, 2, kBwdWarps, GATE>)
-       : wide ? go(norm_add_norm_bwd_kernel<TY, 4, 4, kBwdWideWarps, GATE>) : go(norm_add_norm_bwd_kernel<TY, 4, 4, kBwdWarps, GATE>);
+int launch(const FwdParams& p, int E, cudaStream_t st, const char* who) {
+  return E == 8 ? launch_fwd<TY, GATE>(Fwd8(), p, st, who) : launch_fwd<TY, GATE>(Fwd4(), p, st, who);
+}
+template <typename TY, bool GATE>
+int launch(const BwdParams& p, int E, int64_t* parts, cudaStream_t st, const char* who) {
+  using Wide = std::conditional_t<GATE, Bwd8Gate, Bwd8>;
+  return E == 8 ? launch_bwd<TY, GATE>(Wide(), p, parts, st, who) : launch_bwd<TY, GATE>(Bwd4(), p, parts, st, who);
 }
 
 }  // namespace
@@ -386,17 +498,18 @@ extern "C" int ulm_norm_add_norm_fwd(const ulm_norm_add_norm_fwd_args* a) {
   if (!ok32(a->x, a->x_stride) || !ok32(a->x_out, a->xout_stride) || !ok32(a->v, 0) || !ok32(a->w, 0) || (a->scale_channels && !ok32(a->scale, 0)) ||
       !ok16(a->branch, a->branch_stride, 4) || !ok16(a->gate, a->gate_stride, 4) || !ok16(a->y, a->y_stride, 4))
     return fail(ULM_ERR_ARG, "%s: fp32 rows must be 16-byte aligned, 16-bit rows 8-byte aligned", who);
-  const int E = a->d % 8 == 0 && ok16(a->branch, a->branch_stride, 8) && ok16(a->gate, a->gate_stride, 8) && ok16(a->y, a->y_stride, 8) ? 8 : 4;
+  const int E = a->d % 8 == 0 && ok16(a->branch, a->branch_stride, 8) && ok16(a->gate, a->gate_stride, 8) && ok16(a->y, a->y_stride, 8) && ok256(a->x, a->x_stride) &&
+                        ok256(a->x_out, a->xout_stride) && ok256(a->v, 0) && ok256(a->w, 0) && (!a->scale_channels || ok256(a->scale, 0)) ? 8 : 4;
   const FwdParams p{a->x, a->branch, a->gate, a->v, a->w, {a->scale, a->scale_value, a->scale_channels}, a->x_out, a->y, a->rstd_branch, a->rstd,
                     a->x_stride, a->branch_stride, a->gate_stride, a->xout_stride, a->y_stride, a->rows, a->d, 1, a->eps};
   cudaStream_t st = (cudaStream_t)a->stream;
-  auto go = [&](auto t) { return a->gate ? launch_fwd<decltype(t), true>(p, E, st, who) : launch_fwd<decltype(t), false>(p, E, st, who); };
+  auto go = [&](auto t) { return a->gate ? launch<decltype(t), true>(p, E, st, who) : launch<decltype(t), false>(p, E, st, who); };
   return a->dtype == ULM_F16 ? go(__half()) : go(__nv_bfloat16());
 }
 
 // one CTA a row, or as many as run at a time
 extern "C" int64_t ulm_norm_add_norm_partial(int64_t rows, int32_t d) {
-  const int64_t most = ulm::kMostBwdCtas * ulm::kNumSMs, n = rows < 1 ? 1 : rows < most ? rows : most;
+  const int64_t most = ulm::kMostCtas * ulm::kNumSMs, n = rows < 1 ? 1 : rows < most ? rows : most;
   return n * (2 * (int64_t)d + 1);
 }
 
@@ -414,14 +527,15 @@ extern "C" int ulm_norm_add_norm_bwd(const ulm_norm_add_norm_bwd_args* a) {
                       !ok16(a->dy, a->dy_stride, 4) || !ok16(a->d_branch, a->dbranch_stride, 4) || !ok16(a->d_gate, a->dgate_stride, 4)))
     return fail(ULM_ERR_ARG, "%s: fp32 rows must be 16-byte aligned, 16-bit rows 8-byte aligned", who);
   const int E = a->d % 8 == 0 && ok16(a->branch, a->branch_stride, 8) && ok16(a->gate, a->gate_stride, 8) && ok16(a->dy, a->dy_stride, 8) &&
-                        ok16(a->d_branch, a->dbranch_stride, 8) && ok16(a->d_gate, a->dgate_stride, 8) ? 8 : 4;
+                        ok16(a->d_branch, a->dbranch_stride, 8) && ok16(a->d_gate, a->dgate_stride, 8) && ok256(a->x, a->x_stride) && ok256(a->dx, a->dx_stride) &&
+                        ok256(a->g_add, a->gadd_stride) && ok256(a->v, 0) && ok256(a->w, 0) && (!a->scale_channels || ok256(a->scale, 0)) ? 8 : 4;
   cudaStream_t st = (cudaStream_t)a->stream;
   const Scale scale{a->scale, a->scale_value, a->scale_channels};
   int64_t blocks = 0;
   if (a->rows > 0) {
     const BwdParams p{a->x, a->branch, a->gate, a->v, a->w, scale, a->dy, a->g_add, a->rstd_branch, a->rstd, a->dx, a->d_branch, a->d_gate, a->partial,
                       a->x_stride, a->branch_stride, a->gate_stride, a->dy_stride, a->gadd_stride, a->dx_stride, a->dbranch_stride, a->dgate_stride, a->rows, a->d, 1};
-    auto go = [&](auto t) { return a->gate ? launch_bwd<decltype(t), true>(p, E, &blocks, st, who) : launch_bwd<decltype(t), false>(p, E, &blocks, st, who); };
+    auto go = [&](auto t) { return a->gate ? launch<decltype(t), true>(p, E, &blocks, st, who) : launch<decltype(t), false>(p, E, &blocks, st, who); };
     if (int rc = a->dtype == ULM_F16 ? go(__half()) : go(__nv_bfloat16())) return rc;
   }
   return launch_dependent(who, norm_add_norm_finish_kernel, (2 * a->d + 1 + 31) / 32, dim3(32, 32), 0, st, a->partial, a->v, scale, a->dw, a->dv, a->dscale, (int)blocks, a->d);
