@@ -309,6 +309,33 @@ int ulm_add_dropout_norm_fwd(const ulm_rmsnorm_fwd_args* a, double p, uint64_t s
 int ulm_add_dropout_norm_bwd(const ulm_rmsnorm_bwd_args* a, double p, uint64_t seed);
 int64_t ulm_add_dropout_norm_partial_rows(int64_t rows);
 
+/* ---- activations in 8 bits between forward and backward --------------------
+ * No counterpart in the reference.  A tensor of n elements in blocks of 32 consecutive ones (row-major index, the last block may be
+ * shorter), each with the exponent e of its largest magnitude, at least -120: the byte e + 127 in exps, and for each element the integer
+ * x / 2^(e - 6) rounded to nearest, ties to even, held to +-127 in codes.  Byte 255: the block had an infinity or a NaN and stands for NaN.
+ * ulm_pack8, ulm_unpack8: n elements of dtype (fp16, bf16 or fp32) and back; ulm_pack8_blocks(n) exponents.  unpack gives code 2^(e - 6),
+ *   which is a number of the packed type.  x and codes 16-byte aligned.
+ * ulm_swiglu8_fwd: y = drop(silu(a) * b) as ulm_swiglu_dropout has it (p = 0: nothing is dropped), and a and b in 8 bits.
+ * ulm_swiglu8_bwd: da and db from dy and the 8 bits alone, and with a non-NULL y also drop(silu(a) * b) of them.
+ *   d = 0: a, b, da, db dense, else rows of d elements, row_stride apart, as in ulm_swiglu_rows; y, dy and the 8 bits are dense.  fp32
+ *   arithmetic from the loads to the one rounding of each store. */
+int64_t ulm_pack8_blocks(int64_t n);
+int ulm_pack8(const void* x, int8_t* codes, uint8_t* exps, int64_t n, int32_t dtype, void* stream);
+int ulm_unpack8(const int8_t* codes, const uint8_t* exps, void* x, int64_t n, int32_t dtype, void* stream);
+typedef struct {
+  const void* a; const void* b;        /* fwd inputs                           */
+  void* y;                             /* fwd output; bwd output or NULL       */
+  int8_t* codes_a; int8_t* codes_b;    /* fwd outputs, bwd inputs: n each      */
+  uint8_t* exps_a; uint8_t* exps_b;    /* ulm_pack8_blocks(n) each             */
+  const void* dy; void* da; void* db;  /* bwd                                  */
+  int64_t n, d, row_stride;
+  double p; uint64_t seed;
+  int32_t dtype, reserved;
+  void* stream;
+} ulm_swiglu8_args;
+int ulm_swiglu8_fwd(const ulm_swiglu8_args* a);
+int ulm_swiglu8_bwd(const ulm_swiglu8_args* a);
+
 /* ---- the norms behind and in front of a block, with the residual add between them ----
  * No counterpart in the reference, whose blocks have the second norm alone (train.py:1989-1993).
  * fwd: u = branch rstd_branch, rstd_branch = rsqrt(mean(branch^2) + eps); x_out = x + s sigmoid(gate) v u; y = w x_out rstd,

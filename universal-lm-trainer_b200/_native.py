@@ -23,8 +23,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
-            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'norm_add_norm.cu', 'rotary.cu']          # slowest first: they are compiled in parallel
-_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'norm_rows.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
+            'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'norm_add_norm.cu', 'rotary.cu', 'pack8.cu']          # slowest first: they are compiled in parallel
+_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'norm_rows.cuh', 'pack8.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
 _EXT_SOURCE = 'torch_ops.cpp'
@@ -112,6 +112,11 @@ class SwigluArgs(C.Structure):
                 ('dtype', i32), ('reserved', i32), ('stream', vp)]
 
 
+class Swiglu8Args(C.Structure):
+    _fields_ = ([(n, vp) for n in ('a', 'b', 'y', 'codes_a', 'codes_b', 'exps_a', 'exps_b', 'dy', 'da', 'db')] + [(n, i64) for n in ('n', 'd', 'row_stride')] +
+                [('p', f64), ('seed', u64), ('dtype', i32), ('reserved', i32), ('stream', vp)])
+
+
 class CeFwdArgs(C.Structure):
     _fields_ = [('logits', vp), ('target', vp), ('lse', vp), ('loss', vp), ('row_stride', i64),
                 ('rows', i64), ('V', i32), ('dtype', i32), ('ignore_index', i64), ('stream', vp)]
@@ -172,6 +177,11 @@ EXPORTS = {
     'ulm_add_dropout_norm_fwd': (C.c_int, [C.POINTER(RmsFwdArgs), f64, u64]),
     'ulm_add_dropout_norm_bwd': (C.c_int, [C.POINTER(RmsBwdArgs), f64, u64]),
     'ulm_add_dropout_norm_partial_rows': (i64, [i64]),
+    'ulm_pack8_blocks': (i64, [i64]),
+    'ulm_pack8': (C.c_int, [vp, vp, vp, i64, i32, vp]),
+    'ulm_unpack8': (C.c_int, [vp, vp, vp, i64, i32, vp]),
+    'ulm_swiglu8_fwd': (C.c_int, [C.POINTER(Swiglu8Args)]),
+    'ulm_swiglu8_bwd': (C.c_int, [C.POINTER(Swiglu8Args)]),
     'ulm_norm_add_norm_fwd': (C.c_int, [C.POINTER(NormAddNormFwdArgs)]),
     'ulm_norm_add_norm_bwd': (C.c_int, [C.POINTER(NormAddNormBwdArgs)]),
     'ulm_norm_add_norm_partial': (i64, [i64, i32]),

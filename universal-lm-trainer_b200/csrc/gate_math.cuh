@@ -69,6 +69,12 @@ __device__ __forceinline__ int64_t operand_vec(int64_t v, const Rows& rw) {
   const uint32_t u = (uint32_t)v, r = u / rw.vpr;        // fewer than 2^32 vectors (checked by the host)
   return (int64_t)r * rw.stride + (u - r * rw.vpr);
 }
+// and element i
+template <typename T, bool ROWS>
+__device__ __forceinline__ int64_t operand_element(int64_t i, const Rows& rw) {
+  if constexpr (!ROWS) return i;
+  return operand_vec<ROWS>(i / VecN<T>::N, rw) * VecN<T>::N + i % VecN<T>::N;
+}
 
 }  // namespace
 }  // namespace ulm

@@ -1325,6 +1325,36 @@ void swiglu_rows(const Tensor& ab, const Tensor& y, const Tensor& dy, const Tens
   check(drop.none() ? ulm_swiglu_rows(&p, backward, d, 2 * d) : ulm_swiglu_dropout(&p, backward, d, 2 * d, drop.p, (uint64_t)drop.seed), backward ? "swiglu backward" : "swiglu forward");
 }
 
+// Gradients of x, w1 and w3 (inputs 0 to 2 of `node`) from those of the two projections: da and db, which lie in dab as its halves, or by
+// themselves where dab is undefined
+variable_list gated_products(OpNode& node, const Tensor& dab, const Tensor& da, const Tensor& db, const Tensor& x2, at::IntArrayRef x_sizes, at::ScalarType x_dtype,
+                             const Tensor& w1, const Tensor& w3, at::ScalarType cd) {
+  const int64_t ff = w1.size(0);
+  Tensor dx, dw1, dw3;
+  if (node.task_should_compute_output(0)) {
+    const Tensor c1 = cast_cached(w1, cd), c3 = cast_cached(w3, cd), both = dab.defined() ? stacked(c1, c3) : Tensor();
+    dx = both.defined() ? at::mm(dab, both) : at::mm(da, c1).addmm_(db, c3);      // one GEMM sums the two branches in fp32
+    dx = dx.view(x_sizes).to(x_dtype);
+  }
+  const bool need1 = node.task_should_compute_output(1), need3 = node.task_should_compute_output(2);
+  if (need1 && need3 && dab.defined()) {
+    const Tensor g1 = w1.grad(), g3 = w3.grad();
+    if (is_16bit(cd) && wgrad_in_place() && g1.defined() && g3.defined() && g1.scalar_type() == at::kFloat) {
+      Tensor both = stacked(g1, g3);
+      if (both.defined()) {
+        at::addmm_out(both, both, dab.t(), x2, at::kFloat);
+        return {dx, Tensor(), Tensor()};
+      }
+    } else if (is_16bit(cd) && w1.scalar_type() == at::kFloat && w3.scalar_type() == at::kFloat) {
+      const Tensor dw = at::mm(dab.t(), x2, at::kFloat);
+      return {dx, dw.narrow(0, 0, ff), dw.narrow(0, ff, ff)};
+    }
+  }
+  if (need1) dw1 = weight_grad(w1, da, x2);
+  if (need3) dw3 = weight_grad(w3, db, x2);
+  return {dx, dw1, dw3};
+}
+
 struct GatedBwd : OpNode {
   at::ScalarType cd, x_dtype;
   Drop drop;
@@ -1333,31 +1363,7 @@ struct GatedBwd : OpNode {
     const Tensor dy = dense16(g[0].reshape({-1, g[0].size(-1)}).to(cd)), x2 = x.reshape({-1, x.size(-1)});
     const Tensor dab = empty_cuda(ab.sizes(), cd, ab);
     swiglu_rows(ab, Tensor(), dy, dab, true, drop);
-    const int64_t ff = w1.size(0);
-    const Tensor da = dab.narrow(1, 0, ff), db = dab.narrow(1, ff, ff);
-    Tensor dx, dw1, dw3;
-    if (task_should_compute_output(0)) {
-      const Tensor c1 = cast_cached(w1, cd), c3 = cast_cached(w3, cd), both = stacked(c1, c3);
-      dx = both.defined() ? at::mm(dab, both) : at::mm(da, c1).addmm_(db, c3);      // one GEMM sums the two branches in fp32
-      dx = dx.view(x.sizes()).to(x_dtype);
-    }
-    const bool need1 = task_should_compute_output(1), need3 = task_should_compute_output(2);
-    if (need1 && need3) {
-      const Tensor g1 = w1.grad(), g3 = w3.grad();
-      if (is_16bit(cd) && wgrad_in_place() && g1.defined() && g3.defined() && g1.scalar_type() == at::kFloat) {
-        Tensor both = stacked(g1, g3);
-        if (both.defined()) {
-          at::addmm_out(both, both, dab.t(), x2, at::kFloat);
-          return {dx, Tensor(), Tensor()};
-        }
-      } else if (is_16bit(cd) && w1.scalar_type() == at::kFloat && w3.scalar_type() == at::kFloat) {
-        const Tensor dw = at::mm(dab.t(), x2, at::kFloat);
-        return {dx, dw.narrow(0, 0, ff), dw.narrow(0, ff, ff)};
-      }
-    }
-    if (need1) dw1 = weight_grad(w1, da, x2);
-    if (need3) dw3 = weight_grad(w3, db, x2);
-    return {dx, dw1, dw3};
+    return gated_products(*this, dab, dab.narrow(1, 0, w1.size(0)), dab.narrow(1, w1.size(0), w1.size(0)), x2, x.sizes(), x_dtype, w1, w3, cd);
   }
   variable_list backward_recorded(variable_list& g, const variable_list& kept) override {
     return drop.none() ? OpNode::backward_recorded(g, kept) : backward_once(g, kept, "gated_linear with dropout");
@@ -1404,6 +1410,234 @@ Tensor gated_linear(const Tensor& x, const Tensor& w1, const Tensor& w3) { retur
 Tensor gated_linear_dropout(const Tensor& x, const Tensor& w1, const Tensor& w3, double p, int64_t seed) {
   check_drop(p, "gated_linear");
   return gated(x, w1, w3, Drop{p, seed});
+}
+
+// ---------------------------------------------------------------------------
+// activations kept in 8 bits between forward and backward
+// ---------------------------------------------------------------------------
+// `count` tensors of n elements each in one buffer: their codes one behind the other, each on a 16-byte boundary, then their exponents
+struct Packed8 {
+  Tensor buffer;
+  int64_t n = 0, count = 1;
+  static int64_t codes_bytes(int64_t n) { return (n + 15) / 16 * 16; }
+  static int64_t bytes(int64_t n, int64_t count) { return count * (codes_bytes(n) + ulm_pack8_blocks(n)); }
+  int8_t* codes(int64_t i = 0) const { return static_cast<int8_t*>(buffer.data_ptr()) + i * codes_bytes(n); }
+  uint8_t* exps(int64_t i = 0) const { return static_cast<uint8_t*>(buffer.data_ptr()) + count * codes_bytes(n) + i * ulm_pack8_blocks(n); }
+  static Packed8 make(int64_t n, int64_t count, const Tensor& like) { return {empty_cuda({bytes(n, count)}, at::kByte, like), n, count}; }
+};
+Packed8 pack8(const Tensor& x) {
+  const Tensor d = dense16(x);
+  const Packed8 p = Packed8::make(d.numel(), 1, d);
+  check(ulm_pack8(d.data_ptr(), p.codes(), p.exps(), p.n, code_of(d.scalar_type()), stream_of(d)), "pack_8bit");
+  return p;
+}
+Tensor unpack8(const Packed8& p, at::IntArrayRef sizes, at::ScalarType dtype) {
+  const Tensor x = empty_cuda(sizes, dtype, p.buffer);
+  check(ulm_unpack8(p.codes(), p.exps(), x.data_ptr(), p.n, code_of(dtype), stream_of(x)), "unpack_8bit");
+  return x;
+}
+
+std::tuple<Tensor, Tensor> pack_8bit(const Tensor& x) {
+  TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()), "pack_8bit needs a CUDA fp16/bf16/fp32 tensor");
+  OpScope scope;
+  c10::cuda::CUDAGuard dev(x.device());
+  const Packed8 p = pack8(x.detach());
+  const int64_t at = Packed8::codes_bytes(p.n);
+  return {p.buffer.narrow(0, 0, p.n).view(at::kChar).view(x.sizes()), p.buffer.narrow(0, at, p.buffer.numel() - at)};
+}
+Tensor unpack_8bit(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(codes_in.is_cuda() && codes_in.scalar_type() == at::kChar && known(dtype), "unpack_8bit needs CUDA int8 codes and a result of fp16, bf16 or fp32");
+  TORCH_CHECK_VALUE(exps_in.device() == codes_in.device() && exps_in.scalar_type() == at::kByte && exps_in.dim() == 1 && exps_in.numel() == ulm_pack8_blocks(codes_in.numel()),
+                    "unpack_8bit needs one uint8 exponent for every 32 codes, on their device");
+  OpScope scope;
+  c10::cuda::CUDAGuard dev(codes_in.device());
+  const Tensor codes = dense16(codes_in), exps = exps_in.contiguous(), x = empty_cuda(codes.sizes(), dtype, codes);
+  check(ulm_unpack8(static_cast<int8_t*>(codes.data_ptr()), static_cast<uint8_t*>(exps.data_ptr()), x.data_ptr(), codes.numel(), code_of(dtype), stream_of(x)), "unpack_8bit");
+  return x;
+}
+
+// The gate over dense operands, or (d > 0) the two column halves of one [rows, 2 d] matrix
+ulm_swiglu8_args gate8_args(const Packed8& kept, at::ScalarType dtype, int64_t d, const Drop& drop) {
+  ulm_swiglu8_args a{};
+  a.codes_a = kept.codes(0); a.codes_b = kept.codes(1); a.exps_a = kept.exps(0); a.exps_b = kept.exps(1);
+  a.n = kept.n; a.d = d; a.row_stride = 2 * d; a.p = drop.p; a.seed = (uint64_t)drop.seed;
+  a.dtype = code_of(dtype); a.stream = stream_of(kept.buffer);
+  return a;
+}
+Packed8 gate8_forward(const Tensor& a_t, const Tensor& b_t, int64_t d, int64_t n, const Tensor& y, const Drop& drop) {
+  const Packed8 kept = Packed8::make(n, 2, y);
+  ulm_swiglu8_args a = gate8_args(kept, y.scalar_type(), d, drop);
+  a.a = a_t.data_ptr(); a.b = b_t.data_ptr(); a.y = y.data_ptr();
+  check(ulm_swiglu8_fwd(&a), "swiglu_8bit forward");
+  return kept;
+}
+void gate8_backward(const Packed8& kept, const Tensor& dy, const Tensor& da, const Tensor& db, int64_t d, const Tensor& y, const Drop& drop) {
+  ulm_swiglu8_args a = gate8_args(kept, dy.scalar_type(), d, drop);
+  a.dy = dy.data_ptr(); a.da = da.data_ptr(); a.db = db.data_ptr(); a.y = y.defined() ? y.data_ptr() : nullptr;
+  check(ulm_swiglu8_bwd(&a), "swiglu_8bit backward");
+}
+
+struct Swiglu8Bwd : OpNode {
+  Drop drop;
+  std::vector<int64_t> shape;
+  at::ScalarType dtype;
+  int64_t n = 0;
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor dy = dense16(as_type(g[0], dtype)), da = empty_cuda(shape, dtype, dy), db = empty_cuda(shape, dtype, dy);
+    gate8_backward({kept[0], n, 2}, dy, da, db, 0, Tensor(), drop);
+    return {da, db};
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "swiglu_8bit"); }
+};
+
+Tensor swiglu_8bit(const Tensor& a_in, const Tensor& b_in, double p, int64_t seed) {
+  TORCH_CHECK_VALUE(a_in.is_cuda() && known(a_in.scalar_type()) && b_in.scalar_type() == a_in.scalar_type() && b_in.sizes() == a_in.sizes() && b_in.device() == a_in.device(),
+                    "swiglu_8bit needs two tensors of one CUDA device, of one shape and one of fp16/bf16/fp32");
+  check_drop(p, "swiglu_8bit");
+  const Drop drop{p, seed};
+  Tensor y;
+  Packed8 kept;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(a_in.device());
+    const Tensor a = dense16(a_in), b = dense16(b_in);
+    y = empty_cuda(a.sizes(), a.scalar_type(), a);
+    kept = gate8_forward(a, b, 0, a.numel(), y, drop);
+  }
+  if (!no_graph(a_in, b_in)) {
+    auto node = make_node<Swiglu8Bwd>(a_in, b_in);
+    node->drop = drop; node->shape = y.sizes().vec(); node->dtype = y.scalar_type(); node->n = kept.n;
+    node->keep(kept.buffer);
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+struct Linear8Bwd : OpNode {
+  at::ScalarType cd, x_dtype;
+  std::vector<int64_t> shape;                              // of x
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor weight = kept[0], buffer = kept[1];
+    const Tensor dy = g[0].reshape({-1, weight.size(0)}).to(cd);
+    const int64_t d = shape.back(), rows = dy.size(0);
+    Tensor dx, dw;
+    if (task_should_compute_output(0)) dx = at::mm(dy, cast_cached(weight, cd)).view(shape).to(x_dtype);
+    if (task_should_compute_output(1)) dw = weight_grad(weight, dy, unpack8({buffer, rows * d, 1}, {rows, d}, cd));
+    return {dx, dw};
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "linear_8bit"); }
+};
+
+at::ScalarType compute_dtype(const Tensor& x) { return at::autocast::is_autocast_enabled(at::kCUDA) ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type(); }
+void check_projection(const Tensor& x, const Tensor& w, const char* who) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.is_floating_point() && x.dim() >= 1 && w.device() == x.device() && w.is_floating_point() && w.dim() == 2 && w.size(1) == x.size(-1),
+                    who, " needs x [.., d] and weights [.., d] on one CUDA device");
+  TORCH_CHECK_VALUE(known(compute_dtype(x)), who, " computes in fp16, bf16 or fp32");
+}
+
+Tensor linear_8bit(const Tensor& x, const Tensor& weight) {
+  check_projection(x, weight, "linear_8bit");
+  const at::ScalarType cd = compute_dtype(x);
+  Tensor y;
+  Packed8 kept;
+  const bool graph = !no_graph(x, weight);
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(x.device());
+    const Tensor xc = x.to(cd);
+    auto n = xc.sizes().vec();
+    n.back() = weight.size(0);
+    y = at::mm(xc.reshape({-1, xc.size(-1)}), cast_cached(weight, cd).t()).view(n);
+    if (graph && weight.requires_grad()) kept = pack8(xc);
+  }
+  if (graph) {
+    auto node = make_node<Linear8Bwd>(x, weight);
+    node->cd = cd; node->x_dtype = x.scalar_type(); node->shape = x.sizes().vec();
+    node->keep(weight);
+    node->keep(kept.buffer);
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+struct FeedForward8Bwd : OpNode {
+  at::ScalarType cd, x_dtype;
+  Drop drop;
+  std::vector<int64_t> shape;                              // of x
+  int64_t rows = 0;
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor w1 = kept[0], w3 = kept[1], w2 = kept[2], px = kept[3], pab = kept[4];
+    const int64_t d = w1.size(1), ff = w1.size(0);
+    const bool need_x = task_should_compute_output(0), need1 = task_should_compute_output(1), need3 = task_should_compute_output(2), need2 = task_should_compute_output(3);
+    const Tensor go = g[0].reshape({-1, w2.size(0)}).to(cd);
+    const Tensor dy = dense16(at::mm(go, cast_cached(w2, cd)));
+    const bool halves = ff % (16 / (int64_t)c10::elementSize(cd)) == 0;
+    Tensor dab, da, db, y;
+    if (halves) {
+      dab = empty_cuda({rows, 2 * ff}, cd, dy);
+      da = dab.narrow(1, 0, ff); db = dab.narrow(1, ff, ff);
+    } else {
+      da = empty_cuda({rows, ff}, cd, dy); db = empty_cuda({rows, ff}, cd, dy);
+    }
+    if (need2) y = empty_cuda({rows, ff}, cd, dy);
+    gate8_backward({pab, rows * ff, 2}, dy, da, db, halves ? ff : 0, y, drop);
+    Tensor dw2;
+    if (need2) dw2 = weight_grad(w2, go, y);
+    y = Tensor();
+    const Tensor x2 = need1 || need3 ? unpack8({px, rows * d, 1}, {rows, d}, cd) : Tensor();
+    variable_list r = need_x || need1 || need3 ? gated_products(*this, dab, da, db, x2, shape, x_dtype, w1, w3, cd) : variable_list(3);
+    r.push_back(dw2);
+    return r;
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "feed_forward_8bit"); }
+};
+
+// linear(drop(silu(x w1^T) * (x w3^T)), w2), of which x, the two projections and nothing else are kept, all three in 8 bits
+Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, double p, int64_t seed) {
+  check_projection(x, w1, "feed_forward_8bit");
+  TORCH_CHECK_VALUE(w3.device() == x.device() && w3.sizes() == w1.sizes() && w3.is_floating_point() && w2.device() == x.device() && w2.dim() == 2 && w2.size(1) == w1.size(0) && w2.is_floating_point(),
+                    "feed_forward_8bit needs w1 and w3 [ff, d] and w2 [.., ff] on one CUDA device");
+  check_drop(p, "feed_forward_8bit");
+  const Drop drop{p, seed};
+  const at::ScalarType cd = compute_dtype(x);
+  const int64_t ff = w1.size(0);
+  Tensor out;
+  Packed8 px, pab;
+  int64_t rows = 0;
+  const bool graph = !no_graph(x, w1, w3, w2);
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(x.device());
+    const Tensor xc = x.to(cd), x2 = xc.reshape({-1, xc.size(-1)}), c1 = cast_cached(w1, cd), c3 = cast_cached(w3, cd);
+    rows = x2.size(0);
+    const Tensor y = empty_cuda({rows, ff}, cd, x2);
+    if (ff % (16 / (int64_t)c10::elementSize(cd)) == 0) {
+      const Tensor both = stacked(c1, c3);
+      Tensor ab;
+      if (both.defined()) {
+        ab = at::mm(x2, both.t());
+      } else {
+        ab = empty_cuda({rows, 2 * ff}, cd, x2);
+        Tensor a = ab.narrow(1, 0, ff), b = ab.narrow(1, ff, ff);
+        at::mm_out(a, x2, c1.t());
+        at::mm_out(b, x2, c3.t());
+      }
+      pab = gate8_forward(ab, ab.narrow(1, ff, ff), ff, rows * ff, y, drop);
+    } else {
+      pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), 0, rows * ff, y, drop);
+    }
+    if (graph && (w1.requires_grad() || w3.requires_grad())) px = pack8(x2);
+    auto n = xc.sizes().vec();
+    n.back() = w2.size(0);
+    out = at::mm(y, cast_cached(w2, cd).t()).view(n);
+  }
+  if (graph) {
+    auto node = make_node<FeedForward8Bwd>(x, w1, w3, w2);
+    node->cd = cd; node->x_dtype = x.scalar_type(); node->drop = drop; node->shape = x.sizes().vec(); node->rows = rows;
+    node->keep(w1); node->keep(w3); node->keep(w2); node->keep(px.buffer); node->keep(pab.buffer);
+    torch::autograd::set_history(out, node);
+  }
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -1705,6 +1939,11 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "linear", &::linear);
   def_op(m, "gated_linear", &::gated_linear);
   def_op(m, "gated_linear_dropout", &::gated_linear_dropout);
+  m.def("pack_8bit", &pack_8bit, no_gil());
+  m.def("unpack_8bit", &unpack_8bit, no_gil());
+  def_op(m, "swiglu_8bit", &::swiglu_8bit);
+  def_op(m, "linear_8bit", &::linear_8bit);
+  def_op(m, "feed_forward_8bit", &::feed_forward_8bit);
   m.def("lm_head_lse", &lm_head_lse, no_gil());
   m.def("lm_head_score", &lm_head_score, no_gil());
   m.def("token_targets", &token_targets, no_gil());

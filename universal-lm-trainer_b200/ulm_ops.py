@@ -8,6 +8,7 @@ below keep those names and argument meanings.
 import contextlib
 import ctypes as C
 import math
+import typing
 
 import torch
 import torch.nn as nn
@@ -302,6 +303,50 @@ def linear(x, weight):
     if not x.is_cuda and not N.have_ext():
         return nn.functional.linear(x, weight.to(x.dtype))
     return N.ext().linear(x, weight)
+
+
+# ---------------------------------------------------------------------------
+# Activations kept in 8 bits between forward and backward
+# ---------------------------------------------------------------------------
+class Packed8(typing.NamedTuple):
+    """A tensor in 8 bits (`pack_8bit`): ``codes`` int8 of its shape, ``exponents`` uint8, one for every 32 elements of its row-major order,
+    and the type it had.  33/32 bytes an element."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    dtype: torch.dtype
+
+
+def pack_8bit(x):
+    """A CUDA fp16/bf16/fp32 tensor in 8 bits: of every 32 consecutive elements the exponent e of the largest magnitude (at least -120) and
+    for each the integer nearest x / 2^(e - 6), ties to even, held to +-127.  What comes back (`unpack_8bit`) is off by at most 1/128 of the
+    block's largest magnitude (1/64 where 127 holds it), and is a number of x's own type; its rms error is 0.7 % of normally distributed values.  A
+    block with an infinity or a NaN comes back as NaN, so that a loss scaler sees it.  No gradient."""
+    return Packed8(*N.ext().pack_8bit(x), x.dtype)
+
+
+def unpack_8bit(packed, dtype=None):
+    """The values that `pack_8bit` kept, in the type they had, or rounded to ``dtype``."""
+    return N.ext().unpack_8bit(packed.codes, packed.exponents, packed.dtype if dtype is None else dtype)
+
+
+def swiglu_8bit(a, b, p=0.0, seed=0):
+    """`swiglu_dropout` (p = 0: without dropout), whose backward has a and b in 8 bits alone (`pack_8bit`): a graph keeps 2 1/16 bytes an
+    element in place of two tensors.  The result is that of the operands themselves, rounded once; the gradients are those at
+    the 8-bit operands."""
+    return N.ext().swiglu_8bit(a, b, float(p), _as_i64(seed))
+
+
+def linear_8bit(x, weight):
+    """`linear`, whose backward has its input in 8 bits alone (`pack_8bit`; nothing of it where the weight takes no gradient): the
+    result and x's gradient are those of `linear`, the weight's is that of the 8-bit input.  CUDA only."""
+    return N.ext().linear_8bit(x, weight)
+
+
+def feed_forward_8bit(x, w1, w3, w2, dropout_p=0.0, seed=0):
+    """``linear(gated_linear(x, w1, w3, dropout_p, seed), w2)`` (train.py:1975) as one op that keeps x and the two projections in 8 bits and nothing
+    else: d + 2 d_ff bytes a token (and 1/32 of that) where the ops by themselves keep 2 d + 6 d_ff.  The backward forms the gate's result
+    again from the 8-bit projections, for w2's gradient.  The gate is `swiglu_8bit`'s, the products `linear`'s.  CUDA only."""
+    return N.ext().feed_forward_8bit(x, w1, w3, w2, float(dropout_p), _as_i64(seed))
 
 
 def ce_rows_forward(logits, target, ignore_index):
