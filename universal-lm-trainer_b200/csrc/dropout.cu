@@ -168,7 +168,7 @@ template <typename T>
 int gate_launch(const ulm_swiglu_args* p, bool bwd, int64_t d, int64_t stride, const DropMask& mask, const char* who) {
   cudaStream_t st = (cudaStream_t)p->stream;
   const int64_t nvec = p->n / VecN<T>::N;
-  const Rows rw{(uint32_t)(d / VecN<T>::N), stride / VecN<T>::N};
+  const Rows rw = make_rows(d / VecN<T>::N, stride / VecN<T>::N);
   const T *a = (const T*)p->a, *b = (const T*)p->b, *dy = (const T*)p->dy;
   T *y = (T*)p->y, *da = (T*)p->da, *db = (T*)p->db;
   const unsigned grid = grid_for(nvec, kVecsGate);

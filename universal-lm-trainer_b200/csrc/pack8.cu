@@ -19,7 +19,7 @@ namespace {
 
 constexpr int kThreads = 256;
 // 16-byte vectors of the operands a thread takes
-constexpr int kVecsPack = 2, kVecsFwd = 2, kVecsBwd = 2;
+constexpr int kVecsPack = 4, kVecsFwd = 4, kVecsBwd = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -243,7 +243,7 @@ template <typename T, bool DROP>
 int gate8_launch(const ulm_swiglu8_args* p, bool bwd, const char* who) {
   cudaStream_t st = (cudaStream_t)p->stream;
   const int64_t nvec = whole_vecs<T>(p->n);
-  const Rows rw{(uint32_t)(p->d / VecN<T>::N), p->row_stride / VecN<T>::N};
+  const Rows rw = make_rows(p->d / VecN<T>::N, p->row_stride / VecN<T>::N);
   const Gate8 kept{p->codes_a, p->codes_b, p->exps_a, p->exps_b};
   const DropMask mask = make_drop_mask(p->p, p->seed);
   const T *a = (const T*)p->a, *b = (const T*)p->b, *dy = (const T*)p->dy;
