@@ -1132,6 +1132,64 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
   return {out[0], out[1]};
 }
 
+// The attention block between the two projections (qkv_attn) with rotary positions of any form on q and k
+struct QkvRotaryBwd : OpNode {
+  AttnArgs p{};
+  Turning how;                                             // of the gradients
+  int64_t B = 0, S = 0, H = 0, rows = -1;                  // rows >= 0: the flattened form with padding rows
+  variable_list backward(variable_list& g, const variable_list& kept) override {
+    const Tensor qkv = kept[0], positions = kept.size() > 6 ? kept[6] : Tensor();
+    const Tensor go = heads_of(g[0].contiguous(), B, S, H);
+    const Tensor d = empty_cuda(qkv.sizes(), qkv.scalar_type(), qkv);
+    if (rows > B * S) d.narrow(0, B * S, rows - B * S).zero_();
+    const Tensor dq = qkv_part(d, 0, B, S, H), dk = qkv_part(d, 1, B, S, H);
+    attn_backward(kept[1], kept[2], qkv_part(qkv, 2, B, S, H), heads_of(kept[3], B, S, H), kept[4], go, dq, dk, qkv_part(d, 2, B, S, H), p);
+    rotary_launch(dq, dk, dq, dk, kept[5], positions, how);
+    return {d};
+  }
+  variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "qkv_rope_flash_attn with rotary positions"); }
+};
+
+Tensor qkv_rotary_attn(const Tensor& qkv, int64_t H, const Tensor& turns, const OptTensor& positions_o, bool interleaved, double factor, double dropout_p, bool causal,
+                       double scale, int64_t seed, int64_t flat_b, int64_t flat_s) {
+  const char* who = "qkv_rope_flash_attn with rotary positions";
+  const bool flat = flat_b >= 0;
+  TORCH_CHECK_VALUE(!flat || (qkv.dim() == 2 && qkv.size(0) >= flat_b * flat_s), "flat_shape=(n, L) needs a 2-D qkv with at least n*L rows");
+  TORCH_CHECK_VALUE(qkv.is_cuda() && is_16bit(qkv.scalar_type()) && (flat || qkv.dim() == 3) && qkv.is_contiguous() && qkv.size(-1) == 3 * H * 64 &&
+                        !(reinterpret_cast<uintptr_t>(qkv.data_ptr()) & 31),
+                    "qkv_rope_flash_attn needs a contiguous CUDA fp16/bf16 [n, L, 3*n_heads*64] tensor");
+  const int64_t B = flat ? flat_b : qkv.size(0), S = flat ? flat_s : qkv.size(1), rows = flat ? qkv.size(0) : -1;
+  const Tensor positions = positions_o.value_or(Tensor());
+  check_turns(turns, positions, qkv, B, S, 64, who);
+  if (B * S == 0) {
+    auto n = qkv.sizes().vec();
+    n.back() = H * 64;
+    return at::zeros(n, qkv.options()) + 0 * qkv.sum();
+  }
+  const AttnArgs p{dropout_p, causal, scale, seed};
+  Tensor out, lse, qr, kr;
+  {
+    OpScope scope;
+    c10::cuda::CUDAGuard dev(qkv.device());
+    out = flat ? empty_cuda({rows, H * 64}, qkv.scalar_type(), qkv) : empty_cuda({B, S, H * 64}, qkv.scalar_type(), qkv);
+    if (rows > B * S) out.narrow(0, B * S, rows - B * S).zero_();
+    const Tensor q = qkv_part(qkv, 0, B, S, H), k = qkv_part(qkv, 1, B, S, H);
+    lse = empty_lse(q);
+    qr = empty_bshd(B, H, S, q);
+    kr = empty_bshd(B, H, S, q);
+    rotary_launch(q, k, qr, kr, turns, positions, {interleaved, false, factor});
+    attn_forward(qr, kr, qkv_part(qkv, 2, B, S, H), heads_of(out, B, S, H), lse, p);
+  }
+  if (!no_graph(qkv)) {
+    auto node = make_node<QkvRotaryBwd>(qkv);
+    node->p = p; node->how = {interleaved, true, factor}; node->B = B; node->S = S; node->H = H; node->rows = rows;
+    torch::autograd::set_history(out, node);
+    node->keep(qkv); node->keep(qr); node->keep(kr); node->keep(out, true); node->keep(lse); node->keep(turns);
+    if (positions.defined()) node->keep(positions);
+  }
+  return out;
+}
+
 // ---------------------------------------------------------------------------
 // linear layers
 // ---------------------------------------------------------------------------
@@ -1464,7 +1522,12 @@ ulm_swiglu8_args gate8_args(const Packed8& kept, at::ScalarType dtype, int64_t d
   a.dtype = code_of(dtype); a.stream = stream_of(kept.buffer);
   return a;
 }
-Packed8 gate8_forward(const Tensor& a_t, const Tensor& b_t, int64_t d, int64_t n, const Tensor& y, const Drop& drop) {
+Packed8 gate8_forward(const Tensor& a_t, const Tensor& b_t, int64_t d, int64_t n, const Tensor& y, const Drop& drop, bool graph) {
+  if (!graph) {                                            // the same values, and nothing to keep
+    ulm_swiglu_args p{a_t.data_ptr(), b_t.data_ptr(), y.data_ptr(), nullptr, nullptr, nullptr, n, code_of(y.scalar_type()), 0, stream_of(y)};
+    check(ulm_swiglu_dropout(&p, false, d, 2 * d, drop.p, (uint64_t)drop.seed), "swiglu_8bit forward");
+    return {};
+  }
   const Packed8 kept = Packed8::make(n, 2, y);
   ulm_swiglu8_args a = gate8_args(kept, y.scalar_type(), d, drop);
   a.a = a_t.data_ptr(); a.b = b_t.data_ptr(); a.y = y.data_ptr();
@@ -1495,6 +1558,7 @@ Tensor swiglu_8bit(const Tensor& a_in, const Tensor& b_in, double p, int64_t see
                     "swiglu_8bit needs two tensors of one CUDA device, of one shape and one of fp16/bf16/fp32");
   check_drop(p, "swiglu_8bit");
   const Drop drop{p, seed};
+  const bool graph = !no_graph(a_in, b_in);
   Tensor y;
   Packed8 kept;
   {
@@ -1502,9 +1566,9 @@ Tensor swiglu_8bit(const Tensor& a_in, const Tensor& b_in, double p, int64_t see
     c10::cuda::CUDAGuard dev(a_in.device());
     const Tensor a = dense16(a_in), b = dense16(b_in);
     y = empty_cuda(a.sizes(), a.scalar_type(), a);
-    kept = gate8_forward(a, b, 0, a.numel(), y, drop);
+    kept = gate8_forward(a, b, 0, a.numel(), y, drop, graph);
   }
-  if (!no_graph(a_in, b_in)) {
+  if (graph) {
     auto node = make_node<Swiglu8Bwd>(a_in, b_in);
     node->drop = drop; node->shape = y.sizes().vec(); node->dtype = y.scalar_type(); node->n = kept.n;
     node->keep(kept.buffer);
@@ -1622,9 +1686,9 @@ Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, co
         at::mm_out(a, x2, c1.t());
         at::mm_out(b, x2, c3.t());
       }
-      pab = gate8_forward(ab, ab.narrow(1, ff, ff), ff, rows * ff, y, drop);
+      pab = gate8_forward(ab, ab.narrow(1, ff, ff), ff, rows * ff, y, drop, graph);
     } else {
-      pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), 0, rows * ff, y, drop);
+      pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), 0, rows * ff, y, drop, graph);
     }
     if (graph && (w1.requires_grad() || w3.requires_grad())) px = pack8(x2);
     auto n = xc.sizes().vec();
@@ -1919,6 +1983,7 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "norm_add_norm_gate", &::norm_add_norm_gate);
   def_op(m, "norm_add_norm_scale", &::norm_add_norm_scale);
   def_op(m, "norm_add_norm_gate_scale", &::norm_add_norm_gate_scale);
+  def_op(m, "qkv_rotary_attn", &::qkv_rotary_attn);
   def_op(m, "rotary", &::rotary);
   def_op(m, "rotary_one", &::rotary_one);
   def_op(m, "dropout", &::dropout);

@@ -190,7 +190,7 @@ def rope_flash_attn(q, k, v, cos2d, sin2d, dropout_p: float = 0.0, causal: bool 
 
 
 def qkv_rope_flash_attn(qkv, n_heads, cos2d=None, sin2d=None, dropout_p: float = 0.0, causal: bool = True,
-                        softmax_scale=None, fuse=None, flat_shape=None):
+                        softmax_scale=None, fuse=None, flat_shape=None, rotary=None, positions=None):
     """qkv [n, L, 3*n_heads*64] (the fused projection, 16-bit, contiguous) -> attention output
     [n, L, n_heads*64]; RoPE with the fp32 (L,64) tables when they are given.  With ``flat_shape=(n, L)``
     qkv is the flattened [T', 3*n_heads*64] tensor with T' >= n*L (padding rows at the end) and the output is
@@ -200,13 +200,23 @@ def qkv_rope_flash_attn(qkv, n_heads, cos2d=None, sin2d=None, dropout_p: float =
     (train.py:1935-1939), RoPE on q and k, causal attention, heads merged back (train.py:1963).  Nothing is copied
     that the reference copies around the kernels: q, k, v are strided views of qkv, the output comes out of the kernel
     in (n, L, H, 64) order, and the backward kernels write dq, dk, dv straight into the three slices of one gradient
-    tensor (autograd would otherwise concatenate them)."""
+    tensor (autograd would otherwise concatenate them).
+
+    ``rotary``: a `ulm_ops.Rotary` of at most 64 columns turns q and k in place of the tables, at ``positions`` (`ulm_ops.rotary`; 0, 1, 2, ..
+    without)."""
     n, L = (-1, -1) if flat_shape is None else flat_shape
     if flat_shape is not None and min(n, L) < 0:
         raise ValueError('flat_shape=(n, L) takes sizes')
     code = _fuse_code(fuse)
     if softmax_scale is None:
         softmax_scale = 64 ** -0.5
+    if rotary is not None:
+        if cos2d is not None or sin2d is not None or fuse is not None:
+            raise ValueError('rotary positions take the place of the tables: give one of them, and no fuse')
+        return N.ext().qkv_rotary_attn(qkv, n_heads, rotary.turns, positions, bool(rotary.interleaved), float(rotary.factor), dropout_p, bool(causal), softmax_scale,
+                                       _seed_for(dropout_p), n, L)
+    if positions is not None:
+        raise ValueError('positions are for rotary=; the tables have a row for each')
     return N.ext().qkv_attn(qkv, n_heads, cos2d, sin2d, dropout_p, bool(causal), softmax_scale, _seed_for(dropout_p), code, n, L)
 
 

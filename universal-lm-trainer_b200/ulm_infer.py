@@ -21,14 +21,29 @@ import numpy as np
 import torch
 
 import _native as N
+import flash_attn_v100_cuda as fa
 import ulm_model
 import ulm_ops
 
 
-def causal_attention(qkv, n_heads, cos=None, sin=None, softmax_scale=None):
+def causal_attention(qkv, n_heads, cos=None, sin=None, softmax_scale=None, rotary=None, positions=None):
     """qkv [n, L, 3*n_heads*64] 16-bit, rows contiguous -> (attention output [n, L, n_heads*64], k, v) with k
     rotated, both as (n, n_heads, L, 64) views.  ``cos``/``sin``: the model's [1, L, >=64] or [L, >=64]
-    fp32 RoPE tables (None: no rotation).  No autograd graph is built and nothing is saved."""
+    fp32 RoPE tables (None: no rotation), or ``rotary``: a `ulm_ops.Rotary` of at most 64 columns, at ``positions``.
+    No autograd graph is built and nothing is saved."""
+    if rotary is not None:
+        if cos is not None or sin is not None:
+            raise ValueError('rotary positions take the place of the tables: give one of them')
+        if not (qkv.is_cuda and qkv.dtype in (torch.float16, torch.bfloat16) and qkv.dim() == 3 and qkv.shape[2] == 3 * n_heads * 64):
+            raise ValueError('causal_attention needs a CUDA fp16/bf16 [n, L, 3*n_heads*64] tensor with contiguous rows')
+        with torch.no_grad():
+            n, L = qkv.shape[:2]
+            q, k, v = (qkv.unflatten(2, (3, n_heads, 64))[:, :, i].transpose(1, 2) for i in range(3))
+            q, k = rotary(q, k, positions)
+            out = fa.flash_attn_v100(q, k, v, 0.0, True, softmax_scale)
+        return out.transpose(1, 2).reshape(n, L, n_heads * 64), k, v
+    if positions is not None:
+        raise ValueError('positions are for rotary=; the tables have a row for each')
     return N.ext().causal_attention(qkv, n_heads, cos, sin, 64 ** -0.5 if softmax_scale is None else float(softmax_scale))
 
 

@@ -8,6 +8,7 @@ no SDPA or eager fallback in here: a shape the kernels do not take (head_dim
 other than 64, CPU tensors) raises.
 """
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -15,7 +16,7 @@ import torch.nn.functional as F
 
 import flash_attn_v100_cuda as _fa
 import ulm_ops
-from ulm_ops import FusedRMSNorm, gated_linear, linear
+from ulm_ops import BranchNorm, FusedRMSNorm, Rotary, feed_forward_8bit, gated_linear, linear, linear_8bit
 
 
 @dataclass
@@ -33,6 +34,12 @@ class ModelConfig:  # train.py:725-737
     # not the reference's: what a training step need not store between forward and backward
     counter_dropout: bool = False   # feed-forward and residual dropout by ulm_ops.Dropout, inside the gate and the residual add + norm; not to be captured in a CUDA graph
     streamed_loss: bool = False     # ulm_ops.streamed_cross_entropy: no logits
+    activations_8bit: bool = False  # inputs of wqkv, w1 and w3 and the gate's operands kept in 8 bits (ulm_ops.linear_8bit, feed_forward_8bit); dropout in the gate by counter_dropout alone
+    # not the reference's: other blocks.  They add parameters (branch_*) or leave the tables out (rotary)
+    rotary: Optional[dict] = None   # arguments of ulm_ops.Rotary, in place of the d_model-wide tables; rotary_dim 64 unless it says less
+    branch_norm: bool = False       # a norm behind attention and feed-forward (ulm_ops.BranchNorm) ...
+    branch_gate: bool = False       # ... with a gate from the branch's input ...
+    branch_scale: Optional[float] = None    # ... and a learned scale that starts here
 
 
 def _option(config, name):
@@ -106,15 +113,16 @@ class MultiHeadAttention(nn.Module):  # train.py:1920-1964
         self.wqkv = nn.Linear(config.d_model, 3 * config.d_model, bias=False)
         self.wo = nn.Linear(config.d_model, config.d_model, bias=False)
         self.dropout = config.dropout
+        self.activations_8bit = _option(config, 'activations_8bit')
 
-    def forward(self, x, cos=None, sin=None, shape=None):
+    def forward(self, x, cos=None, sin=None, shape=None, rotary=None):
         """``x``: [n, L, d], or -- with ``shape=(n, L)`` -- the flattened tokens [T', d] with T' >= n*L (rows
-        beyond n*L are padding that only the projections see)."""
+        beyond n*L are padding that only the projections see).  ``rotary``: a `ulm_ops.Rotary` in place of the tables."""
         flat = shape is not None
         n, L = shape if flat else x.shape[:2]
         T = n * L
         x2d = x if flat else x.reshape(T, x.shape[-1])
-        qkv = linear(x2d, self.wqkv.weight)
+        qkv = linear_8bit(x2d, self.wqkv.weight) if self.activations_8bit else linear(x2d, self.wqkv.weight)
         if qkv.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError('attention runs in fp16/bf16: call the model under torch.autocast')
         # train.py:1935-1964 between the two projections as one op on the fused tensor: chunk, RoPE, causal
@@ -126,7 +134,7 @@ class MultiHeadAttention(nn.Module):  # train.py:1920-1964
             cos2d, sin2d = _tables_2d(cos, sin, self.head_dim)
         # on the flattened tensor: the op reads the first n*L rows as [n, L, 3d] and returns [T', d] with zero
         # padding rows, its backward a [T', 3d] gradient with zero padding rows (no pad or slice copies)
-        a2d = _fa.qkv_rope_flash_attn(qkv, self.n_heads, cos2d, sin2d, dropout_p=p_drop, causal=True, flat_shape=(n, L))
+        a2d = _fa.qkv_rope_flash_attn(qkv, self.n_heads, cos2d, sin2d, dropout_p=p_drop, causal=True, flat_shape=(n, L), rotary=rotary)
         out = linear(a2d, self.wo.weight)
         return out if flat else out.view(n, L, out.shape[-1])
 
@@ -145,6 +153,11 @@ def _drop(dropout, x):
     return x if idle else dropout(x)
 
 
+def _idle(dropout):
+    """Whether calling ``dropout`` is known to change nothing."""
+    return (_plain(dropout, nn.Dropout) or _plain(dropout, ulm_ops.Dropout)) and not (dropout.training and dropout.p > 0.0)
+
+
 def _mask_of(dropout):
     """(p, seed) where ``dropout`` is a plain `ulm_ops.Dropout` at work, for the kernel that works in its place; None where it has
     to be called (or is idle)."""
@@ -156,8 +169,9 @@ def _make_dropout(p, counter):
 
 
 class FeedForward(nn.Module):  # train.py:1966-1975
-    def __init__(self, d_model: int, d_ff: int, dropout: float, counter_dropout: bool = False):
+    def __init__(self, d_model: int, d_ff: int, dropout: float, counter_dropout: bool = False, activations_8bit: bool = False):
         super().__init__()
+        self.activations_8bit = activations_8bit
         self.w1 = nn.Linear(d_model, d_ff, bias=False)
         self.w3 = nn.Linear(d_model, d_ff, bias=False)
         self.w2 = nn.Linear(d_ff, d_model, bias=False)
@@ -165,6 +179,8 @@ class FeedForward(nn.Module):  # train.py:1966-1975
 
     def forward(self, x):
         mask = _mask_of(self.dropout)
+        if self.activations_8bit and (mask is not None or _idle(self.dropout)):
+            return feed_forward_8bit(x, self.w1.weight, self.w3.weight, self.w2.weight, *(mask or ()))
         if mask is not None:
             return linear(gated_linear(x, self.w1.weight, self.w3.weight, *mask), self.w2.weight)
         return linear(_drop(self.dropout, gated_linear(x, self.w1.weight, self.w3.weight)), self.w2.weight)
@@ -176,26 +192,37 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
     two), so a block receives the residual stream together with the branch output that has not been
     added yet (`pending`: the previous block's feed-forward output, None for the first block) and hands
     its own feed-forward output on in the same way; the model's final norm absorbs the last one.  With
-    `counter_dropout` the output is handed on undropped, as (output, p, seed), and dropped where it is added.
+    `counter_dropout` the output is handed on undropped, as (output, p, seed), and dropped where it is added; with `branch_norm` it is
+    handed on with the norm behind it, as (output, p, seed, norm, gate).
     Same values, same parameter names."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
         self.self_attn = MultiHeadAttention(config)
         counter = _option(config, 'counter_dropout')
-        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout, counter)
+        self.ff = FeedForward(config.d_model, config.d_ff, config.dropout, counter, _option(config, 'activations_8bit'))
         self.norm1 = FusedRMSNorm(config.d_model)
         self.norm2 = FusedRMSNorm(config.d_model)
         self.dropout = _make_dropout(config.dropout, counter)
+        gated, scale = _option(config, 'branch_gate'), getattr(config, 'branch_scale', None)
+        if not _option(config, 'branch_norm') and (gated or scale is not None):
+            raise ValueError('branch_gate and branch_scale belong to a branch_norm')
+        self.attn_post, self.ff_post = (BranchNorm(config.d_model, gated, scale) if _option(config, 'branch_norm') else None for _ in range(2))
 
-    def forward(self, x, pending=None, cos=None, sin=None, shape=None):
+    def forward(self, x, pending=None, cos=None, sin=None, shape=None, rotary=None):
         if pending is None:
             h = self.norm1(x)
         else:
             x, h = self.norm1.add_forward(x, *_branch(pending))       # train.py:1993 of the previous block + 1988
-        x, h = self.norm2.add_forward(x, self.self_attn(h, cos=cos, sin=sin, shape=shape))   # train.py:1989 + 1991
+        a = self.self_attn(h, cos=cos, sin=sin, shape=shape, rotary=rotary)
+        if self.attn_post is not None:
+            x, h = self.norm2.add_forward(x, a, post=self.attn_post, gate=self.attn_post.gate_of(h))
+        else:
+            x, h = self.norm2.add_forward(x, a)                       # train.py:1989 + 1991
         out = self.ff(h)                                              # added by whoever normalises next
         mask = _mask_of(self.dropout)
+        if self.ff_post is not None:
+            return x, (out if mask is not None else _drop(self.dropout, out), *(mask or (0.0, 0)), self.ff_post, self.ff_post.gate_of(h))
         return x, (out, *mask) if mask is not None else _drop(self.dropout, out)
 
 
@@ -212,7 +239,12 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
         self.config = config
         self.embedding = nn.Embedding(config.vocab_size, config.d_model)
         self.use_gradient_checkpointing = config.use_gradient_checkpointing
-        if config.use_rope:
+        self.rotary = None
+        if _option(config, 'rotary'):
+            self.rotary = Rotary(**{'rotary_dim': 64, **config.rotary})
+            if self.rotary.rotary_dim > 64:
+                raise ValueError('heads have 64 columns: rotary_dim goes up to that')
+        elif config.use_rope:
             self.rope = RotaryPositionalEmbedding(config.d_model, config.max_seq_len)
         self.layers = nn.ModuleList([DecoderOnlyBlock(config) for _ in range(config.n_layers)])
         self.norm = FusedRMSNorm(config.d_model)
@@ -239,14 +271,14 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
                 flat_ids = torch.cat([flat_ids, flat_ids.new_zeros(Tp - T)])
         x = self.embedding(flat_ids)
         cos = sin = None
-        if self.config.use_rope:
+        if self.rotary is None and self.config.use_rope:
             cos, sin = _tables_2d(*self.rope(L), self.layers[0].self_attn.head_dim if len(self.layers) else 64)
         pending = None
         for layer in self.layers:
             if self.use_gradient_checkpointing and self.training:
-                x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), use_reentrant=False)
+                x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), self.rotary, use_reentrant=False)
             else:
-                x, pending = layer(x, pending, cos=cos, sin=sin, shape=(n, L))
+                x, pending = layer(x, pending, cos=cos, sin=sin, shape=(n, L), rotary=self.rotary)
         x = self.norm(x) if pending is None else self.norm.add_forward(x, *_branch(pending))[1]
         return x, T
 

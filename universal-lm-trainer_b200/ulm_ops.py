@@ -55,10 +55,13 @@ class FusedRMSNorm(nn.Module):
     def forward(self, x):
         return rms_norm(x, self.weight, self.eps)
 
-    def add_forward(self, x, branch, dropout_p=0.0, seed=0):
+    def add_forward(self, x, branch, dropout_p=0.0, seed=0, post=None, gate=None):
         """(x + branch, norm(x + branch)); the fused kernel when the tensors have the training layout
         (fp32 residual stream, 16-bit branch, d <= 1024), the two separate ops otherwise.  With ``dropout_p`` the branch
-        is dropped first, in the fused kernel (d <= 8192) or by `dropout`."""
+        is dropped first, in the fused kernel (d <= 8192) or by `dropout`.  With ``post`` (`BranchNorm`) it is then normalised, multiplied by the
+        sigmoid of ``gate`` and by post's scale before it is added: `norm_add_norm` in the training layout (d <= 8192), its separate ops otherwise."""
+        if post is not None:
+            return self._post_add(x, dropout(branch, dropout_p, seed) if dropout_p else branch, post, gate)
         d = x.shape[-1]
         if (x.is_cuda and x.dtype == torch.float32 and branch.dtype in _16BIT and d <= (8192 if dropout_p else 1024)
                 and d % 4 == 0 and torch.is_autocast_enabled('cuda')
@@ -68,6 +71,33 @@ class FusedRMSNorm(nn.Module):
             return add_rms_norm(x, branch, self.weight, self.eps)
         x = x + (dropout(branch, dropout_p, seed) if dropout_p else branch)
         return x, rms_norm(x, self.weight, self.eps)
+
+    def _post_add(self, x, branch, post, gate):
+        d = x.shape[-1]
+        if (x.is_cuda and x.dtype == torch.float32 and branch.dtype in _16BIT and d <= 8192 and d % 4 == 0 and self.eps == post.eps
+                and torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == branch.dtype and (gate is None or gate.dtype == branch.dtype)):
+            return norm_add_norm(x, branch, post.weight, self.weight, gate=gate, scale=post.scale, eps=self.eps)
+        branch = rms_norm(branch, post.weight, post.eps).to(x.dtype)
+        if gate is not None:
+            branch = branch * torch.sigmoid(gate.to(x.dtype))
+        x = x + (branch if post.scale is None else branch * post.scale.to(x.dtype))
+        return x, rms_norm(x, self.weight, self.eps)
+
+
+class BranchNorm(nn.Module):
+    """What stands behind a block's branch before it is added: a norm's ``weight``, with ``gated`` the projection ``gate`` of the branch's input whose sigmoid
+    multiplies it, and a learned ``scale`` that starts at the number given (None: there is none; 0: the branch is off at the start)."""
+
+    def __init__(self, d_model: int, gated=False, scale=None, eps: float = 1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d_model))
+        self.gate = nn.Linear(d_model, d_model, bias=False) if gated else None
+        self.scale = None if scale is None else nn.Parameter(torch.tensor(float(scale)))
+        self.eps = eps
+
+    def gate_of(self, x):
+        """The gate before its sigmoid, of the branch's input."""
+        return None if self.gate is None else linear(x, self.gate.weight)
 
 
 def swiglu(a, b):
