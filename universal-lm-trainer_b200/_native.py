@@ -24,7 +24,7 @@ _CSRC = os.path.join(_HERE, 'csrc')
 _LIB_PATH = os.path.join(_HERE, 'libulm_b200.so')
 _SOURCES = ['attn_bwd.cu', 'attn_fwd.cu', 'lmhead.cu', 'lib.cu', 'tc_host.cu', 'rope.cu', 'rmsnorm.cu', 'ce.cu', 'swiglu.cu',
             'grad_post.cu', 'selftest.cu', 'dropout.cu', 'dropout_norm.cu', 'streamed_ce.cu', 'norm_add_norm.cu', 'rotary.cu', 'pack8.cu']          # slowest first: they are compiled in parallel
-_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'norm_rows.cuh', 'pack8.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
+_HEADERS = ['common.cuh', 'tc.cuh', 'rope_math.cuh', 'gate_math.cuh', 'philox.cuh', 'col_sum.cuh', 'norm_rows.cuh', 'pairs.cuh', 'pack8.cuh', 'lmhead_tiles.cuh', os.path.join('..', '..', 'include', 'ulm_b200.h')]
 
 _EXT_PATH = os.path.join(_HERE, '_ulm_torch.so')
 _EXT_SOURCE = 'torch_ops.cpp'

@@ -17,30 +17,12 @@
 
 #include "common.cuh"
 #include "norm_rows.cuh"
+#include "pairs.cuh"
 
 namespace ulm {
 namespace {
 
 constexpr int kMaxRow = 8192;
-
-// Two fp32 values at a time: half the instructions of the multiply-add pipe, which had 37 of the backward's 82 an element.
-__device__ __forceinline__ uint64_t bits(const float2& v) { return reinterpret_cast<const uint64_t&>(v); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
-  return reinterpret_cast<float2&>(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
-  return reinterpret_cast<float2&>(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return reinterpret_cast<float2&>(r);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The sigmoid as its smaller side s = sig(-|g|) with the sign of g: sig(g) is s or 1 - s, its slope s (1 - s) without a difference that cancels.
 // 2^x and the reciprocal are the special-function unit's, within 2^-22 and 2^-23; with the exponent's rounding s is within 2^-21 + |g| 2^-24 of
