@@ -323,3 +323,28 @@ def test_refusals(bad):
     if bad == 'x on the host': x = x.cpu()
     with pytest.raises(ValueError):
         ulm_ops.norm_add_norm(x, b, v, w, gate=gate, scale=scale)
+
+
+@pytest.mark.parametrize('gated', [False, True])
+@pytest.mark.parametrize('scale', [None, 0.5])
+@pytest.mark.parametrize('autocast', [False, True])
+def test_the_module_in_and_out_of_the_training_layout(gated, scale, autocast):
+    """`FusedRMSNorm.add_forward` behind a `BranchNorm`: the fused op under autocast, its separate ops for fp32 branches."""
+    norm, post = ulm_ops.FusedRMSNorm(64).cuda(), ulm_ops.BranchNorm(64, gated, scale).cuda()
+    for p in (*norm.parameters(), *post.parameters()):
+        p.data.add_(randn(p.shape, F32, p.numel(), 0.1))
+    x, h = randn((2, 5, 64), F32, 1, 2.0), randn((2, 5, 64), F32, 2)
+    with torch.autocast('cuda', dtype=BF16, enabled=autocast):
+        b = randn((2, 5, 64), BF16 if autocast else F32, 3).requires_grad_()
+        gate = post.gate_of(h)
+        x_new, y = norm.add_forward(x, b, post=post, gate=gate)
+    s = dict(x=x, b=b.detach(), v=post.weight.detach(), w=norm.weight.detach())
+    if gated:
+        s['gate'] = gate.detach()
+    if scale is not None:
+        s['scale'] = post.scale.detach()
+    f = forward64(s, 1e-6)
+    within(x_new, f['x_new'], 2.0 ** -18 * (x.double().abs() + f['term'].abs()))
+    within(y, f['y'], (UNIT[b.dtype] if autocast else 0) * f['y'].abs() + 2.0 ** -16 * (1 + f['y'].abs()))
+    params = [*norm.parameters(), *post.parameters(), b]
+    assert all(torch.isfinite(g).all() and g.any() for g in torch.autograd.grad(x_new.sum() + (y.float() ** 2).sum(), params))

@@ -254,3 +254,33 @@ def test_refusals(bad):
     if bad == 'k on the host': k = k.cpu()
     with pytest.raises(ValueError):
         ulm_ops.rotary(q, k, turns, at)
+
+
+def test_negative_positions_of_32_bits_and_both_forms_agree():
+    x = laid_out(2, 3, 5, 64, F32, 3, 'B,S,H,D')
+    at = torch.tensor([[-3, -1, 0, 1, -(1 << 31)], [(1 << 31) - 1, 7, -7, 5, 2]], dtype=torch.int32)
+    case(x, x, ulm_ops.rotary_turns(64)[0], at.cuda(), at.numpy())
+    turns = ulm_ops.rotary_turns(64)[0].cuda()
+    assert torch.equal(ulm_ops.rotary(x, None, turns, at.cuda())[0], ulm_ops.rotary(x, None, turns, at.long().cuda())[0])
+
+
+@pytest.mark.parametrize('D,R', [(64, 64), (80, 20), (65, 62), (9, 4)])
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_in_place_through_the_library(D, R, interleaved):
+    """Outputs may be the inputs; what passes through is then left alone."""
+    import ctypes as C
+
+    import _native as N
+    x = randn((2, 7, 3, D), BF16, 1)
+    turns = ulm_ops.rotary_turns(R)[0].cuda()
+    want, _ = ulm_ops.rotary(x.transpose(1, 2), None, turns, None, interleaved)
+    a = N.RotaryArgs()
+    a.q = a.qo = x.data_ptr()
+    a.turns = turns.data_ptr()
+    a.q_sb = a.qo_sb = 21 * D
+    a.q_ss = a.qo_ss = 3 * D
+    a.q_sh = a.qo_sh = D
+    a.B, a.Hq, a.Hk, a.S, a.D, a.R, a.dtype, a.interleaved, a.factor = 2, 3, 0, 7, D, R, N.ULM_BF16, int(interleaved), 1.0
+    a.stream = torch.cuda.current_stream().cuda_stream
+    N.check(N.lib().ulm_rotary(C.byref(a)), 'rotary')
+    assert torch.equal(x.transpose(1, 2), want)

@@ -190,12 +190,15 @@ norm_add_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
   }
 }
 
+// Asks for a row that will be wanted soon, into L2; `from` on 16 bytes, their number a multiple of 16.
+__device__ __forceinline__ void fetch_to_l2(const void* from, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory"); }
+
 struct BwdParams {
   const float* z; const void* branch; const void* gate; const float* v; const float* w; Scale scale;
   const void* dy; const float* gz; const float* rstd1; const float* rstd2;
   float* dx; void* db; void* dg; float* partial;
   int64_t z_stride, branch_stride, gate_stride, dy_stride, gz_stride, dx_stride, db_stride, dg_stride, rows;
-  int d, L;
+  int d, L, ahead;                                       // ahead: whether the next row is asked for
 };
 
 // Three sums over the L lanes of a row, one barrier where they are more than a warp.  Every exchange between lanes halves the number of sums
@@ -244,7 +247,7 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
   const int L = p.L, group = threadIdx.x / L, groups = blockDim.x / L, nvec = p.d / E, first = threadIdx.x - group * L, hop = L;
   const float inv_d = 1.f / (float)p.d, whole = whole_scale(p.scale);
   // a lane has the same columns of every row: their weights stay in registers where there are few
-  constexpr bool kHold = NV * E <= 16;
+  constexpr bool kHold = NV * E <= 16, kKeepGate = GATE && NV * E <= 16;      // as do the gate's values of a row, formed twice otherwise
   float2 wv[kHold ? NV : 1][E / 2], tv[kHold ? NV : 1][E / 2], acc_w[NV][E / 2], acc_c[NV][E / 2];
   float acc_s = 0.f;
 #pragma unroll
@@ -258,7 +261,7 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
   }
   int phase = 0;
   for (int64_t r = (int64_t)blockIdx.x * groups + group; r < p.rows; r += (int64_t)gridDim.x * groups, phase ^= 1) {
-    float2 z[NV][E / 2], gz[NV][E / 2], shuts[GATE ? NV : 1][E / 2];
+    float2 z[NV][E / 2], gz[NV][E / 2], shuts[kKeepGate ? NV : 1][E / 2];
     Raw<E> b[NV], q[NV], g[GATE ? NV : 1];
 #pragma unroll
     for (int it = 0; it < NV; ++it) {                    // the whole row is requested before any of it is used
@@ -276,11 +279,21 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
         }
       }
     }
+    if (E == 8 && p.ahead && first == 0) {               // the group's next row is on its way to L2 while this one is worked on
+      const int64_t next = r + (int64_t)gridDim.x * groups;
+      if (next < p.rows) {
+        fetch_to_l2(p.z + next * p.z_stride, 4 * p.d);
+        fetch_to_l2(dy + next * p.dy_stride, 2 * p.d);
+        fetch_to_l2(br + next * p.branch_stride, 2 * p.d);
+        if (p.gz) fetch_to_l2(p.gz + next * p.gz_stride, 4 * p.d);
+        if constexpr (GATE) fetch_to_l2(gt + next * p.gate_stride, 2 * p.d);
+      }
+    }
     const float r1 = p.rstd1[r], r2 = p.rstd2[r];
     float2 gh2 = both(0.f), pt2 = gh2, ht2 = gh2;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      const int vi = first + it * hop, at = kHold ? it : 0;
+      const int vi = first + it * hop, at = kHold ? it : 0, keep = kKeepGate ? it : 0;
       if (vi < nvec) {
         float2 G[E / 2], u[E / 2];
         if constexpr (!kHold) {
@@ -290,14 +303,14 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
         unpack_row<TY, E>(q[it], G);
         unpack_row<TY, E>(b[it], u);
         if constexpr (GATE) {
-          unpack_row<TY, E>(g[it], shuts[it]);
+          unpack_row<TY, E>(g[it], shuts[keep]);
 #pragma unroll
-          for (int j = 0; j < E / 2; ++j) shuts[it][j] = shut(shuts[it][j]);
+          for (int j = 0; j < E / 2; ++j) shuts[keep][j] = shut(shuts[keep][j]);
         }
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
           z[it][j] = mul2(z[it][j], both(r2));           // h from here on
-          const float2 tu = mul2(GATE ? mul2(tv[at][j], opened(shuts[it][j])) : tv[at][j], mul2(u[j], both(r1))), a = mul2(G[j], z[it][j]);
+          const float2 tu = mul2(GATE ? mul2(tv[at][j], opened(shuts[keep][j])) : tv[at][j], mul2(u[j], both(r1))), a = mul2(G[j], z[it][j]);
           acc_w[it][j] = add2(acc_w[it][j], a);
           gh2 = fma2(a, wv[at][j], gh2);
           gz[it][j] = fma2(mul2(G[j], wv[at][j]), both(r2), gz[it][j]);      // p from here on
@@ -312,20 +325,25 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
     acc_s += nu;
 #pragma unroll
     for (int it = 0; it < NV; ++it) {
-      const int vi = first + it * hop, at = kHold ? it : 0;
+      const int vi = first + it * hop, at = kHold ? it : 0, keep = kKeepGate ? it : 0;
       if (vi < nvec) {
         float2 u[E / 2], o[E / 2];
         unpack_row<TY, E>(b[it], u);
         if constexpr (!kHold) load_tv<E>(p.v, p.scale, vi * E, tv[0]);
+        if constexpr (GATE && !kKeepGate) {
+          unpack_row<TY, E>(g[it], shuts[0]);
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j) shuts[0][j] = shut(shuts[0][j]);
+        }
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) gz[it][j] = fma2(both(-m), z[it][j], gz[it][j]);      // dz from here on
         store_row<E>(p.dx + r * p.dx_stride + vi * E, gz[it]);
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
-          const float2 ds = GATE ? mul2(gz[it][j], opened(shuts[it][j])) : gz[it][j];
+          const float2 ds = GATE ? mul2(gz[it][j], opened(shuts[keep][j])) : gz[it][j];
           acc_c[it][j] = fma2(ds, mul2(u[j], both(r1)), acc_c[it][j]);
           o[j] = fma2(mul2(ds, both(rs)), tv[at][j], mul2(u[j], both(-k)));
-          if constexpr (GATE) gz[it][j] = mul2(mul2(gz[it][j], slope(shuts[it][j])), mul2(mul2(u[j], both(rs)), tv[at][j]));
+          if constexpr (GATE) gz[it][j] = mul2(mul2(gz[it][j], slope(shuts[keep][j])), mul2(mul2(u[j], both(rs)), tv[at][j]));
         }
         store_row16<TY, E>(db + r * p.db_stride + vi * E, o);
         if constexpr (GATE) store_row16<TY, E>(dg + r * p.dg_stride + vi * E, gz[it]);
@@ -370,8 +388,10 @@ norm_add_norm_finish_kernel(const float* partial, const float* v, const Scale sc
   grid_dependency_wait();
   const int c = blockIdx.x * 32 + threadIdx.x, width = 2 * d + 1;
   float t = 0.f;
-  if (c < width)
+  if (c < width) {
+#pragma unroll 5
     for (int p = threadIdx.y; p < nparts; p += 32) t += partial[(int64_t)p * width + c];
+  }
   sub[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
   if (threadIdx.y != 0 || c >= width) return;
@@ -404,12 +424,17 @@ template <int E_, int NV_, int WARPS_, int CTAS_, int ROWS> struct Form {
 };
 template <typename...> struct Forms {};
 // The first form whose columns suffice.  us at us of the bytes alone (bf16, without a gate, then with one):
-//   forward   32768 x 768 47.2 (46.1), x 1024 63.1 (61.4), 16396 x 4096 125 (123); 48044 x 1024 105 (105), 16396 x 4096 145 (144).  One warp a row up to
+//   forward   32768 x 768 47 (46), x 1024 63 (61), 16396 x 4096 125 (123); 48044 x 1024 105 (105), 16396 x 4096 146 (144).  One warp a row up to
 //             1024 columns: with eight columns a lane, and so three warps and two barriers for 768, 32768 x 768 took 65
-//   backward  32768 x 768 78 (69), x 1024 102 (92), 16396 x 4096 208 (184); 48044 x 1024 181 (165), 16396 x 4096 300 (225).  Eight columns a lane and
+//   backward  32768 x 768 76 (69), x 1024 99 (92), 16396 x 4096 196 (184); 48044 x 1024 169 (165), 16396 x 4096 252 (225).  Eight columns a lane and
 //             24 warps an SM without a gate up to 1024 (sixteen a lane: 87 at 768); the gate's values do not fit the 80 registers of that,
-//             and with sixteen a lane 48044 x 1024 went from 204 to 181.  Thirty-two from where two rows no longer fit a CTA: 16396 x 4096
-//             with a gate 340 -> 300.  There one or two rows are on an SM's way through load, sums, barrier and stores at a time, which is what bounds it
+//             and with sixteen a lane 48044 x 1024 went from 204 to 181.  Thirty-two from where two rows no longer fit a CTA, the gate formed at both uses:
+//             16396 x 4096 with a gate 340 -> 281.  A group then waits for a row, meets at a barrier and stores before it loads the
+//             next, and few rows are on an SM at a time: the next row asked for into L2 meanwhile took 48044 x 1024 from 181 to 169,
+//             16396 x 4096 with a gate from 281 to 252, 5000 x 2816 from 55 to 48; rows of 128 and 256 columns, of which many are under
+//             way, from 18.5 to 20.6 (so from kAheadFrom on only: 512 with a gate 38.9 -> 38.0).  Copies of the row itself, by cp.async into shared memory
+//             a row ahead, cost more load and store instructions than the wait they saved: 32768 x 768 98, 4099 x 4096 with a gate 94
+constexpr int kAheadFrom = 512;
 using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 1>>;
 using Bwd8 = Forms<Form<8, 1, 12, 2, 3>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
 using Bwd8Gate = Forms<Form<8, 1, 20, 1, 6>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
@@ -449,6 +474,7 @@ int launch_bwd(Forms<F, Rest...>, BwdParams p, int64_t* parts, cudaStream_t st, 
     if (p.d > F::kMost) return launch_bwd<TY, GATE>(Forms<Rest...>(), p, parts, st, who);
   const Deal s = deal<F>(p.rows, p.d);
   p.L = s.L;
+  p.ahead = p.d >= kAheadFrom;
   const size_t smem = (size_t)s.groups * p.d * sizeof(float);       // a warp has E NV 32 columns at most
   static_assert(F::CTAS <= kMostCtas && (F::E * F::NV * F::WARPS * 32 + 8 * F::WARPS) * sizeof(float) <= 48 * 1024, "partial rows; shared memory without an opt-in");
   auto kern = norm_add_norm_bwd_kernel<TY, F::E, F::NV, F::WARPS, F::CTAS, GATE>;

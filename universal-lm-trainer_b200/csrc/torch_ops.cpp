@@ -872,22 +872,21 @@ struct NormAddNormBwd : OpNode {
     const Tensor dy = g[1].defined() ? rows_on(as_type(g[1], bdtype), 8) : at::zeros({rows, d}, x.options().dtype(bdtype));
     const Tensor ga = g[0].defined() ? rows_on(as_type(g[0], at::kFloat), 16) : Tensor();
     const Tensor dx = empty_cuda(x.sizes(), at::kFloat, x), db = empty_cuda(x.sizes(), bdtype, x), dg = has_gate ? empty_cuda(x.sizes(), bdtype, x) : Tensor();
-    // dw, dv, dscale, then the CTAs' partial rows
-    const int64_t n_scale = !has_scale ? 0 : channels ? d : 4;
-    const Tensor sums = empty_cuda({2 * d + n_scale}, at::kFloat, x), partial = empty_cuda({ulm_norm_add_norm_partial(rows, (int32_t)d)}, at::kFloat, x);
+    const Tensor dw = empty_cuda({d}, at::kFloat, x), dv = empty_cuda({d}, at::kFloat, x), ds = has_scale ? empty_cuda(scale_shape, at::kFloat, x) : Tensor();
+    const Tensor partial = empty_cuda({ulm_norm_add_norm_partial(rows, (int32_t)d)}, at::kFloat, x);
     ulm_norm_add_norm_bwd_args a{};
     a.x = x.data_ptr<float>(); a.branch = b.data_ptr(); a.gate = has_gate ? gate.data_ptr() : nullptr;
     a.v = v.data_ptr<float>(); a.w = w.data_ptr<float>(); a.scale = has_scale ? scale.data_ptr<float>() : nullptr;
     a.dy = dy.data_ptr(); a.g_add = ga.defined() ? ga.data_ptr<float>() : nullptr; a.rstd_branch = rstd1.data_ptr<float>(); a.rstd = rstd2.data_ptr<float>();
     a.dx = dx.data_ptr<float>(); a.d_branch = db.data_ptr(); a.d_gate = has_gate ? dg.data_ptr() : nullptr;
-    a.dw = sums.data_ptr<float>(); a.dv = a.dw + d; a.dscale = has_scale ? a.dv + d : nullptr; a.partial = partial.data_ptr<float>();
+    a.dw = dw.data_ptr<float>(); a.dv = dv.data_ptr<float>(); a.dscale = has_scale ? ds.data_ptr<float>() : nullptr; a.partial = partial.data_ptr<float>();
     a.x_stride = a.dx_stride = a.dbranch_stride = a.dgate_stride = d;
     a.branch_stride = b.stride(0); a.gate_stride = has_gate ? gate.stride(0) : d; a.dy_stride = dy.stride(0); a.gadd_stride = ga.defined() ? ga.stride(0) : d;
     a.rows = rows; a.d = (int32_t)d; a.dtype = code_of(bdtype); a.scale_channels = channels; a.scale_value = (float)scale_value; a.stream = stream_of(x);
     check(ulm_norm_add_norm_bwd(&a), "norm_add_norm backward");
-    variable_list r{dx, db, as_type(sums.narrow(0, d, d), vdtype), as_type(sums.narrow(0, 0, d), wdtype)};
+    variable_list r{dx, db, as_type(dv, vdtype), as_type(dw, wdtype)};
     if (has_gate) r.push_back(dg);
-    if (has_scale) r.push_back(as_type(sums.narrow(0, 2 * d, channels ? d : 1), sdtype).view(scale_shape));
+    if (has_scale) r.push_back(as_type(ds, sdtype));
     return r;
   }
   variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "norm_add_norm"); }
@@ -1499,9 +1498,9 @@ std::tuple<Tensor, Tensor> pack_8bit(const Tensor& x) {
   TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()), "pack_8bit needs a CUDA fp16/bf16/fp32 tensor");
   OpScope scope;
   c10::cuda::CUDAGuard dev(x.device());
-  const Packed8 p = pack8(x.detach());
-  const int64_t at = Packed8::codes_bytes(p.n);
-  return {p.buffer.narrow(0, 0, p.n).view(at::kChar).view(x.sizes()), p.buffer.narrow(0, at, p.buffer.numel() - at)};
+  const Tensor d = dense16(x), codes = empty_cuda(x.sizes(), at::kChar, x), exps = empty_cuda({ulm_pack8_blocks(x.numel())}, at::kByte, x);
+  check(ulm_pack8(d.data_ptr(), static_cast<int8_t*>(codes.data_ptr()), static_cast<uint8_t*>(exps.data_ptr()), d.numel(), code_of(d.scalar_type()), stream_of(d)), "pack_8bit");
+  return {codes, exps};
 }
 Tensor unpack_8bit(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType dtype) {
   TORCH_CHECK_VALUE(codes_in.is_cuda() && codes_in.scalar_type() == at::kChar && known(dtype), "unpack_8bit needs CUDA int8 codes and a result of fp16, bf16 or fp32");
