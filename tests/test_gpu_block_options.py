@@ -134,6 +134,7 @@ def test_state_dicts_go_round_and_the_options_add_what_they_say():
     assert keys['plain'] - keys['rotary'] == {'rope.inv_freq', 'rope.cos_cached', 'rope.sin_cached'} and not keys['rotary'] - keys['plain']
     assert keys['norms'] - keys['plain'] == {f'layers.0.{n}.weight' for n in ('attn_post', 'ff_post')}
     assert keys['norms, gate and scale'] - keys['norms'] == {f'layers.0.{n}.{k}' for n in ('attn_post', 'ff_post') for k in ('gate.weight', 'scale')}
+    assert ulm_train.build('tiny64', 'cpu', rotary={})[0].rotary.rotary_dim == 64 and ulm_train.build('tiny64', 'cpu')[0].rotary is None
     a, b = tiny(1, **OPTIONS['all']), tiny(2, **OPTIONS['all'])
     b.load_state_dict(a.state_dict(), strict=True)
     with torch.autocast('cuda', dtype=BF16):

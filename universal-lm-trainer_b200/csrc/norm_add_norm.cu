@@ -425,7 +425,8 @@ template <int E_, int NV_, int WARPS_, int CTAS_, int ROWS> struct Form {
 template <typename...> struct Forms {};
 // The first form whose columns suffice.  us at us of the bytes alone (bf16, without a gate, then with one):
 //   forward   32768 x 768 47 (46), x 1024 63 (61), 16396 x 4096 125 (123); 48044 x 1024 105 (105), 16396 x 4096 146 (144).  One warp a row up to
-//             1024 columns: with eight columns a lane, and so three warps and two barriers for 768, 32768 x 768 took 65
+//             1024 columns: with eight columns a lane, and so three warps and two barriers for 768, 32768 x 768 took 65.  Nine warps where a row takes
+//             three: 8192 x 2560 53 -> 45, 5000 x 2816 36 -> 32
 //   backward  32768 x 768 76 (69), x 1024 99 (92), 16396 x 4096 196 (184); 48044 x 1024 169 (165), 16396 x 4096 252 (225).  Eight columns a lane and
 //             24 warps an SM without a gate up to 1024 (sixteen a lane: 87 at 768); the gate's values do not fit the 80 registers of that,
 //             and with sixteen a lane 48044 x 1024 went from 204 to 181.  Thirty-two from where two rows no longer fit a CTA, the gate formed at both uses:
@@ -435,7 +436,7 @@ template <typename...> struct Forms {};
 //             way, from 18.5 to 20.6 (so from kAheadFrom on only: 512 with a gate 38.9 -> 38.0).  Copies of the row itself, by cp.async into shared memory
 //             a row ahead, cost more load and store instructions than the wait they saved: 32768 x 768 98, 4099 x 4096 with a gate 94
 constexpr int kAheadFrom = 512;
-using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 1>>;
+using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 4>, Form<8, 4, 9, 2, 3>, Form<8, 4, 8, 2, 1>>;
 using Bwd8 = Forms<Form<8, 1, 12, 2, 3>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
 using Bwd8Gate = Forms<Form<8, 1, 20, 1, 6>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
 // widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only

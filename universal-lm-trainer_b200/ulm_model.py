@@ -240,7 +240,7 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
         self.embedding = nn.Embedding(config.vocab_size, config.d_model)
         self.use_gradient_checkpointing = config.use_gradient_checkpointing
         self.rotary = None
-        if _option(config, 'rotary'):
+        if getattr(config, 'rotary', None) is not None:
             self.rotary = Rotary(**{'rotary_dim': 64, **config.rotary})
             if self.rotary.rotary_dim > 64:
                 raise ValueError('heads have 64 columns: rotary_dim goes up to that')
