@@ -23,6 +23,7 @@ namespace ulm {
 namespace {
 
 constexpr int kMaxRow = 8192;
+constexpr int kMostCtas = 2;                             // on an SM, of all forms of the backward: each leaves one partial row
 
 // The sigmoid as its smaller side s = sig(-|g|) with the sign of g: sig(g) is s or 1 - s, its slope s (1 - s) without a difference that cancels.
 // 2^x and the reciprocal are the special-function unit's, within 2^-22 and 2^-23; with the exponent's rounding s is within 2^-21 + |g| 2^-24 of
@@ -387,10 +388,16 @@ norm_add_norm_finish_kernel(const float* partial, const float* v, const Scale sc
   __shared__ float sub[32][33];
   grid_dependency_wait();
   const int c = blockIdx.x * 32 + threadIdx.x, width = 2 * d + 1;
-  float t = 0.f;
+  constexpr int kParts = (kMostCtas * kNumSMs + 31) / 32;
+  float t = 0.f, part[kParts];                           // all requested before the first is added
   if (c < width) {
-#pragma unroll 5
-    for (int p = threadIdx.y; p < nparts; p += 32) t += partial[(int64_t)p * width + c];
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      const int row = threadIdx.y + 32 * k;
+      part[k] = row < nparts ? partial[(int64_t)row * width + c] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) t += part[k];
   }
   sub[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
@@ -456,7 +463,6 @@ template <typename F> Deal deal(int64_t rows, int d) {
   s.groups = s.threads / s.L;
   return s;
 }
-constexpr int kMostCtas = 2;                             // on an SM, of all forms of the backward
 
 template <typename TY, bool GATE, typename F, typename... Rest>
 int launch_fwd(Forms<F, Rest...>, FwdParams p, cudaStream_t st, const char* who) {
