@@ -291,3 +291,112 @@ def test_a_cached_context_is_continued():
     cache = torch.cat([rotary(q[:, :, s:e], k[:, :, s:e], torch.arange(s, e, device='cuda'))[1] for s, e in ((0, 20), (20, 40))], 2)
     new_q, new_k = rotary(q[:, :, 40:], k[:, :, 40:], torch.full((n, 1), 40, device='cuda'))
     assert torch.equal(torch.cat([cache, new_k], 2), whole_k) and torch.equal(new_q, whole_q[:, :, 40:])
+
+
+# ---------------------------------------------------------------------------
+# what a differentiable op owes its callers
+# ---------------------------------------------------------------------------
+class Traced(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.w, self.s = torch.nn.Parameter(torch.ones(64, device='cuda')), torch.nn.Parameter(torch.tensor(0.5, device='cuda'))
+        self.rotary = ulm_ops.Rotary(16, interleaved=True).cuda()
+
+    def forward(self, x):
+        q, k = self.rotary(x.view(1, -1, 2, 32).transpose(1, 2), x.view(1, -1, 2, 32).transpose(1, 2))
+        b = (q + k).transpose(1, 2).reshape(x.shape).half()
+        x_new, y = ulm_ops.norm_add_norm(x, b, self.w, self.w, gate=b, scale=self.s)
+        return x_new + ulm_ops.swiglu_8bit(y.float(), x_new)
+
+
+def test_traced_ops_run_again_on_other_inputs():
+    m, x = Traced(), randn((24, 64), torch.float32, 1)
+    got, want = torch.jit.trace(m, randn((24, 64), torch.float32, 2))(x), m(x)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got.sum(), list(m.parameters())), torch.autograd.grad(want.sum(), list(m.parameters()))):
+        assert float((a - b).norm()) <= 2.0 ** -10 * float(b.norm())       # 16-bit gradients rounded once more by the trace's casts
+
+
+OPS = {
+    'rotary': lambda x: ulm_ops.rotary(x.view(1, 1, 4, 64), None, ulm_ops.rotary_turns(64)[0].cuda())[0],
+    'norm_add_norm': lambda x: ulm_ops.norm_add_norm(x, torch.ones(4, 64, device='cuda').half(), torch.ones(64, device='cuda'), torch.ones(64, device='cuda'))[0],
+    'swiglu_8bit': lambda x: ulm_ops.swiglu_8bit(x, x),
+    'linear_8bit': lambda x: ulm_ops.linear_8bit(x, torch.ones(8, 64, device='cuda')),
+    'feed_forward_8bit': lambda x: ulm_ops.feed_forward_8bit(x, *(torch.ones(64, 64, device='cuda') for _ in range(3))),
+}
+
+
+@pytest.mark.parametrize('name', list(OPS))
+def test_transforms_without_a_rule_are_refused(name):
+    with pytest.raises((RuntimeError, NotImplementedError), match='autograd.Function'):
+        torch.func.grad(lambda x: OPS[name](x).sum())(torch.ones(4, 64, device='cuda'))
+
+
+@pytest.mark.parametrize('name', list(OPS))
+def test_without_a_graph_and_through_saved_tensor_hooks(name):
+    x = randn((4, 64), torch.float32, 1)
+    want = OPS[name](x)
+    with torch.inference_mode():
+        assert torch.equal(OPS[name](x), want)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        parked = OPS[name](a)
+    y = OPS[name](b)
+    assert torch.equal(y.detach(), want) and torch.equal(*(torch.autograd.grad(t.sum(), u)[0] for t, u in ((parked, a), (y, b))))
+    first, again = (torch.autograd.grad(OPS[name](b).sum(), b, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(first, again)
+
+
+def test_a_graph_runs_backward_twice():
+    x = randn((4, 64), torch.float32, 1).requires_grad_()
+    for f in OPS.values():
+        y = f(x)
+        assert torch.equal(*(torch.autograd.grad(y.sum(), x, retain_graph=True)[0] for _ in range(2)))
+
+
+def test_two_threads_at_once():
+    import threading
+    model, ids, out = tiny(**OPTIONS['all']), ids_of(), {}
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()), torch.autocast('cuda', dtype=BF16):
+            for _ in range(3):
+                loss = model.compute_loss(ids)
+                out[i] = (loss.detach(), torch.autograd.grad(loss, list(model.parameters())))
+            torch.cuda.current_stream().synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert torch.equal(out[0][0], out[1][0]) and all(torch.equal(a, b) for a, b in zip(out[0][1], out[1][1]))
+
+
+def test_a_whole_step_replays():
+    """Forward and backward of a block's ops captured once, replayed on other values."""
+    rotary, w = ulm_ops.Rotary(64).cuda(), torch.ones(128, device='cuda')
+    qkv, x, up = randn((2, 33, 384), BF16, 1), randn((2, 33, 128), torch.float32, 2), randn((2, 33, 128), BF16, 3)
+    w1, w3, w2 = randn((96, 128), BF16, 4, 0.1), randn((96, 128), BF16, 5, 0.1), randn((128, 96), BF16, 6, 0.1)
+    leaves = [t.requires_grad_() for t in (qkv, x, w1, w3, w2)]
+
+    def step():
+        a = fa.qkv_rope_flash_attn(qkv, 2, rotary=rotary)
+        x_new, h = ulm_ops.norm_add_norm(x, a, w, w, gate=a, scale=0.5)
+        y = ulm_ops.feed_forward_8bit(h, w1, w3, w2)
+        return (x_new.detach(), y.detach(), *torch.autograd.grad([x_new, y], leaves, [x_new.detach(), up]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    with torch.no_grad():
+        qkv.mul_(-1.5), x.add_(1), w1.mul_(2)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, step()):
+        assert float((a - b).float().norm()) <= 2.0 ** -7 * float(b.float().norm())       # library products may be summed in another order

@@ -111,6 +111,15 @@ def test_another_type_and_codes_of_any_layout():
             ulm_ops.unpack_8bit(bad)
 
 
+def test_every_exponent_and_code():
+    """Also those that no tensor packed here has."""
+    codes = torch.arange(-128, 128, dtype=torch.int16).to(torch.int8).repeat(256).cuda()
+    exps = torch.arange(256, dtype=torch.int16).to(torch.uint8).repeat_interleave(8).cuda()
+    back = ulm_ops.unpack_8bit(ulm_ops.Packed8(codes, exps, F32))
+    want = torch.from_numpy(op.unpack(codes.cpu().numpy(), exps.cpu().numpy())).float().cuda()
+    assert same(back, want)
+
+
 def test_past_32_bit_offsets():
     n = (1 << 32) + 77
     x = torch.empty(n, dtype=F16, device='cuda')

@@ -47,7 +47,8 @@ __device__ __forceinline__ uint32_t exponent_byte(uint32_t magnitude) {
   return e < 7u ? 7u : e;                                // 255 for infinities and NaN already
 }
 __device__ __forceinline__ float per_step(uint32_t byte) { return __uint_as_float(byte == 255u ? 0u : (260u - byte) << 23); }            // 2^(6 - e)
-__device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : (byte - 6u) << 23); }     // 2^(e - 6)
+// 2^(e - 6); bytes below 7 do not come from a tensor packed here, and their steps are subnormal
+__device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte > 6u ? (byte - 6u) << 23 : 1u << (byte + 16u)); }
 
 // whether a block's largest rounds to 128, which 127 holds: an element of it may have to be held
 __device__ __forceinline__ bool rounds_past(uint32_t magnitude) { return (magnitude & 0x7fffffu) >= 0x7f0000u; }

@@ -77,7 +77,7 @@ class FusedRMSNorm(nn.Module):
         if (x.is_cuda and x.dtype == torch.float32 and branch.dtype in _16BIT and d <= 8192 and d % 4 == 0 and self.eps == post.eps
                 and torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == branch.dtype and (gate is None or gate.dtype == branch.dtype)):
             return norm_add_norm(x, branch, post.weight, self.weight, gate=gate, scale=post.scale, eps=self.eps)
-        branch = rms_norm(branch, post.weight, post.eps).to(x.dtype)
+        branch = rms_norm(branch, post.weight, post.eps, branch.dtype).to(x.dtype)
         if gate is not None:
             branch = branch * torch.sigmoid(gate.to(x.dtype))
         x = x + (branch if post.scale is None else branch * post.scale.to(x.dtype))
