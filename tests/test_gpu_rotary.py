@@ -57,7 +57,8 @@ def case(q, k, turns, positions=None, at=None, interleaved=False, factor=1.0):
 
 @pytest.mark.parametrize('interleaved', [False, True])
 @pytest.mark.parametrize('dtype', [F16, BF16, F32])
-@pytest.mark.parametrize('D,R', [(2, 2), (6, 2), (6, 6), (10, 4), (20, 20), (64, 64), (64, 32), (64, 2), (65, 64), (80, 20), (80, 80), (96, 48), (128, 64), (128, 128), (256, 256), (256, 6)])
+@pytest.mark.parametrize('D,R', [(2, 2), (6, 2), (6, 6), (10, 4), (20, 20), (64, 64), (64, 32), (64, 2), (65, 64), (80, 20), (80, 80), (96, 48), (128, 64), (128, 128), (256, 256), (256, 6), (96, 2), (96, 50), (128, 66), (64, 34),
+                                 (256, 210), (512, 130), (4096, 2), (24, 10)])
 def test_widths(D, R, dtype, interleaved):
     q, k = laid_out(2, 5, 7, D, dtype, D, 'B,S,H,D'), laid_out(2, 3, 7, D, dtype, R + 1, 'B,S,H,D')
     case(q, k, ulm_ops.rotary_turns(R)[0], interleaved=interleaved)
@@ -68,6 +69,15 @@ def test_widths(D, R, dtype, interleaved):
 def test_head_counts_and_lengths(B, Hq, Hk, S, interleaved):
     dtype = BF16 if S % 2 else F16
     case(laid_out(B, Hq, S, 64, dtype, S, 'part of a projection'), laid_out(B, Hk, S, 64, dtype, S + 1, 'part of a projection'), ulm_ops.rotary_turns(64)[0], interleaved=interleaved)
+
+
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('D,R', [(96, 50), (256, 2), (16, 6), (512, 66)])
+@pytest.mark.parametrize('B,Hq,Hk,S', [(1, 1, 1, 1), (2, 7, 2, 17), (5, 4, 3, 16), (3, 2, 1, 129), (1, 6, 5, 700)])
+def test_rows_of_columns_that_turn_in_no_whole_vectors(D, R, B, Hq, Hk, S, interleaved):
+    dtype = (F16, BF16, F32)[(S + Hq) % 3]
+    at = torch.randint(-9999, 9999, (B, S), generator=torch.Generator().manual_seed(S))
+    case(laid_out(B, Hq, S, D, dtype, S, 'part of a projection'), laid_out(B, Hk, S, D, dtype, S + 1, 'B,H,S,D'), ulm_ops.rotary_turns(R)[0], at.cuda(), at.numpy(), interleaved, 1.25)
 
 
 @pytest.mark.parametrize('interleaved', [False, True])
@@ -264,7 +274,7 @@ def test_negative_positions_of_32_bits_and_both_forms_agree():
     assert torch.equal(ulm_ops.rotary(x, None, turns, at.cuda())[0], ulm_ops.rotary(x, None, turns, at.long().cuda())[0])
 
 
-@pytest.mark.parametrize('D,R', [(64, 64), (80, 20), (65, 62), (9, 4)])
+@pytest.mark.parametrize('D,R', [(64, 64), (80, 20), (65, 62), (9, 4), (96, 50), (64, 2)])
 @pytest.mark.parametrize('interleaved', [False, True])
 def test_in_place_through_the_library(D, R, interleaved):
     """Outputs may be the inputs; what passes through is then left alone."""

@@ -16,6 +16,8 @@ namespace ulm {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kMaxTile = 16, kTileBytes = 16384;         // positions and bytes of a CTA that works on whole rows (8 and 32 KB: no faster)
+constexpr int kRowsBelow = 4;                            // which it does where vectors of what turns have at most so many bytes
 constexpr unsigned kGroup = kThreads;                    // positions; a multiple of kThreads
 
 // V elements that lie on a multiple of A
@@ -30,8 +32,16 @@ struct RotaryParams {
   unsigned turning, passing, chunks;                     // units of a head that turn and that pass through; groups of heads of both tensors
   unsigned turn_tasks, per_group, count;                 // threads of a group of positions: for what turns, in all; positions
   int S, R, D, pos_32, pass_wide;                        // pass_wide: whole 16-byte vectors whatever V is
+  int tile;                                              // positions of a CTA that works on whole rows, or 0
   float factor, sign;                                    // sign: -1 backward
 };
+
+// negative positions wrap, as their product with a share of a turn does
+__device__ __forceinline__ uint64_t position_of(const RotaryParams& p, int b, int s) {
+  if (!p.positions) return (uint64_t)s;
+  const int64_t o = b * p.pos_sb + s * p.pos_ss;
+  return p.pos_32 ? (uint64_t)(int64_t)static_cast<const int32_t*>(p.positions)[o] : (uint64_t)static_cast<const int64_t*>(p.positions)[o];
+}
 
 // cos and sin of `share` / 2^64 turns, times f; the sine also times sign
 __device__ __forceinline__ void turn(uint64_t share, float f, float sign, float& c, float& s) {
@@ -106,11 +116,7 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
       lo[i] = *reinterpret_cast<const W*>(in + i * d.in_sh + col);
       if constexpr (!INTER) hi[i] = *reinterpret_cast<const W*>(in + i * d.in_sh + col + half);
     }
-  uint64_t position = (uint64_t)s;                       // negative positions wrap, as the product does
-  if (p.positions) {
-    const int64_t o = b * p.pos_sb + s * p.pos_ss;
-    position = p.pos_32 ? (uint64_t)(int64_t)static_cast<const int32_t*>(p.positions)[o] : (uint64_t)static_cast<const int64_t*>(p.positions)[o];
-  }
+  const uint64_t position = position_of(p, b, s);
   constexpr int kPairs = INTER ? V / 2 : V;
   float cs[kPairs], sn[kPairs];
 #pragma unroll
@@ -131,8 +137,81 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
     }
 }
 
+// Where what turns is made of vectors of 4 bytes at most (R / 2 is a multiple of little, or R for neighbours) though the rows are whole 16-byte
+// vectors: a CTA brings the rows of kHeads heads at p.tile positions into shared memory, turns them there element by element and stores
+// them by whole vectors again.  us with the widest vectors that fit / this way (the bytes alone), 4 x 16 heads x 4096 positions fp16: 128 columns, 66 turn,
+// halves 55 / 27 (20), 68 turn 32 / 27, 126 turn 49 / 36; 96 columns, 50 turn, halves 42 / 21 (15), neighbours 29 / 21; 13 x 4 heads x 10550 x 96, 2 turn,
+// neighbours 108 / 37 (32).  With vectors of 8 bytes the direct way is the faster: 72 of 128 turn 23 / 30, fp32 36 of 80 28 / 29.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(kThreads)
+rotary_rows_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int H = kHeads, N = 16 / sizeof(T);
+  extern __shared__ __align__(16) char mem[];            // [tile][H][D]
+  __shared__ int64_t from[kMaxTile], to[kMaxTile];       // where a position's heads lie, in elements
+  __shared__ uint64_t place[kMaxTile];
+  T* rows = reinterpret_cast<T*>(mem);
+  grid_dependents_go();
+  grid_dependency_wait();
+  const int chunk = (int)(blockIdx.x % p.chunks), tile = p.tile, tid = threadIdx.x;
+  const unsigned first = blockIdx.x / p.chunks * (unsigned)tile;
+  const bool second = chunk >= p.side[0].chunks;
+  const Side& d = p.side[second];
+  const int h0 = (second ? chunk - p.side[0].chunks : chunk) * H, nh = d.heads - h0 < H ? d.heads - h0 : H;
+  const int held = p.count - first < (unsigned)tile ? (int)(p.count - first) : tile;       // positions
+  if (tid < held) {
+    const unsigned at = first + (unsigned)tid;
+    const int b = (int)(at / (unsigned)p.S), s = (int)(at - (unsigned)b * (unsigned)p.S);
+    from[tid] = b * d.in_sb + s * d.in_ss + h0 * d.in_sh;
+    to[tid] = b * d.out_sb + s * d.out_ss + h0 * d.out_sh;
+    place[tid] = position_of(p, b, s);
+  }
+  __syncthreads();
+  // thread beside thread over the columns of the rows, counted on without divisions
+  auto over = [&](int per_row, int rows, auto&& use) {
+    const int hop_row = kThreads / per_row, hop = kThreads - hop_row * per_row;
+    int row = tid / per_row, i = tid - row * per_row;
+    while (row < rows) {
+      use(row, i);
+      row += hop_row; i += hop;
+      if (i >= per_row) { i -= per_row; ++row; }
+    }
+  };
+  const int inverse = 65536 / nh + 1;                    // row / nh is row * inverse / 65536: rows below kMaxTile H
+  over(p.D / N, held * nh, [&](int row, int v) {
+    const int at = row * inverse >> 16, h = row - at * nh;
+    const uint32_t to_smem = (uint32_t)__cvta_generic_to_shared(rows + (at * H + h) * p.D + v * N);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to_smem), "l"(static_cast<const T*>(d.in) + from[at] + h * d.in_sh + v * N) : "memory");
+  });
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  const int pairs = p.R >> 1, second_of = INTER ? 1 : pairs;
+  over(pairs, held, [&](int at, int pair) {
+    float c, sn;
+    turn(place[at] * p.turns[pair], p.factor, p.sign, c, sn);
+    T* row = rows + at * H * p.D + (INTER ? 2 * pair : pair);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (h < nh) {
+        T *a = row + h * p.D, *b = a + second_of;
+        const float xa = Cvt<T>::to_f(*a), xb = Cvt<T>::to_f(*b);
+        *a = Cvt<T>::from_f(fmaf(xa, c, -(xb * sn)));
+        *b = Cvt<T>::from_f(fmaf(xb, c, xa * sn));
+      }
+  });
+  __syncthreads();
+  over(p.D / N, held * nh, [&](int row, int v) {
+    const int at = row * inverse >> 16, h = row - at * nh;
+    *reinterpret_cast<uint4*>(static_cast<T*>(d.out) + to[at] + h * d.out_sh + v * N) = *reinterpret_cast<const uint4*>(rows + (at * H + h) * p.D + v * N);
+  });
+}
+
 template <typename T, bool INTER>
 int launch(const RotaryParams& p, int V, cudaStream_t st, const char* who) {
+  if (p.tile) {
+    const unsigned blocks = (p.count + (unsigned)p.tile - 1) / (unsigned)p.tile * p.chunks;
+    return launch_dependent(who, rotary_rows_kernel<T, INTER>, blocks, kThreads, (size_t)p.tile * kHeads * p.D * sizeof(T), st, p);
+  }
   const unsigned grid = (p.count + kGroup - 1) / kGroup * (p.per_group / kThreads);
   auto go = [&](auto kern) { return launch_dependent(who, kern, grid, kThreads, 0, st, p); };
   if constexpr (sizeof(T) == 2)
@@ -196,6 +275,10 @@ extern "C" int ulm_rotary(const ulm_rotary_args* a) {
   p.count = (unsigned)positions;
   p.turn_tasks = (unsigned)(kGroup * p.turning * p.chunks);
   p.per_group = (unsigned)(kGroup * per_position);
+  // whole rows: where vectors are at most kRowsBelow bytes though the rows are made of whole ones, and a few rows fit 16 KB
+  const int64_t row_bytes = (int64_t)a->D * es;
+  if (V * es <= kRowsBelow && a->D % wide == 0 && starts_on(wide) && kHeads * row_bytes <= kTileBytes)
+    p.tile = (int)(kTileBytes / (kHeads * row_bytes) < kMaxTile ? kTileBytes / (kHeads * row_bytes) : kMaxTile);
   p.factor = a->factor; p.sign = a->backward ? -1.f : 1.f;
   cudaStream_t st = (cudaStream_t)a->stream;
   auto go = [&](auto t) {
