@@ -191,8 +191,11 @@ norm_add_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
   }
 }
 
-// Asks for a row that will be wanted soon, into L2; `from` on 16 bytes, their number a multiple of 16.
-__device__ __forceinline__ void fetch_to_l2(const void* from, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory"); }
+// Asks for a row that will be wanted soon, into L2: the whole 16 bytes of it.
+__device__ __forceinline__ void fetch_to_l2(const void* from, int bytes) {
+  const uint64_t begin = (reinterpret_cast<uint64_t>(from) + 15) & ~15ull, end = (reinterpret_cast<uint64_t>(from) + bytes) & ~15ull;
+  if (end > begin) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(begin), "r"((uint32_t)(end - begin)) : "memory");
+}
 
 struct BwdParams {
   const float* z; const void* branch; const void* gate; const float* v; const float* w; Scale scale;
@@ -280,7 +283,7 @@ norm_add_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
         }
       }
     }
-    if (E == 8 && p.ahead && first == 0) {               // the group's next row is on its way to L2 while this one is worked on
+    if (p.ahead && first == 0) {               // the group's next row is on its way to L2 while this one is worked on
       const int64_t next = r + (int64_t)gridDim.x * groups;
       if (next < p.rows) {
         fetch_to_l2(p.z + next * p.z_stride, 4 * p.d);
@@ -446,9 +449,10 @@ constexpr int kAheadFrom = 512;
 using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 4>, Form<8, 4, 9, 2, 3>, Form<8, 4, 8, 2, 1>>;
 using Bwd8 = Forms<Form<8, 1, 12, 2, 3>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
 using Bwd8Gate = Forms<Form<8, 1, 20, 1, 6>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
-// widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only
-using Fwd4 = Forms<Form<4, 1, 8, 4, 8>, Form<4, 8, 8, 2, 1>>;
-using Bwd4 = Forms<Form<4, 1, 16, 2, 16>, Form<4, 2, 12, 2, 4>, Form<4, 4, 12, 1, 2>, Form<4, 8, 8, 1, 1>>;
+// widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only: 20000 x 772 with a gate 49 + 82 (33 + 52), 22721 x 796 49 + 65 (33 + 50),
+// 30000 x 300 with a gate 30 + 64 (19 + 30; eight vectors a lane 43 + 64)
+using Fwd4 = Forms<Form<4, 1, 8, 4, 8>, Form<4, 4, 8, 3, 8>, Form<4, 6, 8, 2, 8>, Form<4, 8, 8, 2, 1>>;
+using Bwd4 = Forms<Form<4, 1, 16, 2, 16>, Form<4, 2, 12, 2, 4>, Form<4, 4, 12, 1, 2>, Form<4, 8, 8, 1, 2>, Form<4, 4, 16, 1, 1>>;
 
 // Lanes a row and rows a CTA.  Few rows (less than the SMs take at full CTAs) are spread over more, smaller CTAs.
 struct Deal { int L, groups, threads; };
