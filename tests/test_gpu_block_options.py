@@ -141,6 +141,14 @@ def test_state_dicts_go_round_and_the_options_add_what_they_say():
         assert torch.equal(a.compute_loss(ids_of()).detach(), b.compute_loss(ids_of()).detach())
 
 
+def test_a_model_built_on_the_device():
+    with torch.device('cuda'):
+        model, _ = ulm_train.build('tiny64', 'cuda', **OPTIONS['all'])
+    with torch.autocast('cuda', dtype=BF16):
+        model.compute_loss(ids_of()).backward()
+    assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+
+
 @pytest.mark.parametrize('bad', [dict(branch_gate=True), dict(branch_scale=1.0), dict(rotary=dict(rotary_dim=66)), dict(rotary=dict(rotary_dim=31)), dict(rotary=dict(width=64))])
 def test_options_that_do_not_fit_are_refused(bad):
     with pytest.raises((ValueError, TypeError)):

@@ -50,7 +50,8 @@ def test_stretched_frequencies(dim):
     dict(rotary_dim=8, base=float('inf')), dict(rotary_dim=8, scaling=dict(factor=2.0)), dict(rotary_dim=8, scaling=dict(kind='longer', factor=2.0)),
     dict(rotary_dim=8, scaling=dict(kind='linear')), dict(rotary_dim=8, scaling=dict(kind='linear', factor=-1.0)), dict(rotary_dim=8, scaling=dict(kind='linear', factor=2.0, slow=1.0)),
     dict(rotary_dim=8, scaling=dict(kind='parts', factor=2.0)), dict(rotary_dim=8, scaling=dict(kind='parts', factor=2.0, original_length=64, slow=4.0, fast=4.0)),
-    dict(rotary_dim=8, scaling=dict(kind='linear', factor=2.0, attention_factor=-1.0)),
+    dict(rotary_dim=8, scaling=dict(kind='linear', factor=2.0, attention_factor=-1.0)), dict(rotary_dim=8, scaling=dict(kind='yarn', factor=2.0, original_length=8, attention_factor=0.0)),
+    dict(rotary_dim=8, scaling={}), dict(rotary_dim=8, scaling=dict(kind='yarn', factor=1e-9, original_length=8)),
 ])
 def test_refused_frequencies(args):
     with pytest.raises(ValueError):

@@ -211,7 +211,7 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
     kind = spec.pop('kind', None)
     if scaling is not None and kind not in ('linear', 'ntk', 'parts', 'yarn'):
         raise ValueError(f"scaling is one of kind 'linear', 'ntk', 'parts' and 'yarn', but got {scaling}")
-    multiplier = float(spec.pop('attention_factor', 0.0))
+    multiplier = spec.pop('attention_factor', None)
     w = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
     if kind is not None:
         f = float(spec.pop('factor', 0.0))
@@ -228,15 +228,16 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
                 raise ValueError(f"scaling of kind '{kind}' needs an original_length and slow < fast, but got {scaling}")
             keep = [min(1.0, max(0.0, (length * x / (2.0 * math.pi) - slow) / (fast - slow))) for x in w]
             w = [x * k + x / f * (1.0 - k) for x, k in zip(w, keep)]
-            if kind == 'yarn' and not multiplier:
+            if kind == 'yarn' and multiplier is None:
                 multiplier = 0.1 * math.log(f) + 1.0
     if spec:
         raise ValueError(f'scaling does not know {sorted(spec)}')
-    if not math.isfinite(multiplier) or multiplier < 0.0:
+    multiplier = 1.0 if multiplier is None else float(multiplier)
+    if not multiplier > 0.0 or not math.isfinite(multiplier):
         raise ValueError(f'the attention factor has to be a positive number, but got {multiplier}')
     # w / 2 pi of 2^64, as a signed number of the same bits: a float has 53 of them, so that an angle is off by 2^-54 of itself
     turns = [round(math.ldexp(x / (2.0 * math.pi), 64)) % (1 << 64) for x in w]
-    return torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device), multiplier or 1.0
+    return torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device), multiplier
 
 
 def rotary(q, k, turns, positions=None, interleaved=False, factor=1.0, inverse=False):
@@ -252,12 +253,13 @@ def rotary(q, k, turns, positions=None, interleaved=False, factor=1.0, inverse=F
 
 
 class Rotary(nn.Module):
-    """`rotary` with the frequencies of `rotary_turns`, which are no parameters and not part of a state dict."""
+    """`rotary` with the frequencies of `rotary_turns`, which are no parameters and not part of a state dict: a buffer that moves with the
+    module (made anew, not loaded: a module built on the meta device has none to move)."""
 
     def __init__(self, rotary_dim, base=10000.0, interleaved=False, scaling=None):
         super().__init__()
         self.rotary_dim, self.base, self.interleaved, self.scaling = rotary_dim, base, interleaved, scaling
-        turns, self.factor = rotary_turns(rotary_dim, base, scaling, device='cpu')
+        turns, self.factor = rotary_turns(rotary_dim, base, scaling)
         self.register_buffer('turns', turns, persistent=False)
 
     def forward(self, q, k, positions=None):
