@@ -177,6 +177,26 @@ def test_gate(dtype, shape, p):
         assert torch.equal(y, ulm_ops.swiglu_dropout(a, b, p, 1 << 40))
 
 
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+@pytest.mark.parametrize('form', ['halves', 'halves of three dimensions', 'columns apart', 'off its alignment', 'odd width', 'every other row', 'rows unequally apart', 'one transposed', 'broadcast', 'one row'])
+@pytest.mark.parametrize('graph', [True, False])
+def test_gate_of_operands_of_any_layout(dtype, form, graph):
+    base = randn((6, 10, 160), dtype, 1)
+    flat = base.view(60, 160)
+    a, b = {'halves': lambda: (flat[:, :80], flat[:, 80:]), 'halves of three dimensions': lambda: (base[..., :80], base[..., 80:]), 'columns apart': lambda: (flat[:, :80:2], flat[:, 80::2]),
+            'off its alignment': lambda: (flat[:, 1:73], flat[:, 81:153]), 'odd width': lambda: (flat[:, :75], flat[:, 80:155]), 'every other row': lambda: (flat[::2, :80], flat[::2, 80:]),
+            'rows unequally apart': lambda: (base[:, ::3, :80], base[:, ::3, 80:]), 'one transposed': lambda: (flat[:, :60], flat[:, :60].t()),
+            'broadcast': lambda: (flat[:1, :80].expand(60, 80), flat[1:2, 80:].expand(60, 80)), 'one row': lambda: (flat[3:4, :80], flat[3:4, 80:])}[form]()
+    gy = randn(a.shape, dtype, 2)
+
+    def call(p, q):
+        p, q = p.detach().requires_grad_(graph), q.detach().requires_grad_(graph)
+        y = ulm_ops.swiglu_8bit(p, q, 0.2, 3)
+        return (y.detach(), *torch.autograd.grad(y, [p, q], gy)) if graph else (y,)
+    for got, want in zip(call(a, b), call(a.contiguous(), b.contiguous())):
+        assert torch.equal(got, want)
+
+
 def test_gate_keeps_little():
     a, b = randn((4096, 2048), BF16, 1).requires_grad_(), randn((4096, 2048), BF16, 2).requires_grad_()
     torch.cuda.synchronize()

@@ -6,7 +6,7 @@
 //        dw = sum over rows of dy h;  C = sum over rows of dz sig(g) u;  dv = s C;  ds = v C, for one s its sum over the columns
 //
 // x, z and their gradients fp32; b, g, y and theirs 16-bit; s one number or one a column, g may be left out.  Statistics and sums fp32,
-// one rounding to 16 bits; exponent and division of the sigmoid in full, because z keeps what they leave.
+// one rounding to 16 bits.
 //
 // What bounds it: HBM, 12 bytes an element forward and 18 backward, 2 and 4 more with a gate.  A row belongs to L lanes of a CTA (half a warp, or
 // whole ones) and stays in registers between its uses; a lane owns vectors of E elements.  The backward's second mean needs dz and so the first one:
@@ -470,8 +470,11 @@ template <typename F> Deal deal(int64_t rows, int d) {
 
 template <typename TY, bool GATE, typename F, typename... Rest>
 int launch_fwd(Forms<F, Rest...>, FwdParams p, cudaStream_t st, const char* who) {
-  if constexpr (sizeof...(Rest) > 0)
+  if constexpr (sizeof...(Rest) > 0) {
     if (p.d > F::kMost) return launch_fwd<TY, GATE>(Forms<Rest...>(), p, st, who);
+  } else {
+    static_assert(F::kMost >= kMaxRow, "the last form takes every row");
+  }
   const Deal s = deal<F>(p.rows, p.d);
   p.L = s.L;
   const int64_t blocks = (p.rows + s.groups - 1) / s.groups;
@@ -481,8 +484,11 @@ int launch_fwd(Forms<F, Rest...>, FwdParams p, cudaStream_t st, const char* who)
 
 template <typename TY, bool GATE, typename F, typename... Rest>
 int launch_bwd(Forms<F, Rest...>, BwdParams p, int64_t* parts, cudaStream_t st, const char* who) {
-  if constexpr (sizeof...(Rest) > 0)
+  if constexpr (sizeof...(Rest) > 0) {
     if (p.d > F::kMost) return launch_bwd<TY, GATE>(Forms<Rest...>(), p, parts, st, who);
+  } else {
+    static_assert(F::kMost >= kMaxRow, "the last form takes every row");
+  }
   const Deal s = deal<F>(p.rows, p.d);
   p.L = s.L;
   p.ahead = p.d >= kAheadFrom;

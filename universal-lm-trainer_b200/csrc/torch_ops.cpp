@@ -1513,28 +1513,39 @@ Tensor unpack_8bit(const Tensor& codes_in, const Tensor& exps_in, at::ScalarType
   return x;
 }
 
-// The gate over dense operands, or (d > 0) the two column halves of one [rows, 2 d] matrix
-ulm_swiglu8_args gate8_args(const Packed8& kept, at::ScalarType dtype, int64_t d, const Drop& drop) {
+// Operands of the gate: dense (d = 0), or rows of d elements, `stride` apart
+struct GateRows { int64_t d = 0, stride = 0; };
+// those of a and b where neither is dense and the kernel can read both in place, as column blocks of a wider matrix are; d = 0 otherwise
+GateRows gate_rows(const Tensor& a, const Tensor& b) {
+  const int64_t n = a.dim(), vec = 16 / (int64_t)a.element_size();
+  if (n < 2 || a.numel() == 0 || a.strides() != b.strides() || a.is_contiguous()) return {};
+  const int64_t d = a.size(-1), stride = a.stride(-2);
+  if (a.stride(-1) != 1 || d % vec || stride % vec || stride < d || !aligned_to(a, 16) || !aligned_to(b, 16)) return {};
+  for (int64_t i = n - 2; i > 0; --i)
+    if (a.stride(i - 1) != a.size(i) * a.stride(i)) return {};       // the rows are not equally far apart
+  return {d, stride};
+}
+ulm_swiglu8_args gate8_args(const Packed8& kept, at::ScalarType dtype, const GateRows& rows, const Drop& drop) {
   ulm_swiglu8_args a{};
   a.codes_a = kept.codes(0); a.codes_b = kept.codes(1); a.exps_a = kept.exps(0); a.exps_b = kept.exps(1);
-  a.n = kept.n; a.d = d; a.row_stride = 2 * d; a.p = drop.p; a.seed = (uint64_t)drop.seed;
+  a.n = kept.n; a.d = rows.d; a.row_stride = rows.stride; a.p = drop.p; a.seed = (uint64_t)drop.seed;
   a.dtype = code_of(dtype); a.stream = stream_of(kept.buffer);
   return a;
 }
-Packed8 gate8_forward(const Tensor& a_t, const Tensor& b_t, int64_t d, int64_t n, const Tensor& y, const Drop& drop, bool graph) {
+Packed8 gate8_forward(const Tensor& a_t, const Tensor& b_t, const GateRows& rows, int64_t n, const Tensor& y, const Drop& drop, bool graph) {
   if (!graph) {                                            // the same values, and nothing to keep
     ulm_swiglu_args p{a_t.data_ptr(), b_t.data_ptr(), y.data_ptr(), nullptr, nullptr, nullptr, n, code_of(y.scalar_type()), 0, stream_of(y)};
-    check(ulm_swiglu_dropout(&p, false, d, 2 * d, drop.p, (uint64_t)drop.seed), "swiglu_8bit forward");
+    check(ulm_swiglu_dropout(&p, false, rows.d, rows.stride, drop.p, (uint64_t)drop.seed), "swiglu_8bit forward");
     return {};
   }
   const Packed8 kept = Packed8::make(n, 2, y);
-  ulm_swiglu8_args a = gate8_args(kept, y.scalar_type(), d, drop);
+  ulm_swiglu8_args a = gate8_args(kept, y.scalar_type(), rows, drop);
   a.a = a_t.data_ptr(); a.b = b_t.data_ptr(); a.y = y.data_ptr();
   check(ulm_swiglu8_fwd(&a), "swiglu_8bit forward");
   return kept;
 }
-void gate8_backward(const Packed8& kept, const Tensor& dy, const Tensor& da, const Tensor& db, int64_t d, const Tensor& y, const Drop& drop) {
-  ulm_swiglu8_args a = gate8_args(kept, dy.scalar_type(), d, drop);
+void gate8_backward(const Packed8& kept, const Tensor& dy, const Tensor& da, const Tensor& db, const GateRows& rows, const Tensor& y, const Drop& drop) {
+  ulm_swiglu8_args a = gate8_args(kept, dy.scalar_type(), rows, drop);
   a.dy = dy.data_ptr(); a.da = da.data_ptr(); a.db = db.data_ptr(); a.y = y.defined() ? y.data_ptr() : nullptr;
   check(ulm_swiglu8_bwd(&a), "swiglu_8bit backward");
 }
@@ -1546,7 +1557,7 @@ struct Swiglu8Bwd : OpNode {
   int64_t n = 0;
   variable_list backward(variable_list& g, const variable_list& kept) override {
     const Tensor dy = dense16(as_type(g[0], dtype)), da = empty_cuda(shape, dtype, dy), db = empty_cuda(shape, dtype, dy);
-    gate8_backward({kept[0], n, 2}, dy, da, db, 0, Tensor(), drop);
+    gate8_backward({kept[0], n, 2}, dy, da, db, {}, Tensor(), drop);
     return {da, db};
   }
   variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "swiglu_8bit"); }
@@ -1563,9 +1574,9 @@ Tensor swiglu_8bit(const Tensor& a_in, const Tensor& b_in, double p, int64_t see
   {
     OpScope scope;
     c10::cuda::CUDAGuard dev(a_in.device());
-    const Tensor a = dense16(a_in), b = dense16(b_in);
-    y = empty_cuda(a.sizes(), a.scalar_type(), a);
-    kept = gate8_forward(a, b, 0, a.numel(), y, drop, graph);
+    y = empty_cuda(a_in.sizes(), a_in.scalar_type(), a_in);
+    const GateRows rows = gate_rows(a_in, b_in);
+    kept = rows.d ? gate8_forward(a_in, b_in, rows, y.numel(), y, drop, graph) : gate8_forward(dense16(a_in), dense16(b_in), {}, y.numel(), y, drop, graph);
   }
   if (graph) {
     auto node = make_node<Swiglu8Bwd>(a_in, b_in);
@@ -1643,7 +1654,7 @@ struct FeedForward8Bwd : OpNode {
       da = empty_cuda({rows, ff}, cd, dy); db = empty_cuda({rows, ff}, cd, dy);
     }
     if (need2) y = empty_cuda({rows, ff}, cd, dy);
-    gate8_backward({pab, rows * ff, 2}, dy, da, db, halves ? ff : 0, y, drop);
+    gate8_backward({pab, rows * ff, 2}, dy, da, db, halves ? GateRows{ff, 2 * ff} : GateRows{}, y, drop);
     Tensor dw2;
     if (need2) dw2 = weight_grad(w2, go, y);
     y = Tensor();
@@ -1685,9 +1696,9 @@ Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, co
         at::mm_out(a, x2, c1.t());
         at::mm_out(b, x2, c3.t());
       }
-      pab = gate8_forward(ab, ab.narrow(1, ff, ff), ff, rows * ff, y, drop, graph);
+      pab = gate8_forward(ab, ab.narrow(1, ff, ff), {ff, 2 * ff}, rows * ff, y, drop, graph);
     } else {
-      pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), 0, rows * ff, y, drop, graph);
+      pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), {}, rows * ff, y, drop, graph);
     }
     if (graph && (w1.requires_grad() || w3.requires_grad())) px = pack8(x2);
     auto n = xc.sizes().vec();
