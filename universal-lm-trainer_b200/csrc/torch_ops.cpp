@@ -1965,6 +1965,18 @@ void def_op(pybind11::module_& m, const char* name, R (*f)(A...)) {
     return pybind11::cast(run());
   });
 }
+// An op without a gradient: only a tracer has to see it, or its results would be constants of the trace.
+template <typename R, typename... A>
+void def_traced(pybind11::module_& m, const char* name, R (*f)(A...)) {
+  m.def(name, [name, f](A... a) -> pybind11::object {
+    if (torch::jit::tracer::isTracing()) return pybind11::module_::import("ulm_recorded").attr("Recorded").attr("apply")(name, a...);
+    auto run = [&]() -> R {
+      pybind11::gil_scoped_release nogil;
+      return f(a...);
+    };
+    return pybind11::cast(run());
+  });
+}
 
 }  // namespace
 
@@ -2014,8 +2026,8 @@ PYBIND11_MODULE(_ulm_torch, m) {
   def_op(m, "linear", &::linear);
   def_op(m, "gated_linear", &::gated_linear);
   def_op(m, "gated_linear_dropout", &::gated_linear_dropout);
-  m.def("pack_8bit", &pack_8bit, no_gil());
-  m.def("unpack_8bit", &unpack_8bit, no_gil());
+  def_traced(m, "pack_8bit", &::pack_8bit);
+  def_traced(m, "unpack_8bit", &::unpack_8bit);
   def_op(m, "swiglu_8bit", &::swiglu_8bit);
   def_op(m, "linear_8bit", &::linear_8bit);
   def_op(m, "feed_forward_8bit", &::feed_forward_8bit);
