@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import ulm_infer
 import ulm_ops
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +36,14 @@ def test_packing_has_no_gradient_and_needs_none():
     with torch.autograd.forward_ad.dual_level():
         dual = ulm_ops.pack_8bit(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)))
     assert torch.equal(dual.codes, packed.codes) and torch.equal(dual.exponents, packed.exponents)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('autocast', [False, True])
+def test_prefill_builds_no_graph(autocast):
+    qkv = randn((2, 7, 384), BF16, 1).requires_grad_()
+    with torch.autocast('cuda', dtype=BF16, enabled=autocast):
+        out = ulm_infer.causal_attention(qkv, 2, rotary=ulm_ops.Rotary(64).cuda())
+    assert not any(t.requires_grad for t in out)           # the keys and values go into a cache

@@ -38,7 +38,7 @@ def causal_attention(qkv, n_heads, cos=None, sin=None, softmax_scale=None, rotar
             raise ValueError('causal_attention needs a CUDA fp16/bf16 [n, L, 3*n_heads*64] tensor with contiguous rows')
         with torch.no_grad():
             n, L = qkv.shape[:2]
-            q, k, v = (qkv.unflatten(2, (3, n_heads, 64))[:, :, i].transpose(1, 2) for i in range(3))
+            q, k, v = (qkv.detach().unflatten(2, (3, n_heads, 64))[:, :, i].transpose(1, 2) for i in range(3))
             q, k = rotary(q, k, positions)
             out = fa.flash_attn_v100(q, k, v, 0.0, True, softmax_scale)
         return out.transpose(1, 2).reshape(n, L, n_heads * 64), k, v
