@@ -64,6 +64,19 @@ def test_the_module_keeps_nothing_in_a_state_dict_and_survives_casts():
     assert torch.equal(m.turns, ulm_ops.rotary_turns(64, scaling=dict(kind='linear', factor=2.0))[0])
 
 
+def test_a_module_without_memory_gets_its_frequencies_with_it():
+    kw = dict(base=5000.0, scaling=dict(kind='linear', factor=2.0))
+    want = ulm_ops.rotary_turns(32, **kw)[0]
+    with torch.device('meta'):
+        whole = torch.nn.ModuleDict({'inner': ulm_ops.Rotary(32, **kw)})
+    assert whole['inner'].to('meta').turns.is_meta
+    assert torch.equal(whole.to_empty(device='cpu')['inner'].turns, want)      # as a model around it does
+    m = ulm_ops.Rotary(32, **kw)
+    assert torch.equal(m.to_empty(device='cpu').turns, want) and torch.equal(m.double().turns, want) and m.turns.dtype == torch.int64
+    m.turns = torch.arange(16)                             # frequencies that somebody else has put there move as they are
+    assert torch.equal(m.to_empty(device='cpu').turns, torch.arange(16)) and 'turns' not in m.state_dict()
+
+
 @pytest.mark.parametrize('where', ['cpu', 'meta'])
 def test_tensors_elsewhere_are_refused(where):
     x = torch.zeros(1, 2, 3, 8, device=where)

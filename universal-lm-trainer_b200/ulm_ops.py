@@ -254,13 +254,21 @@ def rotary(q, k, turns, positions=None, interleaved=False, factor=1.0, inverse=F
 
 class Rotary(nn.Module):
     """`rotary` with the frequencies of `rotary_turns`, which are no parameters and not part of a state dict: a buffer that moves with the
-    module (made anew, not loaded: a module built on the meta device has none to move)."""
+    module, and is made anew where a module built on the meta device gets memory."""
 
     def __init__(self, rotary_dim, base=10000.0, interleaved=False, scaling=None):
         super().__init__()
         self.rotary_dim, self.base, self.interleaved, self.scaling = rotary_dim, base, interleaved, scaling
         turns, self.factor = rotary_turns(rotary_dim, base, scaling)
         self.register_buffer('turns', turns, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        before = self.turns
+        super()._apply(fn, recurse)
+        if self.turns is not before and not self.turns.is_meta:        # to_empty brings memory of any content, and nothing loads over it
+            device = self.turns.device
+            self.turns = rotary_turns(self.rotary_dim, self.base, self.scaling, device)[0] if before.is_meta else before.to(device)
+        return self
 
     def forward(self, q, k, positions=None):
         return rotary(q, k, self.turns, positions, self.interleaved, self.factor)
