@@ -4,6 +4,7 @@ import torch
 
 import ulm_infer
 import ulm_ops
+from oracle import rotary as ro
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,18 @@ def test_prefill_builds_no_graph(autocast):
     with torch.autocast('cuda', dtype=BF16, enabled=autocast):
         out = ulm_infer.causal_attention(qkv, 2, rotary=ulm_ops.Rotary(64).cuda())
     assert not any(t.requires_grad for t in out)           # the keys and values go into a cache
+
+
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('at', [1, -1, 2, 3, 100, -4097, 1 << 20])
+def test_slow_pairs_turn_by_their_own_small_angle(at, interleaved):
+    """The sine alone (a pair of 0 and 1), relative to itself, in units of 2^-24: the angle's lower part, the factor and their product one
+    each, what is cut off behind 2^-58 of a turn two at 2^-35 of a turn, the slowest here, or instead the sum's rounding where an upper part is there too;
+    the polynomial's last step one.  Times 1 and plus 0 the result is the sine."""
+    turns = torch.cat([ulm_ops.rotary_turns(d, base, dict(kind='linear', factor=f))[0] for d, base, f in ((64, 1e4, 1.0), (128, 1e6, 8.0), (256, 1e8, 64.0))])
+    n = len(turns)
+    x = torch.zeros(1, 1, 1, 2 * n, device='cuda')
+    (x[..., 1::2] if interleaved else x[..., n:]).fill_(1)
+    y = ulm_ops.rotary(x, None, turns.cuda(), torch.tensor([at], device='cuda'), interleaved)[0].double().cpu()
+    y, want = (t[..., 0::2] if interleaved else t[..., :n] for t in (y, ro.rotary(x, [at], turns, interleaved)))
+    assert bool(((y - want).abs() <= 6 * 2.0 ** -24 * want.abs()).all()), float(((y - want) / want).abs().max())

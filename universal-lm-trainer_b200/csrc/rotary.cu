@@ -4,8 +4,9 @@
 //
 // for the R / 2 pairs (i, j) of a head's first R columns: j = i + R / 2, or neighbours (interleaved).  The other D - R pass through.
 // turns_i is the share of a full turn per position as a 64-bit fixed-point fraction, so that position * turns_i modulo 2^64 is the
-// exact share of a turn at any position, of any sign: no large angle is ever formed and none is rounded.  The angle is reduced to an
-// eighth of a turn on either side of a quarter in integers, and sine and cosine are the Taylor polynomials there (first
+// share of a turn at any position, of any sign, without an error beyond turns_i's own: no large angle is ever formed.  It is reduced to an
+// eighth of a turn on either side of a quarter in integers, cut to 2^-58 of a turn, and rounded once, to fp32: a sine is good
+// relative to itself, also a slow pair's near position 0.  Sine and cosine are the Taylor polynomials there (first
 // terms left out: x^11 / 11! < 1.8e-9 and x^12 / 12! < 1.2e-10 for |x| <= pi / 4).  Products and sums fp32, one rounding at the store.
 //
 // What bounds it: HBM; every element is read once and written once.  A thread owns the same columns of up to kHeads heads of one
@@ -46,12 +47,14 @@ __device__ __forceinline__ uint64_t position_of(const RotaryParams& p, int b, in
 // cos and sin of `share` / 2^64 turns, times f; the sine also times sign
 __device__ __forceinline__ void turn(uint64_t share, float f, float sign, float& c, float& s) {
   const uint32_t top = (uint32_t)(share >> 32), quarter = (top + 0x20000000u) >> 30;
-  const int rest = (int)(top - (quarter << 30));         // [-2^29, 2^29): an eighth of a turn either way
-  // x = rest 2 pi / 2^32 rounded once: the integer in two floats, the factor in two
-  const float hi = __int2float_rn(rest), lo = __int2float_rn(rest - __float2int_rn(hi));
+  const int rest = (int)(top - (quarter << 30));         // [-2^29, 2^29): an eighth of a turn either way, and the lower word behind it
+  // the nearest multiple of 64, which an fp32 number holds, and 32 bits below it, of which the first six are the rest's: a slow pair
+  // near position 0 turns by less than 2^-32, so that the lower word is all of its angle
+  const float hi = __int2float_rn((rest + 32) & ~63), lo = __int2float_rn((int)__funnelshift_r((uint32_t)share, top, 6));
+  // x = (hi + lo / 2^26) 2 pi / 2^32, rounded once: the factor in two floats
   constexpr double kUnit = 6.283185307179586476925 / 4294967296.0;
-  constexpr float u_hi = (float)kUnit, u_lo = (float)(kUnit - (double)u_hi);
-  const float x = fmaf(hi, u_hi, fmaf(hi, u_lo, lo * u_hi)), z = x * x;
+  constexpr float u_hi = (float)kUnit, u_lo = (float)(kUnit - (double)u_hi), u_26 = (float)(kUnit / 67108864.0);
+  const float x = fmaf(hi, u_hi, fmaf(hi, u_lo, lo * u_26)), z = x * x;
   float sp = fmaf(z, 1.f / 362880.f, -1.f / 5040.f), cp = fmaf(z, -1.f / 3628800.f, 1.f / 40320.f);
   sp = fmaf(z, sp, 1.f / 120.f);
   cp = fmaf(z, cp, -1.f / 720.f);
@@ -70,8 +73,9 @@ __device__ __forceinline__ void turn(uint64_t share, float f, float sign, float&
 // (floor 50.0), as against both in one warp, which waited for memory twice.
 constexpr int kHeads = 4;
 
+// Seven CTAs on an SM are 72 registers; at 80, and so six, 8x12x4096x64 bf16 takes 34.4 us for 33.
 template <typename T, int V, int A, bool INTER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 7)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int H = kHeads;
   grid_dependents_go();

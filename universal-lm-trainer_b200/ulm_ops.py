@@ -235,7 +235,7 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
     multiplier = 1.0 if multiplier is None else float(multiplier)
     if not multiplier > 0.0 or not math.isfinite(multiplier):
         raise ValueError(f'the attention factor has to be a positive number, but got {multiplier}')
-    # w / 2 pi of 2^64, as a signed number of the same bits: a float has 53 of them, so that an angle is off by 2^-54 of itself
+    # w / 2 pi of 2^64, as a signed number of the same bits: off by w's own roundings, a few 2^-53 of itself, and half of the last bit
     turns = [round(math.ldexp(x / (2.0 * math.pi), 64)) % (1 << 64) for x in w]
     return torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device), multiplier
 
@@ -245,8 +245,8 @@ def rotary(q, k, turns, positions=None, interleaved=False, factor=1.0, inverse=F
     views of any stride, of one type -> both turned, in the memory order they came in; ``k`` may be None (None comes back).
     ``turns`` (`rotary_turns`) has one number for each pair of columns: i with i + len(turns), or with ``interleaved`` 2i with 2i + 1;
     columns beyond 2 len(turns) pass through.  ``positions``: int32 or int64 [S] or [B, S] (packed sequences, single tokens of a cached
-    context; negative ones turn the other way), 0, 1, 2, .. without.  Exact at any distance: the angle is a 64-bit fraction of a turn.
-    fp32 arithmetic, one rounding.  ``inverse`` turns the other way (times the same ``factor``), which is also the gradient."""
+    context; negative ones turn the other way), 0, 1, 2, .. without.  The angle is positions * turns as a 64-bit fraction of a turn at any
+    distance, so that what it is off by is what turns are (a few 2^-53 of themselves from `rotary_turns`); fp32 sine, cosine and products, one rounding.  ``inverse`` turns the other way (times the same ``factor``), which is also the gradient."""
     if k is None:
         return N.ext().rotary_one(q, turns, positions, bool(interleaved), float(factor), bool(inverse)), None
     return N.ext().rotary(q, k, turns, positions, bool(interleaved), float(factor), bool(inverse))
