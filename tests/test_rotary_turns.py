@@ -45,6 +45,48 @@ def test_stretched_frequencies(dim):
     assert get(kind='linear', factor=1.0)[0].equal(ulm_ops.rotary_turns(dim)[0])
 
 
+@pytest.mark.parametrize('kind', ['parts', 'yarn'])
+@pytest.mark.parametrize('dim,base,length,slow,fast', [(64, 10000.0, 4096, 1.0, 32.0), (128, 1e6, 32768, 1.0, 4.0), (64, 10000.0, 64, 1.0, 32.0), (8, 10000.0, 4096, 15.0, 16.0), (2, 2.0, 4096, 1.0, 32.0)])
+def test_the_ramp_over_the_pairs(kind, dim, base, length, slow, fast):
+    """Against borders found by counting the pairs: the last that turns at least `fast` times, the first that turns at most `slow` times."""
+    f, n = 8.0, dim // 2
+    got, factor = ulm_ops.rotary_turns(dim, base, dict(kind=kind, factor=f, original_length=length, slow=slow, fast=fast, ramp='pairs'))
+    assert factor == (1.0 if kind == 'parts' else pytest.approx(0.1 * math.log(f) + 1.0))
+    turned = [length * base ** (-2 * i / dim) / (2 * math.pi) for i in range(4 * n + 16)]      # and of pairs that a wider head would have
+    first = max([i for i, t in enumerate(turned) if t >= fast], default=0)
+    last = min([i for i, t in enumerate(turned) if t <= slow])
+    for i, w in enumerate(radians(got)):
+        stays = 1.0 if i <= first else 0.0 if i >= last else 1.0 - (i - first) / (last - first)
+        plain = base ** (-2 * i / dim)
+        assert abs(float(w) - (plain * stays + plain / f * (1 - stays))) <= 2.0 ** -45 * plain + 2.0 ** -62      # half of 2^-64 turns
+
+
+def test_the_two_ramps_are_told_apart():
+    get = lambda **kw: [float(w) for w in radians(ulm_ops.rotary_turns(64, scaling=dict(kind='yarn', factor=8.0, original_length=4096, **kw))[0])]      # noqa: E731
+    turns, pairs = get(), get(ramp='pairs')
+    assert get(ramp='turns') == turns
+    off = [b / a for a, b in zip(turns, pairs)]
+    # 652 10000^(-i/32) turns in 4096 positions: 36.7 of pair 10, 27.5 of pair 11, 1.16 of pair 22, 0.87 of pair 23; 3.67 of pair 18, of which
+    # 2.67 / 31 = 0.086 and 5 / 13 = 0.385 stay: (0.385 + 0.615 / 8) / (0.086 + 0.914 / 8) = 2.3
+    assert [i for i, r in enumerate(off) if abs(r - 1) > 1e-9] == list(range(11, 23)) and 2.25 < off[18] == max(off) < 2.35
+
+
+def test_frequencies_of_the_callers_own():
+    w = [1.0, 0.25, -0.03, 0.0]
+    got, factor = ulm_ops.rotary_turns(8, scaling=dict(kind='list', radians=torch.tensor(w, dtype=torch.float64), attention_factor=1.5))
+    assert factor == 1.5 and all(abs(float(a) - b) <= 2.0 ** -50 * abs(b) + 2.0 ** -61 for a, b in zip([r if r < math.pi else r - 2 * Fraction(math.pi) for r in radians(got)], w))
+    m = ulm_ops.Rotary(8, scaling=dict(kind='list', radians=[10000.0 ** (-i / 4) for i in range(4)]))
+    assert torch.equal(m.turns, ulm_ops.rotary_turns(8)[0])
+
+
+@pytest.mark.parametrize('scaling', [
+    dict(kind='list'), dict(kind='list', radians=[1.0, 0.5, 0.1]), dict(kind='list', radians=[1.0, 0.5, 0.1, float('nan')]), dict(kind='list', radians=[1.0, 0.5, 0.1, 0.1], factor=2.0),
+    dict(kind='yarn', factor=2.0, original_length=64, ramp='columns'), dict(kind='parts', factor=2.0, original_length=64, slow=0.0, ramp='pairs'), dict(kind='linear', factor=2.0, ramp='pairs')])
+def test_refused_lists_and_ramps(scaling):
+    with pytest.raises(ValueError):
+        ulm_ops.rotary_turns(8, scaling=scaling)
+
+
 @pytest.mark.parametrize('args', [
     dict(rotary_dim=0), dict(rotary_dim=-2), dict(rotary_dim=7), dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, base=float('nan')),
     dict(rotary_dim=8, base=float('inf')), dict(rotary_dim=8, scaling=dict(factor=2.0)), dict(rotary_dim=8, scaling=dict(kind='longer', factor=2.0)),

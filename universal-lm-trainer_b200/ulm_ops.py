@@ -201,6 +201,12 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
                                         are f times slower, those between in proportion
       dict(kind='yarn', ...)            'parts' (a = 1, b = 32 by default), and q and k multiplied by 0.1 ln f + 1 each (Peng, Quesnelle, Fan
                                         and Shippole, "YaRN: efficient context window extension of large language models", 2023)
+      dict(kind='list', radians=w)      the w_i themselves, one of any sign for each pair (``base`` then does not count)
+
+    With 'parts' and 'yarn' "in proportion" is to the number of turns, as in the paper.  Released checkpoints are mostly trained
+    with ``ramp='pairs'``: in proportion to the pair's number i, from the pair that turns b times within L positions (a whole number, rounded down) to the
+    one that turns a times (rounded up).  The two differ by up to a factor of two and more between the borders, and nothing in a
+    checkpoint's weights tells them apart: its configuration has to.
 
     ``attention_factor=`` beside any of them replaces the multiplier.  Computed on the host in 64 bits."""
     if rotary_dim <= 0 or rotary_dim % 2:
@@ -209,11 +215,15 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
         raise ValueError(f'base has to be a finite number above 1, but got {base}')
     spec = dict(scaling or {})
     kind = spec.pop('kind', None)
-    if scaling is not None and kind not in ('linear', 'ntk', 'parts', 'yarn'):
-        raise ValueError(f"scaling is one of kind 'linear', 'ntk', 'parts' and 'yarn', but got {scaling}")
+    if scaling is not None and kind not in ('linear', 'ntk', 'parts', 'yarn', 'list'):
+        raise ValueError(f"scaling is one of kind 'linear', 'ntk', 'parts', 'yarn' and 'list', but got {scaling}")
     multiplier = spec.pop('attention_factor', None)
     w = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-    if kind is not None:
+    if kind == 'list':
+        w = [float(x) for x in spec.pop('radians', ())]
+        if len(w) != rotary_dim // 2 or not all(math.isfinite(x) for x in w):
+            raise ValueError(f'a list has a finite number of radians for each of the {rotary_dim // 2} pairs, but got {scaling}')
+    elif kind is not None:
         f = float(spec.pop('factor', 0.0))
         if not f > 0.0 or not math.isfinite(f):
             raise ValueError(f'scaling needs a positive factor, but got {scaling}')
@@ -226,7 +236,15 @@ def rotary_turns(rotary_dim, base=10000.0, scaling=None, device=None):
             length, slow, fast = (float(spec.pop(n, d)) for n, d in (('original_length', 0.0), ('slow', 1.0), ('fast', 32.0)))
             if not length > 0.0 or not fast > slow:
                 raise ValueError(f"scaling of kind '{kind}' needs an original_length and slow < fast, but got {scaling}")
-            keep = [min(1.0, max(0.0, (length * x / (2.0 * math.pi) - slow) / (fast - slow))) for x in w]
+            ramp = spec.pop('ramp', 'turns')
+            if ramp == 'turns':
+                keep = [min(1.0, max(0.0, (length * x / (2.0 * math.pi) - slow) / (fast - slow))) for x in w]
+            elif ramp == 'pairs' and slow > 0.0:
+                pair = lambda turns: rotary_dim * math.log(length / (2.0 * math.pi * turns)) / (2.0 * math.log(base))      # noqa: E731
+                first, last = max(math.floor(pair(fast)), 0), math.ceil(pair(slow))
+                keep = [1.0 if i <= first else max(0.0, (last - i) / (last - first)) if i < last else 0.0 for i in range(len(w))]
+            else:
+                raise ValueError(f"ramp is 'turns', or 'pairs' with a positive slow, but got {scaling}")
             w = [x * k + x / f * (1.0 - k) for x, k in zip(w, keep)]
             if kind == 'yarn' and multiplier is None:
                 multiplier = 0.1 * math.log(f) + 1.0
