@@ -1494,6 +1494,26 @@ Tensor unpack8(const Packed8& p, at::IntArrayRef sizes, at::ScalarType dtype) {
   return x;
 }
 
+// A projection's input x in 8 bits, as its node keeps it: packed for this node alone, or the caller's own codes and exponents, which several
+// nodes may keep.  `first` is the buffer or the codes; both are undefined where nothing asks for x.
+struct Input8 {
+  Tensor first, exps;
+  static Input8 keep(const Tensor& x, const OptTensor& codes, const OptTensor& exps) { return codes ? Input8{*codes, *exps} : Input8{pack8(x).buffer, Tensor()}; }
+  Tensor unpack(int64_t rows, int64_t d, at::ScalarType dtype) const {
+    if (!exps.defined()) return unpack8({first, rows * d, 1}, {rows, d}, dtype);
+    const Tensor c = dense16(first), e = exps.contiguous(), x = empty_cuda({rows, d}, dtype, c);
+    check(ulm_unpack8(static_cast<int8_t*>(c.data_ptr()), static_cast<uint8_t*>(e.data_ptr()), x.data_ptr(), rows * d, code_of(dtype), stream_of(x)), "unpack_8bit");
+    return x;
+  }
+};
+void check_packed(const Tensor& x, at::ScalarType cd, const OptTensor& codes, const OptTensor& exps, std::optional<at::ScalarType> dtype, const char* who) {
+  if (!codes && !exps && !dtype) return;
+  TORCH_CHECK_VALUE(codes && exps && dtype && codes->device() == x.device() && codes->scalar_type() == at::kChar && codes->sizes() == x.sizes() && exps->device() == x.device() &&
+                        exps->scalar_type() == at::kByte && exps->dim() == 1 && exps->numel() == ulm_pack8_blocks(x.numel()),
+                    who, " takes its input in 8 bits as pack_8bit makes it of that input");
+  TORCH_CHECK_VALUE(*dtype == cd, who, " takes its input in 8 bits of the type it computes in");
+}
+
 std::tuple<Tensor, Tensor> pack_8bit(const Tensor& x) {
   TORCH_CHECK_VALUE(x.is_cuda() && known(x.scalar_type()), "pack_8bit needs a CUDA fp16/bf16/fp32 tensor");
   OpScope scope;
@@ -1591,12 +1611,12 @@ struct Linear8Bwd : OpNode {
   at::ScalarType cd, x_dtype;
   std::vector<int64_t> shape;                              // of x
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor weight = kept[0], buffer = kept[1];
+    const Tensor weight = kept[0];
     const Tensor dy = g[0].reshape({-1, weight.size(0)}).to(cd);
     const int64_t d = shape.back(), rows = dy.size(0);
     Tensor dx, dw;
     if (task_should_compute_output(0)) dx = at::mm(dy, cast_cached(weight, cd)).view(shape).to(x_dtype);
-    if (task_should_compute_output(1)) dw = weight_grad(weight, dy, unpack8({buffer, rows * d, 1}, {rows, d}, cd));
+    if (task_should_compute_output(1)) dw = weight_grad(weight, dy, Input8{kept[1], kept[2]}.unpack(rows, d, cd));
     return {dx, dw};
   }
   variable_list backward_recorded(variable_list& g, const variable_list& kept) override { return backward_once(g, kept, "linear_8bit"); }
@@ -1609,11 +1629,12 @@ void check_projection(const Tensor& x, const Tensor& w, const char* who) {
   TORCH_CHECK_VALUE(known(compute_dtype(x)), who, " computes in fp16, bf16 or fp32");
 }
 
-Tensor linear_8bit(const Tensor& x, const Tensor& weight) {
+Tensor linear_8bit(const Tensor& x, const Tensor& weight, const OptTensor& codes, const OptTensor& exps, std::optional<at::ScalarType> packed_dtype) {
   check_projection(x, weight, "linear_8bit");
   const at::ScalarType cd = compute_dtype(x);
+  check_packed(x, cd, codes, exps, packed_dtype, "linear_8bit");
   Tensor y;
-  Packed8 kept;
+  Input8 kept;
   const bool graph = !no_graph(x, weight);
   {
     OpScope scope;
@@ -1622,13 +1643,13 @@ Tensor linear_8bit(const Tensor& x, const Tensor& weight) {
     auto n = xc.sizes().vec();
     n.back() = weight.size(0);
     y = at::mm(xc.reshape({-1, xc.size(-1)}), cast_cached(weight, cd).t()).view(n);
-    if (graph && weight.requires_grad()) kept = pack8(xc);
+    if (graph && weight.requires_grad()) kept = Input8::keep(xc, codes, exps);
   }
   if (graph) {
     auto node = make_node<Linear8Bwd>(x, weight);
     node->cd = cd; node->x_dtype = x.scalar_type(); node->shape = x.sizes().vec();
     node->keep(weight);
-    node->keep(kept.buffer);
+    node->keep(kept.first); node->keep(kept.exps);
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -1640,7 +1661,7 @@ struct FeedForward8Bwd : OpNode {
   std::vector<int64_t> shape;                              // of x
   int64_t rows = 0;
   variable_list backward(variable_list& g, const variable_list& kept) override {
-    const Tensor w1 = kept[0], w3 = kept[1], w2 = kept[2], px = kept[3], pab = kept[4];
+    const Tensor w1 = kept[0], w3 = kept[1], w2 = kept[2], pab = kept[3];
     const int64_t d = w1.size(1), ff = w1.size(0);
     const bool need_x = task_should_compute_output(0), need1 = task_should_compute_output(1), need3 = task_should_compute_output(2), need2 = task_should_compute_output(3);
     const Tensor go = g[0].reshape({-1, w2.size(0)}).to(cd);
@@ -1658,7 +1679,7 @@ struct FeedForward8Bwd : OpNode {
     Tensor dw2;
     if (need2) dw2 = weight_grad(w2, go, y);
     y = Tensor();
-    const Tensor x2 = need1 || need3 ? unpack8({px, rows * d, 1}, {rows, d}, cd) : Tensor();
+    const Tensor x2 = need1 || need3 ? Input8{kept[4], kept[5]}.unpack(rows, d, cd) : Tensor();
     variable_list r = need_x || need1 || need3 ? gated_products(*this, dab, da, db, x2, shape, x_dtype, w1, w3, cd) : variable_list(3);
     r.push_back(dw2);
     return r;
@@ -1667,16 +1688,19 @@ struct FeedForward8Bwd : OpNode {
 };
 
 // linear(drop(silu(x w1^T) * (x w3^T)), w2), of which x, the two projections and nothing else are kept, all three in 8 bits
-Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, double p, int64_t seed) {
+Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, double p, int64_t seed, const OptTensor& codes, const OptTensor& exps,
+                         std::optional<at::ScalarType> packed_dtype) {
   check_projection(x, w1, "feed_forward_8bit");
   TORCH_CHECK_VALUE(w3.device() == x.device() && w3.sizes() == w1.sizes() && w3.is_floating_point() && w2.device() == x.device() && w2.dim() == 2 && w2.size(1) == w1.size(0) && w2.is_floating_point(),
                     "feed_forward_8bit needs w1 and w3 [ff, d] and w2 [.., ff] on one CUDA device");
   check_drop(p, "feed_forward_8bit");
   const Drop drop{p, seed};
   const at::ScalarType cd = compute_dtype(x);
+  check_packed(x, cd, codes, exps, packed_dtype, "feed_forward_8bit");
   const int64_t ff = w1.size(0);
   Tensor out;
-  Packed8 px, pab;
+  Input8 px;
+  Packed8 pab;
   int64_t rows = 0;
   const bool graph = !no_graph(x, w1, w3, w2);
   {
@@ -1700,7 +1724,7 @@ Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, co
     } else {
       pab = gate8_forward(dense16(at::mm(x2, c1.t())), dense16(at::mm(x2, c3.t())), {}, rows * ff, y, drop, graph);
     }
-    if (graph && (w1.requires_grad() || w3.requires_grad())) px = pack8(x2);
+    if (graph && (w1.requires_grad() || w3.requires_grad())) px = Input8::keep(x2, codes, exps);
     auto n = xc.sizes().vec();
     n.back() = w2.size(0);
     out = at::mm(y, cast_cached(w2, cd).t()).view(n);
@@ -1708,7 +1732,7 @@ Tensor feed_forward_8bit(const Tensor& x, const Tensor& w1, const Tensor& w3, co
   if (graph) {
     auto node = make_node<FeedForward8Bwd>(x, w1, w3, w2);
     node->cd = cd; node->x_dtype = x.scalar_type(); node->drop = drop; node->shape = x.sizes().vec(); node->rows = rows;
-    node->keep(w1); node->keep(w3); node->keep(w2); node->keep(px.buffer); node->keep(pab.buffer);
+    node->keep(w1); node->keep(w3); node->keep(w2); node->keep(pab.buffer); node->keep(px.first); node->keep(px.exps);
     torch::autograd::set_history(out, node);
   }
   return out;

@@ -16,7 +16,7 @@ import torch.nn.functional as F
 
 import flash_attn_v100_cuda as _fa
 import ulm_ops
-from ulm_ops import BranchNorm, FusedRMSNorm, Rotary, feed_forward_8bit, gated_linear, linear, linear_8bit
+from ulm_ops import BranchNorm, FusedRMSNorm, Rotary, feed_forward_8bit, gated_linear, linear, linear_8bit, pack_8bit
 
 
 @dataclass
@@ -34,7 +34,7 @@ class ModelConfig:  # train.py:725-737
     # not the reference's: what a training step need not store between forward and backward
     counter_dropout: bool = False   # feed-forward and residual dropout by ulm_ops.Dropout, inside the gate and the residual add + norm; not to be captured in a CUDA graph
     streamed_loss: bool = False     # ulm_ops.streamed_cross_entropy: no logits
-    activations_8bit: bool = False  # inputs of wqkv, w1 and w3 and the gate's operands kept in 8 bits (ulm_ops.linear_8bit, feed_forward_8bit); dropout in the gate by counter_dropout alone
+    activations_8bit: bool = False  # inputs of wqkv, w1 and w3 (and of a branch_gate, which are the same) and the gate's operands kept in 8 bits (ulm_ops.linear_8bit, feed_forward_8bit); dropout in the gate by counter_dropout alone
     # not the reference's: other blocks.  They add parameters (branch_*) or leave the tables out (rotary)
     rotary: Optional[dict] = None   # arguments of ulm_ops.Rotary, in place of the d_model-wide tables; rotary_dim 64 unless it says less
     branch_norm: bool = False       # a norm behind attention and feed-forward (ulm_ops.BranchNorm) ...
@@ -115,14 +115,17 @@ class MultiHeadAttention(nn.Module):  # train.py:1920-1964
         self.dropout = config.dropout
         self.activations_8bit = _option(config, 'activations_8bit')
 
-    def forward(self, x, cos=None, sin=None, shape=None, rotary=None):
+    def forward(self, x, cos=None, sin=None, shape=None, rotary=None, packed=None):
         """``x``: [n, L, d], or -- with ``shape=(n, L)`` -- the flattened tokens [T', d] with T' >= n*L (rows
-        beyond n*L are padding that only the projections see).  ``rotary``: a `ulm_ops.Rotary` in place of the tables."""
+        beyond n*L are padding that only the projections see).  ``rotary``: a `ulm_ops.Rotary` in place of the tables.  ``packed``: x as
+        for `ulm_ops.linear_8bit`, with activations_8bit."""
         flat = shape is not None
         n, L = shape if flat else x.shape[:2]
         T = n * L
         x2d = x if flat else x.reshape(T, x.shape[-1])
-        qkv = linear_8bit(x2d, self.wqkv.weight) if self.activations_8bit else linear(x2d, self.wqkv.weight)
+        if packed is not None and not flat:
+            packed = packed._replace(codes=packed.codes.reshape(T, -1))
+        qkv = linear_8bit(x2d, self.wqkv.weight, packed) if self.activations_8bit else linear(x2d, self.wqkv.weight)
         if qkv.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError('attention runs in fp16/bf16: call the model under torch.autocast')
         # train.py:1935-1964 between the two projections as one op on the fused tensor: chunk, RoPE, causal
@@ -158,10 +161,15 @@ def _idle(dropout):
     return (_plain(dropout, nn.Dropout) or _plain(dropout, ulm_ops.Dropout)) and not (dropout.training and dropout.p > 0.0)
 
 
+def _counted(dropout):
+    """Whether ``dropout`` is a plain `ulm_ops.Dropout` at work."""
+    return _plain(dropout, ulm_ops.Dropout) and dropout.active()
+
+
 def _mask_of(dropout):
     """(p, seed) where ``dropout`` is a plain `ulm_ops.Dropout` at work, for the kernel that works in its place; None where it has
     to be called (or is idle)."""
-    return (dropout.p, ulm_ops.next_dropout_seed()) if _plain(dropout, ulm_ops.Dropout) and dropout.active() else None
+    return (dropout.p, ulm_ops.next_dropout_seed()) if _counted(dropout) else None
 
 
 def _make_dropout(p, counter):
@@ -177,13 +185,26 @@ class FeedForward(nn.Module):  # train.py:1966-1975
         self.w2 = nn.Linear(d_ff, d_model, bias=False)
         self.dropout = _make_dropout(dropout, counter_dropout)
 
-    def forward(self, x):
+    def keeps_8bit(self):
+        """Whether `forward` keeps 8 bits: not where a dropout that has to be called stands between the gate and w2."""
+        return self.activations_8bit and (_counted(self.dropout) or _idle(self.dropout))
+
+    def forward(self, x, packed=None):
+        """``packed``: x as for `ulm_ops.feed_forward_8bit`, where `keeps_8bit`."""
+        bits = self.keeps_8bit()
         mask = _mask_of(self.dropout)
-        if self.activations_8bit and (mask is not None or _idle(self.dropout)):
-            return feed_forward_8bit(x, self.w1.weight, self.w3.weight, self.w2.weight, *(mask or ()))
+        if bits:
+            return feed_forward_8bit(x, self.w1.weight, self.w3.weight, self.w2.weight, *(mask or (0.0, 0)), packed)
         if mask is not None:
             return linear(gated_linear(x, self.w1.weight, self.w3.weight, *mask), self.w2.weight)
         return linear(_drop(self.dropout, gated_linear(x, self.w1.weight, self.w3.weight)), self.w2.weight)
+
+
+def _packed_once(x, post, *linears):
+    """x in 8 bits, for a branch that keeps it so and the gate behind it to share; None where nobody would."""
+    if post is None or post.gate is None or not torch.is_grad_enabled() or not any(m.weight.requires_grad for m in (post.gate, *linears)):
+        return None
+    return pack_8bit(x.detach().to(torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else x.dtype))
 
 
 class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
@@ -214,15 +235,20 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
             h = self.norm1(x)
         else:
             x, h = self.norm1.add_forward(x, *_branch(pending))       # train.py:1993 of the previous block + 1988
-        a = self.self_attn(h, cos=cos, sin=sin, shape=shape, rotary=rotary)
+        # only modules that nobody watches or has changed are sure to project h as it is
+        attn, ff, packed = self.self_attn, self.ff, None
+        if _plain(attn, MultiHeadAttention) and attn.activations_8bit:
+            packed = _packed_once(h, self.attn_post, attn.wqkv)
+        a = attn(h, cos=cos, sin=sin, shape=shape, rotary=rotary, **({} if packed is None else {'packed': packed}))
         if self.attn_post is not None:
-            x, h = self.norm2.add_forward(x, a, post=self.attn_post, gate=self.attn_post.gate_of(h))
+            x, h = self.norm2.add_forward(x, a, post=self.attn_post, gate=self.attn_post.gate_of(h, packed))
         else:
             x, h = self.norm2.add_forward(x, a)                       # train.py:1989 + 1991
-        out = self.ff(h)                                              # added by whoever normalises next
+        packed = _packed_once(h, self.ff_post, ff.w1, ff.w3) if _plain(ff, FeedForward) and ff.keeps_8bit() else None
+        out = ff(h) if packed is None else ff(h, packed)              # added by whoever normalises next
         mask = _mask_of(self.dropout)
         if self.ff_post is not None:
-            return x, (out if mask is not None else _drop(self.dropout, out), *(mask or (0.0, 0)), self.ff_post, self.ff_post.gate_of(h))
+            return x, (out if mask is not None else _drop(self.dropout, out), *(mask or (0.0, 0)), self.ff_post, self.ff_post.gate_of(h, packed))
         return x, (out, *mask) if mask is not None else _drop(self.dropout, out)
 
 

@@ -95,9 +95,11 @@ class BranchNorm(nn.Module):
         self.scale = None if scale is None else nn.Parameter(torch.tensor(float(scale)))
         self.eps = eps
 
-    def gate_of(self, x):
-        """The gate before its sigmoid, of the branch's input."""
-        return None if self.gate is None else linear(x, self.gate.weight)
+    def gate_of(self, x, packed=None):
+        """The gate before its sigmoid, of the branch's input; ``packed``: as for `linear_8bit`, which then is the projection."""
+        if self.gate is None:
+            return None
+        return linear(x, self.gate.weight) if packed is None else linear_8bit(x, self.gate.weight, packed)
 
 
 def swiglu(a, b):
@@ -394,17 +396,19 @@ def swiglu_8bit(a, b, p=0.0, seed=0):
     return N.ext().swiglu_8bit(a, b, float(p), _as_i64(seed))
 
 
-def linear_8bit(x, weight):
+def linear_8bit(x, weight, packed=None):
     """`linear`, whose backward has its input in 8 bits alone (`pack_8bit`; nothing of it where the weight takes no gradient): the
-    result and x's gradient are those of `linear`, the weight's is that of the 8-bit input.  CUDA only."""
-    return N.ext().linear_8bit(x, weight)
+    result and x's gradient are those of `linear`, the weight's is that of the 8-bit input.  CUDA only.  ``packed``: `pack_8bit` of x in the type of
+    the product (autocast's, or x's own), for several projections of one x to keep it once between them; without it each packs its own."""
+    return N.ext().linear_8bit(x, weight, *(packed or (None, None, None)))
 
 
-def feed_forward_8bit(x, w1, w3, w2, dropout_p=0.0, seed=0):
+def feed_forward_8bit(x, w1, w3, w2, dropout_p=0.0, seed=0, packed=None):
     """``linear(gated_linear(x, w1, w3, dropout_p, seed), w2)`` (train.py:1975) as one op that keeps x and the two projections in 8 bits and nothing
     else: d + 2 d_ff bytes a token (and 1/32 of that) where the ops by themselves keep 2 d + 6 d_ff.  The backward forms the gate's result
-    again from the 8-bit projections, for w2's gradient.  The gate is `swiglu_8bit`'s, the products `linear`'s.  CUDA only."""
-    return N.ext().feed_forward_8bit(x, w1, w3, w2, float(dropout_p), _as_i64(seed))
+    again from the 8-bit projections, for w2's gradient.  The gate is `swiglu_8bit`'s, the products `linear`'s.  ``packed``: x as for
+    `linear_8bit`.  CUDA only."""
+    return N.ext().feed_forward_8bit(x, w1, w3, w2, float(dropout_p), _as_i64(seed), *(packed or (None, None, None)))
 
 
 def ce_rows_forward(logits, target, ignore_index):
