@@ -239,7 +239,9 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
         attn, ff, packed = self.self_attn, self.ff, None
         if _plain(attn, MultiHeadAttention) and attn.activations_8bit:
             packed = _packed_once(h, self.attn_post, attn.wqkv)
-        a = attn(h, cos=cos, sin=sin, shape=shape, rotary=rotary, **({} if packed is None else {'packed': packed}))
+        # what a model without the options does not have is not handed on: a module put in the attention's place need not know of it
+        options = {k: v for k, v in (('rotary', rotary), ('packed', packed)) if v is not None}
+        a = attn(h, cos=cos, sin=sin, shape=shape, **options)
         if self.attn_post is not None:
             x, h = self.norm2.add_forward(x, a, post=self.attn_post, gate=self.attn_post.gate_of(h, packed))
         else:
@@ -300,11 +302,12 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
         if self.rotary is None and self.config.use_rope:
             cos, sin = _tables_2d(*self.rope(L), self.layers[0].self_attn.head_dim if len(self.layers) else 64)
         pending = None
+        options = {} if self.rotary is None else {'rotary': self.rotary}       # as for the attention in a block
         for layer in self.layers:
             if self.use_gradient_checkpointing and self.training:
-                x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), self.rotary, use_reentrant=False)
+                x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), use_reentrant=False, **options)
             else:
-                x, pending = layer(x, pending, cos=cos, sin=sin, shape=(n, L), rotary=self.rotary)
+                x, pending = layer(x, pending, cos=cos, sin=sin, shape=(n, L), **options)
         x = self.norm(x) if pending is None else self.norm.add_forward(x, *_branch(pending))[1]
         return x, T
 
