@@ -69,3 +69,15 @@ def test_modules_that_know_of_no_options(wrapped, checkpointing, options):
     assert torch.allclose(out.reshape(15, 64), x * 0.5, rtol=0, atol=2.0 ** -20)      # eight roundings of numbers below 2
     out.sum().backward()
     assert model.layers[0].self_attn.w.weight.grad.any()
+
+
+def test_a_model_pickled_whole_before_the_options():
+    model, ids = model_of(False, dropout=0.0), torch.arange(15).view(3, 5)
+    want = model.forward_hidden(ids)
+    del model.rotary
+    for layer in model.layers:
+        del layer.attn_post, layer.ff_post
+    assert torch.equal(model.forward_hidden(ids), want)
+    for module in (ulm_model.MultiHeadAttention(model.config), ulm_model.FeedForward(64, 128, 0.0)):
+        del module.activations_8bit
+        assert module.activations_8bit is False

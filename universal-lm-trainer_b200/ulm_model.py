@@ -106,6 +106,8 @@ def apply_rotary_pos_emb(q, k, cos, sin):
 
 
 class MultiHeadAttention(nn.Module):  # train.py:1920-1964
+    activations_8bit = False                               # of a module pickled whole before there was the option
+
     def __init__(self, config: ModelConfig):
         super().__init__()
         self.d_model, self.n_heads = config.d_model, config.n_heads
@@ -177,6 +179,8 @@ def _make_dropout(p, counter):
 
 
 class FeedForward(nn.Module):  # train.py:1966-1975
+    activations_8bit = False                               # as in MultiHeadAttention
+
     def __init__(self, d_model: int, d_ff: int, dropout: float, counter_dropout: bool = False, activations_8bit: bool = False):
         super().__init__()
         self.activations_8bit = activations_8bit
@@ -235,22 +239,23 @@ class DecoderOnlyBlock(nn.Module):  # train.py:1977-1994
             h = self.norm1(x)
         else:
             x, h = self.norm1.add_forward(x, *_branch(pending))       # train.py:1993 of the previous block + 1988
+        attn_post, ff_post = (getattr(self, n, None) for n in ('attn_post', 'ff_post'))      # absent where pickled whole before there were any
         # only modules that nobody watches or has changed are sure to project h as it is
         attn, ff, packed = self.self_attn, self.ff, None
         if _plain(attn, MultiHeadAttention) and attn.activations_8bit:
-            packed = _packed_once(h, self.attn_post, attn.wqkv)
+            packed = _packed_once(h, attn_post, attn.wqkv)
         # what a model without the options does not have is not handed on: a module put in the attention's place need not know of it
         options = {k: v for k, v in (('rotary', rotary), ('packed', packed)) if v is not None}
         a = attn(h, cos=cos, sin=sin, shape=shape, **options)
-        if self.attn_post is not None:
-            x, h = self.norm2.add_forward(x, a, post=self.attn_post, gate=self.attn_post.gate_of(h, packed))
+        if attn_post is not None:
+            x, h = self.norm2.add_forward(x, a, post=attn_post, gate=attn_post.gate_of(h, packed))
         else:
             x, h = self.norm2.add_forward(x, a)                       # train.py:1989 + 1991
-        packed = _packed_once(h, self.ff_post, ff.w1, ff.w3) if _plain(ff, FeedForward) and ff.keeps_8bit() else None
+        packed = _packed_once(h, ff_post, ff.w1, ff.w3) if _plain(ff, FeedForward) and ff.keeps_8bit() else None
         out = ff(h) if packed is None else ff(h, packed)              # added by whoever normalises next
         mask = _mask_of(self.dropout)
-        if self.ff_post is not None:
-            return x, (out if mask is not None else _drop(self.dropout, out), *(mask or (0.0, 0)), self.ff_post, self.ff_post.gate_of(h, packed))
+        if ff_post is not None:
+            return x, (out if mask is not None else _drop(self.dropout, out), *(mask or (0.0, 0)), ff_post, ff_post.gate_of(h, packed))
         return x, (out, *mask) if mask is not None else _drop(self.dropout, out)
 
 
@@ -299,10 +304,11 @@ class DecoderOnlyTransformer(nn.Module):  # train.py:1996-2082
                 flat_ids = torch.cat([flat_ids, flat_ids.new_zeros(Tp - T)])
         x = self.embedding(flat_ids)
         cos = sin = None
-        if self.rotary is None and self.config.use_rope:
+        rotary = getattr(self, 'rotary', None)             # absent in a model pickled whole before there was the option
+        if rotary is None and self.config.use_rope:
             cos, sin = _tables_2d(*self.rope(L), self.layers[0].self_attn.head_dim if len(self.layers) else 64)
         pending = None
-        options = {} if self.rotary is None else {'rotary': self.rotary}       # as for the attention in a block
+        options = {} if rotary is None else {'rotary': rotary}       # as for the attention in a block
         for layer in self.layers:
             if self.use_gradient_checkpointing and self.training:
                 x, pending = torch.utils.checkpoint.checkpoint(layer, x, pending, cos, sin, (n, L), use_reentrant=False, **options)
