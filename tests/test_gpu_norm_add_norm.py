@@ -155,6 +155,46 @@ def test_gates_open_and_closed():
         assert torch.isfinite(t).all()
 
 
+def test_open_gates_are_no_gates():
+    """A gate that is open to the last bit leaves the very bits of the call without one, gradients included; a closed one passes x alone."""
+    s = inputs(12, 64, F16, True, 'channels')
+    s['gate'][:6], s['gate'][6:] = torch.tensor([float('inf'), 60000.0, 88.0, 17.5, 200.0, 1000.0], device='cuda')[:, None], float('inf')
+    plain = {k: v for k, v in s.items() if k != 'gate'}
+    got, want = call(s), call(plain)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    assert not got['dgate'][[0, 1, 4, 5]].any()
+    check(s, got)
+    s['gate'][1::2] *= -1
+    got = call(s)
+    assert torch.equal(got['x_new'][[0, 2, 4]], want['x_new'][[0, 2, 4]]) and torch.equal(got['x_new'][[1, 5]], s['x'][[1, 5]])
+    check(s, got)
+
+
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('d,rows', [(100, 10007), (300, 4001), (772, 2003), (1020, 2003), (1028, 2003), (2052, 1001), (3076, 701), (4100, 401), (5124, 401), (8188, 401),
+                                    (128, 9001), (2048, 1501), (2560, 1001), (4096, 701), (5120, 401), (6144, 401), (8192, 401)])
+def test_groups_that_take_a_third_row(d, rows, gate):
+    """The backward's groups take row after row; their sums alternate between two sets of slots, and the row after next is asked for ahead."""
+    s = inputs(rows, d, F16 if d % 3 else BF16, gate, SCALES[d // 4 % 5], seed=d)
+    check(s, call(s))
+
+
+@pytest.mark.parametrize('gate', [False, True])
+@pytest.mark.parametrize('d,rows', [(4100, 19001), (8192, 19001), (2560, 60001)])
+def test_forward_groups_that_take_a_third_row(d, rows, gate):
+    """The same of the forward, whose grid is far larger."""
+    s = inputs(rows, d, BF16, gate, 'scalar', seed=d)
+    x_new, y = ulm_ops.norm_add_norm(s['x'], s['b'], s['v'], s['w'], gate=s.get('gate'), scale=s['scale'])
+    stat = 64 * UNIT[F32]
+    for at in range(0, rows, 2048):
+        part = {k: v[at:at + 2048] if v.dim() == 2 else v for k, v in s.items()}
+        f = forward64(part, 1e-6)
+        big = f['t']['x'].abs() + f['term'].abs()
+        within(x_new[at:at + 2048], f['x_new'], (stat + 8 * UNIT[F32]) * f['term'].abs() + 2 * UNIT[F32] * big)
+        within(y[at:at + 2048], f['y'], (UNIT[BF16] + stat) * f['y'].abs() + 2 * stat * (big * f['r2']).amax(-1, keepdim=True) * f['t']['w'].abs() + TINY[BF16])
+
+
 def test_a_bad_row_spoils_no_other():
     s = inputs(9, 128, BF16, True, 'channels')
     good = call(s)
