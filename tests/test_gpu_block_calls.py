@@ -90,6 +90,24 @@ def test_changed_codes_are_noticed_and_frozen_weights_keep_none():
     assert torch.equal(torch.autograd.grad(parked.sum(), w[0])[0], torch.autograd.grad(ulm_ops.linear_8bit(x, w[0]).sum(), w[0])[0])
 
 
+def test_a_traced_projection_of_a_packed_input():
+    w = torch.nn.ParameterList([randn((64, 64), F32, 2 + i) for i in range(3)])
+
+    class Both(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = w
+
+        def forward(self, x):
+            packed = ulm_ops.pack_8bit(x)
+            return LAYERS['linear'](x, self.w, packed) + LAYERS['feed-forward'](x, self.w, packed)
+    m, x = Both(), randn((4, 64), F32, 7)
+    got, want = torch.jit.trace(m, randn((4, 64), F32, 1))(x), m(x)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got.sum(), list(w)), torch.autograd.grad(want.sum(), list(w))):
+        assert float((a - b).norm()) <= 2.0 ** -20 * float(b.norm())       # the sums of two gradients may be taken in another order
+
+
 @pytest.mark.parametrize('dropout', [0.0, 0.2])
 def test_a_branch_gate_shares_the_packed_input(dropout):
     """With a gate behind the branches a layer keeps no more of its two normalised inputs than without one."""
