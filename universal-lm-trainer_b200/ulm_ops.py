@@ -283,11 +283,15 @@ class Rotary(nn.Module):
         self.register_buffer('turns', turns, persistent=False)
 
     def _apply(self, fn, recurse=True):
-        before = self.turns
-        super()._apply(fn, recurse)
-        if self.turns is not before and not self.turns.is_meta:        # to_empty brings memory of any content, and nothing loads over it
-            device = self.turns.device
-            self.turns = rotary_turns(self.rotary_dim, self.base, self.scaling, device)[0] if before.is_meta else before.to(device)
+        # where fn would have the frequencies is asked with none of them, as to_empty would leave memory of any content, and nothing loads over it
+        turns = self._buffers.pop('turns')
+        try:
+            super()._apply(fn, recurse)
+            device = fn(turns[:0]).device
+            if device != turns.device:
+                turns = rotary_turns(self.rotary_dim, self.base, self.scaling, device)[0] if turns.is_meta else turns.to(device)
+        finally:
+            self._buffers['turns'] = turns
         return self
 
     def forward(self, q, k, positions=None):
