@@ -440,7 +440,7 @@ template <typename...> struct Forms {};
 //   backward  32768 x 768 76 (69), x 1024 99 (92), 16396 x 4096 196 (184); 48044 x 1024 169 (165), 16396 x 4096 252 (225).  Eight columns a lane and
 //             24 warps an SM without a gate up to 1024 (sixteen a lane: 87 at 768); the gate's values do not fit the 80 registers of that,
 //             and with sixteen a lane 48044 x 1024 went from 204 to 181.  Thirty-two from where two rows no longer fit a CTA, the gate formed at both uses:
-//             16396 x 4096 with a gate 340 -> 281.  A group then waits for a row, meets at a barrier and stores before it loads the
+//             16396 x 4096 with a gate 340 -> 281; above 4096 columns one row is on an SM: 4096 x 5120 90 (58), x 8192 110 (92).  A group then waits for a row, meets at a barrier and stores before it loads the
 //             next, and few rows are on an SM at a time: the next row asked for into L2 meanwhile took 48044 x 1024 from 181 to 169,
 //             16396 x 4096 with a gate from 281 to 252, 5000 x 2816 from 55 to 48; rows of 128 and 256 columns, of which many are under
 //             way, from 18.5 to 20.6 (so from kAheadFrom on only: 512 with a gate 38.9 -> 38.0).  Copies of the row itself, by cp.async into shared memory
@@ -449,8 +449,9 @@ constexpr int kAheadFrom = 512;
 using Fwd8 = Forms<Form<8, 1, 8, 4, 8>, Form<8, 2, 8, 3, 8>, Form<8, 3, 8, 3, 8>, Form<8, 4, 8, 2, 4>, Form<8, 4, 9, 2, 3>, Form<8, 4, 8, 2, 1>>;
 using Bwd8 = Forms<Form<8, 1, 12, 2, 3>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
 using Bwd8Gate = Forms<Form<8, 1, 20, 1, 6>, Form<8, 2, 12, 1, 2>, Form<8, 4, 8, 1, 1>>;
-// widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only: 20000 x 772 with a gate 49 + 82 (33 + 52), 22721 x 796 49 + 65 (33 + 50),
-// 30000 x 300 with a gate 30 + 64 (19 + 30; eight vectors a lane 43 + 64)
+// widths of 4 modulo 8, and tensors that lie on multiples of 8 or 16 bytes only: 20000 x 772 with a gate 50 + 85 (33 + 52), 22721 x 796 49 + 65 (33 + 50),
+// 30000 x 300 with a gate 30 + 70 (19 + 30; eight vectors a lane 43 + 64), 4096 x 4100 53 + 120 (31 + 46), with a gate 61 + 166 (36 + 56).  The backward's
+// forms were chosen without a gate; with one, 80 registers spill (184 bytes a thread for 132 to 768 columns), and 128 do above 4096 (420; 188 without)
 using Fwd4 = Forms<Form<4, 1, 8, 4, 8>, Form<4, 4, 8, 3, 8>, Form<4, 6, 8, 2, 8>, Form<4, 8, 8, 2, 1>>;
 using Bwd4 = Forms<Form<4, 1, 16, 2, 16>, Form<4, 2, 12, 2, 4>, Form<4, 4, 12, 1, 2>, Form<4, 8, 8, 1, 2>, Form<4, 4, 16, 1, 1>>;
 
